@@ -64,8 +64,9 @@ def listed():
 
 
 def _log_int(rng, lo, hi):
-    """A whole number spread evenly over the logarithm of [lo, hi]."""
-    return max(lo, min(hi, int(round(lo * (hi / lo) ** rng.random()))))
+    """A whole number spread evenly over the logarithm of [lo, hi]; odd, so never whole tiles, where it is large."""
+    n = max(lo, min(hi, int(round(lo * (hi / lo) ** rng.random()))))
+    return n if n < 1024 else (n - 1) | 1
 
 
 def draw(rng):
@@ -83,15 +84,16 @@ def draw(rng):
     group = rng.choice([g for g in (32, 64, 128, dim) if dim % g == 0])
     page = rng.choice([8, 16, 32, 64, 128])
     if op == "append":
-        return dict(op=op, tokens=_log_int(rng, 1, 16000), heads=kv * ratio, kv=kv, dim=dim,
+        prompt = rng.random() < 0.5
+        return dict(op=op, tokens=_log_int(rng, 1, 16000 if prompt else 256), heads=kv * ratio, kv=kv, dim=dim,
                     rot=rng.choice([dim, dim // 2, 32]), layout=rng.choice(["half", "interleaved"]), type=kind,
-                    group=group, page=page, prompt=rng.random() < 0.5)
+                    group=group, page=page, prompt=prompt)
     way = rng.choice(["decode", "decode", "verify", "prompt"])
     case = dict(op=op, heads=kv * ratio, kv=kv, dim=dim, group=group, page=page, type=kind,
                 window=rng.choice([0, 0, _log_int(rng, 16, 4096)]))
     if way == "prompt":
         hi = _log_int(rng, 64, min(2048, 2048 * 4096 // max(4096, kv * ratio * dim)))
-        return dict(case, batch=rng.randint(1, 4), lo=hi // 2, hi=hi + rng.randint(0, 1000), q_lo=max(1, hi // 3),
+        return dict(case, batch=rng.randint(1, 4), lo=hi // 2, hi=(hi + rng.randint(0, 1000)) | 1, q_lo=max(1, hi // 3),
                     q_hi=hi)
     batch = _log_int(rng, 1, 128)
     hi = _log_int(rng, 1, max(2, min(131072, 350000 // batch * 128 // dim)))
