@@ -416,6 +416,93 @@ UP_API int up_sm100_w4a16_gemm(const uint8_t* w, const uint16_t* scale, const ui
                         size_t workspace_bytes, void* stream);
 UP_API size_t up_sm100_w4a16_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t group);
 
+/* ---- Serving operators: rotary positions and attention over a 4-bit cache --------------------------------
+ *
+ * No counterpart in the reference, which has no attention. They stand beside the int4 weights: what lies between the
+ * W4A16 products of a decode step. */
+
+/* Pairs of a rotation: dimensions (i, i + rot/2), or (2i, 2i + 1). */
+typedef enum up_rope_layout { UP_ROPE_HALF = 0, UP_ROPE_INTERLEAVED = 1 } up_rope_layout;
+/* How a rotation's frequencies are scaled for contexts longer than a model was trained on (up_sm100_rope_table). */
+typedef enum up_rope_scaling {
+  UP_ROPE_NONE = 0, UP_ROPE_LINEAR = 1, UP_ROPE_BASE = 2, UP_ROPE_WAVELENGTH = 3, UP_ROPE_RAMP = 4
+} up_rope_scaling;
+
+/* Rotary positions of x [batch, seq, heads, dim] (F32, F16 or BF16; strides in elements, the dimension contiguous). The
+ * first `rot` dimensions of each head turn by the token's position p, with c = table[p][i] and s = table[p][rot/2 + i]:
+ * the pair (x0, x1) becomes (x0 c - x1 s, x1 c + x0 s), in f32 with every product and sum rounded by itself, then
+ * rounded once to x's type. The other dimensions are copied. `backward` != 0 applies the transposed map, the gradient
+ * with respect to x. `positions` (I32 or I64) holds position [b, s] at b * pos_stride_b + s; NULL is s itself. `table`
+ * is f32 [n_pos, rot]; a position outside it gives NaN in the rotated dimensions. `out` may be x with x's strides;
+ * its rows must not overlap (each stride at least dim where its extent is above 1). */
+UP_API int up_sm100_rope(const void* x, int dtype, int64_t batch, int64_t seq, int64_t heads, int64_t dim,
+                         int64_t x_stride_b, int64_t x_stride_s, int64_t x_stride_h, const void* positions,
+                         int index_dtype, int64_t pos_stride_b, const float* table, int64_t n_pos, int64_t rot,
+                         int layout, int backward, void* out, int64_t out_stride_b, int64_t out_stride_s,
+                         int64_t out_stride_h, void* stream);
+
+/* The table of up_sm100_rope: gain * cos(p f_i) at [p][i] and gain * sin(p f_i) at [p][rot/2 + i], computed in f64 and
+ * rounded once, with f_i = base^(-2i/rot) scaled by:
+ *  LINEAR      f_i / factor
+ *  BASE        base * factor^(rot/(rot - 2)) in place of base
+ *  WAVELENGTH  (1 - t) f_i / factor + t f_i, t = clamp((orig f_i / (2 pi) - low) / (high - low), 0, 1)
+ *  RAMP        the same blend, t = 1 - clamp((i - i_high) / (i_low - i_high), 0, 1), where i_n = rot ln(orig / (2 pi n)) /
+ *              (2 ln base), i_high rounded down and at least 0, i_low rounded up and at most rot - 1. */
+UP_API int up_sm100_rope_table(float* table, int64_t n_pos, int64_t rot, double base, int scaling, double factor,
+                               double low, double high, double orig, double gain, void* stream);
+
+/* A paged key/value cache in 4 bits: k and v int4 [pages, kv_heads, page, dim], packed two per byte along dim (low
+ * nibble = even), k_scale and v_scale f16 [pages, kv_heads, page, dim / group], all dense and 16-byte aligned. A value is
+ * nibble * scale (up_sm100_dequant_i4_bf16 reads the arrays as [pages * kv_heads * page, dim]). `page` (tokens a page) is
+ * a power of two from 8 to 4096; dim a multiple of 32 up to 256; group a multiple of 32 that divides dim. Slot s is
+ * token s % page of page s / page. */
+typedef struct up_kv4_cache {
+  void* k;
+  void* v;
+  void* k_scale;
+  void* v_scale;
+  int64_t pages, kv_heads, page, dim, group;
+} up_kv4_cache;
+
+/* Writes `tokens` new tokens into the cache and rotates their queries, in one launch. q [tokens, q_heads, dim] (or NULL
+ * with q_heads 0) is rotated as by up_sm100_rope into q_out (which may be q with q's strides); k [tokens, kv_heads, dim]
+ * is rotated, v is not; both are quantised per group: with a the largest magnitude of the (f32, rotated) group,
+ * scale = f16(min(a * f32(1/7), 65504)) and nibble = clamp(rint(x * (1 / scale)), -8, 7), 0 where scale is 0. A group
+ * with an infinity or a NaN gets a NaN scale and reads back as NaN. `dtype`: BF16 or F16. Strides in elements, the
+ * dimension contiguous. positions (I32 or I64, one a token) and table as for up_sm100_rope, rot 0 for no rotation. slots
+ * (I32 or I64): a token whose slot is outside [0, pages * page) is left out of the cache; its queries are rotated. Slots
+ * are distinct; with equal ones, which token's bytes stay is not defined. */
+UP_API int up_sm100_kv4_append(const void* q, const void* k, const void* v, int dtype, int64_t tokens,
+                               int64_t q_heads, int64_t q_stride_t, int64_t q_stride_h, int64_t k_stride_t,
+                               int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h, const void* positions,
+                               int pos_dtype, const float* table, int64_t n_pos, int64_t rot, int layout,
+                               const void* slots, int slot_dtype, const up_kv4_cache* cache, void* q_out,
+                               int64_t q_out_stride_t, int64_t q_out_stride_h, void* stream);
+
+/* Attention of query tokens over a paged 4-bit cache. q [tokens, q_heads, dim] (BF16 or F16; q_heads a multiple of
+ * cache->kv_heads, query head h reading key/value head h / (q_heads / kv_heads)). Sequence b's queries are the tokens
+ * [cu_q[b], cu_q[b + 1]) (I32, batch + 1 entries, not falling; NULL: one token a sequence, tokens = batch); its cached
+ * tokens are seq_lens[b] (I32), token j on page block_table[b * table_stride + j / page] (I32). With nq queries and L
+ * cached tokens, query i stands at position L - nq + i and sees the tokens j <= that position (`causal` != 0; else all),
+ * and only j > position - window where window > 0.
+ *   out[i] = sum_j softmax_j(scale * q_i . k_j) v_j,   lse[i] = log sum_j exp(scale * q_i . k_j)  (f32, or NULL)
+ * over the visible tokens, accumulated in f32, rounded once to q's type. A query that sees nothing gives 0 and -inf.
+ * What a masked token's page or slot holds (a NaN scale included) has no effect. seq_lens beyond table_width * page count
+ * as that much; cached tokens on a page outside [0, pages) are left out; query tokens that no sequence names are not
+ * written. `workspace` from up_sm100_kv4_attention_workspace_bytes, 256-byte aligned, zero-filled before its first use;
+ * launches leave it ready for the next one, of any shape that needs no more bytes. The result does not depend on the
+ * order in which the parts of a split sequence finish. q is 16-byte aligned with strides of whole 8 elements, out 8-byte
+ * aligned with strides of whole 4 (UP_ERR_UNSUPPORTED else); at most 2^30 cached tokens a sequence and 2^30 query rows
+ * (tokens * q_heads / kv_heads). Launches that overlap on the GPU need separate workspaces. */
+UP_API int up_sm100_kv4_attention(const void* q, int dtype, int64_t tokens, int64_t q_heads, int64_t q_stride_t,
+                                  int64_t q_stride_h, const up_kv4_cache* cache, const int32_t* block_table,
+                                  int64_t table_stride, int64_t table_width, const int32_t* seq_lens,
+                                  const int32_t* cu_q, int64_t batch, int causal, int64_t window, float scale, void* out,
+                                  int64_t out_stride_t, int64_t out_stride_h, float* lse, int64_t lse_stride_t,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+UP_API size_t up_sm100_kv4_attention_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t batch, int64_t kv_heads,
+                                                     int64_t dim);
+
 /* ---- Several GPUs of one node ------------------------------------------------------------------------
  *
  * The reference models a launch over several devices as the same kernel run per device on its slice of the

@@ -31,6 +31,9 @@ KERNEL = dict(NONE=-1, ROW_SUM_F32=1, ROW_MAX_ARGMAX_BF16=2, SCAN_I32=3, GATHER_
               W4A16_GEMM=6, REDUCE2D_F32=7, REDUCE2D_I32=8, SCATTER=9, BINCOUNT=10, REDUCE_F32=11, REDUCE_I32=12,
               ROW_REDUCE_F32=13, COL_SUM_SPLITK=14, WINDOW=15, IM2COL=16)
 ROW_REDUCE_FORM = dict(NONE=0, SOFTMAX=1, RMS_NORM=2, CENTRED=3)
+# up_rope_layout, up_rope_scaling
+ROPE_LAYOUT = dict(HALF=0, INTERLEAVED=1)
+ROPE_SCALING = dict(NONE=0, LINEAR=1, BASE=2, WAVELENGTH=3, RAMP=4)
 # WriteCombine ordinals (crates/unpopped/src/ir.rs:2723-2732)
 COMBINE = dict(ASSIGN=0, ADD=1, MAX=2, MIN=3)
 LOWER_ERROR = {0: "Ok", 1: "UnsupportedDtype", 2: "UnsupportedSchedule", 3: "UnsupportedOp",
@@ -67,6 +70,12 @@ class UpLowered(ctypes.Structure):
                 ("detail", ctypes.c_char * 160), ("scalars", ctypes.c_int64 * 8), ("n_scalars", ctypes.c_int32)]
 
 
+class UpKv4Cache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("page", ctypes.c_int64), ("dim", ctypes.c_int64), ("group", ctypes.c_int64)]
+
+
 class UpError(RuntimeError):
     def __init__(self, status: int, where: str, detail: str = ""):
         self.status = status
@@ -75,6 +84,7 @@ class UpError(RuntimeError):
 
 # Every symbol include/up_sm100.h declares, with its ctypes signature.
 _P, _I, _I64, _U64, _SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64, ctypes.c_size_t
+_F64, _F32, _KV4 = ctypes.c_double, ctypes.c_float, ctypes.POINTER(UpKv4Cache)
 SIGNATURES = {
     "up_sm100_version": ([], _I),
     "up_sm100_name": ([], ctypes.c_char_p),
@@ -110,6 +120,14 @@ SIGNATURES = {
     "up_sm100_dequant_i4_bf16": ([_P, _P, _I64, _I64, _I64, _P, _P], _I),
     "up_sm100_w4a16_gemm": ([_P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _SZ, _P], _I),
     "up_sm100_w4a16_workspace_bytes": ([_I64, _I64, _I64, _I64], _SZ),
+    "up_sm100_rope": ([_P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I, _I64, _P, _I64, _I64, _I, _I, _P, _I64,
+                       _I64, _I64, _P], _I),
+    "up_sm100_rope_table": ([_P, _I64, _I64, _F64, _I, _F64, _F64, _F64, _F64, _F64, _P], _I),
+    "up_sm100_kv4_append": ([_P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I, _P, _I64, _I64, _I,
+                             _P, _I, _KV4, _P, _I64, _I64, _P], _I),
+    "up_sm100_kv4_attention": ([_P, _I, _I64, _I64, _I64, _I64, _KV4, _P, _I64, _I64, _P, _P, _I64, _I, _I64, _F32, _P,
+                                _I64, _I64, _P, _I64, _P, _SZ, _P], _I),
+    "up_sm100_kv4_attention_workspace_bytes": ([_I64, _I64, _I64, _I64, _I64], _SZ),
     "up_sm100_set_wait_limit_ns": ([_U64], None),
     "up_sm100_set_test_withhold_flag": ([_I], None),
     "up_sm100_set_test_scan_epoch": ([_U64], None),

@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import ACCUM, COMBINE, EK, OOB, OP, check
+from ._lib import ACCUM, COMBINE, EK, OOB, OP, ROPE_LAYOUT, ROPE_SCALING, UpKv4Cache, check
 
 _OPS = {"sum": OP["SUM"], "max": OP["MAX"], "min": OP["MIN"]}
 _OOBS = {"skip": OOB["SKIP"], "clamp": OOB["CLAMP"], "zero_fill": OOB["ZERO_FILL"]}
@@ -371,6 +371,214 @@ def w4a16(w_packed: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, group: i
     check(L.up_sm100_w4a16_gemm(w_packed.data_ptr(), scale.data_ptr(), x.data_ptr(), m, n, k, group, out.data_ptr(),
                                 ws.data_ptr(), ws.numel(), _stream(x)), "w4a16")
     return out
+
+
+# ---- rotary positions, the 4-bit paged cache and its attention ----
+_ROPE_EK = {torch.float32: EK["F32"], torch.float16: EK["F16"], torch.bfloat16: EK["BF16"]}
+_KV4_EK = {torch.float16: EK["F16"], torch.bfloat16: EK["BF16"]}
+_POS = {torch.int32: EK["I32"], torch.int64: EK["I64"]}
+_LAYOUTS = {"half": ROPE_LAYOUT["HALF"], "interleaved": ROPE_LAYOUT["INTERLEAVED"]}
+
+
+def _same_device(device, *tensors):
+    """Everything lies on one CUDA device, which is the current one (where the library launches)."""
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise ValueError("the tensors must be on the current CUDA device")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError("all tensors must be on one CUDA device")
+
+
+def rope_table(n_pos: int, rot: int, base: float = 10000.0, scaling: tuple | None = None, gain: float = 1.0,
+               device="cuda") -> torch.Tensor:
+    """The f32 [n_pos, rot] table that `rope` and `kv4_append` read: gain * cos(p f_i) in the first rot/2 columns, gain *
+    sin(p f_i) in the others, f_i = base^(-2i/rot). `scaling` for contexts longer than a model was trained on:
+    ("linear", factor), ("base", factor), ("wavelength", factor, low, high, orig_len) or
+    ("ramp", factor, low, high, orig_len); up_sm100.h has their formulas."""
+    out = torch.empty((n_pos, rot), dtype=torch.float32, device=device)
+    kind, rest = ("none", ()) if scaling is None else (scaling[0], scaling[1:])
+    if len(rest) != {"none": 0, "linear": 1, "base": 1, "wavelength": 4, "ramp": 4}.get(kind, -1):
+        raise ValueError(f"rope_table: no such scaling {scaling!r}")
+    factor, low, high, orig = tuple(float(v) for v in rest) + (1.0, 0.0, 0.0, 0.0)[len(rest):]
+    _same_device(out.device)
+    check(_lib.load().up_sm100_rope_table(out.data_ptr(), n_pos, rot, base, ROPE_SCALING[kind.upper()], factor, low,
+                                          high, orig, gain, _stream(out)), "rope_table")
+    return out
+
+
+def _rope(x, positions, table, layout, backward, out, where):
+    _cuda(x, "x")
+    if x.dtype not in _ROPE_EK or x.dim() not in (3, 4) or (x.stride(-1) != 1 and x.shape[-1] > 1):
+        raise ValueError(f"{where} takes float32, float16 or bfloat16 [tokens, heads, dim] or [batch, seq, heads, dim] "
+                         "with the dimension contiguous")
+    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous():
+        raise ValueError("table is float32 [positions, rot], contiguous (rope_table)")
+    shape = x.shape
+    four = len(shape) == 4
+    batch, seq, heads, dim = shape if four else (1,) + tuple(shape)
+    pos_ptr, pos_kind, pos_stride = None, 0, 0
+    if positions is not None:
+        if positions.dtype not in _POS or not positions.is_contiguous():
+            raise ValueError("positions are contiguous int32 or int64")
+        if tuple(positions.shape) == (seq,):
+            pos_stride = 0
+        elif four and tuple(positions.shape) == (batch, seq):
+            pos_stride = seq
+        else:
+            raise ValueError("positions are one a token: [tokens], [seq] or [batch, seq]")
+        pos_ptr, pos_kind = positions.data_ptr(), _POS[positions.dtype]
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif out.shape != shape or out.dtype != x.dtype or (out.stride(-1) != 1 and dim > 1):
+        raise ValueError("out has x's shape and type, with the dimension contiguous")
+    _same_device(x.device, positions, table, out)
+    xs, os = x.stride(), out.stride()
+    check(_lib.load().up_sm100_rope(x.data_ptr(), _ROPE_EK[x.dtype], batch, seq, heads, dim, xs[0] if four else 0, xs[-3],
+                                    xs[-2], pos_ptr, pos_kind, pos_stride, table.data_ptr(), table.shape[0],
+                                    table.shape[1], _LAYOUTS[layout], backward, out.data_ptr(), os[0] if four else 0,
+                                    os[-3], os[-2], _stream(x)), where)
+    return out
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor | None, table: torch.Tensor, layout: str = "half",
+         out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions: x [tokens, heads, dim] or [batch, seq, heads, dim] (float32, float16, bfloat16; any strides with
+    the dimension contiguous) with the first table.shape[1] dimensions of each head turned by the token's position.
+    layout "half" pairs dimensions (i, i + rot/2), "interleaved" (2i, 2i + 1). positions: int32 or int64, one a token
+    ([seq] serves every sequence of a batch), None counts from 0; one outside the table gives NaN. out may be x."""
+    return _rope(x, positions, table, layout, 0, out, "rope")
+
+
+def rope_backward(grad: torch.Tensor, positions: torch.Tensor | None, table: torch.Tensor, layout: str = "half",
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of `rope` with respect to its input, from the gradient of its output."""
+    return _rope(grad, positions, table, layout, 1, out, "rope_backward")
+
+
+def kv4_cache(pages: int, kv_heads: int, dim: int, page: int = 16, group: int = 32, device="cuda") -> tuple:
+    """A new paged 4-bit cache, the tuple (k, v, k_scale, v_scale) that `kv4_append` and `kv4_attention` take: k and v
+    uint8 [pages, kv_heads, page, dim/2] (int4 two per byte, low nibble = even dimension), the scales float16
+    [pages, kv_heads, page, dim/group]. A slot reads as zeros until it is written."""
+    rows = (pages, kv_heads, page)
+    return tuple(torch.zeros(rows + (n,), dtype=t, device=device)
+                 for n, t in ((dim // 2, torch.uint8), (dim // 2, torch.uint8), (dim // group, torch.float16),
+                              (dim // group, torch.float16)))
+
+
+def _kv4(cache, where):
+    k, v, ks, vs = cache
+    shape, sshape = k.shape, ks.shape
+    if k.dtype != torch.uint8 or v.dtype != torch.uint8 or ks.dtype != torch.float16 or vs.dtype != torch.float16:
+        raise ValueError(f"{where}: a cache is (k uint8, v uint8, k_scale float16, v_scale float16)")
+    if len(shape) != 4 or v.shape != shape or vs.shape != sshape or sshape[:3] != shape[:3] or len(sshape) != 4:
+        raise ValueError(f"{where}: cache arrays are [pages, kv_heads, page, dim/2] and [pages, kv_heads, page, dim/group]")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError(f"{where}: cache arrays are contiguous")
+    dim, groups = 2 * shape[3], sshape[3]
+    if groups == 0 or dim % groups:
+        raise ValueError(f"{where}: the scales' groups divide the head size")
+    return UpKv4Cache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), shape[0], shape[1], shape[2], dim,
+                      dim // groups)
+
+
+def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: tuple, slots: torch.Tensor,
+               positions: torch.Tensor | None = None, table: torch.Tensor | None = None,
+               q: torch.Tensor | None = None, layout: str = "half",
+               q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Writes new tokens into a paged 4-bit cache (`kv4_cache`) in one launch and returns their rotated queries.
+
+    k, v [tokens, kv_heads, dim] and q [tokens, heads, dim] (or None) are bfloat16 or float16, of any strides with the
+    dimension contiguous (views of one projection's output, say). With a table (`rope_table`), q and k turn by their
+    token's position first, as `rope` does; without one they do not. k and v are quantised to int4 with an f16 scale a
+    group. slots (int32 or int64, one a token): the token's place, page * page_size + place in the page; a slot outside the
+    cache (-1: padding) leaves the token out. q_out may be q."""
+    _cuda(k, "k")
+    c = _kv4(cache, "kv4_append")
+    tokens, shape = k.shape[0], (k.shape[0], c.kv_heads, c.dim)
+    if k.dtype not in _KV4_EK or v.dtype != k.dtype:
+        raise ValueError("kv4_append takes bfloat16 or float16, q, k and v alike")
+    if tuple(k.shape) != shape or tuple(v.shape) != shape or k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError("k and v are [tokens, kv_heads, dim] of the cache, with the dimension contiguous")
+    if slots.dtype not in _POS or tuple(slots.shape) != (tokens,) or not slots.is_contiguous():
+        raise ValueError("slots are contiguous int32 or int64, one a token")
+    rot, n_pos, pos_kind = 0, 0, 0
+    if table is not None:
+        if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous():
+            raise ValueError("table is float32 [positions, rot], contiguous (rope_table)")
+        if positions is None or positions.dtype not in _POS or tuple(positions.shape) != (tokens,) or \
+                not positions.is_contiguous():
+            raise ValueError("positions are contiguous int32 or int64, one a token")
+        n_pos, rot = table.shape
+        pos_kind = _POS[positions.dtype]
+    heads, qs, qos = 0, (0, 0), (0, 0)
+    if q is not None:
+        if q.dim() != 3 or q.dtype != k.dtype or q.shape[0] != tokens or q.shape[2] != c.dim or q.stride(2) != 1:
+            raise ValueError("q is [tokens, heads, dim] of k's type, with the dimension contiguous")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(2) != 1:
+            raise ValueError("q_out has q's shape and type, with the dimension contiguous")
+        heads, qs, qos = q.shape[1], q.stride(), q_out.stride()
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    _same_device(k.device, v, slots, positions, table, q, q_out, *cache)
+    ks, vs = k.stride(), v.stride()
+    check(_lib.load().up_sm100_kv4_append(
+        q.data_ptr() if heads else None, k.data_ptr(), v.data_ptr(), _KV4_EK[k.dtype], tokens, heads, qs[0], qs[1], ks[0],
+        ks[1], vs[0], vs[1], positions.data_ptr() if rot else None, pos_kind, table.data_ptr() if rot else None, n_pos,
+        rot, _LAYOUTS[layout], slots.data_ptr(), _POS[slots.dtype], ctypes.byref(c), q_out.data_ptr() if heads else None,
+        qos[0], qos[1], _stream(k)), "kv4_append")
+    return q_out
+
+
+def kv4_attention(q: torch.Tensor, cache: tuple, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                  cu_q: torch.Tensor | None = None, causal: bool = True, window: int = 0,
+                  scale: float | None = None, out: torch.Tensor | None = None, want_lse: bool = False,
+                  ws: torch.Tensor | None = None):
+    """Attention of query tokens over a paged 4-bit cache (`kv4_cache`): out [tokens, heads, dim] of q's type, and with
+    want_lse the f32 [tokens, heads] log-sum-exp of each query's logits.
+
+    q [tokens, heads, dim] bfloat16 or float16 (rows 16-byte aligned), heads a multiple of the cache's; query head h reads
+    key/value head h // (heads // kv_heads). seq_lens int32 [batch]: a sequence's cached tokens, the new ones included;
+    block_table int32 [batch, width]: its pages. cu_q int32 [batch + 1]: where each sequence's query tokens begin in q;
+    None: one token a sequence. The query tokens are the last of their sequence: each sees the cached tokens up to its own
+    (`causal`), and of these the last `window` where window > 0. A query that sees nothing gives 0 (and -inf)."""
+    _cuda(q, "q")
+    c = _kv4(cache, "kv4_attention")
+    if q.dtype not in _KV4_EK or q.dim() != 3 or q.shape[2] != c.dim or q.stride(2) != 1:
+        raise ValueError("q is bfloat16 or float16 [tokens, heads, dim] of the cache's dim, with the dimension contiguous")
+    tokens, heads, dim = q.shape
+    if heads % c.kv_heads:
+        raise ValueError("q's heads are a multiple of the cache's")
+    batch = seq_lens.shape[0]
+    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens is contiguous int32 [batch]")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != batch or \
+            (block_table.stride(1) != 1 and block_table.shape[1] > 1):
+        raise ValueError("block_table is int32 [batch, width] with contiguous rows")
+    if cu_q is None:
+        if tokens != batch:
+            raise ValueError("without cu_q there is one query token a sequence")
+    elif cu_q.dtype != torch.int32 or tuple(cu_q.shape) != (batch + 1,) or not cu_q.is_contiguous():
+        raise ValueError("cu_q is contiguous int32 [batch + 1]")
+    if window < 0:
+        raise ValueError("window is not negative")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError("out has q's shape and type, with the dimension contiguous")
+    _same_device(q.device, block_table, seq_lens, cu_q, out, *cache)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if want_lse else None
+    L = _lib.load()
+    if ws is None:
+        ws = workspace("kv4", L.up_sm100_kv4_attention_workspace_bytes(tokens, heads, batch, c.kv_heads, dim), q.device)
+    qs, os = q.stride(), out.stride()
+    check(L.up_sm100_kv4_attention(
+        q.data_ptr(), _KV4_EK[q.dtype], tokens, heads, qs[0], qs[1], ctypes.byref(c), block_table.data_ptr(),
+        block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), batch,
+        int(causal), window, dim ** -0.5 if scale is None else scale, out.data_ptr(), os[0], os[1],
+        None if lse is None else lse.data_ptr(), heads, ws.data_ptr(), ws.numel(), _stream(q)), "kv4_attention")
+    return (out, lse) if want_lse else out
 
 
 def launch_count() -> int:
