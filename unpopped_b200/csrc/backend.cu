@@ -59,10 +59,15 @@ uint64_t context_id() {
       get_id = reinterpret_cast<GetId>(p);
   });
   if (get_current == nullptr || get_id == nullptr) return 0;
-  cudaFree(nullptr);  // makes the device's primary context current if no context is yet
   CUcontext c = nullptr;
   unsigned long long id = 0;
-  if (get_current(&c) != CUDA_SUCCESS || c == nullptr || get_id(c, &id) != CUDA_SUCCESS) return 0;
+  if (get_current(&c) != CUDA_SUCCESS) return 0;
+  if (c == nullptr) {
+    // Makes the device's primary context current. Not called where one is: it would invalidate a stream capture.
+    cudaFree(nullptr);
+    if (get_current(&c) != CUDA_SUCCESS || c == nullptr) return 0;
+  }
+  if (get_id(c, &id) != CUDA_SUCCESS) return 0;
   return (uint64_t)id;
 }
 

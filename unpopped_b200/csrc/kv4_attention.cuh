@@ -96,11 +96,19 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
 // d += a b: 16 x 8 x 16, f16 operands, f32 sums.
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
       "%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// d = a b + {c0, c1, c0, c1}: the same start for both of a thread's rows.
+__device__ __forceinline__ void mma_f16_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1, float c0, float c1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, "
+      "%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -109,15 +117,28 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// (v & mask) ^ flip
+__device__ __forceinline__ uint32_t pick(uint32_t v, uint32_t mask, uint32_t flip) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(d) : "r"(v), "r"(mask), "r"(flip));
+  return d;
+}
+
+// The nibbles of a word as f16 pairs without a conversion: a nibble with its sign bit flipped is n + 8, and as an f16's
+// low bits the subnormal (n + 8) 2^-24; the odd nibbles, four bits higher, are 16 times that. e[i] holds nibbles i and
+// i + 4. The product's other side takes the 2^24, the 16 and the sum of the eights.
+__device__ __forceinline__ void expand_raw(uint32_t w, uint32_t (&e)[4]) {
+  const uint32_t x = w >> 8;
+  e[0] = pick(w, 0x000f000fu, 0x00080008u);
+  e[1] = pick(w, 0x00f000f0u, 0x00800080u);
+  e[2] = pick(x, 0x000f000fu, 0x00080008u);
+  e[3] = pick(x, 0x00f000f0u, 0x00800080u);
+}
+
 // The nibbles of a word as f16 pairs, exactly: e[i] holds nibbles i and i + 4 (signed). A nibble's two's complement bits
 // with the sign bit flipped are n + 8; OR-ed into the mantissa of 1024 they give 1024 + (n + 8), and 16 steps higher
 // 1024 + 16 (n + 8), so that the odd nibbles need no shift of their own.
 __device__ __forceinline__ void expand(uint32_t w, uint32_t (&e)[4]) {
-  auto pick = [](uint32_t v, uint32_t mask, uint32_t flip) {
-    uint32_t d;
-    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(d) : "r"(v), "r"(mask), "r"(flip));  // (v & mask) ^ flip
-    return d;
-  };
   const uint32_t x = w >> 8;
   const __half2 off = __half2half2(__ushort_as_half(0x6408));  // 1032
   const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00)), off16 = __half2half2(__ushort_as_half(0xd480));  // -72
@@ -171,7 +192,8 @@ constexpr int kSplitThreads = 32 * kSplitWarps;
 constexpr int kUnitTokens = 32 * kSplitWarps;  // cached tokens of one unit: 32 a warp
 constexpr int kMaxCtas = 1024;                 // counters in the workspace
 constexpr int kMaxRows = 16;                   // query rows of a tile at most
-constexpr size_t kCounterBytes = kMaxCtas * sizeof(uint32_t);
+constexpr int kGroupCtas = 16;                 // parts of a split tile that are added at once
+constexpr size_t kCounterBytes = 3 * kMaxCtas * sizeof(uint32_t);
 
 // Query rows a tile has in the split kernel: 8 a column group, a second one where the head size leaves registers.
 inline int split_rows(int64_t rows_a_sequence, int64_t dim) {

@@ -9,15 +9,17 @@
 // products run transposed, cached tokens or dimensions as the 16 rows and query rows as the 8 columns of mma m16n8k16,
 // so one query head wastes no more than the 8 columns:
 //  * K: ldmatrix gives lane (g, t) the word t (8 dimensions) of token g's 16-byte chunk. Its nibble pairs (0,4), (1,5),
-//    (2,6), (3,7) are the A fragments of two k-steps; q's B fragments are laid out in the same order once a tile.
+//    (2,6), (3,7) are the A fragments of two k-steps; q's B fragments are laid out in the same order once a tile. The
+//    fragments are the masked bits themselves, f16 subnormals (n + 8) 2^-24 and, for odd nibbles, 16 times that: q is
+//    divided by 16 there, and the sums begin at -8 sum q.
 //  * V: ldmatrix.trans moves 16-bit units, four nibbles: lane (g, t) gets dimensions 4g .. 4g + 3 of tokens 2t and 2t + 1
 //    in the two halves of a word, which is the A fragment of V transposed after the same conversion.
 //  * Probabilities: the score fragment times v_scale, rounded to f16, transposed by movmatrix, is the B fragment.
-// q is scaled by a power of two a row to fit f16 (exactly, where it is within 2^-22 of the row's largest); the
+// q is scaled by a power of two a row to fit f16 (exactly, where it is within 2^-24 of the row's largest); the
 // probabilities by a power of two a warp, the largest exponent of the v_scale seen, so that p * v_scale fits f16 with
-// 2^-23 of range below its largest value. p is rounded to f16 (2^-12); every sum is f32.
-// The running maximum moves only when a logit exceeds it by more than 2^8 (f32 sums and the f16 range above hold that),
-// so most steps need no reduction across lanes and no rescaling.
+// 2^-24 of range below its largest value. p * v_scale is rounded to f16; every sum is f32.
+// The running maximum moves only when a step's probabilities sum to more than 2^9 (f32 sums and the f16 range above hold
+// that), so most steps need one vote, no reduction across lanes and no rescaling.
 //
 // Work. Units of 128 cached tokens, over sequences, tiles and heads in order, are split evenly over the launch's CTAs
 // (each sequence's count comes from its length on the device: no host read, no launch bound by the longest sequence).
@@ -42,6 +44,7 @@ struct SplitCfg {
   static constexpr int kRing = kSplitWarps * kStages * kStage;
   static constexpr int kMerge = kSplitWarps * kRows * kPitch * 4;
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+  static_assert(kSmem >= 2 * kMaxCtas / kGroupCtas * kRows * 4, "room for the parts' references and sums");
   static constexpr int kOcc = D <= 128 ? (NT == 1 ? 4 : 3) : 2;
 };
 
@@ -52,12 +55,25 @@ __device__ __forceinline__ int swizzle(int r) {
   return (r / (8 / z)) & (z - 1);
 }
 
-__device__ __forceinline__ int64_t cta_of(int64_t u, int64_t U, int64_t P) {
-  int64_t c = (u * P) / U;
-  while (c + 1 < P && ((c + 1) * U) / P <= u) ++c;
-  while (c > 0 && (c * U) / P > u) --c;
-  return c;
+// a / b for a >= 0, b > 0, in 32 bits where both fit (a 64-bit division is a long sequence).
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
+
+// U units in order over P CTAs: the first `extra` take `each` + 1, the others `each`.
+struct Shares {
+  int64_t P, each, extra;
+  __device__ __forceinline__ Shares(int64_t U, int64_t grid) {
+    P = min(grid, U);
+    each = P > 0 ? divide(U, P) : 0;
+    extra = U - each * P;
+  }
+  __device__ __forceinline__ int64_t begin(int64_t cta) const { return cta * each + min(cta, extra); }
+  __device__ __forceinline__ int64_t cta_of(int64_t u) const {
+    const int64_t in_first = extra * (each + 1);
+    return u < in_first ? divide(u, each + 1) : extra + divide(u - in_first, each);
+  }
+};
 
 // Units of one (tile, head) of a sequence: at least one, which writes the rows that see nothing.
 template <int ROWS>
@@ -109,10 +125,11 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
     if (w < warp) before += s_scan[w];
     U += s_scan[w];
   }
-  const int64_t P = min((int64_t)gridDim.x, U), cta = blockIdx.x;
-  if (cta >= P) return;
-  int64_t u = cta * U / P;
-  const int64_t u1 = (cta + 1) * U / P;
+  const Shares shares(U, gridDim.x);
+  const int64_t cta = blockIdx.x;
+  if (cta >= shares.P) return;
+  int64_t u = shares.begin(cta);
+  const int64_t u1 = shares.begin(cta + 1);
   if (u >= before && u < before + mine) {
     int64_t base = before;
     int b = my0;
@@ -128,12 +145,23 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
   int b = s_seq;
   int64_t off = u - s_base;
 
-  const uint32_t ring = smem_addr(smem) + warp * (C::kStages * C::kStage);
+  const uint32_t smem_base = smem_addr(smem), ring = smem_base + warp * (C::kStages * C::kStage);
   float* merge = reinterpret_cast<float*>(smem);
   // the scale runs of 8 tokens are 16 * groups bytes: `groups` 16-byte pieces
   const int groups = EXACT ? GT : a.groups;
-  const int sc_run = lane / groups, sc_part = lane - sc_run * groups;
   const bool sc_mine = lane < 4 * groups;
+  // where piece lane + 32 i of a step's K (or V) lies in its stage
+  auto copy_at = [&](int i) -> uint32_t {
+    if constexpr (32 % CH == 0 && 32 / CH >= 8) {  // the swizzle repeats: one offset a lane, the rest are constants
+      return ((lane / CH) * CH + ((lane % CH) ^ swizzle<D>(lane / CH))) * 16 + i * 512;
+    } else {
+      const int r = (lane + 32 * i) / CH, c = (lane + 32 * i) % CH;
+      return (r * CH + (c ^ swizzle<D>(r))) * 16;
+    }
+  };
+  // where row `lane` of chunk c lies
+  auto chunk_at = [&](int c) -> uint32_t { return (lane * CH + (c ^ swizzle<D>(lane))) * 16; };
+  const int sc_run = sc_mine ? lane / groups * 8 : 0, sc_part = lane % groups;
 
   while (u < u1) {
     const Seq seq = load_seq(a, b);
@@ -150,49 +178,136 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
       off = 0;
       continue;
     }
-    const int head = (int)(in_tile / n_units), first = (int)(in_tile - (int64_t)head * n_units);
+    const int head = (int)divide(in_tile, n_units), first = (int)(in_tile - (int64_t)head * n_units);
     const int count = (int)min((int64_t)(n_units - first), u1 - u);
     const int64_t tile_u0 = u - first;
 
-    // ---- the tile's queries: B fragments, and per column (query row) its logit factor and visible range ----
-    uint32_t qf[NT][CH][4];
-    float qs[NT][2];
-    int last[NT][2], past[NT][2];  // a column sees the tokens past < j <= last
+    const int tok0 = (unit0 + first) * kUnitTokens + warp * 32;
+    const int32_t* pages = a.table + (int64_t)b * a.table_stride;
+    // the page of this lane's token of step k, -1 where it has none
+    auto page_of = [&](int k) {
+      const int j = tok0 + k * kUnitTokens + lane;
+      if (k >= count || j >= seq.len) return -1;
+      const int p = __ldg(pages + (j >> a.page_log2));
+      return p >= 0 && (int64_t)p < a.pages ? p : -1;
+    };
+    int page0[C::kStages];
+#pragma unroll
+    for (int k = 0; k < C::kStages; ++k) page0[k] = page_of(k);
+    // ---- the tile's queries (loads), and the first copies ----
+    uint4 raw[NT][CH];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = tile * ROWS + nt * 8 + g;
-      const bool in = row < rows;
-      const int i = in ? row / a.ratio : 0;
-      const char* src = static_cast<const char*>(a.q) +
-                        2 * ((seq.q0 + i) * a.qs + (int64_t)(head * a.ratio + (in ? row - i * a.ratio : 0)) * a.qh);
-      uint4 raw[CH];
+      const int row = tile * ROWS + nt * 8 + g, i = row / a.ratio;
+      const char* src = static_cast<const char*>(a.q) + 2 * ((seq.q0 + i) * a.qs + (int64_t)(head * a.ratio + row - i * a.ratio) * a.qh);
 #pragma unroll
       for (int c = 0; c < CH; ++c)
-        raw[c] = in ? __ldg(reinterpret_cast<const uint4*>(src + 2 * (32 * c + 8 * t))) : make_uint4(0, 0, 0, 0);
-      float mx = 0.f;
+        raw[nt][c] = row < rows ? __ldg(reinterpret_cast<const uint4*>(src + 2 * (32 * c + 8 * t))) : make_uint4(0, 0, 0, 0);
+    }
+    // A run is 8 tokens, which lie on one page. Rows past the sequence's end come with their run; they are masked. Offsets
+    // count 16-byte pieces: a page of one head is page * CH of them (page * groups / 8 of scales).
+    const uint32_t page_kv = (uint32_t)a.kv_heads << a.page_log2, head_kv = (uint32_t)head << a.page_log2;
+    const uint32_t in_page = (1u << a.page_log2) - 1;
+    const uint4* k_base = reinterpret_cast<const uint4*>(a.k4) + (uint64_t)head_kv * CH;
+    const uint4* v_base = reinterpret_cast<const uint4*>(a.v4) + (uint64_t)head_kv * CH;
+    const uint4* ks_base = reinterpret_cast<const uint4*>(a.k_scale) + ((uint64_t)head_kv * groups >> 3);
+    const uint4* vs_base = reinterpret_cast<const uint4*>(a.v_scale) + ((uint64_t)head_kv * groups >> 3);
+    // Copies step k into the stage at `st` (its word of s_mask: `slot`).
+    auto issue = [&](int k, int page, uint32_t st, int slot) {
+      if (k < count) {
+        const uint32_t tok = (uint32_t)(tok0 + k * kUnitTokens) & in_page;
+        const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) s_mask[warp][slot] = have;
+        if (a.page_log2 >= 5) {  // one page holds the step's 32 tokens
+          const int pg = __shfl_sync(0xffffffffu, page, 0);
+          const uint32_t bytes = pg >= 0 ? 16u : 0u;
+          const uint64_t at = (uint64_t)(uint32_t)max(pg, 0) * (page_kv * CH) + (tok * CH + lane);
+          const uint4 *k_at = k_base + at, *v_at = v_base + at;
+#pragma unroll
+          for (int i = 0; i < CH; ++i) {
+            const uint32_t dst = st + copy_at(i);
+            cp_async16(dst, k_at + 32 * i, bytes);
+            cp_async16(dst + C::kKV, v_at + 32 * i, bytes);
+          }
+          if (sc_mine) {
+            const uint64_t sc = (uint64_t)(uint32_t)max(pg, 0) * ((page_kv >> 3) * groups) + ((tok >> 3) * groups + lane);
+            const uint32_t dst = st + 2 * C::kKV + lane * 16;
+            cp_async16(dst, ks_base + sc, bytes);
+            cp_async16(dst + C::kSc, vs_base + sc, bytes);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < CH; ++i) {
+            const int r = (lane + 32 * i) / CH, run = r & ~7;
+            const int pg = __shfl_sync(0xffffffffu, page, run);
+            const uint32_t bytes = pg >= 0 ? 16u : 0u;
+            const uint64_t at = (uint64_t)(uint32_t)max(pg, 0) * (page_kv * CH) +
+                                (((tok + run) & in_page) * CH + (lane + 32 * i - run * CH));
+            const uint32_t dst = st + copy_at(i);
+            cp_async16(dst, k_base + at, bytes);
+            cp_async16(dst + C::kKV, v_base + at, bytes);
+          }
+          const int pg = __shfl_sync(0xffffffffu, page, sc_run);
+          if (sc_mine) {
+            const uint32_t bytes = pg >= 0 ? 16u : 0u;
+            const uint64_t at = (uint64_t)(uint32_t)max(pg, 0) * ((page_kv >> 3) * groups) +
+                                ((((tok + sc_run) & in_page) >> 3) * groups + sc_part);
+            const uint32_t dst = st + 2 * C::kKV + lane * 16;
+            cp_async16(dst, ks_base + at, bytes);
+            cp_async16(dst + C::kSc, vs_base + at, bytes);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+
+#pragma unroll
+    for (int k = 0; k < C::kStages - 1; ++k) issue(k, page0[k], ring + k * C::kStage, k);
+    int page = page0[C::kStages - 1];
+
+    // ---- B fragments of the queries, and per column (query row) its logit factor and visible range ----
+    uint32_t qf[NT][CH][4];
+    float qs[NT][2], zero[NT][GT][2];  // zero: where a group's sum begins, -8 sum q
+    int last[NT][2], past[NT][2];      // a column sees the tokens past < j <= last
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float big = 0.f;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         float f[8];
-        unpack8(raw[c], a.bf16, f);
+        unpack8(raw[nt][c], a.bf16, f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(f[k]));
+        for (int k = 0; k < 8; ++k) big = fmaxf(big, fabsf(f[k]));
       }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const int ex = (int)(__float_as_uint(mx) >> 23) - 127;  // the row's largest magnitude becomes 2^7 .. 2^8
-      const int sh = mx == 0.f || ex == 128 ? 0 : min(7 - ex, 126);
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      const int ex = (int)(__float_as_uint(big) >> 23) - 127;  // the row's largest magnitude becomes 2^14 .. 2^15
+      const int sh = big == 0.f || ex == 128 ? 0 : min(14 - ex, 126);
       const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        float f[8];
-        unpack8(raw[c], a.bf16, f);
+      for (int z = 0; z < GT; ++z) {
+        float total = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) qf[nt][c][k] = pack2_f16(f[k] * up, f[k + 4] * up);
+        for (int cc = 0; cc < CPG; ++cc) {
+          const int c = z * CPG + cc;
+          float f[8];
+          unpack8(raw[nt][c], a.bf16, f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) total += f[k] *= up;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            qf[nt][c][k] = (k & 1) ? pack2_f16(f[k] * 0.0625f, f[k + 4] * 0.0625f) : pack2_f16(f[k], f[k + 4]);
+        }
+        total += __shfl_xor_sync(0xffffffffu, total, 1);
+        total += __shfl_xor_sync(0xffffffffu, total, 2);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          zero[nt][z][j] = __shfl_sync(0xffffffffu, total, 4 * (2 * t + j)) * -0x1p-21f;  // -8 2^-24
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int s2 = __shfl_sync(0xffffffffu, sh, 4 * (2 * t + j));
-        qs[nt][j] = a.scale_log2 * __uint_as_float((uint32_t)(127 - s2) << 23);
+        qs[nt][j] = a.scale_log2 * 0x1p24f * __uint_as_float((uint32_t)(127 - s2) << 23);
         const int r2 = tile * ROWS + nt * 8 + 2 * t + j;
         const int pos = seq.len - seq.nq + r2 / a.ratio;
         last[nt][j] = r2 >= rows ? -1 : a.causal ? min(pos, seq.len - 1) : seq.len - 1;
@@ -205,12 +320,15 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
     const int all_past = a.window > 0 ? seq.len - seq.nq + i1 - a.window : -1;
 
     float O[CH][2][NT][4];
+    // p = 2^(logit - ref) with ref = mx + vexp: mx a recent maximum of the row's logits, vexp of the exponents of v_scale
     float ref[NT][2], sum[NT][2], mx[NT][2];
     int vexp = -24;  // the smallest exponent of an f16
+    uint32_t vbits = 0x0002u;  // the f16 2^(vexp + 1): scales from here on raise vexp
+    float most = 0x1p33f;      // 2^(9 - vexp): a step's sum from here on raises mx
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) ref[nt][j] = mx[nt][j] = kNoMax, sum[nt][j] = 0.f;
+      for (int j = 0; j < 2; ++j) ref[nt][j] = mx[nt][j] = kNoMax, sum[nt][j] = 0.f;  // (-3e38 + vexp is -3e38)
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -219,125 +337,139 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
           for (int i = 0; i < 4; ++i) O[c][z][nt][i] = 0.f;
     }
 
-    const int tok0 = (unit0 + first) * kUnitTokens + warp * 32;
-    const int32_t* pages = a.table + (int64_t)b * a.table_stride;
-    // the page of this lane's token of step k, -1 where it has none
-    auto page_of = [&](int k) {
-      const int j = tok0 + k * kUnitTokens + lane;
-      if (k >= count || j >= seq.len) return -1;
-      const int p = __ldg(pages + (j >> a.page_log2));
-      return p >= 0 && (int64_t)p < a.pages ? p : -1;
-    };
-    auto issue = [&](int k, int page) {
-      if (k < count) {
-        const uint32_t st = ring + (k % C::kStages) * C::kStage;
-        const int tok = tok0 + k * kUnitTokens;
-        const int in_page = (1 << a.page_log2) - 1;
-        const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
-        if (lane == 0) s_mask[warp][k % C::kStages] = have;
-        // this lane's token as a row of the cache
-        const int64_t line = ((((int64_t)page * a.kv_heads + head)) << a.page_log2) + ((tok + lane) & in_page);
+    // The scales of this lane's four tokens (g, g + 8, g + 16, g + 24): all groups where the count is known.
+    auto scales = [&](const __half* sc, float (&f)[4][GT]) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          const int p = lane + 32 * i, r = p / CH, c = p - r * CH;
-          const int64_t ln = __shfl_sync(0xffffffffu, line, r);
-          const bool ok = (have >> r) & 1u;
-          const int64_t src = ok ? ln * (D / 2) + c * 16 : 0;
-          const uint32_t dst = st + (r * CH + (c ^ swizzle<D>(r))) * 16;
-          cp_async16(dst, a.k4 + src, ok ? 16 : 0);
-          cp_async16(dst + C::kKV, a.v4 + src, ok ? 16 : 0);
-        }
-        const int r8 = (8 * sc_run) & 31;
-        const int64_t ln = __shfl_sync(0xffffffffu, line, r8);
-        if (sc_mine) {
-          const bool ok = (have >> r8) & 1u;
-          const int64_t src = ok ? ln * groups + sc_part * 8 : 0;
-          const uint32_t dst = st + 2 * C::kKV + lane * 16;
-          cp_async16(dst, a.k_scale + src, ok ? 16 : 0);
-          cp_async16(dst + C::kSc, a.v_scale + src, ok ? 16 : 0);
+      for (int i = 0; i < 4; ++i) {
+        const __half* row = sc + (g + 8 * i) * groups;
+        if constexpr (EXACT && GT % 2 == 0) {
+          uint32_t w[GT / 2];
+          if constexpr (GT == 2) {
+            w[0] = *reinterpret_cast<const uint32_t*>(row);
+          } else if constexpr (GT == 4) {
+            const uint2 v = *reinterpret_cast<const uint2*>(row);
+            w[0] = v.x, w[1] = v.y;
+          } else {
+            const uint4 v = *reinterpret_cast<const uint4*>(row);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+          }
+#pragma unroll
+          for (int z = 0; z < GT / 2; ++z) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[z]));
+            f[i][2 * z] = v.x, f[i][2 * z + 1] = v.y;
+          }
+        } else {
+#pragma unroll
+          for (int z = 0; z < GT; ++z) f[i][z] = __half2float(row[EXACT ? z : z / a.cpg]);
         }
       }
-      cp_async_commit();
     };
 
-    // The scales of group z of this lane's four tokens (g, g + 8, g + 16, g + 24).
-    auto scales = [&](const __half* sc, int z, float (&f)[4]) {
-      const int at = EXACT ? z : z / a.cpg;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = __half2float(sc[(g + 8 * i) * groups + at]);
-    };
-
-    auto consume = [&](int k, auto masked) {
+    auto consume = [&](int tok, uint32_t have, uint32_t st, auto masked) {
       constexpr bool MASKED = decltype(masked)::value;
-      const int slot = k % C::kStages, tok = tok0 + k * kUnitTokens;
-      const uint32_t st = ring + slot * C::kStage;
-      const uint8_t* sp = smem + warp * (C::kStages * C::kStage) + slot * C::kStage;
-      const __half* ks = reinterpret_cast<const __half*>(sp + 2 * C::kKV);
+      const uint8_t* sp = smem + (st - smem_base);
       const __half* vs = reinterpret_cast<const __half*>(sp + 2 * C::kKV + C::kSc);
-      const uint32_t have = MASKED ? s_mask[warp][slot] : 0xffffffffu;
+      // ---- scores ----
       float S[2][NT][4];
+      {
+        float f[4][GT];
+        scales(reinterpret_cast<const __half*>(sp + 2 * C::kKV), f);
 #pragma unroll
-      for (int z = 0; z < GT; ++z) {
-        float acc[2][NT][4] = {};
+        for (int z = 0; z < GT; ++z) {
+          float acc[2][NT][4];
 #pragma unroll
-        for (int cc = 0; cc < CPG; ++cc) {
-          const int c = z * CPG + cc;
-          uint32_t w[4], e[4][4];
-          ldmatrix_x4(st + (lane * CH + (c ^ swizzle<D>(lane))) * 16, w);
+          for (int cc = 0; cc < CPG; ++cc) {
+            const int c = z * CPG + cc;
+            uint32_t w[4], e[4][4];
+            ldmatrix_x4(st + chunk_at(c), w);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) expand(w[i], e[i]);
+            for (int i = 0; i < 4; ++i) expand_raw(w[i], e[i]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                if (cc == 0)
+                  mma_f16_from(acc[h][nt], e[2 * h][0], e[2 * h + 1][0], e[2 * h][1], e[2 * h + 1][1], qf[nt][c][0],
+                               qf[nt][c][1], zero[nt][z][0], zero[nt][z][1]);
+                else
+                  mma_f16(acc[h][nt], e[2 * h][0], e[2 * h + 1][0], e[2 * h][1], e[2 * h + 1][1], qf[nt][c][0], qf[nt][c][1]);
+                mma_f16(acc[h][nt], e[2 * h][2], e[2 * h + 1][2], e[2 * h][3], e[2 * h + 1][3], qf[nt][c][2], qf[nt][c][3]);
+              }
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_f16(acc[h][nt], e[2 * h][0], e[2 * h + 1][0], e[2 * h][1], e[2 * h + 1][1], qf[nt][c][0], qf[nt][c][1]);
-              mma_f16(acc[h][nt], e[2 * h][2], e[2 * h + 1][2], e[2 * h][3], e[2 * h + 1][3], qf[nt][c][2], qf[nt][c][3]);
-            }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                S[h][nt][i] = z == 0 ? acc[h][nt][i] * f[2 * h + i / 2][0]
+                                     : fmaf(acc[h][nt][i], f[2 * h + i / 2][z], S[h][nt][i]);
         }
-        float f[4];
-        scales(ks, z, f);
+      }
+      if (MASKED) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              S[h][nt][i] = z == 0 ? acc[h][nt][i] * f[2 * h + i / 2] : fmaf(acc[h][nt][i], f[2 * h + i / 2], S[h][nt][i]);
+            for (int i = 0; i < 4; ++i) {
+              const int r = h * 16 + (i / 2) * 8 + g, j = tok + r;
+              const bool see = ((have >> r) & 1u) && j <= last[nt][i & 1] && j > past[nt][i & 1];
+              S[h][nt][i] = see ? S[h][nt][i] * qs[nt][i & 1] : -INFINITY;
+            }
       }
-      // the largest exponent of this step's v_scale; what is not finite or not visible to any row does not count
-      uint32_t big = 0;
-      {
-        const bool mine_in = !MASKED || ((have >> lane) & 1u);
-        for (int z = 0; z < groups; ++z) {
-          const uint32_t bits = __half_as_ushort(vs[lane * groups + z]) & 0x7fffu;
-          if (mine_in && bits < 0x7c00u) big = max(big, bits);
-        }
-        big = __reduce_max_sync(0xffffffffu, big);
-      }
-      const int ve = big ? (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)big))) >> 23) - 127 : -24;
-      bool over = false;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
+      // ---- probabilities, against the running reference ----
+      float p[2][NT][4], part[NT][2];
+      auto raise = [&]() {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            S[h][nt][i] *= qs[nt][i & 1];
-            if (MASKED) {
-              const int r = h * 16 + (i / 2) * 8 + g, j = tok + r;
-              if (!((have >> r) & 1u) || j > last[nt][i & 1] || j <= past[nt][i & 1]) S[h][nt][i] = -INFINITY;
-            }
-            over |= S[h][nt][i] > mx[nt][i & 1] + 8.f;
+          for (int j = 0; j < 2; ++j) {
+            part[nt][j] = 0.f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = j; i < 4; i += 2) {
+                p[h][nt][i] = exp2_approx(MASKED ? S[h][nt][i] - ref[nt][j] : fmaf(S[h][nt][i], qs[nt][j], -ref[nt][j]));
+                part[nt][j] += p[h][nt][i];
+              }
           }
-      if (__any_sync(0xffffffffu, over) || ve > vexp) {
-        vexp = max(vexp, ve);
+      };
+      raise();
+      // this lane's token: the largest of its v_scale, as bits. What is masked, or not finite there, does not count.
+      uint32_t vb = 0;
+      if constexpr (!MASKED && EXACT && GT % 2 == 0) {
+#pragma unroll
+        for (int z = 0; z < GT / 2; ++z) {
+          const uint32_t w = reinterpret_cast<const uint32_t*>(vs + lane * GT)[z] & 0x7fff7fffu;
+          vb = max(vb, max(w >> 16, w & 0xffffu));
+        }
+        vb = min(vb, 0x7bffu);
+      } else {
+        for (int z = 0; z < groups; ++z) {
+          const uint32_t w = __half_as_ushort(vs[lane * groups + z]) & 0x7fffu;
+          vb = max(vb, MASKED ? (((have >> lane) & 1u) && w < 0x7c00u ? w : 0u) : min(w, 0x7bffu));
+        }
+      }
+      bool over = vb >= vbits;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) over |= part[nt][0] > most || part[nt][1] > most;
+      if (__any_sync(0xffffffffu, over)) {
+        vb = __reduce_max_sync(0xffffffffu, vb);
+        if (vb >= vbits) {
+          vexp = (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)vb))) >> 23) - 127;
+          vbits = vexp >= 15 ? 0x8000u : __half_as_ushort(__float2half_rn(__uint_as_float((uint32_t)(vexp + 128) << 23)));
+          most = __uint_as_float((uint32_t)(136 - vexp) << 23);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             float m = mx[nt][j];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) m = fmaxf(m, fmaxf(S[h][nt][j], S[h][nt][2 + j]));
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = j; i < 4; i += 2) m = fmaxf(m, MASKED ? S[h][nt][i] : S[h][nt][i] * qs[nt][j]);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
             const float now = m + (float)vexp, f = exp2_approx(ref[nt][j] - now);
@@ -349,64 +481,59 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
 #pragma unroll
               for (int z = 0; z < 2; ++z) O[c][z][nt][j] *= f, O[c][z][nt][2 + j] *= f;
           }
+        raise();
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            S[h][nt][i] = exp2_approx(S[h][nt][i] - ref[nt][i & 1]);
-            sum[nt][i & 1] += S[h][nt][i];
-          }
+      for (int nt = 0; nt < NT; ++nt) sum[nt][0] += part[nt][0], sum[nt][1] += part[nt][1];
+      // ---- output ----
+      float f[4][GT];
+      scales(vs, f);
 #pragma unroll
       for (int z = 0; z < GT; ++z) {
-        float f[4];
-        scales(vs, z, f);
-        uint32_t p[2][NT][2];
+        uint32_t pf[2][NT][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {  // a masked token's scale may be anything, a NaN too: 0 stays 0
-              const float p0 = S[h][nt][2 * i], p1 = S[h][nt][2 * i + 1], v = f[2 * h + i];
-              p[h][nt][i] = movmatrix_trans(pack2_f16(MASKED && p0 == 0.f ? 0.f : p0 * v, MASKED && p1 == 0.f ? 0.f : p1 * v));
+              const float p0 = p[h][nt][2 * i], p1 = p[h][nt][2 * i + 1], v = f[2 * h + i][z];
+              pf[h][nt][i] = movmatrix_trans(pack2_f16(MASKED && p0 == 0.f ? 0.f : p0 * v, MASKED && p1 == 0.f ? 0.f : p1 * v));
             }
 #pragma unroll
         for (int cc = 0; cc < CPG; ++cc) {
           const int c = z * CPG + cc;
           uint32_t w[4], e[4][4];
-          ldmatrix_x4_trans(st + C::kKV + (lane * CH + (c ^ swizzle<D>(lane))) * 16, w);
+          ldmatrix_x4_trans(st + C::kKV + chunk_at(c), w);
 #pragma unroll
           for (int i = 0; i < 4; ++i) expand(w[i], e[i]);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma_f16(O[c][0][nt], e[2 * h][0], e[2 * h][1], e[2 * h + 1][0], e[2 * h + 1][1], p[h][nt][0], p[h][nt][1]);
-              mma_f16(O[c][1][nt], e[2 * h][2], e[2 * h][3], e[2 * h + 1][2], e[2 * h + 1][3], p[h][nt][0], p[h][nt][1]);
+              mma_f16(O[c][0][nt], e[2 * h][0], e[2 * h][1], e[2 * h + 1][0], e[2 * h + 1][1], pf[h][nt][0], pf[h][nt][1]);
+              mma_f16(O[c][1][nt], e[2 * h][2], e[2 * h][3], e[2 * h + 1][2], e[2 * h + 1][3], pf[h][nt][0], pf[h][nt][1]);
             }
         }
       }
     };
 
     // ---- this warp's 32 tokens of each unit ----
-#pragma unroll
-    for (int k = 0; k < C::kStages - 1; ++k) issue(k, page_of(k));
-    int page = page_of(C::kStages - 1);
+    int slot = 0, slot_in = C::kStages - 1;
     for (int k = 0; k < count; ++k) {
-      issue(k + C::kStages - 1, page);
+      issue(k + C::kStages - 1, page, ring + slot_in * C::kStage, slot_in);
       page = page_of(k + C::kStages);
       cp_async_wait<C::kStages - 1>();
       __syncwarp();
       const int tok = tok0 + k * kUnitTokens;
-      const bool full = s_mask[warp][k % C::kStages] == 0xffffffffu && tok > all_past && tok + 31 <= all_last;
-      if (full)
-        consume(k, std::false_type{});
+      const uint32_t have = s_mask[warp][slot];
+      if (have == 0xffffffffu && tok > all_past && tok + 31 <= all_last)
+        consume(tok, have, ring + slot * C::kStage, std::false_type{});
       else
-        consume(k, std::true_type{});
+        consume(tok, have, ring + slot * C::kStage, std::true_type{});
       __syncwarp();
+      slot_in = slot;
+      slot = slot + 1 == C::kStages ? 0 : slot + 1;
     }
     cp_async_wait<0>();
 
@@ -475,34 +602,61 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
       }
     }
     if (!whole) {
-      // the tile's counter belongs to the CTA that it begins in; whoever arrives last adds the parts in order
-      const int64_t c0 = cta_of(tile_u0, U, P), c1 = cta_of(tile_u0 + n_units - 1, U, P);
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        const bool done = atomicAdd(a.counters + c0, 1u) == (uint32_t)(c1 - c0);
-        if (done) a.counters[c0] = 0;  // ready for the next launch
-        s_last = done;
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_last) {
+      // The tile's parts are added in order, kGroupCtas at a time: the CTA that completes a group adds its parts into the
+      // group's first, and the one that completes the last group adds the groups. The counters belong to CTAs that a
+      // tile begins in (the first group's, the groups') or that it reaches from before (the other groups').
+      const int64_t c0 = shares.cta_of(tile_u0), c1 = shares.cta_of(tile_u0 + n_units - 1);
+      const int n = (int)(c1 - c0) + 1, n_groups = (n + kGroupCtas - 1) / kGroupCtas;
+      const int mine_in = (int)(cta - c0) / kGroupCtas, from = mine_in * kGroupCtas;
+      auto part_of = [&](int i) { return a.partials + ((c0 + i) * 2 + (i == 0 ? 1 : 0)) * PART; };
+      // counts this CTA in; true in the one that completes the count
+      auto arrive = [&](uint32_t* counter, int of) {
+        __syncthreads();  // orders the block's stores before thread 0's release
+        if (threadIdx.x == 0) {
+          uint32_t before;
+          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+          const bool done = before == (uint32_t)(of - 1);
+          if (done) *counter = 0;  // ready for the next launch
+          s_last = done;
+        }
+        __syncthreads();
+        return s_last != 0;
+      };
+      // adds the parts base, base + step, ...: into part base, or as the tile's output
+      auto add = [&](int base, int step, int count_of, bool out) {
+        float* ms = merge;
+        float* ls = merge + kMaxCtas / kGroupCtas * ROWS;
+        for (int at = threadIdx.x; at < count_of * ROWS; at += kSplitThreads) {
+          const float* q = part_of(base + at / ROWS * step) + ROWS * D + at % ROWS;
+          ms[at] = __ldcg(q);
+          ls[at] = __ldcg(q + ROWS);
+        }
+        __syncthreads();
         for (int at = threadIdx.x; at < live * (D / 4); at += kSplitThreads) {
           const int r = at / (D / 4), d = 4 * (at - r * (D / 4));
+          float m = ms[r];
+          for (int i = 1; i < count_of; ++i) m = fmaxf(m, ms[i * ROWS + r]);
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          float l = 0.f, m = kNoMax;
-          for (int64_t c = c0; c <= c1; ++c) {
-            const float* q = a.partials + (c * 2 + (c == c0 ? 1 : 0)) * PART;
-            const float m1 = __ldcg(q + ROWS * D + r), l1 = __ldcg(q + ROWS * D + ROWS + r);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(q + r * D + d));
-            const float now = fmaxf(m, m1), f = exp2_approx(m - now), f1 = exp2_approx(m1 - now);
-            o.x = fmaf(v.x, f1, o.x * f), o.y = fmaf(v.y, f1, o.y * f);
-            o.z = fmaf(v.z, f1, o.z * f), o.w = fmaf(v.w, f1, o.w * f);
-            l = fmaf(l1, f1, l * f);
-            m = now;
+          float l = 0.f;
+#pragma unroll 8
+          for (int i = 0; i < count_of; ++i) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part_of(base + i * step) + r * D + d));
+            const float w = exp2_approx(ms[i * ROWS + r] - m);
+            o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y), o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
+            l = fmaf(ls[i * ROWS + r], w, l);
           }
-          store(r, d, o, m, l);
+          if (out) {
+            store(r, d, o, m, l);
+          } else {  // the sums' places are this thread's alone; the reference and the sum were read above
+            float* q = part_of(base);
+            __stcg(reinterpret_cast<float4*>(q + r * D + d), o);
+            if (d == 0) __stcg(q + ROWS * D + r, m), __stcg(q + ROWS * D + ROWS + r, l);
+          }
         }
+      };
+      if (arrive(a.counters + (mine_in == 0 ? 0 : kMaxCtas) + c0 + from, min(kGroupCtas, n - from))) {
+        add(from, 1, min(kGroupCtas, n - from), n_groups == 1);
+        if (n_groups > 1 && arrive(a.counters + 2 * kMaxCtas + c0, n_groups)) add(0, kGroupCtas, n_groups, true);
       }
     }
     __syncthreads();  // the ring and the small arrays are free again
