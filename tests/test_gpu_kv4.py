@@ -8,7 +8,12 @@ Attention, against 64 bits, for weights w (the softmax), logits s, values v:
 u_p = 2^-11 (p * v_scale is rounded to f16), u the output type's half ulp, ds = 2^-18 max_j scale sum_d |q_d k_jd| (f32
 sums of at most 256 exact products in pieces of 16, and the scales' products), 2^-20 the exponentials and the f32 sums
 of probabilities; the middle term is the f16 range's lower end (2^-25 of the scaled probabilities, times a nibble of at
-most 8), with l the sum of exp(s - max). |lse - exact| <= ds + 2^-19 + 2^-22 |exact|."""
+most 8), with l the sum of exp(s - max). |lse - exact| <= ds + 2^-19 + 2^-22 |exact|.
+
+With 64 query rows a sequence and key/value head or more and heads of 64 or 128, nibble * scale is rounded to f16 before
+the products: ds grows by 2^-11 max_j scale sum_d |q_d k_jd|, and v's rounding adds 2^-11 sum w |v|. Those are worst cases;
+as roundings are independent with a mean square of a third of their bound, the whole output is also held to
+||out - exact|| <= (u / sqrt(3) + 2^-10) ||exact|| for normally distributed inputs (logits and values of order 1)."""
 import pytest
 import torch
 
@@ -183,8 +188,15 @@ def make(batch, kv, dim, group, page, lens, seed=0, spread=1.0, order=True):
     return cache, table, torch.tensor(lens, dtype=torch.int32, device="cuda")
 
 
+def rounds_cache(q, cache, lens):
+    """Whether nibble * scale is rounded to f16 (the kernel for many query rows)."""
+    per = -(-q.shape[0] // len(lens)) * (q.shape[1] // cache[0].shape[1])
+    return per >= 64 and q.shape[2] in (64, 128)
+
+
 def reference(q, cache, table, lens, cu, causal, window, scale):
     """(out, lse, bound of out, bound of lse), in 64 bits."""
+    f16 = 2.0 ** -11 if rounds_cache(q, cache, lens) else 0.0
     page, ratio = cache[0].shape[2], q.shape[1] // cache[0].shape[1]
     out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     tol = torch.zeros_like(out)
@@ -211,12 +223,12 @@ def reference(q, cache, table, lens, cu, causal, window, scale):
         p = torch.where(see, torch.exp(s - torch.where(some[None, :, None], m, torch.zeros_like(m))), torch.zeros_like(s))
         l = p.sum(-1, keepdim=True)
         w = p / torch.where(l > 0, l, torch.ones_like(l))
-        ds = 2.0 ** -18 * mag.masked_fill(~see, 0).amax(-1)
+        ds = (2.0 ** -18 + f16) * mag.masked_fill(~see, 0).amax(-1)
         vs = cache[3][ids].double().nan_to_num(0, 0, 0).abs().max()
         o = torch.einsum("hqk,khd->qhd", w, rows[1])
         near = torch.einsum("hqk,khd->qhd", w, rows[1].abs())
         seen = see.sum(-1)[:, None, None]
-        tol[q0:q0 + nq] = ((2.0 ** -11 + 2.0 ** -20 + 2 * ds.T[..., None]) * near + o.abs() * U[q.dtype] +
+        tol[q0:q0 + nq] = ((2.0 ** -11 + f16 + 2.0 ** -20 + 2 * ds.T[..., None]) * near + o.abs() * U[q.dtype] +
                            seen * 2.0 ** -22 * vs / l.squeeze(-1).T[..., None].clamp(min=1.0) + 2.0 ** -24)
         out[q0:q0 + nq] = o
         z = (m.squeeze(-1) + l.squeeze(-1).log()).T
@@ -233,6 +245,8 @@ def check(q, cache, table, lens, cu=None, causal=True, window=0, scale=None):
     assert bool((off <= tol).all()), (float((off / tol).max()), int((~(off <= tol)).sum()))
     empty = want_lse == float("-inf")
     assert torch.equal(lse.double() == float("-inf"), empty) and bool((out[empty] == 0).all())
+    if rounds_cache(q, cache, lens) and scale is None:
+        assert float((out.double() - want).norm() / want.norm()) <= U[q.dtype] / 3 ** 0.5 + 2.0 ** -10
     off = (lse.double() - want_lse)[~empty].abs()
     assert bool((off <= tol_lse[~empty]).all()), float((off / tol_lse[~empty]).max())
     assert torch.equal(ops.kv4_attention(q, cache, table, lens, cu_q=cu, causal=causal, window=window, scale=scale), out)
@@ -270,13 +284,61 @@ def test_several_tokens_a_sequence(dim, group, causal, window):
     check(q, cache, table, n, cu, causal, window)
 
 
-@pytest.mark.parametrize("dim", [64, 128])
-def test_prompts(dim):
-    lens, nq = [900, 513, 300], [900, 250, 1]
-    cache, table, n = make(3, 2, dim, 64, 32, lens, seed=5)
+@pytest.mark.parametrize("dim,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("ratio", [1, 4, 5])
+def test_prompts(dim, group, ratio):
+    lens, nq = [900, 513, 300, 0, 128, 129], [900, 250, 1, 3, 128, 200]
+    cache, table, n = make(6, 2, dim, group, 32, lens, seed=5)
     cu = torch.tensor([0] + nq, device="cuda").cumsum(0).int()
-    for kind, window in ((torch.bfloat16, 0), (torch.float16, 200)):
-        check(torch.randn(sum(nq), 8, dim, device="cuda").to(kind), cache, table, n, cu, True, window)
+    for kind, window, causal in ((torch.bfloat16, 0, True), (torch.float16, 200, True), (torch.float16, 0, False)):
+        check(torch.randn(sum(nq), 2 * ratio, dim, device="cuda").to(kind), cache, table, n, cu, causal, window)
+
+
+def test_prompts_over_a_longer_context_and_small_pages():
+    cache, table, n = make(2, 1, 128, 128, 8, [3000, 2111], seed=15)
+    cu = torch.tensor([0, 70, 333], device="cuda").int()
+    check(torch.randn(333, 3, 128, device="cuda").bfloat16(), cache, table, n, cu)
+    packed = torch.randn(333, 7, 128, device="cuda").half()
+    out = torch.zeros(333, 7, 128, device="cuda").half()
+    ops.kv4_attention(packed[:, 2:5], cache, table, n, cu_q=cu, out=out[:, 1:4])
+    assert torch.equal(out[:, 1:4], check(packed[:, 2:5], cache, table, n, cu))
+    assert bool((out[:, 0] == 0).all()) and bool((out[:, 4:] == 0).all())
+
+
+def test_prompts_with_scales_far_apart():
+    """Values whose scales fall and rise by 2^12 between tiles, a maximum that rises late: all rows, some of which see
+    only the small ones. The values are not of order 1, so the element-wise bound alone holds (a scale of 1 / 8 given)."""
+    cache, table, n = make(1, 1, 64, 32, 16, [700], seed=21, spread=4.0)
+    j = torch.arange(700, device="cuda")
+    page, at = table[0, j // 16].long(), j % 16
+    cache[2][page, 0, at] *= (0.1 + j / 100)[:, None].half()
+    cache[3][page, 0, at] *= (2.0 ** (12 * (j / 700 - 0.5).abs() - 8))[:, None].half()
+    cu = torch.tensor([0, 700], device="cuda").int()
+    check(torch.randn(700, 2, 64, device="cuda").bfloat16(), cache, table, n, cu, scale=0.125)
+    check((torch.randn(700, 2, 64, device="cuda") * 1e30).bfloat16(), cache, table, n, cu, scale=1e-31)
+
+
+def test_prompts_with_a_nan_and_pages_outside():
+    """A NaN reaches the rows that see it only (where many rows share a tile, all of such a row)."""
+    cache, table, n = make(1, 1, 128, 64, 16, [300], seed=4)
+    j = 200
+    cu = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    q = torch.randn(300, 2, 128, device="cuda").bfloat16()
+    clean = ops.kv4_attention(q, cache, table, n, cu_q=cu)
+    for which in (3, 2):
+        keep = cache[which][int(table[0, j // 16]), 0, j % 16, 1].clone()
+        for bad in (float("nan"), float("inf")):
+            cache[which][int(table[0, j // 16]), 0, j % 16, 1] = bad
+            out = ops.kv4_attention(q, cache, table, n, cu_q=cu)
+            assert torch.equal(out[:j], clean[:j])
+            assert not bool(torch.isfinite(out[j:, :, 64:]).any()) or which == 2
+        cache[which][int(table[0, j // 16]), 0, j % 16, 1] = keep
+    # pages outside the cache: as if those tokens were masked for every row
+    bad = table.clone()
+    bad[0, 3] = -1
+    got = ops.kv4_attention(q, cache, bad, n, cu_q=cu)
+    assert torch.equal(got[:48], clean[:48]) and bool(torch.isfinite(got).all())
+    assert not torch.equal(got[64:], clean[64:])
 
 
 def test_a_long_sequence_is_split_over_the_gpu():

@@ -75,9 +75,13 @@ extern "C" int up_sm100_kv4_attention(const void* q, int dtype, int64_t tokens, 
   a.lens = seq_lens, a.cu = cu_q, a.batch = (int)batch, a.causal = causal != 0;
   a.window = (int)(window > kMaxTokens ? kMaxTokens : window);
   a.scale_log2 = scale * 1.44269504088896341f;
-  a.counters = static_cast<uint32_t*>(workspace);
+  a.header = static_cast<uint32_t*>(workspace);
+  a.counters = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + kHeaderBytes);
   a.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
-  const int rows = split_rows((tokens + batch - 1) / batch * ratio, cache->dim);
+  const int64_t per = (tokens + batch - 1) / batch * ratio;  // query rows a sequence and key/value head
+  if (per >= kPromptRows && (cache->dim == 64 || cache->dim == 128))
+    return prompt_attention(a, (int)cache->dim, static_cast<cudaStream_t>(stream));
+  const int rows = split_rows(per, cache->dim);
   return split_attention(a, (int)cache->dim, rows, split_ctas(), static_cast<cudaStream_t>(stream));
 }
 

@@ -27,7 +27,8 @@ struct Args {
   const int32_t *lens, *cu;
   int batch, causal, window;
   float scale_log2;                    // scale * log2(e): logits are kept in powers of two
-  uint32_t* counters;                  // workspace
+  uint32_t* header;                    // workspace: its error word is header[3]
+  uint32_t* counters;
   float* partials;
 };
 
@@ -193,14 +194,18 @@ constexpr int kUnitTokens = 32 * kSplitWarps;  // cached tokens of one unit: 32 
 constexpr int kMaxCtas = 1024;                 // counters in the workspace
 constexpr int kMaxRows = 16;                   // query rows of a tile at most
 constexpr int kGroupCtas = 16;                 // parts of a split tile that are added at once
-constexpr size_t kCounterBytes = 3 * kMaxCtas * sizeof(uint32_t);
+constexpr size_t kHeaderBytes = 256, kCounterBytes = kHeaderBytes + 3 * kMaxCtas * sizeof(uint32_t);
 
 // Query rows a tile has in the split kernel: 8 a column group, a second one where the head size leaves registers.
 inline int split_rows(int64_t rows_a_sequence, int64_t dim) {
   return rows_a_sequence > 8 && (dim == 64 || dim == 96 || dim == 128) ? 16 : 8;
 }
 
-int split_attention(const Args& a, int dim, int tile_rows, int ctas, cudaStream_t s);   // by head size
+// Query rows a sequence and key/value head from which the prompt kernel runs (head sizes 64 and 128).
+constexpr int64_t kPromptRows = 64;
+int prompt_attention(const Args& a, int dim, cudaStream_t s);
+
+int split_attention(const Args& a, int dim, int tile_rows, int ctas, cudaStream_t s);  // by head size
 int split_attention_small(const Args& a, int dim, int tile_rows, int ctas, cudaStream_t s);
 int split_attention_128(const Args& a, int tile_rows, int ctas, cudaStream_t s);
 int split_attention_large(const Args& a, int dim, int ctas, cudaStream_t s);

@@ -1,0 +1,559 @@
+// kv4_prompt.cu — attention over the paged 4-bit cache for many query rows a key/value head (prompts), on the tcgen05
+// tensor cores: the cache's tiles are turned into f16 once a CTA and serve 256 query rows.
+//
+// What bounds it: the tensor cores (4 dim flops a query row and cached token) and, at dim 128 as much, the exponentials
+// (one a query row and cached token; 16 a clock and SM against 16 x 512 flops).
+//
+// A CTA takes 256 query rows (query token x head of the group) of one sequence and key/value head as two tiles of 128,
+// and walks the cached tokens that any of them sees, 128 at a time. Per tile of tokens, S = Q K^T (128 x 128) and
+// O += P V (128 x dim) run per query tile with f32 accumulators in tensor memory; the two query tiles alternate, so that
+// the tensor cores work on one while the other's probabilities are computed.
+//  * warps 0..7 (probabilities): warp group w holds query tile w, a thread a row. A thread reads its row of S, takes
+//    p = 2^(logit - ref), and writes P as f16 over S: the A operand of the second product. ref moves only when a tile's
+//    probabilities sum to more than 2^9; then the thread scales its row of O.
+//  * warps 8..11 (cache): read 128 tokens' nibbles and scales, a tile ahead in registers, and write K and V as f16 into
+//    128-byte swizzled shared memory, two stages each. Both have a row a token: K is the B operand with its contraction
+//    (the dimensions) contiguous, V the one with its output (the dimensions) contiguous. The nibble conversion pairs
+//    dimensions k and k + 4 of each 8; q is stored in the same order and the output's columns are read in it.
+//  * warp 12 (products): one thread issues every tcgen05.mma.
+// Scales. A tile's scales are divided by the power of two of the largest (separately for K and V), so nibble * scale
+// keeps f16's precision and range whatever their size; the logits take K's power, the probabilities V's, relative to
+// the largest one met (O is scaled when a larger one comes). nibble * scale and p are rounded to f16; all sums are f32.
+// A token with an infinite or NaN v_scale is left out of the products (its rows would reach queries that do not see it)
+// and the queries that do see it become NaN.
+// Every wait is bounded; one that runs out sets the workspace's error word and the CTA unwinds.
+//
+// The tile of 2 x 128 rows is what 512 columns of tensor memory hold (S and O of both tiles at dim 128) and 227 KB of
+// shared memory (q 64 KB, two stages of K and V 128 KB).
+#include "kv4_attention.cuh"
+#include "tc.cuh"
+
+namespace up {
+namespace kv4 {
+
+namespace {
+
+constexpr int kRowsCta = 256, kTok = 128;
+constexpr int kThreads = 32 * 13, kCacheWarp = 8, kMmaWarp = 12;
+constexpr int kBlockBytes = kTok * 128;  // 128 rows of 64 dimensions (128 bytes), swizzled
+
+template <int D>
+struct Cfg {
+  static constexpr int kBlocks = D / 64;
+  static constexpr int kTile = kBlocks * kBlockBytes;       // 128 rows of D f16
+  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + 2 * kTile, kEnd = kV + 2 * kTile;
+  static constexpr int kScale = kEnd;                       // f16 [2 (K, V)][128][up to D / 32]
+  static constexpr int kSmem = kScale + 2 * kTok * (D / 32) * 2 + 1024 /* alignment */;
+  static constexpr int kS = 0, kO = 2 * kTok;               // tensor memory columns: S (and P) of both tiles, then O
+  static constexpr int kCols = 512;
+};
+
+struct Meta {          // what the cache warps say of a tile of tokens
+  int k_exp, v_exp;    // its scales were divided by 2^these
+  uint32_t valid[4];   // tokens that exist
+  uint32_t bad[4];     // of these, the ones with an infinite or NaN v_scale
+};
+
+struct Shared {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], drain;
+  uint32_t tmem;
+  int abort;
+  Meta meta[4];
+  float row_scale[kRowsCta];   // scale * log2(e) / the row's power of two
+  uint32_t big[2][4];
+  int64_t scan[13], base;
+  int seq;
+};
+
+__device__ __forceinline__ uint64_t desc_v(uint32_t addr) {  // dimensions contiguous: 64-dimension blocks kBlockBytes apart
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3fffu);
+  d |= (uint64_t)(kBlockBytes >> 4) << 16;  // leading offset: the next 64 dimensions
+  d |= (uint64_t)(1024u >> 4) << 32;        // stride offset: the next 8 tokens
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;                  // 128-byte swizzle
+  return d;
+}
+
+// kind::f16 with f16 operands and f32 sums; `mn`: B's output dimension is the contiguous one.
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool mn) {
+  return (1u << 4) | (mn ? 1u << 16 : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
+__device__ __forceinline__ void cache_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+__device__ __forceinline__ int64_t seq_ctas(const Args& a, int b) {
+  const Seq s = load_seq(a, b);
+  return (int64_t)((s.nq * a.ratio + kRowsCta - 1) / kRowsCta) * a.kv_heads;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, const uint64_t wait_ns) {
+  using C = Cfg<D>;
+  constexpr int CH = D / 32;
+  extern __shared__ uint8_t raw_smem[];
+  __shared__ Shared sh;
+  uint8_t* smem = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
+  const uint32_t sbase = smem_addr(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // ---- which sequence, tile and head: sequences in order, a sequence's last (longest) tiles first ----
+  const int per = (a.batch + kThreads - 1) / kThreads;
+  const int my0 = min((int)threadIdx.x * per, a.batch), my1 = min(my0 + per, a.batch);
+  int64_t mine = 0;
+  for (int b = my0; b < my1; ++b) mine += seq_ctas(a, b);
+  int64_t incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += v;
+  }
+  if (lane == 31) sh.scan[warp] = incl;
+  __syncthreads();
+  int64_t before = incl - mine, total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += sh.scan[w];
+    total += sh.scan[w];
+  }
+  const int64_t work = blockIdx.x;
+  if (work >= total) return;
+  if (work >= before && work < before + mine) {
+    int64_t base = before;
+    int b = my0;
+    for (;; ++b) {
+      const int64_t n = seq_ctas(a, b);
+      if (work < base + n) break;
+      base += n;
+    }
+    sh.seq = b;
+    sh.base = base;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&sh.k_full[i], 4);    // the cache warps
+      tc::mbar_init(&sh.v_full[i], 4);
+      tc::mbar_init(&sh.k_empty[i], 1);   // a commit
+      tc::mbar_init(&sh.v_empty[i], 1);
+      tc::mbar_init(&sh.s_full[i], 2);    // the issuer (it has seen the tile's meta) and a commit
+      tc::mbar_init(&sh.p_full[i], 4);    // the tile's warps
+      tc::mbar_init(&sh.pv_done[i], 1);
+    }
+    tc::mbar_init(&sh.drain, 1);
+    tc::mbar_fence_init();
+    sh.abort = 0;
+  }
+  if (warp == kMmaWarp) {
+    tc::tmem_alloc(&sh.tmem, C::kCols);
+    tc::tmem_relinquish();
+  }
+  __syncthreads();
+  const int b = sh.seq;
+  const Seq seq = load_seq(a, b);
+  const int rows = seq.nq * a.ratio, tiles = (rows + kRowsCta - 1) / kRowsCta;
+  const int in_seq = (int)(work - sh.base), tile = tiles - 1 - in_seq / a.kv_heads, head = in_seq % a.kv_heads;
+  const int row0 = tile * kRowsCta, live = min(kRowsCta, rows - row0);
+  int lo, hi;
+  visible(a, seq, row0 / a.ratio, (row0 + live - 1) / a.ratio, lo, hi);
+  const int tok0 = lo / kTok * kTok, n = hi > tok0 ? (hi - tok0 + kTok - 1) / kTok : 0;
+
+  // ---- queries: f16 with a power of two a row, swizzled ----
+  constexpr int LPR = D / 8;  // lanes a row
+  for (int r = warp * (32 / LPR) + lane / LPR; r < kRowsCta; r += kThreads / LPR) {
+    const int c = lane % LPR, row = row0 + r, i = row / a.ratio;
+    float f[8] = {};
+    if (r < live)
+      unpack8(__ldg(reinterpret_cast<const uint4*>(
+                  static_cast<const char*>(a.q) +
+                  2 * ((seq.q0 + i) * a.qs + (int64_t)(head * a.ratio + row - i * a.ratio) * a.qh + 8 * c))),
+              a.bf16, f);
+    float big = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) big = fmaxf(big, fabsf(f[k]));
+#pragma unroll
+    for (int d = 1; d < LPR; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d, LPR));
+    const int ex = (int)(__float_as_uint(big) >> 23) - 127;  // the row's largest magnitude becomes 2^7 .. 2^8
+    const int up = big == 0.f || ex == 128 ? 0 : min(7 - ex, 126);
+    const float m = pow2f(up);
+    uint4 w;
+    w.x = pack2_f16(f[0] * m, f[4] * m), w.y = pack2_f16(f[1] * m, f[5] * m);
+    w.z = pack2_f16(f[2] * m, f[6] * m), w.w = pack2_f16(f[3] * m, f[7] * m);
+    *reinterpret_cast<uint4*>(smem + C::kQ + (r / 128) * C::kTile + (c / 8) * kBlockBytes + (r % 128) * 128 +
+                              ((c % 8) ^ (r & 7)) * 16) = w;
+    if (c == 0) sh.row_scale[r] = a.scale_log2 * pow2f(-up);
+  }
+  tc::fence_proxy_async_smem();
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = sh.tmem;
+  volatile int* abort_flag = &sh.abort;
+  auto give_up = [&]() {
+    *abort_flag = 1;
+    a.header[3] = 1u;
+  };
+
+  if (warp < kCacheWarp) {
+    // ---------------- probabilities ----------------
+    const int w = warp >> 2, r = threadIdx.x;  // r: the CTA's row
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const uint32_t ts = tmem + C::kS + w * kTok + lanes, to = tmem + C::kO + w * D + lanes;
+    const int row = row0 + r, pos = seq.len - seq.nq + row / a.ratio;
+    const int last = r >= live ? -1 : a.causal ? min(pos, seq.len - 1) : seq.len - 1;
+    const int past = a.window > 0 ? max(pos - a.window, -1) : -1;
+    const float row_scale = sh.row_scale[r];
+    float mx = kNoMax, sum = 0.f;
+    int vexp = -24;
+    bool ok = true;
+    for (int t = 0; t < n; ++t) {
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(&sh.s_full[w], t & 1, wait_ns, abort_flag))) {
+        ok = false;
+        break;
+      }
+      tc::fence_after_sync();
+      const Meta& meta = sh.meta[t & 3];
+      const int j0 = tok0 + t * kTok;
+      const float c = row_scale * pow2f(meta.k_exp);
+      const int ve = meta.v_exp;
+      const bool all = (meta.valid[0] & meta.valid[1] & meta.valid[2] & meta.valid[3]) == 0xffffffffu;
+      const bool bad = (meta.bad[0] | meta.bad[1] | meta.bad[2] | meta.bad[3]) != 0;
+      const bool masked = !__all_sync(0xffffffffu, all && j0 > past && j0 + kTok - 1 <= last) || bad;
+      // the visible tokens of chunk g (32 of them)
+      auto seen = [&](int g) -> uint32_t {
+        const int from = past + 1 - (j0 + 32 * g), to_ = last + 1 - (j0 + 32 * g);  // in [from, to_)
+        uint32_t m = meta.valid[g];
+        m &= from >= 32 ? 0u : from <= 0 ? 0xffffffffu : 0xffffffffu << from;
+        m &= to_ <= 0 ? 0u : to_ >= 32 ? 0xffffffffu : (1u << to_) - 1u;
+        return m;
+      };
+      uint32_t p[kTok / 2];
+      float part;
+      auto weigh = [&](float add) {  // p = 2^(c S + add), packed, and their sum
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          uint32_t v[32];
+          ld_x32(ts + 32 * g, v);
+          tc::wait_ld();
+          if (masked) {
+            const uint32_t m = seen(g);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              v[i] = (m >> i) & 1u ? __float_as_uint(exp2_approx(fmaf(__uint_as_float(v[i]), c, add))) : 0u;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(v[i]), c, add)));
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            s0 += __uint_as_float(v[i]);
+            s1 += __uint_as_float(v[i + 1]);
+            p[16 * g + i / 2] = pack2_f16(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+          }
+        }
+        part = s0 + s1;
+      };
+      weigh((float)(ve - max(vexp, ve)) - mx);
+      if (__any_sync(0xffffffffu, part > 512.f || ve > vexp)) {
+        float m = mx;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          uint32_t v[32];
+          ld_x32(ts + 32 * g, v);
+          tc::wait_ld();
+          const uint32_t see = masked ? seen(g) : 0xffffffffu;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if ((see >> i) & 1u) m = fmaxf(m, __uint_as_float(v[i]) * c);
+        }
+        const int e = max(vexp, ve);
+        const float f = exp2_approx(mx - m);
+        sum *= f;
+        if (t > 0) {
+          if (!__all_sync(0xffffffffu, tc::mbar_wait(&sh.pv_done[w], (t - 1) & 1, wait_ns, abort_flag))) {
+            ok = false;
+            break;
+          }
+          tc::fence_after_sync();
+          const float fo = f * pow2f(vexp - e);
+#pragma unroll
+          for (int g = 0; g < D / 32; ++g) {
+            uint32_t v[32];
+            ld_x32(to + 32 * g, v);
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * fo);
+            tc::st_32x32b_x32(to + 32 * g, v);
+          }
+          tc::wait_st();
+        }
+        mx = m;
+        vexp = e;
+        weigh((float)(ve - vexp) - mx);
+      }
+      sum = fmaf(part, pow2f(vexp - ve), sum);
+      if (bad) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (seen(g) & meta.bad[g]) sum = __int_as_float(0x7fffffff);
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = p[32 * g + i];
+        tc::st_32x32b_x32(ts + 32 * g, v);
+      }
+      tc::wait_st();
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&sh.p_full[w]);
+    }
+    if (ok && n > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.pv_done[w], (n - 1) & 1, wait_ns, abort_flag));
+    if (!ok) {
+      give_up();
+    } else {
+      tc::fence_after_sync();
+      const int i = row / a.ratio, h = head * a.ratio + row - i * a.ratio;
+      const int64_t tk = seq.q0 + i;
+      const float scale = sum == 0.f ? 0.f : 1.f / sum, power = pow2f(vexp);
+      char* dst = static_cast<char*>(a.out) + 2 * (tk * a.os + (int64_t)h * a.oh);
+#pragma unroll
+      for (int g = 0; g < D / 32; ++g) {
+        uint32_t v[32] = {};
+        if (n > 0) {
+          ld_x32(to + 32 * g, v);
+          tc::wait_ld();
+        }
+        if (r < live) {
+          float o[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = sum == 0.f ? 0.f : __uint_as_float(v[k]) * scale * power;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // columns 0 .. 7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
+            const float* q = o + 8 * k;
+            const uint2 w0 = make_uint2(pack2(q[0], q[2], a.bf16), pack2(q[4], q[6], a.bf16));
+            const uint2 w1 = make_uint2(pack2(q[1], q[3], a.bf16), pack2(q[5], q[7], a.bf16));
+            *reinterpret_cast<uint2*>(dst + 2 * (32 * g + 8 * k)) = w0;
+            *reinterpret_cast<uint2*>(dst + 2 * (32 * g + 8 * k + 4)) = w1;
+          }
+        }
+      }
+      if (a.lse && r < live) a.lse[tk * a.ls + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+    }
+  } else if (warp < kMmaWarp) {
+    // ---------------- cache: nibbles and scales to f16 ----------------
+    const int w = warp - kCacheWarp, tid = threadIdx.x - 32 * kCacheWarp, groups = a.groups;
+    __half* sc = reinterpret_cast<__half*>(smem + C::kScale);
+    const int32_t* pages = a.table + (int64_t)b * a.table_stride;
+    const int in_page = (1 << a.page_log2) - 1;
+    auto page_of = [&](int t) {
+      const int j = tok0 + t * kTok + tid;
+      if (t >= n || j >= seq.len) return -1;
+      const int p = __ldg(pages + (j >> a.page_log2));
+      return p >= 0 && (int64_t)p < a.pages ? p : -1;
+    };
+    // tile t's nibbles: unit u = lane / 8 + 4 i of this warp's 32 tokens is run u / CH (8 tokens, lane % 8), chunk u % CH
+    uint4 rk[CH], rv[CH];
+    uint16_t sk[CH], sv[CH];  // this thread's token's scales (one a group)
+    int64_t line = 0;
+    int page = page_of(0);
+    auto fetch = [&](int t) {
+      const int j = tok0 + t * kTok + tid;
+      line = page < 0 ? -1 : ((((int64_t)page * a.kv_heads + head)) << a.page_log2) + (j & in_page);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int u = (lane >> 3) + 4 * i, run = u / CH, c = u - run * CH;
+        const int64_t ln = __shfl_sync(0xffffffffu, line, 8 * run + (lane & 7));
+        rk[i] = rv[i] = make_uint4(0, 0, 0, 0);
+        if (ln >= 0) {
+          rk[i] = ld_nc_na_v4(a.k4 + ln * (D / 2) + 16 * c);
+          rv[i] = ld_nc_na_v4(a.v4 + ln * (D / 2) + 16 * c);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < CH; ++g) {
+        sk[g] = sv[g] = 0;
+        if (g < groups && line >= 0) {
+          sk[g] = __half_as_ushort(a.k_scale[line * groups + g]);
+          sv[g] = __half_as_ushort(a.v_scale[line * groups + g]);
+        }
+      }
+      page = page_of(t + 1);
+    };
+    auto convert = [&](const uint4 (&raw)[CH], const __half* scale, uint32_t dst) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int u = (lane >> 3) + 4 * i, run = u / CH, c = u - run * CH, tok = 32 * w + 8 * run + (lane & 7);
+        const __half2 s = __half2half2(scale[tok * groups + c / a.cpg]);
+        const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        const uint32_t at = dst + (c / 2) * kBlockBytes + tok * 128;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t e[4];
+          expand(words[k], e);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&e[z]), s);
+            e[z] = *reinterpret_cast<const uint32_t*>(&v);
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + ((((c & 1) * 4 + k) ^ (tok & 7)) << 4)),
+                       "r"(e[0]), "r"(e[1]), "r"(e[2]), "r"(e[3])
+                       : "memory");
+        }
+      }
+    };
+    if (n > 0) fetch(0);
+    for (int t = 0; t < n; ++t) {
+      // the tile's powers of two, and its scales divided by them
+      uint32_t bk = 0, bv = 0;
+      bool bad = false;
+#pragma unroll
+      for (int g = 0; g < CH; ++g) {
+        const uint32_t mk = sk[g] & 0x7fffu, mv = sv[g] & 0x7fffu;
+        if (mk < 0x7c00u) bk = max(bk, mk);
+        if (mv < 0x7c00u) bv = max(bv, mv);
+        bad |= mv >= 0x7c00u;
+      }
+      bk = __reduce_max_sync(0xffffffffu, bk);
+      bv = __reduce_max_sync(0xffffffffu, bv);
+      Meta& meta = sh.meta[t & 3];
+      const uint32_t valid = __ballot_sync(0xffffffffu, line >= 0), bads = __ballot_sync(0xffffffffu, bad);
+      if (lane == 0) {
+        sh.big[0][w] = bk;
+        sh.big[1][w] = bv;
+        meta.valid[w] = valid;
+        meta.bad[w] = bads;
+      }
+      cache_sync();  // also: every warp is done with the last tile's scales
+      bk = max(max(sh.big[0][0], sh.big[0][1]), max(sh.big[0][2], sh.big[0][3]));
+      bv = max(max(sh.big[1][0], sh.big[1][1]), max(sh.big[1][2], sh.big[1][3]));
+      auto exponent = [](uint32_t bits) {
+        return bits ? (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)bits))) >> 23) - 127 : -24;
+      };
+      const int ke = exponent(bk), ve = exponent(bv);
+#pragma unroll
+      for (int g = 0; g < CH; ++g)
+        if (g < groups) {
+          sc[tid * groups + g] = __float2half_rn(__half2float(__ushort_as_half(sk[g])) * pow2f(-ke));
+          sc[kTok * CH + tid * groups + g] =
+              (sv[g] & 0x7fffu) < 0x7c00u ? __float2half_rn(__half2float(__ushort_as_half(sv[g])) * pow2f(-ve)) : __half(0);
+        }
+      if (tid == 0) {
+        meta.k_exp = ke;
+        meta.v_exp = ve;
+      }
+      cache_sync();
+      const int s = t & 1;
+      const uint32_t ph = ((t >> 1) & 1) ^ 1;
+      uint4 nk[CH], nv[CH];
+#pragma unroll
+      for (int i = 0; i < CH; ++i) nk[i] = rk[i], nv[i] = rv[i];
+      if (t + 1 < n) fetch(t + 1);
+      bool ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.k_empty[s], ph, wait_ns, abort_flag));
+      if (ok) {
+        convert(nk, sc, sbase + C::kK + s * C::kTile);
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sh.k_full[s]);
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.v_empty[s], ph, wait_ns, abort_flag));
+      }
+      if (ok) {
+        convert(nv, sc + kTok * CH, sbase + C::kV + s * C::kTile);
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sh.v_full[s]);
+      } else {
+        give_up();  // the named barrier still counts this warp: it keeps step with the others, without the work
+      }
+    }
+  } else if (lane == 0 && n > 0) {
+    // ---------------- products ----------------
+    constexpr uint32_t id_qk = idesc_f16(128, kTok, false), id_pv = idesc_f16(128, D, true);
+    auto qk = [&](int w, int t) {
+      const uint32_t q = sbase + C::kQ + w * C::kTile, k = sbase + C::kK + (t & 1) * C::kTile;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint32_t at = (i / 4) * kBlockBytes + (i % 4) * 32;
+        tc::mma_ss_bf16(tmem + C::kS + w * kTok, tc::sdesc_kmajor_sw128(q + at), tc::sdesc_kmajor_sw128(k + at), id_qk, i > 0);
+      }
+    };
+    auto pv = [&](int w, int t) {
+      const uint32_t v = sbase + C::kV + (t & 1) * C::kTile;
+#pragma unroll
+      for (int i = 0; i < kTok / 16; ++i)
+        tc::mma_ts_bf16(tmem + C::kO + w * D, tmem + C::kS + w * kTok + 8 * i, desc_v(v + i * 2048), id_pv, t > 0 || i > 0);
+    };
+    bool ok = tc::mbar_wait(&sh.k_full[0], 0, wait_ns, abort_flag);
+    if (ok) {
+      tc::fence_after_sync();
+      for (int w = 0; w < 2; ++w) {
+        tc::mbar_arrive(&sh.s_full[w]);
+        qk(w, 0);
+        tc::commit(&sh.s_full[w]);
+      }
+      tc::commit(&sh.k_empty[0]);
+    }
+    for (int t = 0; ok && t < n; ++t) {
+      ok = tc::mbar_wait(&sh.v_full[t & 1], (t >> 1) & 1, wait_ns, abort_flag);
+      for (int w = 0; ok && w < 2; ++w) {
+        ok = tc::mbar_wait(&sh.p_full[w], t & 1, wait_ns, abort_flag);
+        if (!ok) break;
+        tc::fence_after_sync();
+        pv(w, t);
+        tc::commit(&sh.pv_done[w]);
+        if (t + 1 < n) {
+          if (w == 0) ok = tc::mbar_wait(&sh.k_full[(t + 1) & 1], ((t + 1) >> 1) & 1, wait_ns, abort_flag);
+          if (!ok) break;
+          tc::fence_after_sync();
+          tc::mbar_arrive(&sh.s_full[w]);
+          qk(w, t + 1);  // over S and P of tile t: after pv(w, t), which was issued before it
+          tc::commit(&sh.s_full[w]);
+        }
+      }
+      if (!ok) break;
+      tc::commit(&sh.v_empty[t & 1]);
+      if (t + 1 < n) tc::commit(&sh.k_empty[(t + 1) & 1]);
+    }
+    if (!ok) give_up();
+    tc::commit(&sh.drain);  // nothing may be in flight when the tensor memory goes
+    if (!tc::mbar_wait(&sh.drain, 0, wait_ns, nullptr)) give_up();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (warp == kMmaWarp) tc::tmem_dealloc(tmem, C::kCols);
+}
+
+template <int D>
+int launch_prompt(const Args& a, int64_t ctas, cudaStream_t s) {
+  const auto kernel = kv4_prompt_kernel<D>;
+  const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), Cfg<D>::kSmem);
+  if (e != cudaSuccess) return cuda_status(e);
+  kernel<<<(unsigned)ctas, kThreads, Cfg<D>::kSmem, s>>>(a, wait_limit_ns());
+  note_launch();
+  return check_launch();
+}
+
+}  // namespace
+
+int prompt_attention(const Args& a, int dim, cudaStream_t s) {
+  const int64_t ctas = (a.tokens * a.ratio / kRowsCta + a.batch) * a.kv_heads;
+  if (ctas > 0x7fffffff) return UP_ERR_UNSUPPORTED;
+  return dim == 64 ? launch_prompt<64>(a, ctas, s) : launch_prompt<128>(a, ctas, s);
+}
+
+}  // namespace kv4
+}  // namespace up
