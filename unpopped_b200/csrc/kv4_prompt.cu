@@ -6,8 +6,9 @@
 //
 // A CTA takes 256 query rows (query token x head of the group) of one sequence and key/value head as two tiles of 128,
 // and walks the cached tokens that any of them sees, 128 at a time. Per tile of tokens, S = Q K^T (128 x 128) and
-// O += P V (128 x dim) run per query tile with f32 accumulators in tensor memory; the two query tiles alternate, so that
-// the tensor cores work on one while the other's probabilities are computed.
+// O += P V (128 x dim) run per query tile with f32 accumulators in tensor memory. A tile of tokens is two halves of 64,
+// each with an S of its own, so that a query tile's probabilities of one half are computed while the tensor cores work
+// on the other.
 //  * warps 0..7 (probabilities): warp group w holds query tile w, a thread a row. A thread reads its row of S, takes
 //    p = 2^(logit - ref), and writes P as f16 over S: the A operand of the second product. ref moves only when a tile's
 //    probabilities sum to more than 2^9; then the thread scales its row of O.
@@ -15,7 +16,8 @@
 //    128-byte swizzled shared memory, two stages each. Both have a row a token: K is the B operand with its contraction
 //    (the dimensions) contiguous, V the one with its output (the dimensions) contiguous. The nibble conversion pairs
 //    dimensions k and k + 4 of each 8; q is stored in the same order and the output's columns are read in it.
-//  * warp 12 (products): one thread issues every tcgen05.mma.
+//  * warps 12 and 13 (products): one thread each issues the tcgen05.mma of one query tile, so neither tile's products
+//    wait for the other's probabilities.
 // Scales. A tile's scales are divided by the power of two of the largest (separately for K and V), so nibble * scale
 // keeps f16's precision and range whatever their size; the logits take K's power, the probabilities V's, relative to
 // the largest one met (O is scaled when a larger one comes). nibble * scale and p are rounded to f16; all sums are f32.
@@ -33,8 +35,8 @@ namespace kv4 {
 
 namespace {
 
-constexpr int kRowsCta = 256, kTok = 128;
-constexpr int kThreads = 32 * 13, kCacheWarp = 8, kMmaWarp = 12;
+constexpr int kRowsCta = 256, kTok = 128, kHalf = kTok / 2;
+constexpr int kThreads = 32 * 14, kCacheWarp = 8, kMmaWarp = 12;  // 16 warps' worth of registers: 128 a thread
 constexpr int kBlockBytes = kTok * 128;  // 128 rows of 64 dimensions (128 bytes), swizzled
 
 template <int D>
@@ -55,13 +57,14 @@ struct Meta {          // what the cache warps say of a tile of tokens
 };
 
 struct Shared {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2], drain;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], drain;  // [query tile][half]
   uint32_t tmem;
   int abort;
   Meta meta[4];
   float row_scale[kRowsCta];   // scale * log2(e) / the row's power of two
   uint32_t big[2][4];
-  int64_t scan[13], base;
+  int64_t scan[kThreads / 32], base;
   int seq;
 };
 
@@ -145,13 +148,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&sh.k_full[i], 4);    // the cache warps
       tc::mbar_init(&sh.v_full[i], 4);
-      tc::mbar_init(&sh.k_empty[i], 1);   // a commit
-      tc::mbar_init(&sh.v_empty[i], 1);
-      tc::mbar_init(&sh.s_full[i], 2);    // the issuer (it has seen the tile's meta) and a commit
-      tc::mbar_init(&sh.p_full[i], 4);    // the tile's warps
+      tc::mbar_init(&sh.k_empty[i], 2);   // a commit of each issuer
+      tc::mbar_init(&sh.v_empty[i], 2);
+      for (int h = 0; h < 2; ++h) {
+        tc::mbar_init(&sh.s_full[i][h], 2);  // the issuer (it has seen the tile's meta) and a commit
+        tc::mbar_init(&sh.p_full[i][h], 4);  // the tile's warps
+      }
       tc::mbar_init(&sh.pv_done[i], 1);
     }
-    tc::mbar_init(&sh.drain, 1);
+    tc::mbar_init(&sh.drain, 2);
     tc::mbar_fence_init();
     sh.abort = 0;
   }
@@ -217,44 +222,47 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     float mx = kNoMax, sum = 0.f;
     int vexp = -24;
     bool ok = true;
-    for (int t = 0; t < n; ++t) {
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(&sh.s_full[w], t & 1, wait_ns, abort_flag))) {
-        ok = false;
-        break;
-      }
+    // S of half u: 32 columns are in registers (v) or on the way when its turn comes, and P of half u - 1 is handed over
+    // in the middle of it, so that neither direction's latency stands between the exponentials.
+    uint32_t v[32], p[kHalf / 2];
+    auto wait_s = [&](int u) {
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(&sh.s_full[w][u & 1], (u >> 1) & 1, wait_ns, abort_flag))) return false;
       tc::fence_after_sync();
+      return true;
+    };
+    if (n > 0 && (ok = wait_s(0))) ld_x32(ts, v);
+    for (int u = 0; ok && u < 2 * n; ++u) {  // half h of tile t
+      const int t = u >> 1, h = u & 1;
       const Meta& meta = sh.meta[t & 3];
-      const int j0 = tok0 + t * kTok;
+      const int j0 = tok0 + u * kHalf;
+      const uint32_t th = ts + h * kHalf;
       const float c = row_scale * pow2f(meta.k_exp);
       const int ve = meta.v_exp;
-      const bool all = (meta.valid[0] & meta.valid[1] & meta.valid[2] & meta.valid[3]) == 0xffffffffu;
-      const bool bad = (meta.bad[0] | meta.bad[1] | meta.bad[2] | meta.bad[3]) != 0;
-      const bool masked = !__all_sync(0xffffffffu, all && j0 > past && j0 + kTok - 1 <= last) || bad;
+      const uint32_t valid[2] = {meta.valid[2 * h], meta.valid[2 * h + 1]};
+      const uint32_t bad[2] = {meta.bad[2 * h], meta.bad[2 * h + 1]};
+      const bool masked = !__all_sync(0xffffffffu, (valid[0] & valid[1]) == 0xffffffffu && j0 > past && j0 + kHalf - 1 <= last);
       // the visible tokens of chunk g (32 of them)
       auto seen = [&](int g) -> uint32_t {
         const int from = past + 1 - (j0 + 32 * g), to_ = last + 1 - (j0 + 32 * g);  // in [from, to_)
-        uint32_t m = meta.valid[g];
+        uint32_t m = g ? valid[1] : valid[0];
         m &= from >= 32 ? 0u : from <= 0 ? 0xffffffffu : 0xffffffffu << from;
         m &= to_ <= 0 ? 0u : to_ >= 32 ? 0xffffffffu : (1u << to_) - 1u;
         return m;
       };
-      uint32_t p[kTok / 2];
       float part;
-      auto weigh = [&](float add) {  // p = 2^(c S + add), packed, and their sum
+      // p = 2^(c S + add), packed, and their sum; again if the sum was too large for the reference, which then has moved
+      for (int pass = 0;; ++pass) {
+        const float add = (float)(ve - max(vexp, ve)) - mx;
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          uint32_t v[32];
-          ld_x32(ts + 32 * g, v);
+        for (int g = 0; g < 2; ++g) {
           tc::wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(v[i]), c, add)));
           if (masked) {
             const uint32_t m = seen(g);
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              v[i] = (m >> i) & 1u ? __float_as_uint(exp2_approx(fmaf(__uint_as_float(v[i]), c, add))) : 0u;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(v[i]), c, add)));
+            for (int i = 0; i < 32; ++i) v[i] = (m >> i) & 1u ? v[i] : 0u;
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
@@ -262,16 +270,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
             s1 += __uint_as_float(v[i + 1]);
             p[16 * g + i / 2] = pack2_f16(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
           }
+          if (g == 0) ld_x32(th + 32, v);
         }
         part = s0 + s1;
-      };
-      weigh((float)(ve - max(vexp, ve)) - mx);
-      if (__any_sync(0xffffffffu, part > 512.f || ve > vexp)) {
+        if (pass > 0 || !__any_sync(0xffffffffu, part > 512.f || ve > vexp)) break;
         float m = mx;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          uint32_t v[32];
-          ld_x32(ts + 32 * g, v);
+#pragma unroll 1
+        for (int g = 0; g < 2; ++g) {
+          ld_x32(th + 32 * g, v);
           tc::wait_ld();
           const uint32_t see = masked ? seen(g) : 0xffffffffu;
 #pragma unroll
@@ -281,16 +287,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         const int e = max(vexp, ve);
         const float f = exp2_approx(mx - m);
         sum *= f;
-        if (t > 0) {
-          if (!__all_sync(0xffffffffu, tc::mbar_wait(&sh.pv_done[w], (t - 1) & 1, wait_ns, abort_flag))) {
-            ok = false;
-            break;
-          }
+        if (u > 0) {
+          ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.pv_done[w], (u - 1) & 1, wait_ns, abort_flag));
+          if (!ok) break;
           tc::fence_after_sync();
           const float fo = f * pow2f(vexp - e);
-#pragma unroll
+#pragma unroll 1
           for (int g = 0; g < D / 32; ++g) {
-            uint32_t v[32];
             ld_x32(to + 32 * g, v);
             tc::wait_ld();
 #pragma unroll
@@ -301,27 +304,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         }
         mx = m;
         vexp = e;
-        weigh((float)(ve - vexp) - mx);
+        ld_x32(th, v);
       }
+      if (!ok) break;
       sum = fmaf(part, pow2f(vexp - ve), sum);
-      if (bad) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          if (seen(g) & meta.bad[g]) sum = __int_as_float(0x7fffffff);
-      }
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint32_t v[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = p[32 * g + i];
-        tc::st_32x32b_x32(ts + 32 * g, v);
-      }
+      if ((bad[0] | bad[1]) && ((seen(0) & bad[0]) | (seen(1) & bad[1]))) sum = __int_as_float(0x7fffffff);
+      tc::st_32x32b_x32(th, p);
       tc::wait_st();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&sh.p_full[w]);
+      if (lane == 0) tc::mbar_arrive(&sh.p_full[w][h]);
+      if (u + 1 < 2 * n && (ok = wait_s(u + 1))) ld_x32(ts + (h ^ 1) * kHalf, v);
     }
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.pv_done[w], (n - 1) & 1, wait_ns, abort_flag));
+    // A wait tells phases apart by parity, so it may be one behind at most: S of half u says that PV of half u - 2 is done
+    // (it was issued before), and the last two are waited for in turn.
+    if (ok && n > 0)
+      ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.pv_done[w], 0, wait_ns, abort_flag) &&
+                                       tc::mbar_wait(&sh.pv_done[w], 1, wait_ns, abort_flag));
     if (!ok) {
       give_up();
     } else {
@@ -358,46 +357,44 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     const int w = warp - kCacheWarp, tid = threadIdx.x - 32 * kCacheWarp, groups = a.groups;
     __half* sc = reinterpret_cast<__half*>(smem + C::kScale);
     const int32_t* pages = a.table + (int64_t)b * a.table_stride;
-    const int in_page = (1 << a.page_log2) - 1;
+    const int in_page = (1 << a.page_log2) - 1, cpg_log2 = 31 - __clz(a.cpg);  // 1, 2 or 4 chunks a group
     auto page_of = [&](int t) {
       const int j = tok0 + t * kTok + tid;
       if (t >= n || j >= seq.len) return -1;
       const int p = __ldg(pages + (j >> a.page_log2));
       return p >= 0 && (int64_t)p < a.pages ? p : -1;
     };
-    // tile t's nibbles: unit u = lane / 8 + 4 i of this warp's 32 tokens is run u / CH (8 tokens, lane % 8), chunk u % CH
+    // a tile's nibbles: unit u = lane / 8 + 4 i of this warp's 32 tokens is run u / CH (8 tokens, lane % 8), chunk u % CH
     uint4 rk[CH], rv[CH];
     uint16_t sk[CH], sv[CH];  // this thread's token's scales (one a group)
-    int64_t line = 0;
-    int page = page_of(0);
-    auto fetch = [&](int t) {
-      const int j = tok0 + t * kTok + tid;
-      line = page < 0 ? -1 : ((((int64_t)page * a.kv_heads + head)) << a.page_log2) + (j & in_page);
+    const uint32_t page_lines = (uint32_t)a.kv_heads << a.page_log2, head_line = (uint32_t)head << a.page_log2;
+    // a token that does not exist reads line 0's bytes: its scales are zero
+    auto fetch = [&](const uint8_t* src, int t, int page, uint4 (&raw)[CH]) {
+      const int pg = max(page, 0), at = (tok0 + t * kTok + 32 * w) & in_page;  // a run of 8 is on one page
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int u = (lane >> 3) + 4 * i, run = u / CH, c = u - run * CH;
-        const int64_t ln = __shfl_sync(0xffffffffu, line, 8 * run + (lane & 7));
-        rk[i] = rv[i] = make_uint4(0, 0, 0, 0);
-        if (ln >= 0) {
-          rk[i] = ld_nc_na_v4(a.k4 + ln * (D / 2) + 16 * c);
-          rv[i] = ld_nc_na_v4(a.v4 + ln * (D / 2) + 16 * c);
-        }
+        const int64_t ln = (int64_t)(uint32_t)__shfl_sync(0xffffffffu, pg, 8 * run) * page_lines +
+                           (head_line + ((at + 8 * run) & in_page) + (lane & 7));
+        raw[i] = ld_nc_na_v4(src + ln * (D / 2) + 16 * c);
       }
+    };
+    auto fetch_scales = [&](int t, int page) {
+      const int64_t line = (int64_t)(uint32_t)max(page, 0) * page_lines + (head_line + ((tok0 + t * kTok + tid) & in_page));
 #pragma unroll
       for (int g = 0; g < CH; ++g) {
         sk[g] = sv[g] = 0;
-        if (g < groups && line >= 0) {
+        if (g < groups && page >= 0) {
           sk[g] = __half_as_ushort(a.k_scale[line * groups + g]);
           sv[g] = __half_as_ushort(a.v_scale[line * groups + g]);
         }
       }
-      page = page_of(t + 1);
     };
     auto convert = [&](const uint4 (&raw)[CH], const __half* scale, uint32_t dst) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int u = (lane >> 3) + 4 * i, run = u / CH, c = u - run * CH, tok = 32 * w + 8 * run + (lane & 7);
-        const __half2 s = __half2half2(scale[tok * groups + c / a.cpg]);
+        const __half2 s = __half2half2(scale[tok * groups + (c >> cpg_log2)]);
         const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
         const uint32_t at = dst + (c / 2) * kBlockBytes + tok * 128;
 #pragma unroll
@@ -415,7 +412,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         }
       }
     };
-    if (n > 0) fetch(0);
+    int page = page_of(0);
+    if (n > 0) {
+      fetch_scales(0, page);
+      fetch(a.k4, 0, page, rk);
+      fetch(a.v4, 0, page, rv);
+    }
     for (int t = 0; t < n; ++t) {
       // the tile's powers of two, and its scales divided by them
       uint32_t bk = 0, bv = 0;
@@ -430,7 +432,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       bk = __reduce_max_sync(0xffffffffu, bk);
       bv = __reduce_max_sync(0xffffffffu, bv);
       Meta& meta = sh.meta[t & 3];
-      const uint32_t valid = __ballot_sync(0xffffffffu, line >= 0), bads = __ballot_sync(0xffffffffu, bad);
+      const int next = page_of(t + 1);
+      const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0), bads = __ballot_sync(0xffffffffu, bad);
       if (lane == 0) {
         sh.big[0][w] = bk;
         sh.big[1][w] = bv;
@@ -458,74 +461,78 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       cache_sync();
       const int s = t & 1;
       const uint32_t ph = ((t >> 1) & 1) ^ 1;
-      uint4 nk[CH], nv[CH];
-#pragma unroll
-      for (int i = 0; i < CH; ++i) nk[i] = rk[i], nv[i] = rv[i];
-      if (t + 1 < n) fetch(t + 1);
+      page = next;  // from here on the next tile's: loaded as soon as registers are free
+      if (t + 1 < n) fetch_scales(t + 1, page);
       bool ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.k_empty[s], ph, wait_ns, abort_flag));
       if (ok) {
-        convert(nk, sc, sbase + C::kK + s * C::kTile);
+        convert(rk, sc, sbase + C::kK + s * C::kTile);
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&sh.k_full[s]);
+        if (t + 1 < n) fetch(a.k4, t + 1, page, rk);
         ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.v_empty[s], ph, wait_ns, abort_flag));
       }
       if (ok) {
-        convert(nv, sc + kTok * CH, sbase + C::kV + s * C::kTile);
+        convert(rv, sc + kTok * CH, sbase + C::kV + s * C::kTile);
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&sh.v_full[s]);
+        if (t + 1 < n) fetch(a.v4, t + 1, page, rv);
       } else {
         give_up();  // the named barrier still counts this warp: it keeps step with the others, without the work
       }
     }
   } else if (lane == 0 && n > 0) {
-    // ---------------- products ----------------
-    constexpr uint32_t id_qk = idesc_f16(128, kTok, false), id_pv = idesc_f16(128, D, true);
-    auto qk = [&](int w, int t) {
-      const uint32_t q = sbase + C::kQ + w * C::kTile, k = sbase + C::kK + (t & 1) * C::kTile;
+    // ---------------- products of query tile w ----------------
+    constexpr uint32_t id_qk = idesc_f16(128, kHalf, false), id_pv = idesc_f16(128, D, true);
+    const int w = warp - kMmaWarp;
+    const uint32_t ts = tmem + C::kS + w * kTok, to = tmem + C::kO + w * D;
+    // descriptors of the first step; a step further adds its bytes / 16 to the address field
+    const uint64_t q0 = tc::sdesc_kmajor_sw128(sbase + C::kQ + w * C::kTile);
+    const uint64_t k0 = tc::sdesc_kmajor_sw128(sbase + C::kK), v0 = desc_v(sbase + C::kV);
+    auto qk = [&](int t, int h) {
+      const uint64_t k = k0 + (uint64_t)((t & 1) * (C::kTile >> 4) + h * (kHalf * 128 >> 4));
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint32_t at = (i / 4) * kBlockBytes + (i % 4) * 32;
-        tc::mma_ss_bf16(tmem + C::kS + w * kTok, tc::sdesc_kmajor_sw128(q + at), tc::sdesc_kmajor_sw128(k + at), id_qk, i > 0);
+      for (int i = 0; i < D / 16; ++i) {  // 16 dimensions: 32 bytes
+        const uint64_t at = (uint64_t)((i / 4) * (kBlockBytes >> 4) + (i % 4) * 2);
+        tc::mma_ss_bf16(ts + h * kHalf, q0 + at, k + at, id_qk, i > 0);
       }
     };
-    auto pv = [&](int w, int t) {
-      const uint32_t v = sbase + C::kV + (t & 1) * C::kTile;
+    auto pv = [&](int t, int h) {
+      const uint64_t v = v0 + (uint64_t)((t & 1) * (C::kTile >> 4) + h * (kHalf * 128 >> 4));
 #pragma unroll
-      for (int i = 0; i < kTok / 16; ++i)
-        tc::mma_ts_bf16(tmem + C::kO + w * D, tmem + C::kS + w * kTok + 8 * i, desc_v(v + i * 2048), id_pv, t > 0 || i > 0);
+      for (int i = 0; i < kHalf / 16; ++i)  // 16 tokens: 2048 bytes
+        tc::mma_ts_bf16(to, ts + h * kHalf + 8 * i, v + (uint64_t)(i * 128), id_pv, t + h + i > 0);
     };
     bool ok = tc::mbar_wait(&sh.k_full[0], 0, wait_ns, abort_flag);
     if (ok) {
       tc::fence_after_sync();
-      for (int w = 0; w < 2; ++w) {
-        tc::mbar_arrive(&sh.s_full[w]);
-        qk(w, 0);
-        tc::commit(&sh.s_full[w]);
+      for (int h = 0; h < 2; ++h) {
+        tc::mbar_arrive(&sh.s_full[w][h]);
+        qk(0, h);
+        tc::commit(&sh.s_full[w][h]);
       }
       tc::commit(&sh.k_empty[0]);
     }
     for (int t = 0; ok && t < n; ++t) {
       ok = tc::mbar_wait(&sh.v_full[t & 1], (t >> 1) & 1, wait_ns, abort_flag);
-      for (int w = 0; ok && w < 2; ++w) {
-        ok = tc::mbar_wait(&sh.p_full[w], t & 1, wait_ns, abort_flag);
+      for (int h = 0; ok && h < 2; ++h) {
+        ok = tc::mbar_wait(&sh.p_full[w][h], t & 1, wait_ns, abort_flag);
         if (!ok) break;
         tc::fence_after_sync();
-        pv(w, t);
+        pv(t, h);
         tc::commit(&sh.pv_done[w]);
+        if (h == 1) tc::commit(&sh.v_empty[t & 1]);
         if (t + 1 < n) {
-          if (w == 0) ok = tc::mbar_wait(&sh.k_full[(t + 1) & 1], ((t + 1) >> 1) & 1, wait_ns, abort_flag);
+          if (h == 0) ok = tc::mbar_wait(&sh.k_full[(t + 1) & 1], ((t + 1) >> 1) & 1, wait_ns, abort_flag);
           if (!ok) break;
           tc::fence_after_sync();
-          tc::mbar_arrive(&sh.s_full[w]);
-          qk(w, t + 1);  // over S and P of tile t: after pv(w, t), which was issued before it
-          tc::commit(&sh.s_full[w]);
+          tc::mbar_arrive(&sh.s_full[w][h]);
+          qk(t + 1, h);  // over S and P of tile t's half: issued after pv(t, h), which reads them
+          tc::commit(&sh.s_full[w][h]);
+          if (h == 1) tc::commit(&sh.k_empty[(t + 1) & 1]);
         }
       }
-      if (!ok) break;
-      tc::commit(&sh.v_empty[t & 1]);
-      if (t + 1 < n) tc::commit(&sh.k_empty[(t + 1) & 1]);
     }
     if (!ok) give_up();
     tc::commit(&sh.drain);  // nothing may be in flight when the tensor memory goes
