@@ -9,15 +9,16 @@
 // O += P V (128 x dim) run per query tile with f32 accumulators in tensor memory. A tile of tokens is two halves of 64,
 // each with an S of its own, so that a query tile's probabilities of one half are computed while the tensor cores work
 // on the other.
-//  * warps 0..7 (probabilities): warp group w holds query tile w, a thread a row. A thread reads its row of S, takes
-//    p = 2^(logit - ref), and writes P as f16 over S: the A operand of the second product. ref moves only when a tile's
-//    probabilities sum to more than 2^9; then the thread scales its row of O.
-//  * warps 8..11 (cache): read 128 tokens' nibbles and scales, a tile ahead in registers, and write K and V as f16 into
-//    128-byte swizzled shared memory, two stages each. Both have a row a token: K is the B operand with its contraction
-//    (the dimensions) contiguous, V the one with its output (the dimensions) contiguous. The nibble conversion pairs
-//    dimensions k and k + 4 of each 8; q is stored in the same order and the output's columns are read in it.
-//  * warps 12 and 13 (products): one thread each issues the tcgen05.mma of one query tile, so neither tile's products
-//    wait for the other's probabilities.
+//  * warp groups 0 and 1 (probabilities): group w holds query tile w, a thread a row. A thread reads its row of S twice,
+//    for the largest logit and for p = 2^(logit - ref), and writes P as f16 over it: the A operand of the second product.
+//    ref moves only when a logit is more than 2^8 above it; then the thread scales its row of O.
+//  * warp groups 2 and 3 (cache, K and V): read 128 tokens' nibbles and scales, a tile ahead in registers, and write
+//    them as f16 into 128-byte swizzled shared memory, two stages each. Both have a row a token: K is the B operand with
+//    its contraction (the dimensions) contiguous, V the one with its output (the dimensions) contiguous. The nibble
+//    conversion pairs dimensions k and k + 4 of each 8; q is stored in the same order and the output's columns are read
+//    in it.
+//  * warps 16 and 17 (products): each issues the tcgen05.mma of one query tile, so neither tile's products wait for the
+//    other's probabilities.
 // Scales. A tile's scales are divided by the power of two of the largest (separately for K and V), so nibble * scale
 // keeps f16's precision and range whatever their size; the logits take K's power, the probabilities V's, relative to
 // the largest one met (O is scaled when a larger one comes). nibble * scale and p are rounded to f16; all sums are f32.
@@ -36,7 +37,7 @@ namespace kv4 {
 namespace {
 
 constexpr int kRowsCta = 256, kTok = 128, kHalf = kTok / 2;
-constexpr int kThreads = 32 * 14, kCacheWarp = 8, kMmaWarp = 12;  // 16 warps' worth of registers: 128 a thread
+constexpr int kThreads = 32 * 18, kCacheWarp = 8, kMmaWarp = 16;
 constexpr int kBlockBytes = kTok * 128;  // 128 rows of 64 dimensions (128 bytes), swizzled
 
 template <int D>
@@ -57,13 +58,13 @@ struct Meta {          // what the cache warps say of a tile of tokens
 };
 
 struct Shared {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t full[2][2], empty[2][2];  // [K, V][stage]
   uint64_t s_full[2][2], p_full[2][2], pv_done[2], drain;  // [query tile][half]
   uint32_t tmem;
   int abort;
   Meta meta[4];
   float row_scale[kRowsCta];   // scale * log2(e) / the row's power of two
-  uint32_t big[2][4];
+  uint32_t big[2][4];          // [K, V][warp]
   int64_t scan[kThreads / 32], base;
   int seq;
 };
@@ -95,8 +96,31 @@ __device__ __forceinline__ void ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
       : "memory");
 }
 
+// D[tmem] (+)= A B, kind::f16: A from shared memory (a descriptor) or tensor memory. The thread that issues shares its
+// scheduler with warps that compute, so what an issue costs is its instructions: no lane mask, constant tensor memory
+// addresses (the CTA holds all of it, from address 0).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
-__device__ __forceinline__ void cache_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+template <int ID>
+__device__ __forceinline__ void named_sync() { asm volatile("bar.sync %0, 128;" ::"n"(ID) : "memory"); }
+__device__ __forceinline__ void cache_sync(int z) { z ? named_sync<2>() : named_sync<1>(); }  // K's, V's group
 
 __device__ __forceinline__ int64_t seq_ctas(const Args& a, int b) {
   const Seq s = load_seq(a, b);
@@ -146,10 +170,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&sh.k_full[i], 4);    // the cache warps
-      tc::mbar_init(&sh.v_full[i], 4);
-      tc::mbar_init(&sh.k_empty[i], 2);   // a commit of each issuer
-      tc::mbar_init(&sh.v_empty[i], 2);
+      for (int z = 0; z < 2; ++z) {
+        tc::mbar_init(&sh.full[z][i], 4);   // the cache group's warps
+        tc::mbar_init(&sh.empty[z][i], 2);  // a commit of each issuer
+      }
       for (int h = 0; h < 2; ++h) {
         tc::mbar_init(&sh.s_full[i][h], 2);  // the issuer (it has seen the tile's meta) and a commit
         tc::mbar_init(&sh.p_full[i][h], 4);  // the tile's warps
@@ -203,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = sh.tmem;
+  constexpr uint32_t tmem = 0;  // all 512 columns were allocated: they begin at 0
   volatile int* abort_flag = &sh.abort;
   auto give_up = [&]() {
     *abort_flag = 1;
@@ -222,114 +246,114 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     float mx = kNoMax, sum = 0.f;
     int vexp = -24;
     bool ok = true;
-    // S of half u: 32 columns are in registers (v) or on the way when its turn comes, and P of half u - 1 is handed over
-    // in the middle of it, so that neither direction's latency stands between the exponentials.
-    uint32_t v[32], p[kHalf / 2];
-    auto wait_s = [&](int u) {
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(&sh.s_full[w][u & 1], (u >> 1) & 1, wait_ns, abort_flag))) return false;
-      tc::fence_after_sync();
-      return true;
+    auto wait = [&](uint64_t* bar, int parity) {
+      return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity & 1, wait_ns, abort_flag)) != 0;
     };
-    if (n > 0 && (ok = wait_s(0))) ld_x32(ts, v);
-    for (int u = 0; ok && u < 2 * n; ++u) {  // half h of tile t
+#pragma unroll 1
+    for (int u = 0; u < 2 * n; ++u) {  // half h of tile t
       const int t = u >> 1, h = u & 1;
+      ok = wait(&sh.s_full[w][h], t);
+      if (!ok) break;
+      tc::fence_after_sync();
       const Meta& meta = sh.meta[t & 3];
       const int j0 = tok0 + u * kHalf;
       const uint32_t th = ts + h * kHalf;
       const float c = row_scale * pow2f(meta.k_exp);
       const int ve = meta.v_exp;
-      const uint32_t valid[2] = {meta.valid[2 * h], meta.valid[2 * h + 1]};
-      const uint32_t bad[2] = {meta.bad[2 * h], meta.bad[2 * h + 1]};
-      const bool masked = !__all_sync(0xffffffffu, (valid[0] & valid[1]) == 0xffffffffu && j0 > past && j0 + kHalf - 1 <= last);
+      const uint32_t valid0 = meta.valid[2 * h], valid1 = meta.valid[2 * h + 1];
+      const bool masked = !__all_sync(0xffffffffu, (valid0 & valid1) == 0xffffffffu && j0 > past && j0 + kHalf - 1 <= last);
       // the visible tokens of chunk g (32 of them)
       auto seen = [&](int g) -> uint32_t {
         const int from = past + 1 - (j0 + 32 * g), to_ = last + 1 - (j0 + 32 * g);  // in [from, to_)
-        uint32_t m = g ? valid[1] : valid[0];
+        uint32_t m = g ? valid1 : valid0;
         m &= from >= 32 ? 0u : from <= 0 ? 0xffffffffu : 0xffffffffu << from;
         m &= to_ <= 0 ? 0u : to_ >= 32 ? 0xffffffffu : (1u << to_) - 1u;
         return m;
       };
-      float part;
-      // p = 2^(c S + add), packed, and their sum; again if the sum was too large for the reference, which then has moved
-      for (int pass = 0;; ++pass) {
-        const float add = (float)(ve - max(vexp, ve)) - mx;
-        float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          tc::wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(v[i]), c, add)));
-          if (masked) {
-            const uint32_t m = seen(g);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = (m >> i) & 1u ? v[i] : 0u;
-          }
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            s0 += __uint_as_float(v[i]);
-            s1 += __uint_as_float(v[i + 1]);
-            p[16 * g + i / 2] = pack2_f16(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-          }
-          if (g == 0) ld_x32(th + 32, v);
-        }
-        part = s0 + s1;
-        if (pass > 0 || !__any_sync(0xffffffffu, part > 512.f || ve > vexp)) break;
-        float m = mx;
+      // the largest logit, against the reference
+      float m = mx;
 #pragma unroll 1
-        for (int g = 0; g < 2; ++g) {
-          ld_x32(th + 32 * g, v);
-          tc::wait_ld();
-          const uint32_t see = masked ? seen(g) : 0xffffffffu;
+      for (int g = 0; g < 2; ++g) {
+        uint32_t v[32];
+        ld_x32(th + 32 * g, v);
+        tc::wait_ld();
+        if (masked) {
+          const uint32_t see = seen(g);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if ((see >> i) & 1u) m = fmaxf(m, __uint_as_float(v[i]) * c);
+          for (int i = 0; i < 32; ++i) v[i] = (see >> i) & 1u ? v[i] : 0x7fffffffu;  // a NaN is no maximum
         }
+        float m1 = m;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          m = fmaxf(m, __uint_as_float(v[i]) * c);
+          m1 = fmaxf(m1, __uint_as_float(v[i + 1]) * c);
+        }
+        m = fmaxf(m, m1);
+      }
+      if (__any_sync(0xffffffffu, m > mx + 8.f || ve > vexp)) {
         const int e = max(vexp, ve);
-        const float f = exp2_approx(mx - m);
+        const float f = exp2_approx(mx - m), fo = f * pow2f(vexp - e);
         sum *= f;
+        mx = m;
+        vexp = e;
         if (u > 0) {
-          ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.pv_done[w], (u - 1) & 1, wait_ns, abort_flag));
+          ok = wait(&sh.pv_done[w], u - 1);
           if (!ok) break;
           tc::fence_after_sync();
-          const float fo = f * pow2f(vexp - e);
 #pragma unroll 1
           for (int g = 0; g < D / 32; ++g) {
+            uint32_t v[32];
             ld_x32(to + 32 * g, v);
             tc::wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * fo);
             tc::st_32x32b_x32(to + 32 * g, v);
           }
-          tc::wait_st();
         }
-        mx = m;
-        vexp = e;
-        ld_x32(th, v);
       }
-      if (!ok) break;
-      sum = fmaf(part, pow2f(vexp - ve), sum);
-      if ((bad[0] | bad[1]) && ((seen(0) & bad[0]) | (seen(1) & bad[1]))) sum = __int_as_float(0x7fffffff);
-      tc::st_32x32b_x32(th, p);
+      // p = 2^(c S - ref), as f16 over columns that were read, and their sum
+      const float add = (float)(ve - vexp) - mx;
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll 1
+      for (int g = 0; g < 2; ++g) {
+        uint32_t v[32], p[16];
+        ld_x32(th + 32 * g, v);
+        tc::wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(v[i]), c, add)));
+        if (masked) {
+          const uint32_t see = seen(g);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = (see >> i) & 1u ? v[i] : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          s0 += __uint_as_float(v[i]);
+          s1 += __uint_as_float(v[i + 1]);
+          p[i / 2] = pack2_f16(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        }
+        tc::st_32x32b_x16(th + 16 * g, p);
+      }
+      sum = fmaf(s0 + s1, pow2f(vexp - ve), sum);
+      const uint32_t bad0 = meta.bad[2 * h], bad1 = meta.bad[2 * h + 1];
+      if ((bad0 | bad1) && ((seen(0) & bad0) | (seen(1) & bad1))) sum = __int_as_float(0x7fffffff);
       tc::wait_st();
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&sh.p_full[w][h]);
-      if (u + 1 < 2 * n && (ok = wait_s(u + 1))) ld_x32(ts + (h ^ 1) * kHalf, v);
     }
     // A wait tells phases apart by parity, so it may be one behind at most: S of half u says that PV of half u - 2 is done
     // (it was issued before), and the last two are waited for in turn.
-    if (ok && n > 0)
-      ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.pv_done[w], 0, wait_ns, abort_flag) &&
-                                       tc::mbar_wait(&sh.pv_done[w], 1, wait_ns, abort_flag));
+    if (ok && n > 0) ok = wait(&sh.pv_done[w], 0) && wait(&sh.pv_done[w], 1);
     if (!ok) {
       give_up();
     } else {
       tc::fence_after_sync();
-      const int i = row / a.ratio, h = head * a.ratio + row - i * a.ratio;
+      const int i = row / a.ratio, head_q = head * a.ratio + row - i * a.ratio;
       const int64_t tk = seq.q0 + i;
       const float scale = sum == 0.f ? 0.f : 1.f / sum, power = pow2f(vexp);
-      char* dst = static_cast<char*>(a.out) + 2 * (tk * a.os + (int64_t)h * a.oh);
-#pragma unroll
+      char* dst = static_cast<char*>(a.out) + 2 * (tk * a.os + (int64_t)head_q * a.oh);
+#pragma unroll 1
       for (int g = 0; g < D / 32; ++g) {
         uint32_t v[32] = {};
         if (n > 0) {
@@ -337,25 +361,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
           tc::wait_ld();
         }
         if (r < live) {
-          float o[32];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = sum == 0.f ? 0.f : __uint_as_float(v[k]) * scale * power;
+          for (int k = 0; k < 32; ++k) v[k] = sum == 0.f ? 0u : __float_as_uint(__uint_as_float(v[k]) * scale * power);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // columns 0 .. 7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
-            const float* q = o + 8 * k;
-            const uint2 w0 = make_uint2(pack2(q[0], q[2], a.bf16), pack2(q[4], q[6], a.bf16));
-            const uint2 w1 = make_uint2(pack2(q[1], q[3], a.bf16), pack2(q[5], q[7], a.bf16));
-            *reinterpret_cast<uint2*>(dst + 2 * (32 * g + 8 * k)) = w0;
-            *reinterpret_cast<uint2*>(dst + 2 * (32 * g + 8 * k + 4)) = w1;
+            auto two = [&](int x, int y) { return pack2(__uint_as_float(v[8 * k + x]), __uint_as_float(v[8 * k + y]), a.bf16); };
+            *reinterpret_cast<uint2*>(dst + 2 * (32 * g + 8 * k)) = make_uint2(two(0, 2), two(4, 6));
+            *reinterpret_cast<uint2*>(dst + 2 * (32 * g + 8 * k + 4)) = make_uint2(two(1, 3), two(5, 7));
           }
         }
       }
-      if (a.lse && r < live) a.lse[tk * a.ls + h] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+      if (a.lse && r < live) a.lse[tk * a.ls + head_q] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
     }
   } else if (warp < kMmaWarp) {
-    // ---------------- cache: nibbles and scales to f16 ----------------
-    const int w = warp - kCacheWarp, tid = threadIdx.x - 32 * kCacheWarp, groups = a.groups;
-    __half* sc = reinterpret_cast<__half*>(smem + C::kScale);
+    // ---------------- cache: nibbles and scales to f16; group z: 0 K, 1 V ----------------
+    const int z = (warp - kCacheWarp) >> 2, w = warp & 3, tid = threadIdx.x & 127, groups = a.groups;
+    const uint8_t* nibbles = z ? a.v4 : a.k4;
+    const __half* scales = z ? a.v_scale : a.k_scale;
+    __half* sc = reinterpret_cast<__half*>(smem + C::kScale) + z * kTok * CH;
     const int32_t* pages = a.table + (int64_t)b * a.table_stride;
     const int in_page = (1 << a.page_log2) - 1, cpg_log2 = 31 - __clz(a.cpg);  // 1, 2 or 4 chunks a group
     auto page_of = [&](int t) {
@@ -365,36 +388,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       return p >= 0 && (int64_t)p < a.pages ? p : -1;
     };
     // a tile's nibbles: unit u = lane / 8 + 4 i of this warp's 32 tokens is run u / CH (8 tokens, lane % 8), chunk u % CH
-    uint4 rk[CH], rv[CH];
-    uint16_t sk[CH], sv[CH];  // this thread's token's scales (one a group)
+    uint4 raw[CH];
+    uint16_t sk[CH];  // this thread's token's scales (one a group)
     const uint32_t page_lines = (uint32_t)a.kv_heads << a.page_log2, head_line = (uint32_t)head << a.page_log2;
     // a token that does not exist reads line 0's bytes: its scales are zero
-    auto fetch = [&](const uint8_t* src, int t, int page, uint4 (&raw)[CH]) {
+    auto fetch = [&](int t, int page) {
       const int pg = max(page, 0), at = (tok0 + t * kTok + 32 * w) & in_page;  // a run of 8 is on one page
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int u = (lane >> 3) + 4 * i, run = u / CH, c = u - run * CH;
         const int64_t ln = (int64_t)(uint32_t)__shfl_sync(0xffffffffu, pg, 8 * run) * page_lines +
                            (head_line + ((at + 8 * run) & in_page) + (lane & 7));
-        raw[i] = ld_nc_na_v4(src + ln * (D / 2) + 16 * c);
+        raw[i] = ld_nc_na_v4(nibbles + ln * (D / 2) + 16 * c);
       }
     };
     auto fetch_scales = [&](int t, int page) {
       const int64_t line = (int64_t)(uint32_t)max(page, 0) * page_lines + (head_line + ((tok0 + t * kTok + tid) & in_page));
 #pragma unroll
       for (int g = 0; g < CH; ++g) {
-        sk[g] = sv[g] = 0;
-        if (g < groups && page >= 0) {
-          sk[g] = __half_as_ushort(a.k_scale[line * groups + g]);
-          sv[g] = __half_as_ushort(a.v_scale[line * groups + g]);
-        }
+        sk[g] = 0;
+        if (g < groups && page >= 0) sk[g] = __half_as_ushort(__ldg(scales + line * groups + g));
       }
     };
-    auto convert = [&](const uint4 (&raw)[CH], const __half* scale, uint32_t dst) {
+    auto convert = [&](uint32_t dst) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int u = (lane >> 3) + 4 * i, run = u / CH, c = u - run * CH, tok = 32 * w + 8 * run + (lane & 7);
-        const __half2 s = __half2half2(scale[tok * groups + (c >> cpg_log2)]);
+        const __half2 s = __half2half2(sc[tok * groups + (c >> cpg_log2)]);
         const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
         const uint32_t at = dst + (c / 2) * kBlockBytes + tok * 128;
 #pragma unroll
@@ -402,9 +422,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
           uint32_t e[4];
           expand(words[k], e);
 #pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&e[z]), s);
-            e[z] = *reinterpret_cast<const uint32_t*>(&v);
+          for (int x = 0; x < 4; ++x) {
+            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&e[x]), s);
+            e[x] = *reinterpret_cast<const uint32_t*>(&v);
           }
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + ((((c & 1) * 4 + k) ^ (tok & 7)) << 4)),
                        "r"(e[0]), "r"(e[1]), "r"(e[2]), "r"(e[3])
@@ -415,128 +435,109 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     int page = page_of(0);
     if (n > 0) {
       fetch_scales(0, page);
-      fetch(a.k4, 0, page, rk);
-      fetch(a.v4, 0, page, rv);
+      fetch(0, page);
     }
     for (int t = 0; t < n; ++t) {
-      // the tile's powers of two, and its scales divided by them
-      uint32_t bk = 0, bv = 0;
+      const int next = page_of(t + 1);
+      // the tile's power of two, and its scales divided by it
+      uint32_t big = 0;
       bool bad = false;
 #pragma unroll
       for (int g = 0; g < CH; ++g) {
-        const uint32_t mk = sk[g] & 0x7fffu, mv = sv[g] & 0x7fffu;
-        if (mk < 0x7c00u) bk = max(bk, mk);
-        if (mv < 0x7c00u) bv = max(bv, mv);
-        bad |= mv >= 0x7c00u;
+        const uint32_t m = sk[g] & 0x7fffu;
+        if (m < 0x7c00u) big = max(big, m);
+        bad |= m >= 0x7c00u;
       }
-      bk = __reduce_max_sync(0xffffffffu, bk);
-      bv = __reduce_max_sync(0xffffffffu, bv);
+      big = __reduce_max_sync(0xffffffffu, big);
       Meta& meta = sh.meta[t & 3];
-      const int next = page_of(t + 1);
-      const uint32_t valid = __ballot_sync(0xffffffffu, page >= 0), bads = __ballot_sync(0xffffffffu, bad);
+      const uint32_t marks = __ballot_sync(0xffffffffu, z ? bad : page >= 0);
       if (lane == 0) {
-        sh.big[0][w] = bk;
-        sh.big[1][w] = bv;
-        meta.valid[w] = valid;
-        meta.bad[w] = bads;
+        sh.big[z][w] = big;
+        (z ? meta.bad : meta.valid)[w] = marks;
       }
-      cache_sync();  // also: every warp is done with the last tile's scales
-      bk = max(max(sh.big[0][0], sh.big[0][1]), max(sh.big[0][2], sh.big[0][3]));
-      bv = max(max(sh.big[1][0], sh.big[1][1]), max(sh.big[1][2], sh.big[1][3]));
-      auto exponent = [](uint32_t bits) {
-        return bits ? (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)bits))) >> 23) - 127 : -24;
-      };
-      const int ke = exponent(bk), ve = exponent(bv);
+      cache_sync(z);  // also: every warp is done with the last tile's scales
+      big = max(max(sh.big[z][0], sh.big[z][1]), max(sh.big[z][2], sh.big[z][3]));
+      const int e = big ? (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)big))) >> 23) - 127 : -24;
 #pragma unroll
       for (int g = 0; g < CH; ++g)
-        if (g < groups) {
-          sc[tid * groups + g] = __float2half_rn(__half2float(__ushort_as_half(sk[g])) * pow2f(-ke));
-          sc[kTok * CH + tid * groups + g] =
-              (sv[g] & 0x7fffu) < 0x7c00u ? __float2half_rn(__half2float(__ushort_as_half(sv[g])) * pow2f(-ve)) : __half(0);
-        }
-      if (tid == 0) {
-        meta.k_exp = ke;
-        meta.v_exp = ve;
-      }
-      cache_sync();
-      const int s = t & 1;
-      const uint32_t ph = ((t >> 1) & 1) ^ 1;
-      page = next;  // from here on the next tile's: loaded as soon as registers are free
+        if (g < groups)  // a value that is not finite is left out (its token is marked); such a key makes its logit NaN
+          sc[tid * groups + g] = z && (sk[g] & 0x7fffu) >= 0x7c00u
+                                     ? __half(0)
+                                     : __float2half_rn(__half2float(__ushort_as_half(sk[g])) * pow2f(-e));
+      if (tid == 0) (z ? meta.v_exp : meta.k_exp) = e;
+      cache_sync(z);
+      page = next;
       if (t + 1 < n) fetch_scales(t + 1, page);
-      bool ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.k_empty[s], ph, wait_ns, abort_flag));
-      if (ok) {
-        convert(rk, sc, sbase + C::kK + s * C::kTile);
+      const int s = t & 1;
+      if (__all_sync(0xffffffffu, tc::mbar_wait(&sh.empty[z][s], ((t >> 1) & 1) ^ 1, wait_ns, abort_flag))) {
+        convert(sbase + (z ? C::kV : C::kK) + s * C::kTile);
         tc::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sh.k_full[s]);
-        if (t + 1 < n) fetch(a.k4, t + 1, page, rk);
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.v_empty[s], ph, wait_ns, abort_flag));
-      }
-      if (ok) {
-        convert(rv, sc + kTok * CH, sbase + C::kV + s * C::kTile);
-        tc::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sh.v_full[s]);
-        if (t + 1 < n) fetch(a.v4, t + 1, page, rv);
+        if (lane == 0) tc::mbar_arrive(&sh.full[z][s]);
+        if (t + 1 < n) fetch(t + 1, page);
       } else {
         give_up();  // the named barrier still counts this warp: it keeps step with the others, without the work
       }
     }
-  } else if (lane == 0 && n > 0) {
+  } else {
     // ---------------- products of query tile w ----------------
-    constexpr uint32_t id_qk = idesc_f16(128, kHalf, false), id_pv = idesc_f16(128, D, true);
-    const int w = warp - kMmaWarp;
-    const uint32_t ts = tmem + C::kS + w * kTok, to = tmem + C::kO + w * D;
-    // descriptors of the first step; a step further adds its bytes / 16 to the address field
-    const uint64_t q0 = tc::sdesc_kmajor_sw128(sbase + C::kQ + w * C::kTile);
-    const uint64_t k0 = tc::sdesc_kmajor_sw128(sbase + C::kK), v0 = desc_v(sbase + C::kV);
-    auto qk = [&](int t, int h) {
-      const uint64_t k = k0 + (uint64_t)((t & 1) * (C::kTile >> 4) + h * (kHalf * 128 >> 4));
+    if (n > 0) {
+      constexpr uint32_t id_qk = idesc_f16(128, kHalf, false), id_pv = idesc_f16(128, D, true);
+      const int w = warp - kMmaWarp;
+      // descriptors of the first step; a step further adds its bytes / 16 to the address field
+      const uint64_t q0 = tc::sdesc_kmajor_sw128(sbase + C::kQ + w * C::kTile);
+      const uint64_t k0 = tc::sdesc_kmajor_sw128(sbase + C::kK), v0 = desc_v(sbase + C::kV);
+      const uint32_t ts = tmem + C::kS + w * kTok, to = tmem + C::kO + w * D;
+      auto wait = [&](uint64_t* bar, int parity) {
+        return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity & 1, wait_ns, abort_flag)) != 0;
+      };
+      auto qk = [&](int t, int h) {
+        const uint64_t k = k0 + (uint64_t)((t & 1) * (C::kTile >> 4) + h * (kHalf * 128 >> 4));
+        if (elect_one()) {
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {  // 16 dimensions: 32 bytes
-        const uint64_t at = (uint64_t)((i / 4) * (kBlockBytes >> 4) + (i % 4) * 2);
-        tc::mma_ss_bf16(ts + h * kHalf, q0 + at, k + at, id_qk, i > 0);
+          for (int i = 0; i < D / 16; ++i) {  // 16 dimensions: 32 bytes
+            const uint64_t at = (uint64_t)((i / 4) * (kBlockBytes >> 4) + (i % 4) * 2);
+            mma_ss(ts + h * kHalf, q0 + at, k + at, id_qk, i > 0);
+          }
+          tc::mbar_arrive(&sh.s_full[w][h]);
+          tc::commit(&sh.s_full[w][h]);
+          if (h == 1) tc::commit(&sh.empty[0][t & 1]);
+        }
+        __syncwarp();
+      };
+      // a tile's K and V are waited for together: its meta has both groups' part
+      auto cached = [&](int t) { return wait(&sh.full[0][t & 1], t >> 1) && wait(&sh.full[1][t & 1], t >> 1); };
+      bool ok = cached(0);
+      if (ok) {
+        tc::fence_after_sync();
+        qk(0, 0);
+        qk(0, 1);
       }
-    };
-    auto pv = [&](int t, int h) {
-      const uint64_t v = v0 + (uint64_t)((t & 1) * (C::kTile >> 4) + h * (kHalf * 128 >> 4));
-#pragma unroll
-      for (int i = 0; i < kHalf / 16; ++i)  // 16 tokens: 2048 bytes
-        tc::mma_ts_bf16(to, ts + h * kHalf + 8 * i, v + (uint64_t)(i * 128), id_pv, t + h + i > 0);
-    };
-    bool ok = tc::mbar_wait(&sh.k_full[0], 0, wait_ns, abort_flag);
-    if (ok) {
-      tc::fence_after_sync();
-      for (int h = 0; h < 2; ++h) {
-        tc::mbar_arrive(&sh.s_full[w][h]);
-        qk(0, h);
-        tc::commit(&sh.s_full[w][h]);
-      }
-      tc::commit(&sh.k_empty[0]);
-    }
-    for (int t = 0; ok && t < n; ++t) {
-      ok = tc::mbar_wait(&sh.v_full[t & 1], (t >> 1) & 1, wait_ns, abort_flag);
-      for (int h = 0; ok && h < 2; ++h) {
-        ok = tc::mbar_wait(&sh.p_full[w][h], t & 1, wait_ns, abort_flag);
+#pragma unroll 1
+      for (int u = 0; ok && u < 2 * n; ++u) {
+        const int t = u >> 1, h = u & 1;
+        ok = wait(&sh.p_full[w][h], t);
         if (!ok) break;
         tc::fence_after_sync();
-        pv(t, h);
-        tc::commit(&sh.pv_done[w]);
-        if (h == 1) tc::commit(&sh.v_empty[t & 1]);
-        if (t + 1 < n) {
-          if (h == 0) ok = tc::mbar_wait(&sh.k_full[(t + 1) & 1], ((t + 1) >> 1) & 1, wait_ns, abort_flag);
-          if (!ok) break;
-          tc::fence_after_sync();
-          tc::mbar_arrive(&sh.s_full[w][h]);
-          qk(t + 1, h);  // over S and P of tile t's half: issued after pv(t, h), which reads them
-          tc::commit(&sh.s_full[w][h]);
-          if (h == 1) tc::commit(&sh.k_empty[(t + 1) & 1]);
+        const uint64_t v = v0 + (uint64_t)((t & 1) * (C::kTile >> 4) + h * (kHalf * 128 >> 4));
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < kHalf / 16; ++i)  // 16 tokens: 2048 bytes
+            mma_ts(to, ts + h * kHalf + 8 * i, v + (uint64_t)(i * 128), id_pv, u + i > 0);
+          tc::commit(&sh.pv_done[w]);
+          if (h == 1) tc::commit(&sh.empty[1][t & 1]);
         }
+        __syncwarp();
+        if (t + 1 == n) continue;
+        if (h == 0) ok = cached(t + 1);
+        if (!ok) break;
+        tc::fence_after_sync();
+        qk(t + 1, h);  // over S and P of tile t's half: issued after the products that read them
       }
+      if (!ok) give_up();
+      if (elect_one()) tc::commit(&sh.drain);  // nothing may be in flight when the tensor memory goes
+      if (!tc::mbar_wait(&sh.drain, 0, wait_ns, nullptr)) give_up();
     }
-    if (!ok) give_up();
-    tc::commit(&sh.drain);  // nothing may be in flight when the tensor memory goes
-    if (!tc::mbar_wait(&sh.drain, 0, wait_ns, nullptr)) give_up();
   }
   tc::fence_before_sync();
   __syncthreads();
