@@ -59,7 +59,7 @@ struct Meta {          // what the cache warps say of a tile of tokens
 
 struct Shared {
   uint64_t full[2][2], empty[2][2];  // [K, V][stage]
-  uint64_t s_full[2][2], p_full[2][2], pv_done[2], drain;  // [query tile][half]
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], all_done[2], drain;  // [query tile][half]
   uint32_t tmem;
   int abort;
   Meta meta[4];
@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         tc::mbar_init(&sh.p_full[i][h], 4);  // the tile's warps
       }
       tc::mbar_init(&sh.pv_done[i], 1);
+      tc::mbar_init(&sh.all_done[i], 1);
     }
     tc::mbar_init(&sh.drain, 2);
     tc::mbar_fence_init();
@@ -199,18 +200,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
   const int tok0 = lo / kTok * kTok, n = hi > tok0 ? (hi - tok0 + kTok - 1) / kTok : 0;
 
   // ---- queries: f16 with a power of two a row, swizzled ----
-  constexpr int LPR = D / 8;  // lanes a row
-  for (int r = warp * (32 / LPR) + lane / LPR; r < kRowsCta; r += kThreads / LPR) {
-    const int c = lane % LPR, row = row0 + r, i = row / a.ratio;
-    float f[8] = {};
+  constexpr int LPR = D / 8, STEP = kThreads / LPR;  // lanes a row, rows at a time
+  constexpr int QN = (kRowsCta + STEP - 1) / STEP;
+  uint4 qraw[QN];  // every load before the first use
+#pragma unroll
+  for (int k = 0; k < QN; ++k) {
+    const int r = threadIdx.x / LPR + k * STEP, row = row0 + r, i = row / a.ratio;
+    qraw[k] = make_uint4(0, 0, 0, 0);
     if (r < live)
-      unpack8(__ldg(reinterpret_cast<const uint4*>(
-                  static_cast<const char*>(a.q) +
-                  2 * ((seq.q0 + i) * a.qs + (int64_t)(head * a.ratio + row - i * a.ratio) * a.qh + 8 * c))),
-              a.bf16, f);
+      qraw[k] = __ldg(reinterpret_cast<const uint4*>(
+          static_cast<const char*>(a.q) +
+          2 * ((seq.q0 + i) * a.qs + (int64_t)(head * a.ratio + row - i * a.ratio) * a.qh + 8 * (threadIdx.x % LPR))));
+  }
+#pragma unroll
+  for (int k = 0; k < QN; ++k) {
+    const int r = threadIdx.x / LPR + k * STEP, c = threadIdx.x % LPR;
+    if (r >= kRowsCta) break;  // a warp's rows are all in or all out
+    float f[8];
+    unpack8(qraw[k], a.bf16, f);
     float big = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) big = fmaxf(big, fabsf(f[k]));
+    for (int x = 0; x < 8; ++x) big = fmaxf(big, fabsf(f[x]));
 #pragma unroll
     for (int d = 1; d < LPR; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d, LPR));
     const int ex = (int)(__float_as_uint(big) >> 23) - 127;  // the row's largest magnitude becomes 2^7 .. 2^8
@@ -223,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
                               ((c % 8) ^ (r & 7)) * 16) = w;
     if (c == 0) sh.row_scale[r] = a.scale_log2 * pow2f(-up);
   }
+  static_assert(kThreads % LPR == 0 && kRowsCta % (32 / LPR) == 0, "whole rows a warp");
   tc::fence_proxy_async_smem();
   tc::fence_before_sync();
   __syncthreads();
@@ -246,6 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     float mx = kNoMax, sum = 0.f;
     int vexp = -24;
     bool ok = true;
+    const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (uint64_t)(2 * (a.os | a.oh))) & 15) == 0;  // 16-byte stores
     auto wait = [&](uint64_t* bar, int parity) {
       return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity & 1, wait_ns, abort_flag)) != 0;
     };
@@ -297,6 +309,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         mx = m;
         vexp = e;
         if (u > 0) {
+          // Phases are told apart by parity. PV of half u - 2 is done (S of half u was issued after it) and PV of half u
+          // waits for this warp, so the barrier is in the phase asked for or just past it.
           ok = wait(&sh.pv_done[w], u - 1);
           if (!ok) break;
           tc::fence_after_sync();
@@ -342,17 +356,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&sh.p_full[w][h]);
     }
-    // A wait tells phases apart by parity, so it may be one behind at most: S of half u says that PV of half u - 2 is done
-    // (it was issued before), and the last two are waited for in turn.
-    if (ok && n > 0) ok = wait(&sh.pv_done[w], 0) && wait(&sh.pv_done[w], 1);
+    if (ok && n > 0) ok = wait(&sh.all_done[w], 0);
     if (!ok) {
       give_up();
     } else {
       tc::fence_after_sync();
-      const int i = row / a.ratio, head_q = head * a.ratio + row - i * a.ratio;
-      const int64_t tk = seq.q0 + i;
+      // the row, rounded, into the warp's part of the query tile (its products are done), then out in whole rows
       const float scale = sum == 0.f ? 0.f : 1.f / sum, power = pow2f(vexp);
-      char* dst = static_cast<char*>(a.out) + 2 * (tk * a.os + (int64_t)head_q * a.oh);
+      uint8_t* tile_rows = smem + C::kQ + w * C::kTile;
 #pragma unroll 1
       for (int g = 0; g < D / 32; ++g) {
         uint32_t v[32] = {};
@@ -360,17 +371,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
           ld_x32(to + 32 * g, v);
           tc::wait_ld();
         }
-        if (r < live) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] = sum == 0.f ? 0u : __float_as_uint(__uint_as_float(v[k]) * scale * power);
+        for (int k = 0; k < 32; ++k) v[k] = sum == 0.f ? 0u : __float_as_uint(__uint_as_float(v[k]) * scale * power);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {  // columns 0 .. 7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
-            auto two = [&](int x, int y) { return pack2(__uint_as_float(v[8 * k + x]), __uint_as_float(v[8 * k + y]), a.bf16); };
-            *reinterpret_cast<uint2*>(dst + 2 * (32 * g + 8 * k)) = make_uint2(two(0, 2), two(4, 6));
-            *reinterpret_cast<uint2*>(dst + 2 * (32 * g + 8 * k + 4)) = make_uint2(two(1, 3), two(5, 7));
-          }
+        for (int k = 0; k < 4; ++k) {  // columns 0 .. 7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
+          auto two = [&](int x, int y) { return pack2(__uint_as_float(v[8 * k + x]), __uint_as_float(v[8 * k + y]), a.bf16); };
+          const int c = 4 * g + k;  // 16 bytes: 8 dimensions
+          *reinterpret_cast<uint4*>(tile_rows + (c / 8) * kBlockBytes + (r % 128) * 128 + ((c % 8) ^ (r & 7)) * 16) =
+              make_uint4(two(0, 2), two(4, 6), two(1, 3), two(5, 7));
         }
       }
+      __syncwarp();
+#pragma unroll 1
+      for (int k = 0; k < LPR; ++k) {  // 32 / LPR rows at a time
+        const int rr = (r & ~31) + k * (32 / LPR) + lane / LPR, c = lane % LPR, out_row = row0 + rr, i = out_row / a.ratio;
+        if (rr >= live) break;
+        const uint4 v = *reinterpret_cast<const uint4*>(tile_rows + (c / 8) * kBlockBytes + (rr % 128) * 128 +
+                                                        ((c % 8) ^ (rr & 7)) * 16);
+        char* dst = static_cast<char*>(a.out) +
+                    2 * ((seq.q0 + i) * a.os + (int64_t)(head * a.ratio + out_row - i * a.ratio) * a.oh + 8 * c);
+        if (wide) {
+          *reinterpret_cast<uint4*>(dst) = v;
+        } else {
+          *reinterpret_cast<uint2*>(dst) = make_uint2(v.x, v.y);
+          *reinterpret_cast<uint2*>(dst + 8) = make_uint2(v.z, v.w);
+        }
+      }
+      const int i = row / a.ratio, head_q = head * a.ratio + row - i * a.ratio;
+      const int64_t tk = seq.q0 + i;
       if (a.lse && r < live) a.lse[tk * a.ls + head_q] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
     }
   } else if (warp < kMmaWarp) {
@@ -525,6 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
           for (int i = 0; i < kHalf / 16; ++i)  // 16 tokens: 2048 bytes
             mma_ts(to, ts + h * kHalf + 8 * i, v + (uint64_t)(i * 128), id_pv, u + i > 0);
           tc::commit(&sh.pv_done[w]);
+          if (u + 1 == 2 * n) tc::commit(&sh.all_done[w]);
           if (h == 1) tc::commit(&sh.empty[1][t & 1]);
         }
         __syncwarp();
