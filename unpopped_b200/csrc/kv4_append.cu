@@ -9,10 +9,14 @@
 //
 // What bounds it: HBM. q, k and v are read once, q is written once, and a cached row takes dim / 2 + 2 dim / group bytes.
 //
-// A thread owns two 16-byte chunks (8 dimensions each) of a row, so that each rotated pair is in one thread: chunks j
-// and rot / 16 + j of the half layout, two neighbours otherwise. dim / 16 threads make a row, and a block takes as many
-// whole rows as fit into 256 threads. A chunk's magnitude goes through shared memory: groups need not fall on a warp's
-// lanes (dim 96 has 6 threads a row), and a group's maximum is then group / 32 16-byte reads.
+// Some blocks turn the queries as rope.cu does, the others take the rows of keys and values; they alternate over the grid,
+// so that the queries' traffic fills the time in which the other rows wait for their slots, positions and scales. A row of
+// keys or values is dim / 16 threads, and a block takes as many whole rows as fit into 256. A thread owns two 16-byte
+// chunks (8 dimensions each) of its row, so that each rotated pair is in one thread: chunks j and rot / 16 + j of the half
+// layout, two neighbours otherwise. A chunk's magnitude goes through shared memory: groups need not fall on a warp's lanes
+// (dim 96 has 6 threads a row), and a group's maximum is then group / 32 16-byte reads.
+// Four rows a thread, loaded together, measured slower (231 us against 159 us for 16001 tokens of 64 and 8 heads, both with
+// an earlier form of the queries' part): the registers that they take halve the queries' blocks on an SM.
 #include "kv4.cuh"
 #include "rope.cuh"
 
@@ -32,9 +36,10 @@ struct Append {
   int slot_dtype;
   const float* table;
   int64_t n_pos;
-  int rot, half, page_log2, dim, group;
+  int rot, half, page_log2, dim, group, groups;
   uint8_t *k4, *v4;
   __half *k_scale, *v_scale;
+  Divide32 by_tpr, by_heads, by_per;  // threads a row, rows a token, chunks a group
 };
 
 // The 8 elements at dimension e of a row, in f32. VEC: 16-byte aligned.
@@ -47,6 +52,13 @@ __device__ __forceinline__ void load8(const T* row, int e, float (&f)[8]) {
     for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(row[e + i]);
   }
 }
+
+// How the blocks that turn queries and those that take rows of keys and values alternate: `few` of the rarer kind, the
+// last of each of the first `few` runs of `period` blocks.
+struct Mix {
+  uint32_t few, period;
+  int few_are_queries;
+};
 
 // The rotated 8 elements at dimension e, whatever the pairs' other elements' place: each pair is computed from the row.
 template <typename T>
@@ -73,32 +85,50 @@ __device__ __forceinline__ uint32_t magnitude8(const float (&f)[8]) {  // as bit
   return m;
 }
 
-template <typename T, bool VEC>
+// VEC: blocks of queries (items of rope_item, HEADS heads each) and of rows. Else (rows or rotations that are not whole
+// 16-byte chunks) every block takes rows, and the queries are rows like the others.
+template <typename T, bool VEC, int HEADS>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const T* q, const T* __restrict__ k,
-                                                              const T* __restrict__ v, T* q_out, const Append a) {
+                                                              const T* __restrict__ v, T* q_out, const Append a,
+                                                              const Geometry g, const Mix mix,
+                                                              const Items<Divide32> n) {
+  uint32_t block = blockIdx.x;
+  if (VEC) {
+    const uint32_t run = block / mix.period;  // runs before this block
+    const bool rare = run < mix.few && block - run * mix.period == mix.period - 1;
+    block = rare ? run : block - min(run, mix.few);
+    if (rare == (mix.few_are_queries != 0)) {
+      const uint32_t item = block * kThreads + threadIdx.x;
+      if (item < n.count) {
+        if (a.half) rope_item<T, true, HEADS, Divide32>(q, q_out, a.table, g, item, n, 0);
+        else rope_item<T, false, HEADS, Divide32>(q, q_out, a.table, g, item, n, 0);
+      }
+      return;
+    }
+  }
   // the chunks' magnitudes of this block's rows: two chunks a thread
   __shared__ alignas(16) uint32_t mag[2 * kThreads];
   const int tpr = a.dim / 16, rows_per_block = kThreads / tpr;
-  const int r = threadIdx.x / tpr, u = threadIdx.x - r * tpr;
-  const uint32_t heads = (uint32_t)(a.q_heads + 2 * a.kv_heads);  // the launch keeps tokens * heads below 2^31
-  const uint32_t row = blockIdx.x * (uint32_t)rows_per_block + r;
-  const int64_t tok = row / heads, head = row % heads;
+  const int r = (int)a.by_tpr(threadIdx.x), u = (int)threadIdx.x - r * tpr;
+  const uint32_t q_heads = VEC ? 0u : (uint32_t)a.q_heads, kv_heads = (uint32_t)a.kv_heads;
+  const uint32_t heads = q_heads + 2 * kv_heads;  // the launch keeps tokens * heads below 2^31
+  const uint32_t row = block * (uint32_t)rows_per_block + r;
+  const uint32_t tok = a.by_heads(row), head = row - tok * heads;
   const bool live = r < rows_per_block && tok < a.tokens;
-  const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + a.kv_heads;
-  int64_t slot = -1;
-  if (live && !is_q) {
-    slot = load_id(a.slots, a.slot_dtype, tok);
-    if (slot >= (a.pages << a.page_log2)) slot = -1;  // left out, like a negative one
-  }
-  const bool work = live && (is_q || slot >= 0);
+  const bool is_q = !VEC && head < q_heads, is_v = head >= q_heads + kv_heads;
   const int pairs = VEC && a.half ? a.rot / 16 : 0;  // half-layout pairs of chunks come first
   const int c0 = u < pairs ? u : 2 * u, c1 = u < pairs ? u + pairs : 2 * u + 1;
   float x[2][8];
-  const int64_t h = is_q ? head : is_v ? head - a.q_heads - a.kv_heads : head - a.q_heads;
-  if (work) {
+  int64_t slot = -1;
+  const int64_t h = is_q ? head : is_v ? head - q_heads - kv_heads : head - q_heads;
+  if (live) {
     const T* src = is_q ? q + tok * a.qs + h * a.qh : is_v ? v + tok * a.vs + h * a.vh : k + tok * a.ks + h * a.kh;
     load8<T, VEC>(src, 8 * c0, x[0]);
     load8<T, VEC>(src, 8 * c1, x[1]);
+    if (!is_q) {
+      slot = load_id(a.slots, a.slot_dtype, tok);
+      if (slot >= (a.pages << a.page_log2)) slot = -1;  // left out, like a negative one
+    }
     if (!is_v && a.rot > 0) {
       const int64_t p = load_id(a.positions, a.pos_dtype, tok);
       const bool in = p >= 0 && p < a.n_pos;
@@ -142,66 +172,78 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(const T* q, const 
     }
   }
   __syncthreads();
-  if (!work) return;
+  if (!live || (!is_q && slot < 0)) return;
   if (is_q) {
     T* o = q_out + tok * a.qos + h * a.qoh;
 #pragma unroll
-    for (int z = 0; z < 2; ++z) {
-      const int e = 8 * (z ? c1 : c0);
-      if constexpr (VEC) {
-        st_cs_v4(o + e, Chunk<T>::pack(x[z]));
-      } else {
+    for (int z = 0; z < 2; ++z)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[e + i] = from_f32<T>(x[z][i]);
-      }
-    }
+      for (int i = 0; i < 8; ++i) o[8 * (z ? c1 : c0) + i] = from_f32<T>(x[z][i]);
     return;
   }
   // the row's place in the cache
   const int64_t page = slot >> a.page_log2, at = slot & (((int64_t)1 << a.page_log2) - 1);
   const int64_t line = (((page * a.kv_heads + h) << a.page_log2) + at);
-  const int groups = a.dim / a.group, per = a.group / 8;  // chunks a group
+  const int groups = a.groups, per = a.group / 8;  // chunks a group
   uint32_t* words = reinterpret_cast<uint32_t*>((is_v ? a.v4 : a.k4) + line * (a.dim / 2));
   __half* scales = (is_v ? a.v_scale : a.k_scale) + line * groups;
+  __half sc = __half(0);
+  float sf = 0.f, inv = 0.f;
+  int last = -1;
 #pragma unroll
   for (int z = 0; z < 2; ++z) {
-    const int c = z ? c1 : c0, g = c / per;
-    const uint4* m4 = reinterpret_cast<const uint4*>(mag + r * 2 * tpr + g * per);
-    uint32_t m = 0;
-    for (int i = 0; i < per / 4; ++i) {
-      const uint4 w = m4[i];
-      m = max(max(m, max(w.x, w.y)), max(w.z, w.w));
+    const int c = z ? c1 : c0, grp = (int)a.by_per((uint32_t)c);
+    if (grp != last) {
+      const uint4* m4 = reinterpret_cast<const uint4*>(mag + r * 2 * tpr + grp * per);
+      uint32_t m = 0;
+      for (int i = 0; i < per / 4; ++i) {
+        const uint4 w = m4[i];
+        m = max(max(m, max(w.x, w.y)), max(w.z, w.w));
+      }
+      sc = m >= 0x7f800000u ? __ushort_as_half(0x7fff)
+                            : __float2half_rn(fminf(__fmul_rn(__uint_as_float(m), 1.0f / 7.0f), 65504.0f));
+      sf = __half2float(sc);
+      inv = sf > 0.0f ? __fdiv_rn(1.0f, sf) : 0.0f;
+      last = grp;
     }
-    const float amax = __uint_as_float(m);
-    const __half sc = m >= 0x7f800000u ? __ushort_as_half(0x7fff)
-                                       : __float2half_rn(fminf(__fmul_rn(amax, 1.0f / 7.0f), 65504.0f));
-    const float sf = __half2float(sc);
-    const float inv = sf > 0.0f ? __fdiv_rn(1.0f, sf) : 0.0f;
     uint32_t w = 0;
+    if (sf > 0.0f)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float n = fminf(fmaxf(rintf(__fmul_rn(x[z][i], inv)), -8.0f), 7.0f);
-      w |= ((uint32_t)(sf > 0.0f ? (int)n : 0) & 15u) << (4 * i);
-    }
+      for (int i = 0; i < 8; ++i)
+        w |= ((uint32_t)(int)fminf(fmaxf(rintf(__fmul_rn(x[z][i], inv)), -8.0f), 7.0f) & 15u) << (4 * i);
     words[c] = w;
-    if (c == g * per) scales[g] = sc;
+    if (c == grp * per) scales[grp] = sc;
   }
 }
 
 template <typename T>
-int launch_append(const void* q, const void* k, const void* v, void* q_out, const Append& a, cudaStream_t s) {
+int launch_append(const void* q, const void* k, const void* v, void* q_out, Append a, const Geometry& g,
+                  cudaStream_t s) {
+  const bool strides = (a.ks | a.kh | a.vs | a.vh) % 8 == 0;
+  const bool vec = strides && aligned(k, 16) && aligned(v, 16) && a.rot % (a.half ? 16 : 8) == 0 && aligned(a.table, 16) &&
+                   (a.q_heads == 0 || rope_vector<T>(q, q_out, a.table, g, a.half));
+  const int64_t limit = 0x7fffffff - kThreads;  // rows, items and blocks are counted in 32 bits
+  const int64_t heads = (vec ? 0 : a.q_heads) + 2 * a.kv_heads;
+  const int per = rope_heads<T>(g, a.tokens, a.half);
+  const int64_t units = rope_units<T>(g, a.half), groups = (a.q_heads + per - 1) / per;
+  if (heads > limit || a.tokens > limit / heads) return UP_ERR_UNSUPPORTED;
+  if (a.q_heads > limit / units || a.tokens > limit / (a.q_heads > 0 ? a.q_heads * units : 1)) return UP_ERR_UNSUPPORTED;
+  a.by_heads = Divide32(heads);
   const int rows_per_block = kThreads / (a.dim / 16);
-  const int64_t heads = a.q_heads + 2 * a.kv_heads;
-  if (heads > 0x7fffffff || a.tokens > (0x7fffffff - kThreads) / heads) return UP_ERR_UNSUPPORTED;
-  const int64_t rows = a.tokens * heads, blocks = (rows + rows_per_block - 1) / rows_per_block;
-  const bool strides = (a.qs | a.qh | a.ks | a.kh | a.vs | a.vh | a.qos | a.qoh) % 8 == 0;
-  const bool bases = aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(q_out, 16) && aligned(a.table, 16);
-  if (strides && bases && a.rot % (a.half ? 16 : 8) == 0)
-    kv4_append_kernel<T, true><<<(int)blocks, kThreads, 0, s>>>(static_cast<const T*>(q), static_cast<const T*>(k),
-                                                                static_cast<const T*>(v), static_cast<T*>(q_out), a);
-  else
-    kv4_append_kernel<T, false><<<(int)blocks, kThreads, 0, s>>>(static_cast<const T*>(q), static_cast<const T*>(k),
-                                                                 static_cast<const T*>(v), static_cast<T*>(q_out), a);
+  const int64_t rows = a.tokens * heads, row_blocks = (rows + rows_per_block - 1) / rows_per_block;
+  const int64_t q_items = vec ? a.tokens * groups * units : 0, q_blocks = (q_items + kThreads - 1) / kThreads;
+  if (row_blocks + q_blocks > limit) return UP_ERR_UNSUPPORTED;
+  Mix mix;
+  mix.few_are_queries = q_blocks < row_blocks;
+  mix.few = (uint32_t)(mix.few_are_queries ? q_blocks : row_blocks);
+  mix.period = (uint32_t)(mix.few > 0 ? (q_blocks + row_blocks) / mix.few : 1);
+  const Items<Divide32> n{Divide32(units), Divide32(groups > 0 ? groups : 1), Divide32(a.tokens), (uint32_t)q_items};
+  const auto kernel = !vec       ? kv4_append_kernel<T, false, 1>
+                      : per == 4 ? kv4_append_kernel<T, true, 4>
+                      : per == 2 ? kv4_append_kernel<T, true, 2>
+                                 : kv4_append_kernel<T, true, 1>;
+  kernel<<<(unsigned)(row_blocks + q_blocks), kThreads, 0, s>>>(
+      static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), static_cast<T*>(q_out), a, g, mix, n);
   note_launch();
   return check_launch();
 }
@@ -245,11 +287,14 @@ extern "C" int up_sm100_kv4_append(const void* q, const void* k, const void* v, 
   a.positions = positions, a.pos_dtype = pos_dtype, a.slots = slots, a.slot_dtype = slot_dtype;
   a.table = table, a.n_pos = n_pos, a.rot = (int)rot, a.half = layout == UP_ROPE_HALF;
   a.page_log2 = log2_of(cache->page), a.dim = (int)cache->dim, a.group = (int)cache->group;
+  a.groups = (int)(cache->dim / cache->group), a.by_tpr = Divide32(cache->dim / 16), a.by_per = Divide32(cache->group / 8);
   a.k4 = static_cast<uint8_t*>(cache->k), a.v4 = static_cast<uint8_t*>(cache->v);
   a.k_scale = static_cast<__half*>(cache->k_scale), a.v_scale = static_cast<__half*>(cache->v_scale);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == UP_EK_BF16 ? launch_append<__nv_bfloat16>(q, k, v, q_out, a, s)
-                             : launch_append<__half>(q, k, v, q_out, a, s);
+  const Geometry g{tokens, q_heads, cache->dim, rot, 0, q_stride_t, q_stride_h, 0, q_out_stride_t, q_out_stride_h,
+                   positions, pos_dtype, 0, n_pos};
+  return dtype == UP_EK_BF16 ? launch_append<__nv_bfloat16>(q, k, v, q_out, a, g, s)
+                             : launch_append<__half>(q, k, v, q_out, a, g, s);
 }
 
 UP_DEFINE_REVISION(kv4_append)

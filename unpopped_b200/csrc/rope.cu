@@ -3,94 +3,24 @@
 // What bounds it: HBM. Every element of x is read once and written once (2 * size bytes) for 3 flops; the table rows
 // (4 * rot bytes a token, against heads * dim * size of x) are read again for each head, from L1.
 //
-// A thread owns 16-byte chunks whose pairs are complete: in the half layout chunk j of the first half and chunk j of
-// the second, in the interleaved one a single chunk. So a pair is rotated in one thread, nothing is exchanged, and a
-// row may be rotated in place. Consecutive threads take consecutive chunks of a head, then heads, then tokens.
+// A thread owns two 16-byte chunks whose pairs are complete: in the half layout chunk j of the first half and chunk j of
+// the second, in the interleaved one two neighbours. So a pair is rotated in one thread, nothing is exchanged, and a row
+// may be rotated in place. Consecutive threads take consecutive chunks of a head, then heads, then tokens.
 #include "rope.cuh"
+
+#include <type_traits>
 
 namespace up {
 namespace rp {
 
 constexpr int kThreads = 256;
 
-struct Geometry {
-  int64_t seq, heads, dim, rot;
-  int64_t xb, xs, xh, ob, os, oh;  // strides in elements: batch, token, head
-  const void* positions;           // NULL: a token's index in its sequence
-  int index_dtype;
-  int64_t pos_stride_b, n_pos;
-};
-
-__device__ __forceinline__ int64_t position(const Geometry& g, int64_t b, int64_t s) {
-  return g.positions ? load_id(g.positions, g.index_dtype, b * g.pos_stride_b + s) : s;
-}
-
-// U units a head: half layout rot / 2N pairs of chunks, then the (dim - rot) / N chunks that are only copied;
-// interleaved dim / N chunks. HEADS heads a thread (head, head + heads/HEADS rounded up, ...): their loads are in
-// flight together and share the row's cosines and sines.
-template <typename T, bool HALF, int HEADS, typename I>
-__global__ void __launch_bounds__(kThreads) rope_vec_kernel(const T* x, T* out,
-                                                            const float* __restrict__ table, const Geometry g,
-                                                            I items, I units, I head_groups, int backward) {
-  constexpr int N = Chunk<T>::N;
+template <typename T, bool HALF, int HEADS, typename Div>
+__global__ void __launch_bounds__(kThreads) rope_vec_kernel(const T* x, T* out, const float* __restrict__ table,
+                                                            const Geometry g, const Items<Div> n, int backward) {
+  using I = typename Div::Int;
   const I item = (I)blockIdx.x * kThreads + threadIdx.x;
-  if (item >= items) return;
-  const I row = item / units, u = item - row * units;
-  const I tok = row / head_groups, hg = row - tok * head_groups;
-  const I b = tok / (I)g.seq, s = tok - b * (I)g.seq;
-  const I pairs = HALF ? (I)(g.rot / (2 * N)) : (I)(g.rot / N);
-  const bool turn = u < pairs;
-  const int64_t e0 = turn || !HALF ? (int64_t)u * N : g.rot + (int64_t)(u - pairs) * N;
-  const int64_t e1 = e0 + g.rot / 2;  // the other chunk of a half-layout pair
-  const T* xr = x + b * g.xb + s * g.xs;
-  T* orow = out + b * g.ob + s * g.os;
-  uint4 lo[HEADS], hi[HEADS];
-#pragma unroll
-  for (int k = 0; k < HEADS; ++k) {
-    const I h = hg + (I)k * head_groups;
-    if (h >= (I)g.heads) continue;
-    lo[k] = *reinterpret_cast<const uint4*>(xr + h * g.xh + e0);
-    if (HALF && turn) hi[k] = *reinterpret_cast<const uint4*>(xr + h * g.xh + e1);
-  }
-  constexpr int C = HALF ? N : N / 2;  // cosines a unit needs
-  float c[C], sn[C];
-  if (turn) {
-    const int64_t p = position(g, b, s);
-    if (p >= 0 && p < g.n_pos) {
-      const float* t = table + p * g.rot + (HALF ? e0 : e0 / 2);
-      load_row<C>(t, c);
-      load_row<C>(t + g.rot / 2, sn);
-    } else {
-#pragma unroll
-      for (int i = 0; i < C; ++i) c[i] = sn[i] = __int_as_float(0x7fffffff);
-    }
-    if (backward)
-#pragma unroll
-      for (int i = 0; i < C; ++i) sn[i] = -sn[i];
-  }
-#pragma unroll
-  for (int k = 0; k < HEADS; ++k) {
-    const I h = hg + (I)k * head_groups;
-    if (h >= (I)g.heads) continue;
-    T* o = orow + h * g.oh;
-    if (!turn) {
-      st_cs_v4(o + e0, lo[k]);
-    } else if constexpr (HALF) {
-      float a[N], d[N];
-      Chunk<T>::unpack(lo[k], a);
-      Chunk<T>::unpack(hi[k], d);
-#pragma unroll
-      for (int i = 0; i < N; ++i) rotate(a[i], d[i], c[i], sn[i]);
-      st_cs_v4(o + e0, Chunk<T>::pack(a));
-      st_cs_v4(o + e1, Chunk<T>::pack(d));
-    } else {
-      float a[N];
-      Chunk<T>::unpack(lo[k], a);
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) rotate(a[2 * i], a[2 * i + 1], c[i], sn[i]);
-      st_cs_v4(o + e0, Chunk<T>::pack(a));
-    }
-  }
+  if (item < n.count) rope_item<T, HALF, HEADS, Div>(x, out, table, g, item, n, backward);
 }
 
 // Any even rot, stride and alignment: a thread per pair, then per copied element.
@@ -126,19 +56,18 @@ __global__ void __launch_bounds__(kThreads) rope_any_kernel(const T* x, T* out, 
 template <typename T, bool HALF, int HEADS>
 int launch_vec(const void* x, void* out, const float* table, const Geometry& g, int64_t tokens, int backward,
                cudaStream_t s) {
-  constexpr int N = Chunk<T>::N;
-  const int64_t units = HALF ? g.rot / (2 * N) + (g.dim - g.rot) / N : g.dim / N;
-  const int64_t hgs = (g.heads + HEADS - 1) / HEADS;
-  const int64_t items = tokens * hgs * units, blocks = (items + kThreads - 1) / kThreads;
+  const int64_t units = rope_units<T>(g, HALF), groups = (g.heads + HEADS - 1) / HEADS;
+  const int64_t items = tokens * groups * units, blocks = (items + kThreads - 1) / kThreads;
   if (blocks > 0x7fffffff) return UP_ERR_UNSUPPORTED;
-  if (items + kThreads <= 0x7fffffff && tokens * g.heads <= 0x7fffffff)
-    rope_vec_kernel<T, HALF, HEADS, uint32_t><<<(int)blocks, kThreads, 0, s>>>(
-        static_cast<const T*>(x), static_cast<T*>(out), table, g, (uint32_t)items, (uint32_t)units, (uint32_t)hgs,
-        backward);
-  else
-    rope_vec_kernel<T, HALF, HEADS, uint64_t><<<(int)blocks, kThreads, 0, s>>>(
-        static_cast<const T*>(x), static_cast<T*>(out), table, g, (uint64_t)items, (uint64_t)units, (uint64_t)hgs,
-        backward);
+  const T* xt = static_cast<const T*>(x);
+  T* ot = static_cast<T*>(out);
+  if (items + kThreads <= 0x7fffffff && g.heads <= 0x7fffffff) {
+    const Items<Divide32> n{Divide32(units), Divide32(groups), Divide32(g.seq), (uint32_t)items};
+    rope_vec_kernel<T, HALF, HEADS, Divide32><<<(int)blocks, kThreads, 0, s>>>(xt, ot, table, g, n, backward);
+  } else {
+    const Items<Divide64> n{Divide64(units), Divide64(groups), Divide64(g.seq), (uint64_t)items};
+    rope_vec_kernel<T, HALF, HEADS, Divide64><<<(int)blocks, kThreads, 0, s>>>(xt, ot, table, g, n, backward);
+  }
   note_launch();
   return check_launch();
 }
@@ -146,12 +75,15 @@ int launch_vec(const void* x, void* out, const float* table, const Geometry& g, 
 template <typename T>
 int launch(const void* x, void* out, const float* table, const Geometry& g, int64_t tokens, int half, int backward,
            cudaStream_t s) {
-  constexpr int N = Chunk<T>::N;
-  const bool strides = (g.xb | g.xs | g.xh | g.ob | g.os | g.oh) % N == 0;
-  const bool rows = g.dim % N == 0 && g.rot % (half ? 2 * N : N) == 0;
-  if (strides && rows && aligned(x, 16) && aligned(out, 16) && aligned(table, 16)) {
-    if (half) return launch_vec<T, true, 2>(x, out, table, g, tokens, backward, s);
-    return launch_vec<T, false, 2>(x, out, table, g, tokens, backward, s);
+  if (rope_vector<T>(x, out, table, g, half)) {
+    const auto run = [&](auto heads) {
+      constexpr int H = decltype(heads)::value;
+      return half ? launch_vec<T, true, H>(x, out, table, g, tokens, backward, s)
+                  : launch_vec<T, false, H>(x, out, table, g, tokens, backward, s);
+    };
+    const int heads = rope_heads<T>(g, tokens, half);
+    if (heads == 4) return run(std::integral_constant<int, 4>{});
+    return heads == 2 ? run(std::integral_constant<int, 2>{}) : run(std::integral_constant<int, 1>{});
   }
   const int64_t items = tokens * g.heads * (g.rot / 2 + (g.dim - g.rot));
   int64_t blocks = (items + kThreads - 1) / kThreads;
