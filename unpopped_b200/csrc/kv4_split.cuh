@@ -75,6 +75,10 @@ struct Shares {
   }
 };
 
+// What starting a tile costs, in units: its loads wait for one another (length, pages, cache) and its parts are added. The
+// CTAs' shares count it, or CTAs that get many short sequences finish last: 64 sequences of 0 to 4096 tokens take COST.
+constexpr int kTileCost = 2;
+
 // Units of one (tile, head) of a sequence: at least one, which writes the rows that see nothing.
 template <int ROWS>
 __device__ __forceinline__ int tile_units(const Args& a, const Seq& s, int tile, int& unit0) {
@@ -91,7 +95,7 @@ __device__ __forceinline__ int64_t seq_units(const Args& a, int b) {
   const int tiles = (s.nq * a.ratio + ROWS - 1) / ROWS;
   int64_t n = 0;
   int unit0;
-  for (int i = 0; i < tiles; ++i) n += tile_units<ROWS>(a, s, i, unit0);
+  for (int i = 0; i < tiles; ++i) n += kTileCost + tile_units<ROWS>(a, s, i, unit0);
   return n * a.kv_heads;
 }
 
@@ -170,18 +174,22 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
     int64_t in_tile = off;  // off counts from the sequence's first unit
     for (; tile < tiles; ++tile) {
       n_units = tile_units<ROWS>(a, seq, tile, unit0);
-      if (in_tile < (int64_t)n_units * a.kv_heads) break;
-      in_tile -= (int64_t)n_units * a.kv_heads;
+      if (in_tile < (int64_t)(n_units + kTileCost) * a.kv_heads) break;
+      in_tile -= (int64_t)(n_units + kTileCost) * a.kv_heads;
     }
     if (tile == tiles) {  // past this sequence's last unit
       ++b;
       off = 0;
       continue;
     }
-    const int head = (int)divide(in_tile, n_units), first = (int)(in_tile - (int64_t)head * n_units);
-    const int count = (int)min((int64_t)(n_units - first), u1 - u);
-    const int64_t tile_u0 = u - first;
-
+    // a tile's share is its cost and then its units: this CTA has [at, at + take) of it, the units [first, first + count)
+    const int head = (int)divide(in_tile, n_units + kTileCost), at = (int)(in_tile - (int64_t)head * (n_units + kTileCost));
+    const int take = (int)min((int64_t)(n_units + kTileCost - at), u1 - u);
+    const int first = max(at - kTileCost, 0), count = max(at + take - kTileCost, 0) - first;
+    const int64_t tile_u0 = u - at + kTileCost;  // the share of the first unit
+    u += take;
+    off += take;
+    if (count == 0) continue;
     const int tok0 = (unit0 + first) * kUnitTokens + warp * 32;
     const int32_t* pages = a.table + (int64_t)b * a.table_stride;
     // the page of this lane's token of step k, -1 where it has none
@@ -660,8 +668,6 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
       }
     }
     __syncthreads();  // the ring and the small arrays are free again
-    u += count;
-    off += count;
   }
 }
 
