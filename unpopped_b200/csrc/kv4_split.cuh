@@ -427,23 +427,6 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
             }
       }
       // ---- probabilities, against the running reference ----
-      float p[2][NT][4], part[NT][2];
-      auto raise = [&]() {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            part[nt][j] = 0.f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int i = j; i < 4; i += 2) {
-                p[h][nt][i] = exp2_approx(MASKED ? S[h][nt][i] - ref[nt][j] : fmaf(S[h][nt][i], qs[nt][j], -ref[nt][j]));
-                part[nt][j] += p[h][nt][i];
-              }
-          }
-      };
-      raise();
       // this lane's token: the largest of its v_scale, as bits. What is masked, or not finite there, does not count.
       uint32_t vb = 0;
       if constexpr (!MASKED && EXACT && GT % 2 == 0) {
@@ -459,6 +442,23 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
           vb = max(vb, MASKED ? (((have >> lane) & 1u) && w < 0x7c00u ? w : 0u) : min(w, 0x7bffu));
         }
       }
+      float p[2][NT][4], part[NT][2];
+      auto weigh = [&]() {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            part[nt][j] = 0.f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = j; i < 4; i += 2) {
+                p[h][nt][i] = exp2_approx(MASKED ? S[h][nt][i] - ref[nt][j] : fmaf(S[h][nt][i], qs[nt][j], -ref[nt][j]));
+                part[nt][j] += p[h][nt][i];
+              }
+          }
+      };
+      weigh();
       bool over = vb >= vbits;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) over |= part[nt][0] > most || part[nt][1] > most;
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
 #pragma unroll
               for (int z = 0; z < 2; ++z) O[c][z][nt][j] *= f, O[c][z][nt][2 + j] *= f;
           }
-        raise();
+        weigh();
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) sum[nt][0] += part[nt][0], sum[nt][1] += part[nt][1];
@@ -630,32 +630,45 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
         __syncthreads();
         return s_last != 0;
       };
-      // adds the parts base, base + step, ...: into part base, or as the tile's output
-      auto add = [&](int base, int step, int count_of, bool out) {
+      // Adds the parts base, base + step, ...: into part base, or as the tile's output. A place's loads
+      // are on the way together.
+      auto add = [&](int base, int step, int of, bool out) {
         float* ms = merge;
         float* ls = merge + kMaxCtas / kGroupCtas * ROWS;
-        for (int at = threadIdx.x; at < count_of * ROWS; at += kSplitThreads) {
-          const float* q = part_of(base + at / ROWS * step) + ROWS * D + at % ROWS;
+        const float* from_part = part_of(base);
+        const int64_t skip = part_of(base + step) - from_part;  // part 0 of the tile lies apart from the others'
+        const int64_t next = part_of(base + 2 * step) - part_of(base + step);
+        auto at_part = [&](int i) { return from_part + (i == 0 ? 0 : skip + (i - 1) * next); };
+        for (int at = threadIdx.x; at < of * ROWS; at += kSplitThreads) {
+          const float* q = at_part(at / ROWS) + ROWS * D + at % ROWS;
           ms[at] = __ldcg(q);
           ls[at] = __ldcg(q + ROWS);
         }
         __syncthreads();
+#pragma unroll 1
         for (int at = threadIdx.x; at < live * (D / 4); at += kSplitThreads) {
           const int r = at / (D / 4), d = 4 * (at - r * (D / 4));
-          float m = ms[r];
-          for (int i = 1; i < count_of; ++i) m = fmaxf(m, ms[i * ROWS + r]);
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          float l = 0.f;
-#pragma unroll 8
-          for (int i = 0; i < count_of; ++i) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part_of(base + i * step) + r * D + d));
-            const float w = exp2_approx(ms[i * ROWS + r] - m);
-            o.x = fmaf(v.x, w, o.x), o.y = fmaf(v.y, w, o.y), o.z = fmaf(v.z, w, o.z), o.w = fmaf(v.w, w, o.w);
-            l = fmaf(ls[i * ROWS + r], w, l);
+          float l = 0.f, m = ms[r];
+#pragma unroll 1
+          for (int i = 1; i < of; ++i) m = fmaxf(m, ms[i * ROWS + r]);
+#pragma unroll 1
+          for (int i0 = 0; i0 < of; i0 += kGroupCtas) {
+            float4 v[kGroupCtas];
+#pragma unroll
+            for (int i = 0; i < kGroupCtas; ++i)
+              v[i] = i0 + i < of ? __ldcg(reinterpret_cast<const float4*>(at_part(i0 + i) + r * D + d)) : o;
+#pragma unroll
+            for (int i = 0; i < kGroupCtas; ++i)
+              if (i0 + i < of) {
+                const float w = exp2_approx(ms[(i0 + i) * ROWS + r] - m);
+                o.x = fmaf(v[i].x, w, o.x), o.y = fmaf(v[i].y, w, o.y), o.z = fmaf(v[i].z, w, o.z), o.w = fmaf(v[i].w, w, o.w);
+                l = fmaf(ls[(i0 + i) * ROWS + r], w, l);
+              }
           }
           if (out) {
             store(r, d, o, m, l);
-          } else {  // the sums' places are this thread's alone; the reference and the sum were read above
+          } else {  // the reference and the sum were read by all above, and the sums' places are this thread's alone
             float* q = part_of(base);
             __stcg(reinterpret_cast<float4*>(q + r * D + d), o);
             if (d == 0) __stcg(q + ROWS * D + r, m), __stcg(q + ROWS * D + ROWS + r, l);
@@ -663,8 +676,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
         }
       };
       if (arrive(a.counters + (mine_in == 0 ? 0 : kMaxCtas) + c0 + from, min(kGroupCtas, n - from))) {
-        add(from, 1, min(kGroupCtas, n - from), n_groups == 1);
-        if (n_groups > 1 && arrive(a.counters + 2 * kMaxCtas + c0, n_groups)) add(0, kGroupCtas, n_groups, true);
+#pragma unroll 1
+        for (int level = 0;; ++level) {
+          const bool top = level > 0 || n_groups == 1;
+          add(level ? 0 : from, level ? kGroupCtas : 1, level ? n_groups : min(kGroupCtas, n - from), top);
+          if (top || !arrive(a.counters + 2 * kMaxCtas + c0, n_groups)) break;
+        }
       }
     }
     __syncthreads();  // the ring and the small arrays are free again
