@@ -10,9 +10,9 @@ int split_attention(const Args& a, int dim, int rows, int ctas, cudaStream_t s) 
   return split_attention_large(a, dim, ctas, s);
 }
 
-// f32 parts of the split tiles: two a CTA (one tile begins earlier, one ends later), each rows x (dim + 2).
+// f32 parts of the split tiles: two a CTA (one tile begins earlier, one ends later), each rows x (dim + 4).
 static size_t partial_bytes(int64_t ctas, int64_t rows, int64_t dim) {
-  return (size_t)ctas * 2 * rows * (dim + 2) * sizeof(float);
+  return (size_t)ctas * 2 * rows * (dim + 4) * sizeof(float);
 }
 
 static int split_ctas() { return sm_count() * 4 < kMaxCtas ? sm_count() * 4 : kMaxCtas; }

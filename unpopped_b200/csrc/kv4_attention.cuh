@@ -193,7 +193,7 @@ constexpr int kSplitThreads = 32 * kSplitWarps;
 constexpr int kUnitTokens = 32 * kSplitWarps;  // cached tokens of one unit: 32 a warp
 constexpr int kMaxCtas = 1024;                 // counters in the workspace
 constexpr int kMaxRows = 16;                   // query rows of a tile at most
-constexpr int kGroupCtas = 16;                 // parts of a split tile that are added at once
+constexpr int kGroup = 16;                     // parts of a split tile that are added at once
 constexpr size_t kHeaderBytes = 256, kCounterBytes = kHeaderBytes + 3 * kMaxCtas * sizeof(uint32_t);
 
 // Query rows a tile has in the split kernel: 8 a column group, a second one where the head size leaves registers.

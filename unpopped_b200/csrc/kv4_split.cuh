@@ -23,6 +23,9 @@
 //
 // Work. Units of 128 cached tokens, over sequences, tiles and heads in order, are split evenly over the launch's CTAs
 // (each sequence's count comes from its length on the device: no host read, no launch bound by the longest sequence).
+// CTAs do not run at one rate (of a launch that the memory bounds, the slowest take a fifth longer than the mean); drawing
+// the last eighth of the units in items as CTAs finish cost more, by the items' starts, than it gained (attend over 32
+// contexts of 8k to 16k tokens: 100.7 us with it, 95.7 us without).
 // A warp takes 32 tokens of each unit through its own ring of cp.async stages, so no barrier stands in the loop. A tile
 // that ends inside one CTA is written at once; parts of a split tile go to the workspace in f32 and the CTA that
 // finishes last adds them in order. No CTA waits for another.
@@ -44,7 +47,6 @@ struct SplitCfg {
   static constexpr int kRing = kSplitWarps * kStages * kStage;
   static constexpr int kMerge = kSplitWarps * kRows * kPitch * 4;
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
-  static_assert(kSmem >= 2 * kMaxCtas / kGroupCtas * kRows * 4, "room for the parts' references and sums");
   static constexpr int kOcc = D <= 128 ? (NT == 1 ? 4 : 3) : 2;
 };
 
@@ -132,6 +134,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
   const Shares shares(U, gridDim.x);
   const int64_t cta = blockIdx.x;
   if (cta >= shares.P) return;
+  // the sequence in which this CTA's share [u, u1) begins: the thread that counted it says so
   int64_t u = shares.begin(cta);
   const int64_t u1 = shares.begin(cta + 1);
   if (u >= before && u < before + mine) {
@@ -582,8 +585,9 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
       *reinterpret_cast<uint2*>(static_cast<char*>(a.out) + 2 * (tk * a.os + h * a.oh + d)) = w;
       if (a.lse && d == 0) a.lse[tk * a.ls + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
     };
-    // parts: [cta][whether the tile began in an earlier CTA][ROWS][D sums, then the reference and the sum]
-    constexpr int PART = ROWS * (D + 2);
+    // parts: [CTA][whether the tile begins in it]: [ROWS][D] sums, [ROWS] references, [ROWS] sums of p, and the latter
+    // two again once the part holds its group
+    constexpr int PART = ROWS * (D + 4);
     float* part = a.partials + (cta * 2 + (first > 0 ? 0 : 1)) * PART;
     for (int at = threadIdx.x; at < live * (D / 4); at += kSplitThreads) {
       const int r = at / (D / 4), d = 4 * (at - r * (D / 4));
@@ -610,12 +614,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
       }
     }
     if (!whole) {
-      // The tile's parts are added in order, kGroupCtas at a time: the CTA that completes a group adds its parts into the
-      // group's first, and the one that completes the last group adds the groups. The counters belong to CTAs that a
-      // tile begins in (the first group's, the groups') or that it reaches from before (the other groups').
+      // The tile's parts are added in order, kGroup at a time: the CTA that completes a group adds its parts into the
+      // group's first, and the one that completes the last group adds the groups. The counters belong to CTAs that a tile
+      // begins in (the first group's, the groups') or that it reaches from before (the other groups').
       const int64_t c0 = shares.cta_of(tile_u0), c1 = shares.cta_of(tile_u0 + n_units - 1);
-      const int n = (int)(c1 - c0) + 1, n_groups = (n + kGroupCtas - 1) / kGroupCtas;
-      const int mine_in = (int)(cta - c0) / kGroupCtas, from = mine_in * kGroupCtas;
+      const int n = (int)(c1 - c0) + 1, n_groups = (n + kGroup - 1) / kGroup;
+      const int mine_in = (int)(cta - c0) / kGroup, from = mine_in * kGroup;
       auto part_of = [&](int i) { return a.partials + ((c0 + i) * 2 + (i == 0 ? 1 : 0)) * PART; };
       // counts this CTA in; true in the one that completes the count
       auto arrive = [&](uint32_t* counter, int of) {
@@ -630,56 +634,57 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
         __syncthreads();
         return s_last != 0;
       };
-      // Adds the parts base, base + step, ...: into part base, or as the tile's output. A place's loads
-      // are on the way together.
-      auto add = [&](int base, int step, int of, bool out) {
-        float* ms = merge;
-        float* ls = merge + kMaxCtas / kGroupCtas * ROWS;
-        const float* from_part = part_of(base);
-        const int64_t skip = part_of(base + step) - from_part;  // part 0 of the tile lies apart from the others'
+      // Adds the parts base, base + step, ...: into part base, or as the tile's output. kGroup parts' loads are on the way
+      // together.
+      auto add = [&](int base, int step, int of, int level, bool out) {
+        const int refs = ROWS * D + level * 2 * ROWS;
+        const float* begin = part_of(base);
+        const int64_t skip = part_of(base + step) - begin;  // part 0 of the tile lies apart from the others'
         const int64_t next = part_of(base + 2 * step) - part_of(base + step);
-        auto at_part = [&](int i) { return from_part + (i == 0 ? 0 : skip + (i - 1) * next); };
-        for (int at = threadIdx.x; at < of * ROWS; at += kSplitThreads) {
-          const float* q = at_part(at / ROWS) + ROWS * D + at % ROWS;
-          ms[at] = __ldcg(q);
-          ls[at] = __ldcg(q + ROWS);
-        }
-        __syncthreads();
 #pragma unroll 1
         for (int at = threadIdx.x; at < live * (D / 4); at += kSplitThreads) {
           const int r = at / (D / 4), d = 4 * (at - r * (D / 4));
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          float l = 0.f, m = ms[r];
+          float l = 0.f, m = kNoMax;
 #pragma unroll 1
-          for (int i = 1; i < of; ++i) m = fmaxf(m, ms[i * ROWS + r]);
-#pragma unroll 1
-          for (int i0 = 0; i0 < of; i0 += kGroupCtas) {
-            float4 v[kGroupCtas];
+          for (int i0 = 0; i0 < of; i0 += kGroup) {
+            float4 v[kGroup];
+            float vm[kGroup], vl[kGroup];
 #pragma unroll
-            for (int i = 0; i < kGroupCtas; ++i)
-              v[i] = i0 + i < of ? __ldcg(reinterpret_cast<const float4*>(at_part(i0 + i) + r * D + d)) : o;
+            for (int i = 0; i < kGroup; ++i) {
+              const bool is = i0 + i < of;
+              const float* q = begin + (i0 + i == 0 ? 0 : skip + (i0 + i - 1) * next);
+              v[i] = is ? __ldcg(reinterpret_cast<const float4*>(q + r * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+              vm[i] = is ? __ldcg(q + refs + r) : kNoMax;
+              vl[i] = is ? __ldcg(q + refs + ROWS + r) : 0.f;
+            }
+            float now = m;
 #pragma unroll
-            for (int i = 0; i < kGroupCtas; ++i)
-              if (i0 + i < of) {
-                const float w = exp2_approx(ms[(i0 + i) * ROWS + r] - m);
-                o.x = fmaf(v[i].x, w, o.x), o.y = fmaf(v[i].y, w, o.y), o.z = fmaf(v[i].z, w, o.z), o.w = fmaf(v[i].w, w, o.w);
-                l = fmaf(ls[(i0 + i) * ROWS + r], w, l);
-              }
+            for (int i = 0; i < kGroup; ++i) now = fmaxf(now, vm[i]);
+            const float f = exp2_approx(m - now);
+            o.x *= f, o.y *= f, o.z *= f, o.w *= f, l *= f;
+            m = now;
+#pragma unroll
+            for (int i = 0; i < kGroup; ++i) {
+              const float w = exp2_approx(vm[i] - m);
+              o.x = fmaf(v[i].x, w, o.x), o.y = fmaf(v[i].y, w, o.y), o.z = fmaf(v[i].z, w, o.z), o.w = fmaf(v[i].w, w, o.w);
+              l = fmaf(vl[i], w, l);
+            }
           }
           if (out) {
             store(r, d, o, m, l);
-          } else {  // the reference and the sum were read by all above, and the sums' places are this thread's alone
+          } else {
             float* q = part_of(base);
             __stcg(reinterpret_cast<float4*>(q + r * D + d), o);
-            if (d == 0) __stcg(q + ROWS * D + r, m), __stcg(q + ROWS * D + ROWS + r, l);
+            if (d == 0) __stcg(q + refs + 2 * ROWS + r, m), __stcg(q + refs + 3 * ROWS + r, l);
           }
         }
       };
-      if (arrive(a.counters + (mine_in == 0 ? 0 : kMaxCtas) + c0 + from, min(kGroupCtas, n - from))) {
+      if (arrive(a.counters + (mine_in == 0 ? 0 : kMaxCtas) + c0 + from, min(kGroup, n - from))) {
 #pragma unroll 1
         for (int level = 0;; ++level) {
           const bool top = level > 0 || n_groups == 1;
-          add(level ? 0 : from, level ? kGroupCtas : 1, level ? n_groups : min(kGroupCtas, n - from), top);
+          add(level ? 0 : from, level ? kGroup : 1, level ? n_groups : min(kGroup, n - from), level, top);
           if (top || !arrive(a.counters + 2 * kMaxCtas + c0, n_groups)) break;
         }
       }
