@@ -114,7 +114,12 @@ typedef enum up_kernel_id {
   UP_K_ROW_REDUCE_F32 = 13, /* a RowReduce form (softmax, RMS norm, centred quotient) over f32 rows */
   UP_K_COL_SUM_SPLITK = 14,  /* the split-K variant of the outer-axis f32 Sum/Mean (needs a workspace) */
   UP_K_WINDOW = 15,          /* 1-D window pooling (Sum/Mean/Max/Min) along one axis, f32 or i32 */
-  UP_K_IM2COL = 16           /* the 2-D unfold of an NCHW input, raw bits */
+  UP_K_IM2COL = 16,          /* the 2-D unfold of an NCHW input, raw bits */
+  /* The serving operators: named for their interface artifacts. No plan lowers to them and up_sm100_launch declines
+   * them; their typed entry points are below. */
+  UP_K_ROPE = 17,
+  UP_K_KV4_APPEND = 18,
+  UP_K_KV4_ATTENTION = 19
 } up_kernel_id;
 
 /* A buffer argument: the reference's TypedBuffer / OperandDesc. `base` and `stride` count elements
@@ -489,7 +494,8 @@ UP_API int up_sm100_kv4_append(const void* q, const void* k, const void* v, int 
  * over the visible tokens, accumulated in f32, rounded once to q's type. A query that sees nothing gives 0 and -inf.
  * What a masked token's page or slot holds (a NaN scale included) has no effect. seq_lens beyond table_width * page count
  * as that much; cached tokens on a page outside [0, pages) are left out; query tokens that no sequence names are not
- * written. `workspace` from up_sm100_kv4_attention_workspace_bytes, 256-byte aligned, zero-filled before its first use;
+ * written. A NaN in a visible cached value reaches the outputs that it multiplies, or all of the row's (where many query
+ * rows share a tile). `workspace` from up_sm100_kv4_attention_workspace_bytes, 256-byte aligned, zero-filled before its first use;
  * launches leave it ready for the next one, of any shape that needs no more bytes. The result does not depend on the
  * order in which the parts of a split sequence finish. q is 16-byte aligned with strides of whole 8 elements, out 8-byte
  * aligned with strides of whole 4 (UP_ERR_UNSUPPORTED else); at most 2^30 cached tokens a sequence and 2^30 query rows

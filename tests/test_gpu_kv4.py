@@ -444,6 +444,24 @@ def test_many_short_sequences_and_captured_launches():
         assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("nq", [1, 40])
+def test_a_captured_step_of_wide_heads(nq):
+    """Heads of 128 need more shared memory than a launch has by default: setting it must not break a capture."""
+    cache, table, n = make(3, 2, 128, 64, 16, [500, 64, 300], seed=13)
+    cu = torch.arange(4, device="cuda", dtype=torch.int32) * nq
+    q = torch.randn(3 * nq, 8, 128, device="cuda").bfloat16()
+    want = check(q, cache, table, n, cu)
+    out = torch.empty_like(q)
+    ws = torch.zeros(_lib.load().up_sm100_kv4_attention_workspace_bytes(3 * nq, 8, 3, 2, 128), dtype=torch.uint8,
+                     device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.kv4_attention(q, cache, table, n, cu_q=cu, out=out, ws=ws)
+    out.zero_()
+    graph.replay()
+    assert torch.equal(out, want)
+
+
 def test_a_cache_that_passes_32_bits():
     """Pages above 2^32 bytes into the arrays."""
     page, kv, dim, group = 4096, 8, 128, 128

@@ -30,6 +30,8 @@ SCHED = dict(VECTORIZED=0, SCALAR=1, STRIDED=2, REDUCTION=3, ROW_REDUCE=4, CONTR
 KERNEL = dict(NONE=-1, ROW_SUM_F32=1, ROW_MAX_ARGMAX_BF16=2, SCAN_I32=3, GATHER_ROWS=4, DEQUANT_I4=5,
               W4A16_GEMM=6, REDUCE2D_F32=7, REDUCE2D_I32=8, SCATTER=9, BINCOUNT=10, REDUCE_F32=11, REDUCE_I32=12,
               ROW_REDUCE_F32=13, COL_SUM_SPLITK=14, WINDOW=15, IM2COL=16)
+# The serving operators' ids, for their interface artifacts: no plan lowers to them
+SERVING_KERNEL = dict(ROPE=17, KV4_APPEND=18, KV4_ATTENTION=19)
 ROW_REDUCE_FORM = dict(NONE=0, SOFTMAX=1, RMS_NORM=2, CENTRED=3)
 # up_rope_layout, up_rope_scaling
 ROPE_LAYOUT = dict(HALF=0, INTERLEAVED=1)

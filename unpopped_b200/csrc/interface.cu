@@ -15,8 +15,11 @@ uint64_t revision_backend();
 uint64_t revision_colsplit();
 uint64_t revision_dequant();
 uint64_t revision_gather();
+uint64_t revision_kv4_append();
+uint64_t revision_kv4_attention();
 uint64_t revision_reduce();
 uint64_t revision_reduce2d();
+uint64_t revision_rope();
 uint64_t revision_rowreduce();
 uint64_t revision_scan();
 uint64_t revision_scatter();
@@ -46,6 +49,9 @@ extern "C" uint64_t up_sm100_revision_hash(int kernel_id) {
     case UP_K_COL_SUM_SPLITK: return revision_colsplit();
     case UP_K_WINDOW:
     case UP_K_IM2COL: return revision_window();
+    case UP_K_ROPE: return revision_rope();
+    case UP_K_KV4_APPEND: return revision_kv4_append();
+    case UP_K_KV4_ATTENTION: return revision_kv4_attention();
     default: return 0;
   }
 }
@@ -84,6 +90,12 @@ static const char* interface_body(int id) {
       return R"J({"entry_symbol":"up_sm100_window","params":[{"name":"x","role":"read","elem":"F32|I32","rank":-1},{"name":"out","role":"write","elem":"F32|I32","rank":-1},{"name":"op","role":"scalar","elem":"I32"},{"name":"size","role":"scalar","elem":"I32"},{"name":"stride","role":"scalar","elem":"I32"},{"name":"dilation","role":"scalar","elem":"I32"},{"name":"pad_lo","role":"scalar","elem":"I32"},{"name":"count_include_pad","role":"scalar","elem":"I32"},{"name":"axis","role":"scalar","elem":"I32"}],"launch":{"block":[256,1,1],"grid":"a CTA per row (innermost axis; the row staged by cp.async into 32 KiB of static shared memory) or per group of lines, up to 16 per SM","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":256,"min_blocks":0},"cooperative":false,"requires":["sm_100a","cp.async"],"fidelity_notes":[],"workspace":null})J";
     case UP_K_IM2COL:
       return R"J({"entry_symbol":"up_sm100_im2col","params":[{"name":"x","role":"read","elem":"any","rank":4},{"name":"out","role":"write","elem":"any","rank":3},{"name":"kh","role":"scalar","elem":"I32"},{"name":"kw","role":"scalar","elem":"I32"},{"name":"sh","role":"scalar","elem":"I32"},{"name":"sw","role":"scalar","elem":"I32"},{"name":"ph","role":"scalar","elem":"I32"},{"name":"pw","role":"scalar","elem":"I32"},{"name":"dh","role":"scalar","elem":"I32"},{"name":"dw","role":"scalar","elem":"I32"}],"launch":{"block":[256,1,1],"grid":"a CTA per input plane staged in dynamic shared memory (the plane's bytes, at most 96 KiB), else a CTA per output row; up to 16 per SM","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":256,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":[],"workspace":null})J";
+    case UP_K_ROPE:
+      return R"J({"entry_symbol":"up_sm100_rope","params":[{"name":"x","role":"read","elem":"F32|F16|BF16","rank":4},{"name":"positions","role":"read","elem":"I32|I64","rank":2},{"name":"table","role":"read","elem":"F32","rank":2},{"name":"out","role":"write","elem":"F32|F16|BF16","rank":4},{"name":"layout","role":"scalar","elem":"I32"},{"name":"backward","role":"scalar","elem":"I32"}],"launch":{"block":[256,1,1],"grid":"a thread per two 16-byte chunks of one, two or four heads of a token","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":256,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["each product and sum rounded to f32, one rounding to x's type"],"workspace":null})J";
+    case UP_K_KV4_APPEND:
+      return R"J({"entry_symbol":"up_sm100_kv4_append","params":[{"name":"q","role":"read","elem":"F16|BF16","rank":3},{"name":"k","role":"read","elem":"F16|BF16","rank":3},{"name":"v","role":"read","elem":"F16|BF16","rank":3},{"name":"positions","role":"read","elem":"I32|I64","rank":1},{"name":"table","role":"read","elem":"F32","rank":2},{"name":"slots","role":"read","elem":"I32|I64","rank":1},{"name":"cache","role":"readwrite","elem":"I4+F16","rank":4},{"name":"q_out","role":"write","elem":"F16|BF16","rank":3},{"name":"layout","role":"scalar","elem":"I32"}],"launch":{"block":[256,1,1],"grid":"blocks of query chunks and blocks of key and value rows, alternating","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":256,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["packed values and scales are the stated f32 operations bit for bit"],"workspace":null})J";
+    case UP_K_KV4_ATTENTION:
+      return R"J({"entry_symbol":"up_sm100_kv4_attention","params":[{"name":"q","role":"read","elem":"F16|BF16","rank":3},{"name":"cache","role":"read","elem":"I4+F16","rank":4},{"name":"block_table","role":"read","elem":"I32","rank":2},{"name":"seq_lens","role":"read","elem":"I32","rank":1},{"name":"cu_q","role":"read","elem":"I32","rank":1},{"name":"out","role":"write","elem":"F16|BF16","rank":3},{"name":"lse","role":"write","elem":"F32","rank":2},{"name":"causal","role":"scalar","elem":"I32"},{"name":"window","role":"scalar","elem":"I64"},{"name":"scale","role":"scalar","elem":"F32"}],"launch":{"block":[128,1,1],"grid":"few query rows: two to four CTAs per SM over units of 128 cached tokens; prompts (block 576): a CTA per 256 query rows","cluster":null,"dynamic_shared_bytes":"up to 200704"},"launch_bounds":{"max_threads":576,"min_blocks":1},"cooperative":false,"requires":["sm_100a","cp.async","mma.sync","tcgen05","tensor_memory","mbarrier"],"fidelity_notes":["f32 sums; p * v_scale rounded to f16, and in prompts nibble * scale too","split tiles are added in order: deterministic"],"workspace":"counters and parts of split tiles: up_sm100_kv4_attention_workspace_bytes, zero-filled once"})J";
     default: return nullptr;
   }
 }
