@@ -69,7 +69,7 @@ extern "C" int up_sm100_kv4_attention(const void* q, int dtype, int64_t tokens, 
     a.k4 = a.v4 = static_cast<const uint8_t*>(q);
     a.k_scale = a.v_scale = static_cast<const __half*>(q);
   }
-  a.pages = cache->pages, a.kv_heads = (int)cache->kv_heads, a.ratio = (int)ratio, a.page_log2 = log2_of(cache->page);
+  a.pages = (uint32_t)cache->pages, a.kv_heads = (int)cache->kv_heads, a.ratio = (int)ratio, a.page_log2 = log2_of(cache->page);
   a.cpg = (int)(cache->group / 32), a.groups = (int)(cache->dim / cache->group);
   a.table = block_table, a.table_stride = table_stride, a.table_width = table_width;
   a.lens = seq_lens, a.cu = cu_q, a.batch = (int)batch, a.causal = causal != 0;

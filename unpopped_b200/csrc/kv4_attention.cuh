@@ -19,7 +19,7 @@ struct Args {
   int64_t tokens;
   const uint8_t *k4, *v4;
   const __half *k_scale, *v_scale;
-  int64_t pages;
+  uint32_t pages;                      // below 2^31: a negative page number is not below it
   int kv_heads, ratio, page_log2;      // ratio: query heads a key/value head
   int cpg, groups;                     // 32-dimension chunks a group; groups a row
   const int32_t* table;

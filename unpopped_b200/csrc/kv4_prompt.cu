@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       const int j = tok0 + t * kTok + tid;
       if (t >= n || j >= seq.len) return -1;
       const int p = __ldg(pages + (j >> a.page_log2));
-      return p >= 0 && (int64_t)p < a.pages ? p : -1;
+      return (uint32_t)p < a.pages ? p : -1;
     };
     // a tile's nibbles: unit u = lane / 8 + 4 i of this warp's 32 tokens is run u / CH (8 tokens, lane % 8), chunk u % CH
     uint4 raw[CH];

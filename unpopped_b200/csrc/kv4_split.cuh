@@ -39,7 +39,9 @@ namespace kv4 {
 template <int D, int NT>
 struct SplitCfg {
   static constexpr int kChunks = D / 32;
-  static constexpr int kStages = 3;
+  // Two stages: a third made the ring's share of the SM's memory leave 7 KB of L1 (94.3 against 91.7 us for 32 contexts of
+  // 8k to 16k tokens), and a fifth CTA in place of it spilled registers (97.2 us).
+  static constexpr int kStages = 2;
   static constexpr int kRows = 8 * NT;
   // a stage of one warp: 32 tokens of K and V (D / 2 bytes each) and of their scales (at most D / 32 f16 each)
   static constexpr int kKV = 16 * D, kSc = 2 * D, kStage = 2 * kKV + 2 * kSc;
@@ -47,6 +49,7 @@ struct SplitCfg {
   static constexpr int kRing = kSplitWarps * kStages * kStage;
   static constexpr int kMerge = kSplitWarps * kRows * kPitch * 4;
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
+  static_assert(kStages == 2, "the tokens that exist are kept for the step at hand and the next");
   static constexpr int kOcc = D <= 128 ? (NT == 1 ? 4 : 3) : 2;
 };
 
@@ -110,7 +113,6 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
   __shared__ int64_t s_scan[kSplitWarps + 1], s_base;
   __shared__ int s_seq, s_last;
   __shared__ float s_ref[kSplitWarps][ROWS], s_sum[kSplitWarps][ROWS];
-  __shared__ uint32_t s_mask[kSplitWarps][C::kStages];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   // ---- this CTA's share [u, u1) of the units, and the sequence it begins in ----
@@ -156,7 +158,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
   float* merge = reinterpret_cast<float*>(smem);
   // the scale runs of 8 tokens are 16 * groups bytes: `groups` 16-byte pieces
   const int groups = EXACT ? GT : a.groups;
-  const bool sc_mine = lane < 4 * groups;
+  // a lane copies a piece of K's scales (the first 4 * groups lanes) or of V's; one of each where that is more than 32 lanes
+  // or no power of two
+  const bool sc_both = 8 * groups > 32 || (groups & (groups - 1)) != 0, sc_v = !sc_both && lane >= 4 * groups;
+  const int sc_at = sc_both ? lane : lane & (4 * groups - 1);
+  const bool sc_mine = sc_at < 4 * groups && (sc_both || lane < 8 * groups);
+  const int sc_run = sc_mine ? sc_at / groups * 8 : 0, sc_part = sc_at % groups;
   // where piece lane + 32 i of a step's K (or V) lies in its stage
   auto copy_at = [&](int i) -> uint32_t {
     if constexpr (32 % CH == 0 && 32 / CH >= 8) {  // the swizzle repeats: one offset a lane, the rest are constants
@@ -168,7 +175,6 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
   };
   // where row `lane` of chunk c lies
   auto chunk_at = [&](int c) -> uint32_t { return (lane * CH + (c ^ swizzle<D>(lane))) * 16; };
-  const int sc_run = sc_mine ? lane / groups * 8 : 0, sc_part = lane % groups;
 
   while (u < u1) {
     const Seq seq = load_seq(a, b);
@@ -200,7 +206,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
       const int j = tok0 + k * kUnitTokens + lane;
       if (k >= count || j >= seq.len) return -1;
       const int p = __ldg(pages + (j >> a.page_log2));
-      return p >= 0 && (int64_t)p < a.pages ? p : -1;
+      return (uint32_t)p < a.pages ? p : -1;
     };
     int page0[C::kStages];
 #pragma unroll
@@ -221,14 +227,15 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
     const uint32_t in_page = (1u << a.page_log2) - 1;
     const uint4* k_base = reinterpret_cast<const uint4*>(a.k4) + (uint64_t)head_kv * CH;
     const uint4* v_base = reinterpret_cast<const uint4*>(a.v4) + (uint64_t)head_kv * CH;
-    const uint4* ks_base = reinterpret_cast<const uint4*>(a.k_scale) + ((uint64_t)head_kv * groups >> 3);
+    const uint4* ks_base = reinterpret_cast<const uint4*>(sc_v ? a.v_scale : a.k_scale) + ((uint64_t)head_kv * groups >> 3);
     const uint4* vs_base = reinterpret_cast<const uint4*>(a.v_scale) + ((uint64_t)head_kv * groups >> 3);
-    // Copies step k into the stage at `st` (its word of s_mask: `slot`).
-    auto issue = [&](int k, int page, uint32_t st, int slot) {
+    const uint32_t sc_dst = 2 * C::kKV + (sc_v ? C::kSc : 0) + sc_at * 16;
+    uint32_t have = 0, have_next = 0;  // the tokens of the step at hand, and of the last one copied, that exist
+    // Copies step k into the stage at `st`.
+    auto issue = [&](int k, int page, uint32_t st) {
       if (k < count) {
         const uint32_t tok = (uint32_t)(tok0 + k * kUnitTokens) & in_page;
-        const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
-        if (lane == 0) s_mask[warp][slot] = have;
+        have_next = __ballot_sync(0xffffffffu, page >= 0);
         if (a.page_log2 >= 5) {  // one page holds the step's 32 tokens
           const int pg = __shfl_sync(0xffffffffu, page, 0);
           const uint32_t bytes = pg >= 0 ? 16u : 0u;
@@ -241,10 +248,9 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
             cp_async16(dst + C::kKV, v_at + 32 * i, bytes);
           }
           if (sc_mine) {
-            const uint64_t sc = (uint64_t)(uint32_t)max(pg, 0) * ((page_kv >> 3) * groups) + ((tok >> 3) * groups + lane);
-            const uint32_t dst = st + 2 * C::kKV + lane * 16;
-            cp_async16(dst, ks_base + sc, bytes);
-            cp_async16(dst + C::kSc, vs_base + sc, bytes);
+            const uint64_t sc = (uint64_t)(uint32_t)max(pg, 0) * ((page_kv >> 3) * groups) + ((tok >> 3) * groups + sc_at);
+            cp_async16(st + sc_dst, ks_base + sc, bytes);
+            if (sc_both) cp_async16(st + sc_dst + C::kSc, vs_base + sc, bytes);
           }
         } else {
 #pragma unroll
@@ -263,9 +269,8 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
             const uint32_t bytes = pg >= 0 ? 16u : 0u;
             const uint64_t at = (uint64_t)(uint32_t)max(pg, 0) * ((page_kv >> 3) * groups) +
                                 ((((tok + sc_run) & in_page) >> 3) * groups + sc_part);
-            const uint32_t dst = st + 2 * C::kKV + lane * 16;
-            cp_async16(dst, ks_base + at, bytes);
-            cp_async16(dst + C::kSc, vs_base + at, bytes);
+            cp_async16(st + sc_dst, ks_base + at, bytes);
+            if (sc_both) cp_async16(st + sc_dst + C::kSc, vs_base + at, bytes);
           }
         }
       }
@@ -273,7 +278,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
     };
 
 #pragma unroll
-    for (int k = 0; k < C::kStages - 1; ++k) issue(k, page0[k], ring + k * C::kStage, k);
+    for (int k = 0; k < C::kStages - 1; ++k) issue(k, page0[k], ring + k * C::kStage);
     int page = page0[C::kStages - 1];
 
     // ---- B fragments of the queries, and per column (query row) its logit factor and visible range ----
@@ -532,12 +537,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
     // ---- this warp's 32 tokens of each unit ----
     int slot = 0, slot_in = C::kStages - 1;
     for (int k = 0; k < count; ++k) {
-      issue(k + C::kStages - 1, page, ring + slot_in * C::kStage, slot_in);
+      have = have_next;
+      issue(k + C::kStages - 1, page, ring + slot_in * C::kStage);
       page = page_of(k + C::kStages);
       cp_async_wait<C::kStages - 1>();
       __syncwarp();
       const int tok = tok0 + k * kUnitTokens;
-      const uint32_t have = s_mask[warp][slot];
       if (have == 0xffffffffu && tok > all_past && tok + 31 <= all_last)
         consume(tok, have, ring + slot * C::kStage, std::false_type{});
       else
