@@ -341,6 +341,37 @@ def test_prompts_with_a_nan_and_pages_outside():
     assert not torch.equal(got[64:], clean[64:])
 
 
+@pytest.mark.parametrize("dim,group", [(64, 32), (64, 64), (96, 96), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("scale", [None, -0.2])
+def test_prompts_keep_the_logits_of_32_bits(dim, group, scale):
+    """The logsumexp has f32's precision: no nibble * scale is rounded to f16 on the way to a logit. A logit is at most 17
+    sums of exact products (16 dimensions at a time, scales in two parts), each off by 2^-23 of what has been added so far
+    at most, which is of the logits' size: 2^-19 with the sums of the softmax. A rounding to f16 is off by 2^-16 and more."""
+    lens, nq = [900, 300], [700, 150]
+    cache, table, n = make(2, 2, dim, group, 16, lens, seed=31)
+    cu = torch.tensor([0] + nq, device="cuda").cumsum(0).int()
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    q = torch.randn(sum(nq), 6, dim, generator=g, device="cuda").bfloat16()
+    _, lse = ops.kv4_attention(q, cache, table, n, cu_q=cu, scale=scale, want_lse=True)
+    _, want, _, _ = reference(q, cache, table, n, cu, True, 0, dim ** -0.5 if scale is None else scale)
+    assert float((lse.double() - want).norm() / want.norm()) <= 2.0 ** -19
+
+
+def test_prompts_with_a_nan_in_a_token_of_one_scale():
+    cache, table, n = make(1, 1, 64, 64, 16, [300], seed=6)
+    j = 200
+    cu = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    q = torch.randn(300, 2, 64, device="cuda").bfloat16()
+    clean = ops.kv4_attention(q, cache, table, n, cu_q=cu)
+    for which in (3, 2):
+        keep = cache[which][int(table[0, j // 16]), 0, j % 16, 0].clone()
+        for bad in (float("nan"), float("inf")):
+            cache[which][int(table[0, j // 16]), 0, j % 16, 0] = bad
+            out = ops.kv4_attention(q, cache, table, n, cu_q=cu)
+            assert torch.equal(out[:j], clean[:j]) and not bool(torch.isfinite(out[j:]).any())
+        cache[which][int(table[0, j // 16]), 0, j % 16, 0] = keep
+
+
 def test_a_long_sequence_is_split_over_the_gpu():
     lens = [70001]
     cache, table, n = make(1, 1, 128, 128, 64, lens, seed=9)

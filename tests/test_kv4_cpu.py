@@ -127,7 +127,7 @@ def test_interfaces(kid, src):
 
 
 def test_division_by_multiplication():
-    """Divide32 of rope.cuh: exact for every dividend below 2^31, and no intermediate passes 32 bits."""
+    """Divide32 of divide.cuh: exact for every dividend below 2^31, and no intermediate passes 32 bits."""
     rng = random.Random(1)
     for d in list(range(1, 2000)) + [rng.randrange(1, 2 ** 31) for _ in range(2000)] + [2 ** 30, 2 ** 30 + 1, 2 ** 31 - 1]:
         s = 0

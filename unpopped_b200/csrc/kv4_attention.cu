@@ -72,7 +72,7 @@ extern "C" int up_sm100_kv4_attention(const void* q, int dtype, int64_t tokens, 
   a.pages = (uint32_t)cache->pages, a.kv_heads = (int)cache->kv_heads, a.ratio = (int)ratio, a.page_log2 = log2_of(cache->page);
   a.cpg = (int)(cache->group / 32), a.groups = (int)(cache->dim / cache->group);
   a.table = block_table, a.table_stride = table_stride, a.table_width = table_width;
-  a.lens = seq_lens, a.cu = cu_q, a.batch = (int)batch, a.causal = causal != 0;
+  a.lens = seq_lens, a.cu = cu_q, a.batch = (int)batch, a.causal = causal != 0, a.by_ratio = Divide32(ratio);
   a.window = (int)(window > kMaxTokens ? kMaxTokens : window);
   a.scale_log2 = scale * 1.44269504088896341f;
   a.header = static_cast<uint32_t*>(workspace);

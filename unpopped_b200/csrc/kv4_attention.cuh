@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "divide.cuh"
 #include "kv4.cuh"
 
 namespace up {
@@ -26,6 +27,7 @@ struct Args {
   int64_t table_stride, table_width;
   const int32_t *lens, *cu;
   int batch, causal, window;
+  Divide32 by_ratio;
   float scale_log2;                    // scale * log2(e): logits are kept in powers of two
   uint32_t* header;                    // workspace: its error word is header[3]
   uint32_t* counters;

@@ -13,15 +13,18 @@
 //    for the largest logit and for p = 2^(logit - ref), and writes P as f16 over it: the A operand of the second product.
 //    ref moves only when a logit is more than 2^8 above it; then the thread scales its row of O.
 //  * warp groups 2 and 3 (cache, K and V): read 128 tokens' nibbles and scales, a tile ahead in registers, and write
-//    them as f16 into 128-byte swizzled shared memory, two stages each. Both have a row a token: K is the B operand with
-//    its contraction (the dimensions) contiguous, V the one with its output (the dimensions) contiguous. The nibble
-//    conversion pairs dimensions k and k + 4 of each 8; q is stored in the same order and the output's columns are read
-//    in it.
+//    them as f16 into 128-byte swizzled shared memory: V in two stages, K in a place a half, free again when the half's
+//    logits are there. Both have a row a token: K is the B operand with its contraction (the dimensions) contiguous, V
+//    the one with its output (the dimensions) contiguous. The nibble conversion pairs dimensions k and k + 4 of each 8;
+//    q is stored in the same order and the output's columns are read in it.
 //  * warps 16 and 17 (products): each issues the tcgen05.mma of one query tile, so neither tile's products wait for the
 //    other's probabilities.
-// Scales. A tile's scales are divided by the power of two of the largest (separately for K and V), so nibble * scale
-// keeps f16's precision and range whatever their size; the logits take K's power, the probabilities V's, relative to
-// the largest one met (O is scaled when a larger one comes). nibble * scale and p are rounded to f16; all sums are f32.
+// Scales. The logits are exact up to their f32 sums, as the row's logsumexp is in f32. With one scale a token (ONE) K is
+// the nibbles themselves and a column of S is multiplied by its token's scale. With more, a tile's scales are divided by
+// the power of two of the largest and each is split into its first 8 bits and the rest: a nibble times either is exact
+// in f16, and the two products are added in the same S (half as much tensor work again). For V, whose products' sum is
+// rounded to 16 bits, nibble * (scale / the tile's power) and p are rounded to f16. The logits take K's power, the
+// probabilities V's, relative to the largest one met (O is scaled when a larger one comes). All sums are f32.
 // A token with an infinite or NaN v_scale is left out of the products (its rows would reach queries that do not see it)
 // and the queries that do see it become NaN.
 // Every wait is bounded; one that runs out sets the workspace's error word and the CTA unwinds.
@@ -39,14 +42,16 @@ namespace {
 constexpr int kRowsCta = 256, kTok = 128, kHalf = kTok / 2;
 constexpr int kThreads = 32 * 18, kCacheWarp = 8, kMmaWarp = 16;
 constexpr int kBlockBytes = kTok * 128;  // 128 rows of 64 dimensions (128 bytes), swizzled
+constexpr int kKBlockBytes = kHalf * 128;
 
 template <int D>
 struct Cfg {
   static constexpr int kBlocks = D / 64;
   static constexpr int kTile = kBlocks * kBlockBytes;       // 128 rows of D f16
-  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + 2 * kTile, kEnd = kV + 2 * kTile;
-  static constexpr int kScale = kEnd;                       // f16 [2 (K, V)][128][up to D / 32]
-  static constexpr int kSmem = kScale + 2 * kTok * (D / 32) * 2 + 1024 /* alignment */;
+  static constexpr int kPart = kTile / 2;                   // K of a half: 64 rows, its first bits or the rest
+  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + 4 * kPart, kEnd = kV + 2 * kTile;
+  static constexpr int kScale = kEnd;                       // K: f16 pairs [128][up to D / 32]; V: f16, the same
+  static constexpr int kSmem = kScale + kTok * (D / 32) * (4 + 2) + 1024 /* alignment */;
   static constexpr int kS = 0, kO = 2 * kTok;               // tensor memory columns: S (and P) of both tiles, then O
   static constexpr int kCols = 512;
 };
@@ -58,12 +63,13 @@ struct Meta {          // what the cache warps say of a tile of tokens
 };
 
 struct Shared {
-  uint64_t full[2][2], empty[2][2];  // [K, V][stage]
+  uint64_t full[2][2], empty[2][2];  // K: [0][half], V: [1][stage]
   uint64_t s_full[2][2], p_full[2][2], pv_done[2], all_done[2], drain;  // [query tile][half]
   uint32_t tmem;
   int abort;
   Meta meta[4];
-  float row_scale[kRowsCta];   // scale * log2(e) / the row's power of two
+  alignas(16) float k_scale[4][kTok];  // ONE: the tokens' scales
+  float row_scale[kRowsCta];   // |scale| * log2(e) / the row's power of two
   uint32_t big[2][4];          // [K, V][warp]
   int64_t scan[kThreads / 32], base;
   int seq;
@@ -127,7 +133,7 @@ __device__ __forceinline__ int64_t seq_ctas(const Args& a, int b) {
   return (int64_t)((s.nq * a.ratio + kRowsCta - 1) / kRowsCta) * a.kv_heads;
 }
 
-template <int D>
+template <int D, bool ONE>
 __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, const uint64_t wait_ns) {
   using C = Cfg<D>;
   constexpr int CH = D / 32;
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       for (int z = 0; z < 2; ++z) {
-        tc::mbar_init(&sh.full[z][i], 4);   // the cache group's warps
+        tc::mbar_init(&sh.full[z][i], z ? 4 : 2);  // the warps that fill it
         tc::mbar_init(&sh.empty[z][i], 2);  // a commit of each issuer
       }
       for (int h = 0; h < 2; ++h) {
@@ -196,16 +202,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
   const int in_seq = (int)(work - sh.base), tile = tiles - 1 - in_seq / a.kv_heads, head = in_seq % a.kv_heads;
   const int row0 = tile * kRowsCta, live = min(kRowsCta, rows - row0);
   int lo, hi;
-  visible(a, seq, row0 / a.ratio, (row0 + live - 1) / a.ratio, lo, hi);
+  visible(a, seq, (int)a.by_ratio(row0), (int)a.by_ratio(row0 + live - 1), lo, hi);
   const int tok0 = lo / kTok * kTok, n = hi > tok0 ? (hi - tok0 + kTok - 1) / kTok : 0;
 
-  // ---- queries: f16 with a power of two a row, swizzled ----
+  // ---- queries: f16 with a power of two a row and the logits' sign, swizzled ----
   constexpr int LPR = D / 8, STEP = kThreads / LPR;  // lanes a row, rows at a time
   constexpr int QN = (kRowsCta + STEP - 1) / STEP;
   uint4 qraw[QN];  // every load before the first use
 #pragma unroll
   for (int k = 0; k < QN; ++k) {
-    const int r = threadIdx.x / LPR + k * STEP, row = row0 + r, i = row / a.ratio;
+    const int r = threadIdx.x / LPR + k * STEP, row = row0 + r, i = (int)a.by_ratio(row);
     qraw[k] = make_uint4(0, 0, 0, 0);
     if (r < live)
       qraw[k] = __ldg(reinterpret_cast<const uint4*>(
@@ -225,13 +231,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     for (int d = 1; d < LPR; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d, LPR));
     const int ex = (int)(__float_as_uint(big) >> 23) - 127;  // the row's largest magnitude becomes 2^7 .. 2^8
     const int up = big == 0.f || ex == 128 ? 0 : min(7 - ex, 126);
-    const float m = pow2f(up);
+    const float m = a.scale_log2 < 0.f ? -pow2f(up) : pow2f(up);
     uint4 w;
     w.x = pack2_f16(f[0] * m, f[4] * m), w.y = pack2_f16(f[1] * m, f[5] * m);
     w.z = pack2_f16(f[2] * m, f[6] * m), w.w = pack2_f16(f[3] * m, f[7] * m);
     *reinterpret_cast<uint4*>(smem + C::kQ + (r / 128) * C::kTile + (c / 8) * kBlockBytes + (r % 128) * 128 +
                               ((c % 8) ^ (r & 7)) * 16) = w;
-    if (c == 0) sh.row_scale[r] = a.scale_log2 * pow2f(-up);
+    if (c == 0) sh.row_scale[r] = fabsf(a.scale_log2) * pow2f(-up);
   }
   static_assert(kThreads % LPR == 0 && kRowsCta % (32 / LPR) == 0, "whole rows a warp");
   tc::fence_proxy_async_smem();
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     const int w = warp >> 2, r = threadIdx.x;  // r: the CTA's row
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const uint32_t ts = tmem + C::kS + w * kTok + lanes, to = tmem + C::kO + w * D + lanes;
-    const int row = row0 + r, pos = seq.len - seq.nq + row / a.ratio;
+    const int row = row0 + r, pos = seq.len - seq.nq + (int)a.by_ratio(row);
     const int last = r >= live ? -1 : a.causal ? min(pos, seq.len - 1) : seq.len - 1;
     const int past = a.window > 0 ? max(pos - a.window, -1) : -1;
     const float row_scale = sh.row_scale[r];
@@ -270,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       const Meta& meta = sh.meta[t & 3];
       const int j0 = tok0 + u * kHalf;
       const uint32_t th = ts + h * kHalf;
-      const float c = row_scale * pow2f(meta.k_exp);
+      const float c = ONE ? row_scale : row_scale * pow2f(meta.k_exp);
       const int ve = meta.v_exp;
       const uint32_t valid0 = meta.valid[2 * h], valid1 = meta.valid[2 * h + 1];
       const bool masked = !__all_sync(0xffffffffu, (valid0 & valid1) == 0xffffffffu && j0 > past && j0 + kHalf - 1 <= last);
@@ -282,13 +288,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         m &= to_ <= 0 ? 0u : to_ >= 32 ? 0xffffffffu : (1u << to_) - 1u;
         return m;
       };
+      auto logits = [&](int g, uint32_t (&v)[32]) {  // in units of c
+        ld_x32(th + 32 * g, v);
+        tc::wait_ld();
+        if (ONE) {
+          const float4* ks = reinterpret_cast<const float4*>(sh.k_scale[t & 3] + h * kHalf + 32 * g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 k = ks[i];
+            v[4 * i] = __float_as_uint(__uint_as_float(v[4 * i]) * k.x);
+            v[4 * i + 1] = __float_as_uint(__uint_as_float(v[4 * i + 1]) * k.y);
+            v[4 * i + 2] = __float_as_uint(__uint_as_float(v[4 * i + 2]) * k.z);
+            v[4 * i + 3] = __float_as_uint(__uint_as_float(v[4 * i + 3]) * k.w);
+          }
+        }
+      };
       // the largest logit, against the reference
-      float m = mx;
+      float m = -INFINITY;
 #pragma unroll 1
       for (int g = 0; g < 2; ++g) {
         uint32_t v[32];
-        ld_x32(th + 32 * g, v);
-        tc::wait_ld();
+        logits(g, v);
         if (masked) {
           const uint32_t see = seen(g);
 #pragma unroll
@@ -297,11 +317,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         float m1 = m;
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          m = fmaxf(m, __uint_as_float(v[i]) * c);
-          m1 = fmaxf(m1, __uint_as_float(v[i + 1]) * c);
+          m = fmaxf(m, __uint_as_float(v[i]));
+          m1 = fmaxf(m1, __uint_as_float(v[i + 1]));
         }
         m = fmaxf(m, m1);
       }
+      m = fmaxf(mx, m * c);  // c is not negative; where nothing is seen, -infinity or (c = 0) NaN
       if (__any_sync(0xffffffffu, m > mx + 8.f || ve > vexp)) {
         const int e = max(vexp, ve);
         const float f = exp2_approx(mx - m), fo = f * pow2f(vexp - e);
@@ -331,8 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
 #pragma unroll 1
       for (int g = 0; g < 2; ++g) {
         uint32_t v[32], p[16];
-        ld_x32(th + 32 * g, v);
-        tc::wait_ld();
+        logits(g, v);
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(v[i]), c, add)));
         if (masked) {
@@ -384,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       __syncwarp();
 #pragma unroll 1
       for (int k = 0; k < LPR; ++k) {  // 32 / LPR rows at a time
-        const int rr = (r & ~31) + k * (32 / LPR) + lane / LPR, c = lane % LPR, out_row = row0 + rr, i = out_row / a.ratio;
+        const int rr = (r & ~31) + k * (32 / LPR) + lane / LPR, c = lane % LPR, out_row = row0 + rr, i = (int)a.by_ratio(out_row);
         if (rr >= live) break;
         const uint4 v = *reinterpret_cast<const uint4*>(tile_rows + (c / 8) * kBlockBytes + (rr % 128) * 128 +
                                                         ((c % 8) ^ (rr & 7)) * 16);
@@ -397,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
           *reinterpret_cast<uint2*>(dst + 8) = make_uint2(v.z, v.w);
         }
       }
-      const int i = row / a.ratio, head_q = head * a.ratio + row - i * a.ratio;
+      const int i = (int)a.by_ratio(row), head_q = head * a.ratio + row - i * a.ratio;
       const int64_t tk = seq.q0 + i;
       if (a.lse && r < live) a.lse[tk * a.ls + head_q] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
     }
@@ -406,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     const int z = (warp - kCacheWarp) >> 2, w = warp & 3, tid = threadIdx.x & 127, groups = a.groups;
     const uint8_t* nibbles = z ? a.v4 : a.k4;
     const __half* scales = z ? a.v_scale : a.k_scale;
-    __half* sc = reinterpret_cast<__half*>(smem + C::kScale) + z * kTok * CH;
+    uint32_t* sc_k = reinterpret_cast<uint32_t*>(smem + C::kScale);  // f16 pairs: a scale's first 8 bits, the rest
+    __half* sc_v = reinterpret_cast<__half*>(smem + C::kScale + 4 * kTok * CH);
     const int32_t* pages = a.table + (int64_t)b * a.table_stride;
     const int in_page = (1 << a.page_log2) - 1, cpg_log2 = 31 - __clz(a.cpg);  // 1, 2 or 4 chunks a group
     auto page_of = [&](int t) {
@@ -438,25 +459,50 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         if (g < groups && page >= 0) sk[g] = __half_as_ushort(__ldg(scales + line * groups + g));
       }
     };
-    auto convert = [&](uint32_t dst) {
+    auto put = [](uint32_t at, const uint32_t (&e)[4]) {
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(e[0]), "r"(e[1]), "r"(e[2]), "r"(e[3]) : "memory");
+    };
+    auto times = [](const uint32_t (&e)[4], __half2 s, uint32_t (&o)[4]) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&e[x]), s);
+        o[x] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    };
+    auto convert = [&](int t) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int u = (lane >> 3) + 4 * i, run = u / CH, c = u - run * CH, tok = 32 * w + 8 * run + (lane & 7);
-        const __half2 s = __half2half2(sc[tok * groups + (c >> cpg_log2)]);
         const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-        const uint32_t at = dst + (c / 2) * kBlockBytes + tok * 128;
+        const int in_row = tok * groups + (c >> cpg_log2);
+        if (z) {
+          const __half2 s = __half2half2(sc_v[in_row]);
+          const uint32_t at = sbase + C::kV + (t & 1) * C::kTile + (c / 2) * kBlockBytes + tok * 128;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t e[4];
-          expand(words[k], e);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&e[x]), s);
-            e[x] = *reinterpret_cast<const uint32_t*>(&v);
+          for (int k = 0; k < 4; ++k) {
+            uint32_t e[4];
+            expand(words[k], e);
+            times(e, s, e);
+            put(at + ((((c & 1) * 4 + k) ^ (tok & 7)) << 4), e);
           }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + ((((c & 1) * 4 + k) ^ (tok & 7)) << 4)),
-                       "r"(e[0]), "r"(e[1]), "r"(e[2]), "r"(e[3])
-                       : "memory");
+        } else {
+          const __half2 s = ONE ? __half2() : *reinterpret_cast<const __half2*>(&sc_k[in_row]);
+          const uint32_t at = sbase + C::kK + (tok / kHalf) * 2 * C::kPart + (c / 2) * kKBlockBytes + (tok % kHalf) * 128;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t to = at + ((((c & 1) * 4 + k) ^ (tok & 7)) << 4);
+            uint32_t e[4];
+            expand(words[k], e);
+            if (ONE) {
+              put(to, e);
+            } else {
+              uint32_t o[4];
+              times(e, __low2half2(s), o);
+              put(to, o);
+              times(e, __high2half2(s), o);
+              put(to + C::kPart, o);
+            }
+          }
         }
       }
     };
@@ -467,44 +513,59 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     }
     for (int t = 0; t < n; ++t) {
       const int next = page_of(t + 1);
-      // the tile's power of two, and its scales divided by it
-      uint32_t big = 0;
-      bool bad = false;
-#pragma unroll
-      for (int g = 0; g < CH; ++g) {
-        const uint32_t m = sk[g] & 0x7fffu;
-        if (m < 0x7c00u) big = max(big, m);
-        bad |= m >= 0x7c00u;
-      }
-      big = __reduce_max_sync(0xffffffffu, big);
       Meta& meta = sh.meta[t & 3];
-      const uint32_t marks = __ballot_sync(0xffffffffu, z ? bad : page >= 0);
-      if (lane == 0) {
-        sh.big[z][w] = big;
-        (z ? meta.bad : meta.valid)[w] = marks;
-      }
-      cache_sync(z);  // also: every warp is done with the last tile's scales
-      big = max(max(sh.big[z][0], sh.big[z][1]), max(sh.big[z][2], sh.big[z][3]));
-      const int e = big ? (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)big))) >> 23) - 127 : -24;
+      if (ONE && !z) {
+        const float k = __half2float(__ushort_as_half(sk[0]));
+        sh.k_scale[t & 3][tid] = fabsf(k) < INFINITY ? k : __int_as_float(0x7fffffff);
+        const uint32_t marks = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) meta.valid[w] = marks;
+      } else {
+        // the tile's power of two, and its scales divided by it
+        uint32_t big = 0;
+        bool bad = false;
 #pragma unroll
-      for (int g = 0; g < CH; ++g)
-        if (g < groups)  // a value that is not finite is left out (its token is marked); such a key makes its logit NaN
-          sc[tid * groups + g] = z && (sk[g] & 0x7fffu) >= 0x7c00u
-                                     ? __half(0)
-                                     : __float2half_rn(__half2float(__ushort_as_half(sk[g])) * pow2f(-e));
-      if (tid == 0) (z ? meta.v_exp : meta.k_exp) = e;
-      cache_sync(z);
+        for (int g = 0; g < CH; ++g) {
+          const uint32_t m = sk[g] & 0x7fffu;
+          if (m < 0x7c00u) big = max(big, m);
+          bad |= m >= 0x7c00u;
+        }
+        big = __reduce_max_sync(0xffffffffu, big);
+        const uint32_t marks = __ballot_sync(0xffffffffu, z ? bad : page >= 0);
+        if (lane == 0) {
+          sh.big[z][w] = big;
+          (z ? meta.bad : meta.valid)[w] = marks;
+        }
+        cache_sync(z);  // also: every warp is done with the last tile's scales
+        big = max(max(sh.big[z][0], sh.big[z][1]), max(sh.big[z][2], sh.big[z][3]));
+        const int e = big ? (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)big))) >> 23) - 127 : -24;
+#pragma unroll
+        for (int g = 0; g < CH; ++g) {
+          if (g >= groups) continue;
+          const bool finite = (sk[g] & 0x7fffu) < 0x7c00u;
+          const uint32_t s = __half_as_ushort(__float2half_rn(__half2float(__ushort_as_half(sk[g])) * pow2f(-e)));
+          if (z) {  // a value that is not finite is left out: its token is marked
+            sc_v[tid * groups + g] = __ushort_as_half((unsigned short)(finite ? s : 0u));
+          } else {  // such a key makes its logit NaN
+            const uint32_t first = s & 0xfff8u;
+            const __half rest = __hsub(__ushort_as_half((unsigned short)s), __ushort_as_half((unsigned short)first));
+            sc_k[tid * groups + g] = finite ? first | (uint32_t)__half_as_ushort(rest) << 16 : 0x7fff7fffu;
+          }
+        }
+        if (tid == 0) (z ? meta.v_exp : meta.k_exp) = e;
+        cache_sync(z);
+      }
       page = next;
       if (t + 1 < n) fetch_scales(t + 1, page);
-      const int s = t & 1;
-      if (__all_sync(0xffffffffu, tc::mbar_wait(&sh.empty[z][s], ((t >> 1) & 1) ^ 1, wait_ns, abort_flag))) {
-        convert(sbase + (z ? C::kV : C::kK) + s * C::kTile);
+      // where it goes: K's place of this warp's half, filled once a tile; V's stage, every second one
+      const int s = z ? t & 1 : w >> 1, turn = z ? t >> 1 : t;
+      if (__all_sync(0xffffffffu, tc::mbar_wait(&sh.empty[z][s], (turn & 1) ^ 1, wait_ns, abort_flag))) {
+        convert(t);
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&sh.full[z][s]);
         if (t + 1 < n) fetch(t + 1, page);
       } else {
-        give_up();  // the named barrier still counts this warp: it keeps step with the others, without the work
+        give_up();  // a named barrier still counts this warp: it keeps step with the others, without the work
       }
     }
   } else {
@@ -519,27 +580,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       auto wait = [&](uint64_t* bar, int parity) {
         return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity & 1, wait_ns, abort_flag)) != 0;
       };
-      auto qk = [&](int t, int h) {
-        const uint64_t k = k0 + (uint64_t)((t & 1) * (C::kTile >> 4) + h * (kHalf * 128 >> 4));
+      auto qk = [&](int h) {
+        const uint64_t k = k0 + (uint64_t)(h * (2 * C::kPart >> 4));
         if (elect_one()) {
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) {  // 16 dimensions: 32 bytes
-            const uint64_t at = (uint64_t)((i / 4) * (kBlockBytes >> 4) + (i % 4) * 2);
-            mma_ss(ts + h * kHalf, q0 + at, k + at, id_qk, i > 0);
+          for (int x = 0; x < (ONE ? 1 : 2) * (D / 16); ++x) {  // 16 dimensions: 32 bytes; the scales' first bits, the rest
+            const int i = x % (D / 16), part = x / (D / 16);
+            mma_ss(ts + h * kHalf, q0 + (uint64_t)((i / 4) * (kBlockBytes >> 4) + (i % 4) * 2),
+                   k + (uint64_t)(part * (C::kPart >> 4) + (i / 4) * (kKBlockBytes >> 4) + (i % 4) * 2), id_qk, x > 0);
           }
           tc::mbar_arrive(&sh.s_full[w][h]);
           tc::commit(&sh.s_full[w][h]);
-          if (h == 1) tc::commit(&sh.empty[0][t & 1]);
+          tc::commit(&sh.empty[0][h]);
         }
         __syncwarp();
       };
-      // a tile's K and V are waited for together: its meta has both groups' part
-      auto cached = [&](int t) { return wait(&sh.full[0][t & 1], t >> 1) && wait(&sh.full[1][t & 1], t >> 1); };
-      bool ok = cached(0);
-      if (ok) {
+      // K of a half, and with the first one the tile's V: the tile's meta has both groups' part
+      auto cached = [&](int t, int h) { return wait(&sh.full[0][h], t) && (h == 1 || wait(&sh.full[1][t & 1], t >> 1)); };
+      bool ok = true;
+      for (int h = 0; ok && h < 2; ++h) {
+        ok = cached(0, h);
+        if (!ok) break;
         tc::fence_after_sync();
-        qk(0, 0);
-        qk(0, 1);
+        qk(h);
       }
 #pragma unroll 1
       for (int u = 0; ok && u < 2 * n; ++u) {
@@ -558,10 +621,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         }
         __syncwarp();
         if (t + 1 == n) continue;
-        if (h == 0) ok = cached(t + 1);
+        ok = cached(t + 1, h);
         if (!ok) break;
         tc::fence_after_sync();
-        qk(t + 1, h);  // over S and P of tile t's half: issued after the products that read them
+        qk(h);  // over S and P of tile t's half: issued after the products that read them
       }
       if (!ok) give_up();
       if (elect_one()) tc::commit(&sh.drain);  // nothing may be in flight when the tensor memory goes
@@ -574,9 +637,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
   if (warp == kMmaWarp) tc::tmem_dealloc(tmem, C::kCols);
 }
 
-template <int D>
+template <int D, bool ONE>
 int launch_prompt(const Args& a, int64_t ctas, cudaStream_t s) {
-  const auto kernel = kv4_prompt_kernel<D>;
+  const auto kernel = kv4_prompt_kernel<D, ONE>;
   const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), Cfg<D>::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
   kernel<<<(unsigned)ctas, kThreads, Cfg<D>::kSmem, s>>>(a, wait_limit_ns());
@@ -589,7 +652,8 @@ int launch_prompt(const Args& a, int64_t ctas, cudaStream_t s) {
 int prompt_attention(const Args& a, int dim, cudaStream_t s) {
   const int64_t ctas = (a.tokens * a.ratio / kRowsCta + a.batch) * a.kv_heads;
   if (ctas > 0x7fffffff) return UP_ERR_UNSUPPORTED;
-  return dim == 64 ? launch_prompt<64>(a, ctas, s) : launch_prompt<128>(a, ctas, s);
+  if (dim == 64) return a.groups == 1 ? launch_prompt<64, true>(a, ctas, s) : launch_prompt<64, false>(a, ctas, s);
+  return a.groups == 1 ? launch_prompt<128, true>(a, ctas, s) : launch_prompt<128, false>(a, ctas, s);
 }
 
 }  // namespace kv4

@@ -87,7 +87,7 @@ constexpr int kTileCost = 2;
 // Units of one (tile, head) of a sequence: at least one, which writes the rows that see nothing.
 template <int ROWS>
 __device__ __forceinline__ int tile_units(const Args& a, const Seq& s, int tile, int& unit0) {
-  const int rows = s.nq * a.ratio, i0 = tile * ROWS / a.ratio, i1 = (min((tile + 1) * ROWS, rows) - 1) / a.ratio;
+  const int rows = s.nq * a.ratio, i0 = (int)a.by_ratio(tile * ROWS), i1 = (int)a.by_ratio(min((tile + 1) * ROWS, rows) - 1);
   int lo, hi;
   visible(a, s, i0, i1, lo, hi);
   unit0 = lo / kUnitTokens;
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
     s_base = base;
   }
   __syncthreads();
-  int b = s_seq;
+  int b = s_seq, tile = 0;
   int64_t off = u - s_base;
 
   const uint32_t smem_base = smem_addr(smem), ring = smem_base + warp * (C::kStages * C::kStage);
@@ -179,20 +179,20 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
   while (u < u1) {
     const Seq seq = load_seq(a, b);
     const int rows = seq.nq * a.ratio, tiles = (rows + ROWS - 1) / ROWS;
-    int tile = 0, unit0 = 0, n_units = 0;
-    int64_t in_tile = off;  // off counts from the sequence's first unit
-    for (; tile < tiles; ++tile) {
+    int unit0 = 0, n_units = 0;
+    for (; tile < tiles; ++tile) {  // off counts from this tile's first head
       n_units = tile_units<ROWS>(a, seq, tile, unit0);
-      if (in_tile < (int64_t)(n_units + kTileCost) * a.kv_heads) break;
-      in_tile -= (int64_t)(n_units + kTileCost) * a.kv_heads;
+      if (off < (int64_t)(n_units + kTileCost) * a.kv_heads) break;
+      off -= (int64_t)(n_units + kTileCost) * a.kv_heads;
     }
     if (tile == tiles) {  // past this sequence's last unit
       ++b;
+      tile = 0;
       off = 0;
       continue;
     }
     // a tile's share is its cost and then its units: this CTA has [at, at + take) of it, the units [first, first + count)
-    const int head = (int)divide(in_tile, n_units + kTileCost), at = (int)(in_tile - (int64_t)head * (n_units + kTileCost));
+    const int head = (int)divide(off, n_units + kTileCost), at = (int)(off - (int64_t)head * (n_units + kTileCost));
     const int take = (int)min((int64_t)(n_units + kTileCost - at), u1 - u);
     const int first = max(at - kTileCost, 0), count = max(at + take - kTileCost, 0) - first;
     const int64_t tile_u0 = u - at + kTileCost;  // the share of the first unit
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
     uint4 raw[NT][CH];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = tile * ROWS + nt * 8 + g, i = row / a.ratio;
+      const int row = tile * ROWS + nt * 8 + g, i = (int)a.by_ratio(row);
       const char* src = static_cast<const char*>(a.q) + 2 * ((seq.q0 + i) * a.qs + (int64_t)(head * a.ratio + row - i * a.ratio) * a.qh);
 #pragma unroll
       for (int c = 0; c < CH; ++c)
@@ -325,13 +325,13 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
         const int s2 = __shfl_sync(0xffffffffu, sh, 4 * (2 * t + j));
         qs[nt][j] = a.scale_log2 * 0x1p24f * __uint_as_float((uint32_t)(127 - s2) << 23);
         const int r2 = tile * ROWS + nt * 8 + 2 * t + j;
-        const int pos = seq.len - seq.nq + r2 / a.ratio;
+        const int pos = seq.len - seq.nq + (int)a.by_ratio(r2);
         last[nt][j] = r2 >= rows ? -1 : a.causal ? min(pos, seq.len - 1) : seq.len - 1;
         past[nt][j] = a.window > 0 ? max(pos - a.window, -1) : -1;
       }
     }
     // every query of the tile sees the tokens (all_past, all_last]
-    const int i0 = tile * ROWS / a.ratio, i1 = (min((tile + 1) * ROWS, rows) - 1) / a.ratio;
+    const int i0 = (int)a.by_ratio(tile * ROWS), i1 = (int)a.by_ratio(min((tile + 1) * ROWS, rows) - 1);
     const int all_last = a.causal ? seq.len - seq.nq + i0 : seq.len - 1;
     const int all_past = a.window > 0 ? seq.len - seq.nq + i1 - a.window : -1;
 
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
     const int live = min(ROWS, rows - tile * ROWS);
     // a row's output from its sums (in f32) and its place
     auto store = [&](int r, int d, float4 o, float m, float l) {
-      const int row = tile * ROWS + r, i = row / a.ratio;
+      const int row = tile * ROWS + r, i = (int)a.by_ratio(row);
       const int64_t tk = seq.q0 + i;
       const int h = head * a.ratio + row - i * a.ratio;
       const float inv = l == 0.f ? 0.f : 1.f / l;
