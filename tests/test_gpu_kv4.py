@@ -372,6 +372,71 @@ def test_prompts_with_a_nan_in_a_token_of_one_scale():
         cache[which][int(table[0, j // 16]), 0, j % 16, 0] = keep
 
 
+@pytest.mark.parametrize("dim,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("ratio", [12, 29])
+def test_prompts_of_many_rows(dim, group, ratio):
+    """Enough rows that they are shared by tiles of 256 at either head size."""
+    lens, nq = [900, 513, 300, 0, 128, 129], [900, 250, 1, 3, 128, 200]
+    cache, table, n = make(6, 2, dim, group, 32, lens, seed=5)
+    cu = torch.tensor([0] + nq, device="cuda").cumsum(0).int()
+    for kind, window, causal in ((torch.bfloat16, 0, True), (torch.float16, 200, True), (torch.float16, 0, False)):
+        q = torch.randn(sum(nq), 2 * ratio, dim, device="cuda").to(kind)
+        check(q, cache, table, n, cu, causal, window)
+    packed = torch.randn(sum(nq), 2 * ratio + 3, dim, device="cuda").half()
+    out = torch.zeros_like(packed)
+    ops.kv4_attention(packed[:, 2:-1], cache, table, n, cu_q=cu, out=out[:, 1:-2])
+    assert torch.equal(out[:, 1:-2], check(packed[:, 2:-1], cache, table, n, cu))
+    assert bool((out[:, 0] == 0).all()) and bool((out[:, -2:] == 0).all())
+
+
+@pytest.mark.parametrize("dim,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("scale", [None, -0.2])
+def test_prompts_of_many_rows_keep_the_logits_of_32_bits(dim, group, scale):
+    """As test_prompts_keep_the_logits_of_32_bits: the same sums, the same bound."""
+    cache, table, n = make(1, 1, dim, group, 16, [500], seed=31)
+    cu = torch.tensor([0, 400], device="cuda").int()
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    q = torch.randn(400, 45, dim, generator=g, device="cuda").bfloat16()
+    _, lse = ops.kv4_attention(q, cache, table, n, cu_q=cu, scale=scale, want_lse=True)
+    _, want, _, _ = reference(q, cache, table, n, cu, True, 0, dim ** -0.5 if scale is None else scale)
+    assert float((lse.double() - want).norm() / want.norm()) <= 2.0 ** -19
+
+
+def test_prompts_of_many_rows_with_scales_far_apart():
+    cache, table, n = make(1, 1, 64, 32, 16, [700], seed=21, spread=4.0)
+    j = torch.arange(700, device="cuda")
+    page, at = table[0, j // 16].long(), j % 16
+    cache[2][page, 0, at] *= (0.1 + j / 100)[:, None].half()
+    cache[3][page, 0, at] *= (2.0 ** (12 * (j / 700 - 0.5).abs() - 8))[:, None].half()
+    cu = torch.tensor([0, 700], device="cuda").int()
+    check(torch.randn(700, 24, 64, device="cuda").bfloat16(), cache, table, n, cu, scale=0.125)
+    check((torch.randn(700, 24, 64, device="cuda") * 1e30).bfloat16(), cache, table, n, cu, scale=1e-31)
+    check((torch.randn(700, 24, 64, device="cuda") * 1e-3).half(), cache, table, n, cu, scale=-90.0)
+    check(torch.zeros(700, 24, 64, device="cuda").half(), cache, table, n, cu)
+
+
+@pytest.mark.parametrize("dim,group", [(64, 64), (128, 64)])
+def test_prompts_of_many_rows_with_a_nan_and_pages_outside(dim, group):
+    cache, table, n = make(1, 1, dim, group, 16, [300], seed=4)
+    j = 200
+    cu = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    q = torch.randn(300, 60, dim, device="cuda").bfloat16()
+    clean = ops.kv4_attention(q, cache, table, n, cu_q=cu)
+    for which in (3, 2):
+        keep = cache[which][int(table[0, j // 16]), 0, j % 16, -1].clone()
+        for bad in (float("nan"), float("inf")):
+            cache[which][int(table[0, j // 16]), 0, j % 16, -1] = bad
+            out = ops.kv4_attention(q, cache, table, n, cu_q=cu)
+            assert torch.equal(out[:j], clean[:j])
+            assert not bool(torch.isfinite(out[j:, :, -group:]).any())
+        cache[which][int(table[0, j // 16]), 0, j % 16, -1] = keep
+    bad = table.clone()
+    bad[0, 3] = -1
+    got = ops.kv4_attention(q, cache, bad, n, cu_q=cu)
+    assert torch.equal(got[:48], clean[:48]) and bool(torch.isfinite(got).all())
+    assert not torch.equal(got[64:], clean[64:])
+
+
 def test_a_long_sequence_is_split_over_the_gpu():
     lens = [70001]
     cache, table, n = make(1, 1, 128, 128, 64, lens, seed=9)
@@ -540,3 +605,14 @@ def test_refusals():
             ops.kv4_append(x, x, c, n)
         with pytest.raises(_lib.UpError):
             ops.kv4_attention(x, c, table, n)
+
+
+@pytest.mark.parametrize("dim,group", [(64, 64), (128, 128), (96, 32), (256, 256)])
+def test_an_infinite_key_scale_makes_its_logit_nan(dim, group):
+    """A nibble of 0 times it is NaN, so the rows that see the token are, whatever the sign of the other products."""
+    cache, table, n = make(1, 1, dim, group, 16, [200], seed=8)
+    cu = torch.tensor([0, 4], device="cuda").int()
+    q = torch.randn(4, 16, dim, device="cuda").bfloat16()
+    cache[2][int(table[0, 198 // 16]), 0, 198 % 16, 0] = float("inf")
+    out = ops.kv4_attention(q, cache, table, n, cu_q=cu)
+    assert bool(out[2:].isnan().all()) and not bool(out[:2].isnan().any())

@@ -79,7 +79,7 @@ extern "C" int up_sm100_kv4_attention(const void* q, int dtype, int64_t tokens, 
   a.counters = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + kHeaderBytes);
   a.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
   const int64_t per = (tokens + batch - 1) / batch * ratio;  // query rows a sequence and key/value head
-  if (per >= kPromptRows && (cache->dim == 64 || cache->dim == 128))
+  if (many_rows(per, batch * cache->kv_heads, cache->dim, sm_count()))
     return prompt_attention(a, (int)cache->dim, static_cast<cudaStream_t>(stream));
   const int rows = split_rows(per, cache->dim);
   return split_attention(a, (int)cache->dim, rows, split_ctas(), static_cast<cudaStream_t>(stream));

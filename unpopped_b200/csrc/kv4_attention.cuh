@@ -198,13 +198,26 @@ constexpr int kMaxRows = 16;                   // query rows of a tile at most
 constexpr int kGroup = 16;                     // parts of a split tile that are added at once
 constexpr size_t kHeaderBytes = 256, kCounterBytes = kHeaderBytes + 3 * kMaxCtas * sizeof(uint32_t);
 
-// Query rows a tile has in the split kernel: 8 a column group, a second one where the head size leaves registers.
+// Query rows a tile has in the split kernel: 8 a column group, a second one where the head size leaves registers (not
+// above 128) and the rows of a sequence and key/value head need it. Measured with 64 sequences of 2048 tokens, 8 key/value
+// heads of 128: 8 rows 41 us in tiles of 8 and 53 of 16, 12 rows 68 and 55, 32 rows 123 and 97; one sequence of 2048, where
+// little but the start counts: 8 rows 10.1 and 11.7, 32 rows 12.5 and 15.4.
 inline int split_rows(int64_t rows_a_sequence, int64_t dim) {
   return rows_a_sequence > 8 && (dim == 64 || dim == 96 || dim == 128) ? 16 : 8;
 }
 
-// Query rows a sequence and key/value head from which the prompt kernel runs (head sizes 64 and 128).
-constexpr int64_t kPromptRows = 64;
+// Whether the kernel for many query rows (head sizes 64 and 128; 256 rows a CTA, one CTA an SM) takes less time than the
+// split one, given `rows` query rows for each of `pairs` (sequence, key/value head): the first in as many turns as its
+// CTAs fill the SMs, the second in 16-row tiles that are spread evenly. Against as many cached tokens a 256-row tile takes
+// an SM as long as five 16-row ones at head size 128 and seven at 64 (2.75 and 2.4 us a 128 tokens). Measured over one
+// sequence of 32768 tokens to 32 of 2048, 8 key/value heads, 8 to 1024 rows each, the faster one is taken but within 4 %:
+// 12 sequences of 4096 at size 128, 96 rows 99 us split and 116 not, 128 rows 127 and 114; 4 of them, 256 rows 90 and 102,
+// 384 rows 128 and 113; at size 64, 12 of them, 128 rows 82 and 107, 192 rows 116 and 102.
+inline bool many_rows(int64_t rows, int64_t pairs, int64_t dim, int64_t sms) {
+  if (dim != 64 && dim != 128) return false;
+  const int64_t turns = (pairs * ((rows + 255) / 256) + sms - 1) / sms;
+  return turns * sms * (dim == 64 ? 7 : 5) < pairs * ((rows + 15) / 16);
+}
 int prompt_attention(const Args& a, int dim, cudaStream_t s);
 
 int split_attention(const Args& a, int dim, int tile_rows, int ctas, cudaStream_t s);  // by head size

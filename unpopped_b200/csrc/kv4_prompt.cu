@@ -19,12 +19,13 @@
 //    q is stored in the same order and the output's columns are read in it.
 //  * warps 16 and 17 (products): each issues the tcgen05.mma of one query tile, so neither tile's products wait for the
 //    other's probabilities.
-// Scales. The logits are exact up to their f32 sums, as the row's logsumexp is in f32. With one scale a token (ONE) K is
-// the nibbles themselves and a column of S is multiplied by its token's scale. With more, a tile's scales are divided by
-// the power of two of the largest and each is split into its first 8 bits and the rest: a nibble times either is exact
-// in f16, and the two products are added in the same S (half as much tensor work again). For V, whose products' sum is
-// rounded to 16 bits, nibble * (scale / the tile's power) and p are rounded to f16. The logits take K's power, the
-// probabilities V's, relative to the largest one met (O is scaled when a larger one comes). All sums are f32.
+// Scales. A tile's scales are divided by the power of two of the largest (separately for K and V), so nibble * scale
+// keeps f16's range whatever their size; the logits take K's power, the probabilities V's, relative to the largest one
+// met (O is scaled when a larger one comes). The logits are exact up to their f32 sums, as a row's logsumexp is in f32:
+// each of K's scales is split into its first 8 bits and the rest, a nibble times either is exact in f16, and both
+// products are added in one S. That is half as much tensor work again, which the probabilities hide (prompts of 1500 to
+// 2048 tokens 314 -> 320 us; with one scale a token, multiplying the columns of S by it in the softmax instead took
+// 381). V's products end in 16 bits: there nibble * scale, and p, are rounded to f16. All sums are f32.
 // A token with an infinite or NaN v_scale is left out of the products (its rows would reach queries that do not see it)
 // and the queries that do see it become NaN.
 // Every wait is bounded; one that runs out sets the workspace's error word and the CTA unwinds.
@@ -64,15 +65,11 @@ struct Meta {          // what the cache warps say of a tile of tokens
 
 struct Shared {
   uint64_t full[2][2], empty[2][2];  // K: [0][half], V: [1][stage]
-  uint64_t s_full[2][2], p_full[2][2], pv_done[2], all_done[2], drain;  // [query tile][half]
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], all_done[2], q_full, drain;  // [query tile][half]
   uint32_t tmem;
   int abort;
   Meta meta[4];
-  alignas(16) float k_scale[4][kTok];  // ONE: the tokens' scales
-  float row_scale[kRowsCta];   // |scale| * log2(e) / the row's power of two
   uint32_t big[2][4];          // [K, V][warp]
-  int64_t scan[kThreads / 32], base;
-  int seq;
 };
 
 __device__ __forceinline__ uint64_t desc_v(uint32_t addr) {  // dimensions contiguous: 64-dimension blocks kBlockBytes apart
@@ -124,16 +121,11 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23); }
-template <int ID>
-__device__ __forceinline__ void named_sync() { asm volatile("bar.sync %0, 128;" ::"n"(ID) : "memory"); }
-__device__ __forceinline__ void cache_sync(int z) { z ? named_sync<2>() : named_sync<1>(); }  // K's, V's group
+template <int ID, int THREADS>
+__device__ __forceinline__ void named_sync() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(THREADS) : "memory"); }
+__device__ __forceinline__ void cache_sync(int z) { z ? named_sync<2, 128>() : named_sync<1, 128>(); }  // K's, V's group
 
-__device__ __forceinline__ int64_t seq_ctas(const Args& a, int b) {
-  const Seq s = load_seq(a, b);
-  return (int64_t)((s.nq * a.ratio + kRowsCta - 1) / kRowsCta) * a.kv_heads;
-}
-
-template <int D, bool ONE>
+template <int D>
 __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, const uint64_t wait_ns) {
   using C = Cfg<D>;
   constexpr int CH = D / 32;
@@ -143,37 +135,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
   const uint32_t sbase = smem_addr(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // ---- which sequence, tile and head: sequences in order, a sequence's last (longest) tiles first ----
-  const int per = (a.batch + kThreads - 1) / kThreads;
-  const int my0 = min((int)threadIdx.x * per, a.batch), my1 = min(my0 + per, a.batch);
-  int64_t mine = 0;
-  for (int b = my0; b < my1; ++b) mine += seq_ctas(a, b);
-  int64_t incl = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += v;
-  }
-  if (lane == 31) sh.scan[warp] = incl;
-  __syncthreads();
-  int64_t before = incl - mine, total = 0;
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += sh.scan[w];
-    total += sh.scan[w];
-  }
-  const int64_t work = blockIdx.x;
-  if (work >= total) return;
-  if (work >= before && work < before + mine) {
-    int64_t base = before;
-    int b = my0;
-    for (;; ++b) {
-      const int64_t n = seq_ctas(a, b);
-      if (work < base + n) break;
-      base += n;
-    }
-    sh.seq = b;
-    sh.base = base;
-  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       for (int z = 0; z < 2; ++z) {
@@ -187,6 +148,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       tc::mbar_init(&sh.pv_done[i], 1);
       tc::mbar_init(&sh.all_done[i], 1);
     }
+    tc::mbar_init(&sh.q_full, kCacheWarp);
     tc::mbar_init(&sh.drain, 2);
     tc::mbar_fence_init();
     sh.abort = 0;
@@ -195,55 +157,53 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     tc::tmem_alloc(&sh.tmem, C::kCols);
     tc::tmem_relinquish();
   }
+  // ---- which sequence, tile and head: sequences in order, a sequence's last (longest) tiles first ----
+  // Each warp finds it for itself, 32 sequences at a time: no exchange between them.
+  const int64_t work = blockIdx.x;
+  int64_t base = 0;  // CTAs of the sequences before
+  int b = 0;
+  Seq seq;
+  for (;; b += 32) {
+    seq = Seq{0, 0, 0};
+    if (b + lane < a.batch) seq = load_seq(a, b + lane);
+    const int64_t mine = (int64_t)((seq.nq * a.ratio + kRowsCta - 1) / kRowsCta) * a.kv_heads;
+    int64_t incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += v;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, work < base + incl);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      base = __shfl_sync(0xffffffffu, base + incl - mine, at);
+      seq.len = __shfl_sync(0xffffffffu, seq.len, at);
+      seq.nq = __shfl_sync(0xffffffffu, seq.nq, at);
+      seq.q0 = __shfl_sync(0xffffffffu, seq.q0, at);
+      b += at;
+      break;
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
+    if (b + 32 >= a.batch) {  // more CTAs were launched than there are tiles; all warps see this
+      b = -1;
+      break;
+    }
+  }
+  tc::fence_before_sync();
   __syncthreads();
-  const int b = sh.seq;
-  const Seq seq = load_seq(a, b);
+  tc::fence_after_sync();
+  if (b < 0) {
+    if (warp == kMmaWarp) tc::tmem_dealloc(0, C::kCols);
+    return;
+  }
   const int rows = seq.nq * a.ratio, tiles = (rows + kRowsCta - 1) / kRowsCta;
-  const int in_seq = (int)(work - sh.base), tile = tiles - 1 - in_seq / a.kv_heads, head = in_seq % a.kv_heads;
+  const int in_seq = (int)(work - base), tile = tiles - 1 - in_seq / a.kv_heads, head = in_seq % a.kv_heads;
   const int row0 = tile * kRowsCta, live = min(kRowsCta, rows - row0);
   int lo, hi;
   visible(a, seq, (int)a.by_ratio(row0), (int)a.by_ratio(row0 + live - 1), lo, hi);
   const int tok0 = lo / kTok * kTok, n = hi > tok0 ? (hi - tok0 + kTok - 1) / kTok : 0;
 
-  // ---- queries: f16 with a power of two a row and the logits' sign, swizzled ----
-  constexpr int LPR = D / 8, STEP = kThreads / LPR;  // lanes a row, rows at a time
-  constexpr int QN = (kRowsCta + STEP - 1) / STEP;
-  uint4 qraw[QN];  // every load before the first use
-#pragma unroll
-  for (int k = 0; k < QN; ++k) {
-    const int r = threadIdx.x / LPR + k * STEP, row = row0 + r, i = (int)a.by_ratio(row);
-    qraw[k] = make_uint4(0, 0, 0, 0);
-    if (r < live)
-      qraw[k] = __ldg(reinterpret_cast<const uint4*>(
-          static_cast<const char*>(a.q) +
-          2 * ((seq.q0 + i) * a.qs + (int64_t)(head * a.ratio + row - i * a.ratio) * a.qh + 8 * (threadIdx.x % LPR))));
-  }
-#pragma unroll
-  for (int k = 0; k < QN; ++k) {
-    const int r = threadIdx.x / LPR + k * STEP, c = threadIdx.x % LPR;
-    if (r >= kRowsCta) break;  // a warp's rows are all in or all out
-    float f[8];
-    unpack8(qraw[k], a.bf16, f);
-    float big = 0.f;
-#pragma unroll
-    for (int x = 0; x < 8; ++x) big = fmaxf(big, fabsf(f[x]));
-#pragma unroll
-    for (int d = 1; d < LPR; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d, LPR));
-    const int ex = (int)(__float_as_uint(big) >> 23) - 127;  // the row's largest magnitude becomes 2^7 .. 2^8
-    const int up = big == 0.f || ex == 128 ? 0 : min(7 - ex, 126);
-    const float m = a.scale_log2 < 0.f ? -pow2f(up) : pow2f(up);
-    uint4 w;
-    w.x = pack2_f16(f[0] * m, f[4] * m), w.y = pack2_f16(f[1] * m, f[5] * m);
-    w.z = pack2_f16(f[2] * m, f[6] * m), w.w = pack2_f16(f[3] * m, f[7] * m);
-    *reinterpret_cast<uint4*>(smem + C::kQ + (r / 128) * C::kTile + (c / 8) * kBlockBytes + (r % 128) * 128 +
-                              ((c % 8) ^ (r & 7)) * 16) = w;
-    if (c == 0) sh.row_scale[r] = fabsf(a.scale_log2) * pow2f(-up);
-  }
-  static_assert(kThreads % LPR == 0 && kRowsCta % (32 / LPR) == 0, "whole rows a warp");
-  tc::fence_proxy_async_smem();
-  tc::fence_before_sync();
-  __syncthreads();
-  tc::fence_after_sync();
+  constexpr int LPR = D / 8;  // lanes a row of queries
   constexpr uint32_t tmem = 0;  // all 512 columns were allocated: they begin at 0
   volatile int* abort_flag = &sh.abort;
   auto give_up = [&]() {
@@ -254,12 +214,65 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
   if (warp < kCacheWarp) {
     // ---------------- probabilities ----------------
     const int w = warp >> 2, r = threadIdx.x;  // r: the CTA's row
+    const int row = row0 + r, in_q = (int)a.by_ratio(row), head_q = head * a.ratio + row - in_q * a.ratio;
+    const int64_t token = seq.q0 + in_q;
+    // ---- queries: f16 with a power of two a row and the logits' sign, swizzled ----
+    // A warp copies its 32 rows to their places as they are; then each thread turns its row into f16 there.
+    const uint32_t q_rows = sbase + C::kQ + w * C::kTile + (r & 96) * 128;
+    auto place = [&](uint32_t rows, int rr, int o) {  // 8 dimensions of one of the warp's rows
+      return rows + (o / 8) * kBlockBytes + rr * 128 + ((o % 8) ^ (rr & 7)) * 16;
+    };
+    {
+      const int64_t q_off = 2 * (token * a.qs + (int64_t)head_q * a.qh);
+      const int o = lane % LPR;
+#pragma unroll 8
+      for (int k = 0; k < LPR; ++k) {  // 32 / LPR rows at a time
+        const int rr = k * (32 / LPR) + lane / LPR;
+        const int64_t off = __shfl_sync(0xffffffffu, q_off, rr);
+        const bool in = (r & ~31) + rr < live;
+        cp_async16(place(q_rows, rr, o), static_cast<const char*>(a.q) + (in ? off + 16 * o : 0), in ? 16 : 0);
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      __syncwarp();
+    }
+    auto piece = [&](int o) {
+      uint4 x;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                   : "r"(place(q_rows, lane, o))
+                   : "memory");
+      return x;
+    };
+    uint32_t big = 0;  // the row's largest magnitude, by its 16 bits
+#pragma unroll
+    for (int o = 0; o < LPR; ++o) {
+      const uint4 x = piece(o);
+      big = __vmaxu2(big, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+    }
+    big = max(big & 0xffffu, big >> 16);
+    const float most = a.bf16 ? __uint_as_float(big << 16) : __half2float(__ushort_as_half((unsigned short)big));
+    const int ex = (int)(__float_as_uint(most) >> 23) - 127;  // it becomes 2^7 .. 2^8
+    const int up = big == 0 || ex == 128 ? 0 : min(7 - ex, 126);
+    const float q_mul = a.scale_log2 < 0.f ? -pow2f(up) : pow2f(up), row_scale = fabsf(a.scale_log2) * pow2f(-up);
+#pragma unroll 4
+    for (int o = 0; o < LPR; ++o) {
+      float f[8];
+      unpack8(piece(o), a.bf16, f);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) f[x] *= q_mul;
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(q_rows, lane, o)), "r"(pack2_f16(f[0], f[4])),
+                   "r"(pack2_f16(f[1], f[5])), "r"(pack2_f16(f[2], f[6])), "r"(pack2_f16(f[3], f[7]))
+                   : "memory");
+    }
+    tc::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&sh.q_full);
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const uint32_t ts = tmem + C::kS + w * kTok + lanes, to = tmem + C::kO + w * D + lanes;
-    const int row = row0 + r, pos = seq.len - seq.nq + (int)a.by_ratio(row);
+    const int pos = seq.len - seq.nq + in_q;
     const int last = r >= live ? -1 : a.causal ? min(pos, seq.len - 1) : seq.len - 1;
     const int past = a.window > 0 ? max(pos - a.window, -1) : -1;
-    const float row_scale = sh.row_scale[r];
     float mx = kNoMax, sum = 0.f;
     int vexp = -24;
     bool ok = true;
@@ -276,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       const Meta& meta = sh.meta[t & 3];
       const int j0 = tok0 + u * kHalf;
       const uint32_t th = ts + h * kHalf;
-      const float c = ONE ? row_scale : row_scale * pow2f(meta.k_exp);
+      const float c = row_scale * pow2f(meta.k_exp);
       const int ve = meta.v_exp;
       const uint32_t valid0 = meta.valid[2 * h], valid1 = meta.valid[2 * h + 1];
       const bool masked = !__all_sync(0xffffffffu, (valid0 & valid1) == 0xffffffffu && j0 > past && j0 + kHalf - 1 <= last);
@@ -288,27 +301,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         m &= to_ <= 0 ? 0u : to_ >= 32 ? 0xffffffffu : (1u << to_) - 1u;
         return m;
       };
-      auto logits = [&](int g, uint32_t (&v)[32]) {  // in units of c
-        ld_x32(th + 32 * g, v);
-        tc::wait_ld();
-        if (ONE) {
-          const float4* ks = reinterpret_cast<const float4*>(sh.k_scale[t & 3] + h * kHalf + 32 * g);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 k = ks[i];
-            v[4 * i] = __float_as_uint(__uint_as_float(v[4 * i]) * k.x);
-            v[4 * i + 1] = __float_as_uint(__uint_as_float(v[4 * i + 1]) * k.y);
-            v[4 * i + 2] = __float_as_uint(__uint_as_float(v[4 * i + 2]) * k.z);
-            v[4 * i + 3] = __float_as_uint(__uint_as_float(v[4 * i + 3]) * k.w);
-          }
-        }
-      };
       // the largest logit, against the reference
       float m = -INFINITY;
 #pragma unroll 1
       for (int g = 0; g < 2; ++g) {
         uint32_t v[32];
-        logits(g, v);
+        ld_x32(th + 32 * g, v);
+        tc::wait_ld();
         if (masked) {
           const uint32_t see = seen(g);
 #pragma unroll
@@ -352,7 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
 #pragma unroll 1
       for (int g = 0; g < 2; ++g) {
         uint32_t v[32], p[16];
-        logits(g, v);
+        ld_x32(th + 32 * g, v);
+        tc::wait_ld();
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(v[i]), c, add)));
         if (masked) {
@@ -382,8 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     } else {
       tc::fence_after_sync();
       // the row, rounded, into the warp's part of the query tile (its products are done), then out in whole rows
-      const float scale = sum == 0.f ? 0.f : 1.f / sum, power = pow2f(vexp);
-      uint8_t* tile_rows = smem + C::kQ + w * C::kTile;
+      const float scale = sum == 0.f ? 0.f : pow2f(vexp) / sum;  // O is 0 where the sum is
 #pragma unroll 1
       for (int g = 0; g < D / 32; ++g) {
         uint32_t v[32] = {};
@@ -392,24 +391,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
           tc::wait_ld();
         }
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = sum == 0.f ? 0u : __float_as_uint(__uint_as_float(v[k]) * scale * power);
+        for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * scale);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {  // columns 0 .. 7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
           auto two = [&](int x, int y) { return pack2(__uint_as_float(v[8 * k + x]), __uint_as_float(v[8 * k + y]), a.bf16); };
-          const int c = 4 * g + k;  // 16 bytes: 8 dimensions
-          *reinterpret_cast<uint4*>(tile_rows + (c / 8) * kBlockBytes + (r % 128) * 128 + ((c % 8) ^ (r & 7)) * 16) =
-              make_uint4(two(0, 2), two(4, 6), two(1, 3), two(5, 7));
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(q_rows, lane, 4 * g + k)), "r"(two(0, 2)),
+                       "r"(two(4, 6)), "r"(two(1, 3)), "r"(two(5, 7))
+                       : "memory");
         }
       }
       __syncwarp();
-#pragma unroll 1
+      const int64_t out_off = 2 * (token * a.os + (int64_t)head_q * a.oh);
+      const int o = lane % LPR;
+#pragma unroll 4
       for (int k = 0; k < LPR; ++k) {  // 32 / LPR rows at a time
-        const int rr = (r & ~31) + k * (32 / LPR) + lane / LPR, c = lane % LPR, out_row = row0 + rr, i = (int)a.by_ratio(out_row);
-        if (rr >= live) break;
-        const uint4 v = *reinterpret_cast<const uint4*>(tile_rows + (c / 8) * kBlockBytes + (rr % 128) * 128 +
-                                                        ((c % 8) ^ (rr & 7)) * 16);
-        char* dst = static_cast<char*>(a.out) +
-                    2 * ((seq.q0 + i) * a.os + (int64_t)(head * a.ratio + out_row - i * a.ratio) * a.oh + 8 * c);
+        const int rr = k * (32 / LPR) + lane / LPR;
+        char* dst = static_cast<char*>(a.out) + __shfl_sync(0xffffffffu, out_off, rr) + 16 * o;
+        if ((r & ~31) + rr >= live) continue;
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(place(q_rows, rr, o))
+                     : "memory");
         if (wide) {
           *reinterpret_cast<uint4*>(dst) = v;
         } else {
@@ -417,9 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
           *reinterpret_cast<uint2*>(dst + 8) = make_uint2(v.z, v.w);
         }
       }
-      const int i = (int)a.by_ratio(row), head_q = head * a.ratio + row - i * a.ratio;
-      const int64_t tk = seq.q0 + i;
-      if (a.lse && r < live) a.lse[tk * a.ls + head_q] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
+      if (a.lse && r < live) a.lse[token * a.ls + head_q] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) * kLn2;
     }
   } else if (warp < kMmaWarp) {
     // ---------------- cache: nibbles and scales to f16; group z: 0 K, 1 V ----------------
@@ -486,22 +487,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
             put(at + ((((c & 1) * 4 + k) ^ (tok & 7)) << 4), e);
           }
         } else {
-          const __half2 s = ONE ? __half2() : *reinterpret_cast<const __half2*>(&sc_k[in_row]);
+          const __half2 s = *reinterpret_cast<const __half2*>(&sc_k[in_row]);
           const uint32_t at = sbase + C::kK + (tok / kHalf) * 2 * C::kPart + (c / 2) * kKBlockBytes + (tok % kHalf) * 128;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t to = at + ((((c & 1) * 4 + k) ^ (tok & 7)) << 4);
-            uint32_t e[4];
+            uint32_t e[4], o[4];
             expand(words[k], e);
-            if (ONE) {
-              put(to, e);
-            } else {
-              uint32_t o[4];
-              times(e, __low2half2(s), o);
-              put(to, o);
-              times(e, __high2half2(s), o);
-              put(to + C::kPart, o);
-            }
+            times(e, __low2half2(s), o);
+            put(to, o);
+            times(e, __high2half2(s), o);
+            put(to + C::kPart, o);
           }
         }
       }
@@ -514,46 +510,39 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     for (int t = 0; t < n; ++t) {
       const int next = page_of(t + 1);
       Meta& meta = sh.meta[t & 3];
-      if (ONE && !z) {
-        const float k = __half2float(__ushort_as_half(sk[0]));
-        sh.k_scale[t & 3][tid] = fabsf(k) < INFINITY ? k : __int_as_float(0x7fffffff);
-        const uint32_t marks = __ballot_sync(0xffffffffu, page >= 0);
-        if (lane == 0) meta.valid[w] = marks;
-      } else {
-        // the tile's power of two, and its scales divided by it
-        uint32_t big = 0;
-        bool bad = false;
+      // the tile's power of two, and its scales divided by it
+      uint32_t big = 0;
+      bool bad = false;
 #pragma unroll
-        for (int g = 0; g < CH; ++g) {
-          const uint32_t m = sk[g] & 0x7fffu;
-          if (m < 0x7c00u) big = max(big, m);
-          bad |= m >= 0x7c00u;
-        }
-        big = __reduce_max_sync(0xffffffffu, big);
-        const uint32_t marks = __ballot_sync(0xffffffffu, z ? bad : page >= 0);
-        if (lane == 0) {
-          sh.big[z][w] = big;
-          (z ? meta.bad : meta.valid)[w] = marks;
-        }
-        cache_sync(z);  // also: every warp is done with the last tile's scales
-        big = max(max(sh.big[z][0], sh.big[z][1]), max(sh.big[z][2], sh.big[z][3]));
-        const int e = big ? (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)big))) >> 23) - 127 : -24;
-#pragma unroll
-        for (int g = 0; g < CH; ++g) {
-          if (g >= groups) continue;
-          const bool finite = (sk[g] & 0x7fffu) < 0x7c00u;
-          const uint32_t s = __half_as_ushort(__float2half_rn(__half2float(__ushort_as_half(sk[g])) * pow2f(-e)));
-          if (z) {  // a value that is not finite is left out: its token is marked
-            sc_v[tid * groups + g] = __ushort_as_half((unsigned short)(finite ? s : 0u));
-          } else {  // such a key makes its logit NaN
-            const uint32_t first = s & 0xfff8u;
-            const __half rest = __hsub(__ushort_as_half((unsigned short)s), __ushort_as_half((unsigned short)first));
-            sc_k[tid * groups + g] = finite ? first | (uint32_t)__half_as_ushort(rest) << 16 : 0x7fff7fffu;
-          }
-        }
-        if (tid == 0) (z ? meta.v_exp : meta.k_exp) = e;
-        cache_sync(z);
+      for (int g = 0; g < CH; ++g) {
+        const uint32_t m = sk[g] & 0x7fffu;
+        if (m < 0x7c00u) big = max(big, m);
+        bad |= m >= 0x7c00u;
       }
+      big = __reduce_max_sync(0xffffffffu, big);
+      const uint32_t marks = __ballot_sync(0xffffffffu, z ? bad : page >= 0);
+      if (lane == 0) {
+        sh.big[z][w] = big;
+        (z ? meta.bad : meta.valid)[w] = marks;
+      }
+      cache_sync(z);  // also: every warp is done with the last tile's scales
+      big = max(max(sh.big[z][0], sh.big[z][1]), max(sh.big[z][2], sh.big[z][3]));
+      const int e = big ? (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)big))) >> 23) - 127 : -24;
+#pragma unroll
+      for (int g = 0; g < CH; ++g) {
+        if (g >= groups) continue;
+        const bool finite = (sk[g] & 0x7fffu) < 0x7c00u;
+        const uint32_t s = __half_as_ushort(__float2half_rn(__half2float(__ushort_as_half(sk[g])) * pow2f(-e)));
+        if (z) {  // a value that is not finite is left out: its token is marked
+          sc_v[tid * groups + g] = __ushort_as_half((unsigned short)(finite ? s : 0u));
+        } else {  // such a key makes its logit NaN
+          const uint32_t first = s & 0xfff8u;
+          const __half rest = __hsub(__ushort_as_half((unsigned short)s), __ushort_as_half((unsigned short)first));
+          sc_k[tid * groups + g] = finite ? first | (uint32_t)__half_as_ushort(rest) << 16 : 0x7fff7fffu;
+        }
+      }
+      if (tid == 0) (z ? meta.v_exp : meta.k_exp) = e;
+      cache_sync(z);
       page = next;
       if (t + 1 < n) fetch_scales(t + 1, page);
       // where it goes: K's place of this warp's half, filled once a tile; V's stage, every second one
@@ -584,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         const uint64_t k = k0 + (uint64_t)(h * (2 * C::kPart >> 4));
         if (elect_one()) {
 #pragma unroll
-          for (int x = 0; x < (ONE ? 1 : 2) * (D / 16); ++x) {  // 16 dimensions: 32 bytes; the scales' first bits, the rest
+          for (int x = 0; x < 2 * (D / 16); ++x) {  // 16 dimensions: 32 bytes; the scales' first bits, the rest
             const int i = x % (D / 16), part = x / (D / 16);
             mma_ss(ts + h * kHalf, q0 + (uint64_t)((i / 4) * (kBlockBytes >> 4) + (i % 4) * 2),
                    k + (uint64_t)(part * (C::kPart >> 4) + (i / 4) * (kKBlockBytes >> 4) + (i % 4) * 2), id_qk, x > 0);
@@ -597,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       };
       // K of a half, and with the first one the tile's V: the tile's meta has both groups' part
       auto cached = [&](int t, int h) { return wait(&sh.full[0][h], t) && (h == 1 || wait(&sh.full[1][t & 1], t >> 1)); };
-      bool ok = true;
+      bool ok = wait(&sh.q_full, 0);
       for (int h = 0; ok && h < 2; ++h) {
         ok = cached(0, h);
         if (!ok) break;
@@ -637,9 +626,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
   if (warp == kMmaWarp) tc::tmem_dealloc(tmem, C::kCols);
 }
 
-template <int D, bool ONE>
+template <int D>
 int launch_prompt(const Args& a, int64_t ctas, cudaStream_t s) {
-  const auto kernel = kv4_prompt_kernel<D, ONE>;
+  const auto kernel = kv4_prompt_kernel<D>;
   const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), Cfg<D>::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
   kernel<<<(unsigned)ctas, kThreads, Cfg<D>::kSmem, s>>>(a, wait_limit_ns());
@@ -652,8 +641,7 @@ int launch_prompt(const Args& a, int64_t ctas, cudaStream_t s) {
 int prompt_attention(const Args& a, int dim, cudaStream_t s) {
   const int64_t ctas = (a.tokens * a.ratio / kRowsCta + a.batch) * a.kv_heads;
   if (ctas > 0x7fffffff) return UP_ERR_UNSUPPORTED;
-  if (dim == 64) return a.groups == 1 ? launch_prompt<64, true>(a, ctas, s) : launch_prompt<64, false>(a, ctas, s);
-  return a.groups == 1 ? launch_prompt<128, true>(a, ctas, s) : launch_prompt<128, false>(a, ctas, s);
+  return dim == 64 ? launch_prompt<64>(a, ctas, s) : launch_prompt<128>(a, ctas, s);
 }
 
 }  // namespace kv4

@@ -81,7 +81,8 @@ struct Shares {
 };
 
 // What starting a tile costs, in units: its loads wait for one another (length, pages, cache) and its parts are added. The
-// CTAs' shares count it, or CTAs that get many short sequences finish last: 64 sequences of 0 to 4096 tokens take COST.
+// CTAs' shares count it, or CTAs that get many short sequences finish last: 64 sequences of 0 to 4096 tokens
+// took 52.2 us without it and 45.8 with, 24 sequences of a few queries 42.2 and 28.4.
 constexpr int kTileCost = 2;
 
 // Units of one (tile, head) of a sequence: at least one, which writes the rows that see nothing.
@@ -390,6 +391,10 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
       {
         float f[4][GT];
         scales(reinterpret_cast<const __half*>(sp + 2 * C::kKV), f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int z = 0; z < GT; ++z) f[i][z] = fmaf(f[i][z], 0.f, f[i][z]);  // infinity * a nibble of 0 is NaN: so is the logit
 #pragma unroll
         for (int z = 0; z < GT; ++z) {
           float acc[2][NT][4];
