@@ -1,8 +1,12 @@
 // kv4_prompt.cu — attention over the paged 4-bit cache for many query rows a key/value head (prompts), on the tcgen05
 // tensor cores: the cache's tiles are turned into f16 once a CTA and serve 256 query rows.
 //
-// What bounds it: the tensor cores (4 dim flops a query row and cached token) and, at dim 128 as much, the exponentials
-// (one a query row and cached token; 16 a clock and SM against 16 x 512 flops).
+// What bounds it: no one unit. At dim 128 a tile of 256 query rows and 128 cached tokens takes about 5300 cycles, of which
+// the tensor cores are busy 4200 (an M128 N64 K16 product takes 49 cycles, not 32: it reads its A operand from shared
+// memory again), the exponentials 2050 (16 a clock and SM), and the schedulers issue in half. Leaving out half of the
+// products, the exponentials or the conversion of the cache gains 6, 1 and 5 % each: the chain from S to P to the next S
+// is what takes the time. Starting and ending a CTA takes 14000 cycles more. Three sequences of 1500 to 2048 query
+// tokens, 32 heads over 8, dim 128: bf16 310 us (198 GFLOP, 638 TFLOP/s; the second products of the parts not counted).
 //
 // A CTA takes 256 query rows (query token x head of the group) of one sequence and key/value head as two tiles of 128,
 // and walks the cached tokens that any of them sees, 128 at a time. Per tile of tokens, S = Q K^T (128 x 128) and
@@ -13,8 +17,8 @@
 //    for the largest logit and for p = 2^(logit - ref), and writes P as f16 over it: the A operand of the second product.
 //    ref moves only when a logit is more than 2^8 above it; then the thread scales its row of O.
 //  * warp groups 2 and 3 (cache, K and V): read 128 tokens' nibbles and scales, a tile ahead in registers, and write
-//    them as f16 into 128-byte swizzled shared memory: V in two stages, K in a place a half, free again when the half's
-//    logits are there. Both have a row a token: K is the B operand with its contraction (the dimensions) contiguous, V
+//    them as f16 into 128-byte swizzled shared memory, a place a half, free again when the half's products are done. Both
+//    have a row a token: K is the B operand with its contraction (the dimensions) contiguous, V
 //    the one with its output (the dimensions) contiguous. The nibble conversion pairs dimensions k and k + 4 of each 8;
 //    q is stored in the same order and the output's columns are read in it.
 //  * warps 16 and 17 (products): each issues the tcgen05.mma of one query tile, so neither tile's products wait for the
@@ -23,15 +27,16 @@
 // keeps f16's range whatever their size; the logits take K's power, the probabilities V's, relative to the largest one
 // met (O is scaled when a larger one comes). The logits are exact up to their f32 sums, as a row's logsumexp is in f32:
 // each of K's scales is split into its first 8 bits and the rest, a nibble times either is exact in f16, and both
-// products are added in one S. That is half as much tensor work again, which the probabilities hide (prompts of 1500 to
-// 2048 tokens 314 -> 320 us; with one scale a token, multiplying the columns of S by it in the softmax instead took
-// 381). V's products end in 16 bits: there nibble * scale, and p, are rounded to f16. All sums are f32.
+// products are added in one S (with one scale a token, multiplying the columns of S by it in the softmax instead took 381
+// us where this took 320). So is V for f16 outputs. For bf16 ones, which round to 8 bits, nibble * scale is rounded to f16:
+// that is one product, and the second part's memory is a second stage (310 us against 362). p is rounded to f16. All sums
+// are f32.
 // A token with an infinite or NaN v_scale is left out of the products (its rows would reach queries that do not see it)
 // and the queries that do see it become NaN.
 // Every wait is bounded; one that runs out sets the workspace's error word and the CTA unwinds.
 //
 // The tile of 2 x 128 rows is what 512 columns of tensor memory hold (S and O of both tiles at dim 128) and 227 KB of
-// shared memory (q 64 KB, two stages of K and V 128 KB).
+// shared memory (q 64 KB, K and V in two parts 64 KB each).
 #include "kv4_attention.cuh"
 #include "tc.cuh"
 
@@ -42,17 +47,17 @@ namespace {
 
 constexpr int kRowsCta = 256, kTok = 128, kHalf = kTok / 2;
 constexpr int kThreads = 32 * 18, kCacheWarp = 8, kMmaWarp = 16;
-constexpr int kBlockBytes = kTok * 128;  // 128 rows of 64 dimensions (128 bytes), swizzled
-constexpr int kKBlockBytes = kHalf * 128;
+constexpr int kBlockBytes = kTok * 128;       // 128 query rows of 64 dimensions (128 bytes), swizzled
+constexpr int kHalfBlockBytes = kHalf * 128;  // 64 tokens of 64 dimensions
 
 template <int D>
 struct Cfg {
   static constexpr int kBlocks = D / 64;
   static constexpr int kTile = kBlocks * kBlockBytes;       // 128 rows of D f16
-  static constexpr int kPart = kTile / 2;                   // K of a half: 64 rows, its first bits or the rest
-  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + 4 * kPart, kEnd = kV + 2 * kTile;
-  static constexpr int kScale = kEnd;                       // K: f16 pairs [128][up to D / 32]; V: f16, the same
-  static constexpr int kSmem = kScale + kTok * (D / 32) * (4 + 2) + 1024 /* alignment */;
+  static constexpr int kPart = kTile / 2;                   // K or V of a half: 64 rows, with the scales' first bits or the rest
+  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + 4 * kPart;
+  static constexpr int kScale = kV + 4 * kPart;             // f16 pairs [2 (K, V)][128][up to D / 32]
+  static constexpr int kSmem = kScale + 2 * kTok * (D / 32) * 4 + 1024 /* alignment */;
   static constexpr int kS = 0, kO = 2 * kTok;               // tensor memory columns: S (and P) of both tiles, then O
   static constexpr int kCols = 512;
 };
@@ -64,7 +69,10 @@ struct Meta {          // what the cache warps say of a tile of tokens
 };
 
 struct Shared {
-  uint64_t full[2][2], empty[2][2];  // K: [0][half], V: [1][stage]
+  uint64_t k_full[2], k_empty[2], v_full[2][2], v_empty[2][2];  // K: [half], V: [stage][half]
+  // V's part of a tile's meta is there; of tile t in t mod 4, as up to three tiles' come before the first one's is waited
+  // for, and a wait must not find its barrier two phases on.
+  uint64_t v_meta[4];
   uint64_t s_full[2][2], p_full[2][2], pv_done[2], all_done[2], q_full, drain;  // [query tile][half]
   uint32_t tmem;
   int abort;
@@ -72,10 +80,10 @@ struct Shared {
   uint32_t big[2][4];          // [K, V][warp]
 };
 
-__device__ __forceinline__ uint64_t desc_v(uint32_t addr) {  // dimensions contiguous: 64-dimension blocks kBlockBytes apart
+__device__ __forceinline__ uint64_t desc_v(uint32_t addr) {  // dimensions contiguous: 64-dimension blocks kHalfBlockBytes apart
   uint64_t d = 0;
   d |= (uint64_t)((addr >> 4) & 0x3fffu);
-  d |= (uint64_t)(kBlockBytes >> 4) << 16;  // leading offset: the next 64 dimensions
+  d |= (uint64_t)(kHalfBlockBytes >> 4) << 16;  // leading offset: the next 64 dimensions
   d |= (uint64_t)(1024u >> 4) << 32;        // stride offset: the next 8 tokens
   d |= (uint64_t)1u << 46;
   d |= (uint64_t)2u << 61;                  // 128-byte swizzle
@@ -125,7 +133,7 @@ template <int ID, int THREADS>
 __device__ __forceinline__ void named_sync() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(THREADS) : "memory"); }
 __device__ __forceinline__ void cache_sync(int z) { z ? named_sync<2, 128>() : named_sync<1, 128>(); }  // K's, V's group
 
-template <int D>
+template <int D, bool BF16>  // BF16: q and out, else f16
 __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, const uint64_t wait_ns) {
   using C = Cfg<D>;
   constexpr int CH = D / 32;
@@ -137,17 +145,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      for (int z = 0; z < 2; ++z) {
-        tc::mbar_init(&sh.full[z][i], z ? 4 : 2);  // the warps that fill it
-        tc::mbar_init(&sh.empty[z][i], 2);  // a commit of each issuer
-      }
+      tc::mbar_init(&sh.k_full[i], 2);   // the warps that fill it
+      tc::mbar_init(&sh.k_empty[i], 2);  // a commit of each issuer
       for (int h = 0; h < 2; ++h) {
+        tc::mbar_init(&sh.v_full[i][h], 2);
+        tc::mbar_init(&sh.v_empty[i][h], 2);
         tc::mbar_init(&sh.s_full[i][h], 2);  // the issuer (it has seen the tile's meta) and a commit
         tc::mbar_init(&sh.p_full[i][h], 4);  // the tile's warps
       }
       tc::mbar_init(&sh.pv_done[i], 1);
       tc::mbar_init(&sh.all_done[i], 1);
     }
+    for (int i = 0; i < 4; ++i) tc::mbar_init(&sh.v_meta[i], 1);
     tc::mbar_init(&sh.q_full, kCacheWarp);
     tc::mbar_init(&sh.drain, 2);
     tc::mbar_fence_init();
@@ -251,14 +260,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       big = __vmaxu2(big, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
     }
     big = max(big & 0xffffu, big >> 16);
-    const float most = a.bf16 ? __uint_as_float(big << 16) : __half2float(__ushort_as_half((unsigned short)big));
+    const float most = BF16 ? __uint_as_float(big << 16) : __half2float(__ushort_as_half((unsigned short)big));
     const int ex = (int)(__float_as_uint(most) >> 23) - 127;  // it becomes 2^7 .. 2^8
     const int up = big == 0 || ex == 128 ? 0 : min(7 - ex, 126);
     const float q_mul = a.scale_log2 < 0.f ? -pow2f(up) : pow2f(up), row_scale = fabsf(a.scale_log2) * pow2f(-up);
 #pragma unroll 4
     for (int o = 0; o < LPR; ++o) {
       float f[8];
-      unpack8(piece(o), a.bf16, f);
+      unpack8(piece(o), BF16, f);
 #pragma unroll
       for (int x = 0; x < 8; ++x) f[x] *= q_mul;
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(q_rows, lane, o)), "r"(pack2_f16(f[0], f[4])),
@@ -394,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * scale);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {  // columns 0 .. 7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
-          auto two = [&](int x, int y) { return pack2(__uint_as_float(v[8 * k + x]), __uint_as_float(v[8 * k + y]), a.bf16); };
+          auto two = [&](int x, int y) { return pack2(__uint_as_float(v[8 * k + x]), __uint_as_float(v[8 * k + y]), BF16); };
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(q_rows, lane, 4 * g + k)), "r"(two(0, 2)),
                        "r"(two(4, 6)), "r"(two(1, 3)), "r"(two(5, 7))
                        : "memory");
@@ -427,8 +436,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     const int z = (warp - kCacheWarp) >> 2, w = warp & 3, tid = threadIdx.x & 127, groups = a.groups;
     const uint8_t* nibbles = z ? a.v4 : a.k4;
     const __half* scales = z ? a.v_scale : a.k_scale;
-    uint32_t* sc_k = reinterpret_cast<uint32_t*>(smem + C::kScale);  // f16 pairs: a scale's first 8 bits, the rest
-    __half* sc_v = reinterpret_cast<__half*>(smem + C::kScale + 4 * kTok * CH);
+    uint32_t* sc = reinterpret_cast<uint32_t*>(smem + C::kScale) + z * kTok * CH;  // a scale's first 8 bits, the rest
+    const bool two = !BF16 || z == 0;
     const int32_t* pages = a.table + (int64_t)b * a.table_stride;
     const int in_page = (1 << a.page_log2) - 1, cpg_log2 = 31 - __clz(a.cpg);  // 1, 2 or 4 chunks a group
     auto page_of = [&](int t) {
@@ -470,32 +479,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         o[x] = *reinterpret_cast<const uint32_t*>(&v);
       }
     };
-    auto convert = [&](int t) {
+    auto convert = [&](int stage) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int u = (lane >> 3) + 4 * i, run = u / CH, c = u - run * CH, tok = 32 * w + 8 * run + (lane & 7);
         const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
         const int in_row = tok * groups + (c >> cpg_log2);
-        if (z) {
-          const __half2 s = __half2half2(sc_v[in_row]);
-          const uint32_t at = sbase + C::kV + (t & 1) * C::kTile + (c / 2) * kBlockBytes + tok * 128;
+        const __half2 s = *reinterpret_cast<const __half2*>(&sc[in_row]);
+        const uint32_t at = sbase + (z ? C::kV : C::kK) + ((tok / kHalf) * 2 + stage) * C::kPart + (c / 2) * kHalfBlockBytes + (tok % kHalf) * 128;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t e[4];
-            expand(words[k], e);
-            times(e, s, e);
-            put(at + ((((c & 1) * 4 + k) ^ (tok & 7)) << 4), e);
-          }
-        } else {
-          const __half2 s = *reinterpret_cast<const __half2*>(&sc_k[in_row]);
-          const uint32_t at = sbase + C::kK + (tok / kHalf) * 2 * C::kPart + (c / 2) * kKBlockBytes + (tok % kHalf) * 128;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t to = at + ((((c & 1) * 4 + k) ^ (tok & 7)) << 4);
-            uint32_t e[4], o[4];
-            expand(words[k], e);
-            times(e, __low2half2(s), o);
-            put(to, o);
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t to = at + ((((c & 1) * 4 + k) ^ (tok & 7)) << 4);
+          uint32_t e[4], o[4];
+          expand(words[k], e);
+          times(e, __low2half2(s), o);
+          put(to, o);
+          if (two) {
             times(e, __high2half2(s), o);
             put(to + C::kPart, o);
           }
@@ -533,25 +532,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         if (g >= groups) continue;
         const bool finite = (sk[g] & 0x7fffu) < 0x7c00u;
         const uint32_t s = __half_as_ushort(__float2half_rn(__half2float(__ushort_as_half(sk[g])) * pow2f(-e)));
-        if (z) {  // a value that is not finite is left out: its token is marked
-          sc_v[tid * groups + g] = __ushort_as_half((unsigned short)(finite ? s : 0u));
-        } else {  // such a key makes its logit NaN
-          const uint32_t first = s & 0xfff8u;
-          const __half rest = __hsub(__ushort_as_half((unsigned short)s), __ushort_as_half((unsigned short)first));
-          sc_k[tid * groups + g] = finite ? first | (uint32_t)__half_as_ushort(rest) << 16 : 0x7fff7fffu;
-        }
+        const uint32_t first = two ? s & 0xfff8u : s;
+        const __half rest = __hsub(__ushort_as_half((unsigned short)s), __ushort_as_half((unsigned short)first));
+        // where it is not finite, a key makes its logit NaN, a value is left out: its token is marked
+        sc[tid * groups + g] = finite ? first | (uint32_t)__half_as_ushort(rest) << 16 : z ? 0u : 0x7fff7fffu;
       }
-      if (tid == 0) (z ? meta.v_exp : meta.k_exp) = e;
+      if (tid == 0) {
+        (z ? meta.v_exp : meta.k_exp) = e;
+        if (z) tc::mbar_arrive(&sh.v_meta[t & 3]);
+      }
       cache_sync(z);
       page = next;
       if (t + 1 < n) fetch_scales(t + 1, page);
-      // where it goes: K's place of this warp's half, filled once a tile; V's stage, every second one
-      const int s = z ? t & 1 : w >> 1, turn = z ? t >> 1 : t;
-      if (__all_sync(0xffffffffu, tc::mbar_wait(&sh.empty[z][s], (turn & 1) ^ 1, wait_ns, abort_flag))) {
-        convert(t);
+      // this warp's half, of the stage
+      const int h = w >> 1, stage = two ? 0 : t & 1, turn = two ? t : t >> 1;
+      if (__all_sync(0xffffffffu, tc::mbar_wait(z ? &sh.v_empty[stage][h] : &sh.k_empty[h], (turn & 1) ^ 1, wait_ns, abort_flag))) {
+        convert(stage);
         tc::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&sh.full[z][s]);
+        if (lane == 0) tc::mbar_arrive(z ? &sh.v_full[stage][h] : &sh.k_full[h]);
         if (t + 1 < n) fetch(t + 1, page);
       } else {
         give_up();  // a named barrier still counts this warp: it keeps step with the others, without the work
@@ -576,16 +575,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
           for (int x = 0; x < 2 * (D / 16); ++x) {  // 16 dimensions: 32 bytes; the scales' first bits, the rest
             const int i = x % (D / 16), part = x / (D / 16);
             mma_ss(ts + h * kHalf, q0 + (uint64_t)((i / 4) * (kBlockBytes >> 4) + (i % 4) * 2),
-                   k + (uint64_t)(part * (C::kPart >> 4) + (i / 4) * (kKBlockBytes >> 4) + (i % 4) * 2), id_qk, x > 0);
+                   k + (uint64_t)(part * (C::kPart >> 4) + (i / 4) * (kHalfBlockBytes >> 4) + (i % 4) * 2), id_qk, x > 0);
           }
           tc::mbar_arrive(&sh.s_full[w][h]);
           tc::commit(&sh.s_full[w][h]);
-          tc::commit(&sh.empty[0][h]);
+          tc::commit(&sh.k_empty[h]);
         }
         __syncwarp();
       };
-      // K of a half, and with the first one the tile's V: the tile's meta has both groups' part
-      auto cached = [&](int t, int h) { return wait(&sh.full[0][h], t) && (h == 1 || wait(&sh.full[1][t & 1], t >> 1)); };
+      // K of a half, and with the first one V's part of the tile's meta, which the probabilities take
+      auto cached = [&](int t, int h) { return wait(&sh.k_full[h], t) && (h == 1 || wait(&sh.v_meta[t & 3], t >> 2)); };
+      constexpr bool two = !BF16;
       bool ok = wait(&sh.q_full, 0);
       for (int h = 0; ok && h < 2; ++h) {
         ok = cached(0, h);
@@ -596,17 +596,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
 #pragma unroll 1
       for (int u = 0; ok && u < 2 * n; ++u) {
         const int t = u >> 1, h = u & 1;
-        ok = wait(&sh.p_full[w][h], t);
+        const int stage = two ? 0 : t & 1;
+        ok = wait(&sh.v_full[stage][h], two ? t : t >> 1) && wait(&sh.p_full[w][h], t);
         if (!ok) break;
         tc::fence_after_sync();
-        const uint64_t v = v0 + (uint64_t)((t & 1) * (C::kTile >> 4) + h * (kHalf * 128 >> 4));
+        const uint64_t v = v0 + (uint64_t)((2 * h + stage) * (C::kPart >> 4));
         if (elect_one()) {
 #pragma unroll
           for (int i = 0; i < kHalf / 16; ++i)  // 16 tokens: 2048 bytes
             mma_ts(to, ts + h * kHalf + 8 * i, v + (uint64_t)(i * 128), id_pv, u + i > 0);
+          if (two) {
+#pragma unroll
+            for (int i = 0; i < kHalf / 16; ++i)
+              mma_ts(to, ts + h * kHalf + 8 * i, v + (uint64_t)((C::kPart >> 4) + i * 128), id_pv, true);
+          }
           tc::commit(&sh.pv_done[w]);
           if (u + 1 == 2 * n) tc::commit(&sh.all_done[w]);
-          if (h == 1) tc::commit(&sh.empty[1][t & 1]);
+          tc::commit(&sh.v_empty[stage][h]);
         }
         __syncwarp();
         if (t + 1 == n) continue;
@@ -626,9 +632,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
   if (warp == kMmaWarp) tc::tmem_dealloc(tmem, C::kCols);
 }
 
-template <int D>
+template <int D, bool BF16>
 int launch_prompt(const Args& a, int64_t ctas, cudaStream_t s) {
-  const auto kernel = kv4_prompt_kernel<D>;
+  const auto kernel = kv4_prompt_kernel<D, BF16>;
   const cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), Cfg<D>::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
   kernel<<<(unsigned)ctas, kThreads, Cfg<D>::kSmem, s>>>(a, wait_limit_ns());
@@ -641,7 +647,8 @@ int launch_prompt(const Args& a, int64_t ctas, cudaStream_t s) {
 int prompt_attention(const Args& a, int dim, cudaStream_t s) {
   const int64_t ctas = (a.tokens * a.ratio / kRowsCta + a.batch) * a.kv_heads;
   if (ctas > 0x7fffffff) return UP_ERR_UNSUPPORTED;
-  return dim == 64 ? launch_prompt<64>(a, ctas, s) : launch_prompt<128>(a, ctas, s);
+  if (dim == 64) return a.bf16 ? launch_prompt<64, true>(a, ctas, s) : launch_prompt<64, false>(a, ctas, s);
+  return a.bf16 ? launch_prompt<128, true>(a, ctas, s) : launch_prompt<128, false>(a, ctas, s);
 }
 
 }  // namespace kv4

@@ -7,6 +7,7 @@ exception is `scan_host`, whose buffers are in host memory: the library itself s
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 
 import numpy as np
@@ -536,6 +537,11 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: tuple, slots: torch.Tens
     return q_out
 
 
+@functools.lru_cache(maxsize=1024)
+def _kv4_workspace_bytes(device, *sizes) -> int:
+    return _lib.load().up_sm100_kv4_attention_workspace_bytes(*sizes)
+
+
 def kv4_attention(q: torch.Tensor, cache: tuple, block_table: torch.Tensor, seq_lens: torch.Tensor,
                   cu_q: torch.Tensor | None = None, causal: bool = True, window: int = 0,
                   scale: float | None = None, out: torch.Tensor | None = None, want_lse: bool = False,
@@ -583,7 +589,7 @@ def kv4_attention(q: torch.Tensor, cache: tuple, block_table: torch.Tensor, seq_
         lse_ptr = lse.data_ptr()
     L = _lib.load()
     if ws is None:
-        ws = workspace("kv4", L.up_sm100_kv4_attention_workspace_bytes(tokens, heads, batch, kv_heads, dim), q.device)
+        ws = workspace("kv4", _kv4_workspace_bytes(dev, tokens, heads, batch, kv_heads, dim), q.device)
     os = out.stride()
     check(L.up_sm100_kv4_attention(
         q.data_ptr(), kind, tokens, heads, qs[0], qs[1], ctypes.byref(c), block_table.data_ptr(), ps[0], pages[1],
