@@ -616,3 +616,17 @@ def test_an_infinite_key_scale_makes_its_logit_nan(dim, group):
     cache[2][int(table[0, 198 // 16]), 0, 198 % 16, 0] = float("inf")
     out = ops.kv4_attention(q, cache, table, n, cu_q=cu)
     assert bool(out[2:].isnan().all()) and not bool(out[:2].isnan().any())
+
+
+@pytest.mark.parametrize("dim,group", [(64, 32), (128, 128)])
+def test_many_sequences_of_many_rows(dim, group):
+    """More sequences than a warp looks through at once, empty ones among them; no wait inside the launch ran out."""
+    g = torch.Generator().manual_seed(dim)
+    lens = torch.randint(0, 300, (70,), generator=g).tolist()
+    nq = torch.randint(0, 35, (70,), generator=g).tolist()
+    lens[3] = nq[5] = nq[69] = 0
+    cache, table, n = make(70, 1, dim, group, 16, lens, seed=12)
+    cu = torch.tensor([0] + nq, device="cuda").cumsum(0).int()
+    for kind in (torch.bfloat16, torch.float16):
+        check(torch.randn(sum(nq), 16, dim, device="cuda").to(kind), cache, table, n, cu)
+    ops.check_workspace("kv4", cache[0].device)
