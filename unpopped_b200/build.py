@@ -3,7 +3,8 @@
     python -m unpopped_b200.build          # or: python unpopped_b200/build.py
 
 Sources: unpopped_b200/csrc/*.cu. Output: unpopped_b200/libunpopped_sm100.so, which the snapshot carries to
-the GPU box. Objects are compiled in parallel and relinked only when a source or header changed.
+the GPU box. Objects are compiled in parallel and relinked only when a source or header changed. Beside it stands
+unpopped_b200/_bind.so, the serving operators' Python calls (csrc/bind.cpp, host code against torch's headers).
 """
 from __future__ import annotations
 
@@ -13,12 +14,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libunpopped_sm100.so")
+BIND = os.path.join(HERE, "_bind.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -78,9 +81,31 @@ def build(verbose: bool = False, extra=()) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    _build_bind()
     if verbose:
         print(LIB)
     return LIB
+
+
+def _build_bind():
+    src = os.path.join(CSRC, "bind.cpp")
+    if not _stale(BIND, [src, os.path.join(ROOT, "include", "up_sm100.h")]):
+        return
+    import torch
+
+    base = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
+    includes = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
+                sysconfig.get_paths()["include"], cuda, os.path.join(ROOT, "include")]
+    tmp = BIND + ".tmp"
+    cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{d}" for d in includes] +
+           [src, "-o", tmp, "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+            "-L" + HERE, "-l:libunpopped_sm100.so", "-Wl,-rpath,$ORIGIN"])
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on bind.cpp:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BIND)
 
 
 def ptxas_report(src_name: str) -> str:

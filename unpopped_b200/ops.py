@@ -7,14 +7,13 @@ exception is `scan_host`, whose buffers are in host memory: the library itself s
 from __future__ import annotations
 
 import ctypes
-import functools
 import threading
 
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import ACCUM, COMBINE, EK, OOB, OP, ROPE_LAYOUT, ROPE_SCALING, UpKv4Cache, check
+from ._lib import ACCUM, COMBINE, EK, OOB, OP, ROPE_SCALING, check
 
 _OPS = {"sum": OP["SUM"], "max": OP["MAX"], "min": OP["MIN"]}
 _OOBS = {"skip": OOB["SKIP"], "clamp": OOB["CLAMP"], "zero_fill": OOB["ZERO_FILL"]}
@@ -378,21 +377,6 @@ def w4a16(w_packed: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, group: i
 
 
 # ---- rotary positions, the 4-bit paged cache and its attention ----
-_ROPE_EK = {torch.float32: EK["F32"], torch.float16: EK["F16"], torch.bfloat16: EK["BF16"]}
-_KV4_EK = {torch.float16: EK["F16"], torch.bfloat16: EK["BF16"]}
-_POS = {torch.int32: EK["I32"], torch.int64: EK["I64"]}
-_LAYOUTS = {"half": ROPE_LAYOUT["HALF"], "interleaved": ROPE_LAYOUT["INTERLEAVED"]}
-
-
-def _same_device(dev: int, tensors):
-    """Everything lies on CUDA device `dev`, which is the current one (where the library launches)."""
-    if dev != torch.cuda.current_device():
-        raise ValueError("the tensors must be on the current CUDA device")
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError("all tensors must be on one CUDA device")
-
-
 def rope_table(n_pos: int, rot: int, base: float = 10000.0, scaling: tuple | None = None, gain: float = 1.0,
                device="cuda") -> torch.Tensor:
     """The f32 [n_pos, rot] table that `rope` and `kv4_append` read: gain * cos(p f_i) in the first rot/2 columns, gain *
@@ -404,43 +388,25 @@ def rope_table(n_pos: int, rot: int, base: float = 10000.0, scaling: tuple | Non
     if len(rest) != {"none": 0, "linear": 1, "base": 1, "wavelength": 4, "ramp": 4}.get(kind, -1):
         raise ValueError(f"rope_table: no such scaling {scaling!r}")
     factor, low, high, orig = tuple(float(v) for v in rest) + (1.0, 0.0, 0.0, 0.0)[len(rest):]
-    _same_device(out.get_device(), ())
+    if out.get_device() != torch.cuda.current_device():
+        raise ValueError("the table must be on the current CUDA device")
     check(_lib.load().up_sm100_rope_table(out.data_ptr(), n_pos, rot, base, ROPE_SCALING[kind.upper()], factor, low,
                                           high, orig, gain, _stream(out)), "rope_table")
     return out
 
 
-def _rope(x, positions, table, layout, backward, out, where):
-    _cuda(x, "x")
-    kind, shape, xs = _ROPE_EK.get(x.dtype), x.shape, x.stride()
-    four = len(shape) == 4
-    if kind is None or not (four or len(shape) == 3) or (xs[-1] != 1 and shape[-1] > 1):
-        raise ValueError(f"{where} takes float32, float16 or bfloat16 [tokens, heads, dim] or [batch, seq, heads, dim] "
-                         "with the dimension contiguous")
-    batch, seq, heads, dim = shape if four else (1, *shape)
-    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous():
-        raise ValueError("table is float32 [positions, rot], contiguous (rope_table)")
-    n_pos, rot = table.shape
-    pos_ptr, pos_kind, pos_stride = None, 0, 0
-    if positions is not None:
-        pos_kind, at = _POS.get(positions.dtype), positions.shape
-        if pos_kind is None or not positions.is_contiguous():
-            raise ValueError("positions are contiguous int32 or int64")
-        if at == (batch, seq) and four:
-            pos_stride = seq
-        elif at != (seq,):
-            raise ValueError("positions are one a token: [tokens], [seq] or [batch, seq]")
-        pos_ptr = positions.data_ptr()
-    if out is None:
-        out = torch.empty_like(x)
-    elif out.shape != shape or out.dtype != x.dtype or (out.stride(-1) != 1 and dim > 1):
-        raise ValueError("out has x's shape and type, with the dimension contiguous")
-    _same_device(x.get_device(), (positions, table, out))
-    os = out.stride()
-    check(_lib.load().up_sm100_rope(x.data_ptr(), kind, batch, seq, heads, dim, xs[0] if four else 0, xs[-3], xs[-2],
-                                    pos_ptr, pos_kind, pos_stride, table.data_ptr(), n_pos, rot, _LAYOUTS[layout],
-                                    backward, out.data_ptr(), os[0] if four else 0, os[-3], os[-2], _stream(x)), where)
-    return out
+_bound = None
+
+
+def _calls():
+    """The serving operators' calls (csrc/bind.cpp); like the library, there is no substitute for them."""
+    global _bound
+    if _bound is None:
+        from . import _bind
+
+        _bind.init(check, workspace, _ws_cache)
+        _bound = _bind
+    return _bound
 
 
 def rope(x: torch.Tensor, positions: torch.Tensor | None, table: torch.Tensor, layout: str = "half",
@@ -449,13 +415,13 @@ def rope(x: torch.Tensor, positions: torch.Tensor | None, table: torch.Tensor, l
     the dimension contiguous) with the first table.shape[1] dimensions of each head turned by the token's position.
     layout "half" pairs dimensions (i, i + rot/2), "interleaved" (2i, 2i + 1). positions: int32 or int64, one a token
     ([seq] serves every sequence of a batch), None counts from 0; one outside the table gives NaN. out may be x."""
-    return _rope(x, positions, table, layout, 0, out, "rope")
+    return _calls().rope(x, positions, table, layout, out, False)
 
 
 def rope_backward(grad: torch.Tensor, positions: torch.Tensor | None, table: torch.Tensor, layout: str = "half",
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """The gradient of `rope` with respect to its input, from the gradient of its output."""
-    return _rope(grad, positions, table, layout, 1, out, "rope_backward")
+    return _calls().rope(grad, positions, table, layout, out, True)
 
 
 def kv4_cache(pages: int, kv_heads: int, dim: int, page: int = 16, group: int = 32, device="cuda") -> tuple:
@@ -466,23 +432,6 @@ def kv4_cache(pages: int, kv_heads: int, dim: int, page: int = 16, group: int = 
     return tuple(torch.zeros(rows + (n,), dtype=t, device=device)
                  for n, t in ((dim // 2, torch.uint8), (dim // 2, torch.uint8), (dim // group, torch.float16),
                               (dim // group, torch.float16)))
-
-
-def _kv4(cache, where):
-    k, v, ks, vs = cache
-    shape, sshape = k.shape, ks.shape
-    if k.dtype != torch.uint8 or v.dtype != torch.uint8 or ks.dtype != torch.float16 or vs.dtype != torch.float16:
-        raise ValueError(f"{where}: a cache is (k uint8, v uint8, k_scale float16, v_scale float16)")
-    if len(shape) != 4 or len(sshape) != 4 or v.shape != shape or vs.shape != sshape or sshape[:3] != shape[:3]:
-        raise ValueError(f"{where}: cache arrays are [pages, kv_heads, page, dim/2] and [pages, kv_heads, page, dim/group]")
-    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
-        raise ValueError(f"{where}: cache arrays are contiguous")
-    pages, heads, page, half = shape
-    groups = sshape[3]
-    if groups == 0 or 2 * half % groups:
-        raise ValueError(f"{where}: the scales' groups divide the head size")
-    return UpKv4Cache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, heads, page, 2 * half,
-                      2 * half // groups), heads, 2 * half
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: tuple, slots: torch.Tensor,
@@ -496,50 +445,7 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: tuple, slots: torch.Tens
     token's position first, as `rope` does; without one they do not. k and v are quantised to int4 with an f16 scale a
     group. slots (int32 or int64, one a token): the token's place, page * page_size + place in the page; a slot outside the
     cache (-1: padding) leaves the token out. q_out may be q."""
-    _cuda(k, "k")
-    c, kv_heads, dim = _kv4(cache, "kv4_append")
-    kind, shape = _KV4_EK.get(k.dtype), k.shape
-    if kind is None or v.dtype != k.dtype:
-        raise ValueError("kv4_append takes bfloat16 or float16, q, k and v alike")
-    ks, vs = k.stride(), v.stride()
-    if shape[1:] != (kv_heads, dim) or len(shape) != 3 or v.shape != shape or ks[2] != 1 or vs[2] != 1:
-        raise ValueError("k and v are [tokens, kv_heads, dim] of the cache, with the dimension contiguous")
-    tokens = shape[0]
-    slot_kind = _POS.get(slots.dtype)
-    if slot_kind is None or slots.shape != (tokens,) or not slots.is_contiguous():
-        raise ValueError("slots are contiguous int32 or int64, one a token")
-    rot, n_pos, pos_kind, pos_ptr, table_ptr = 0, 0, 0, None, None
-    if table is not None:
-        if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous():
-            raise ValueError("table is float32 [positions, rot], contiguous (rope_table)")
-        pos_kind = None if positions is None else _POS.get(positions.dtype)
-        if pos_kind is None or positions.shape != (tokens,) or not positions.is_contiguous():
-            raise ValueError("positions are contiguous int32 or int64, one a token")
-        n_pos, rot = table.shape
-        pos_ptr, table_ptr = positions.data_ptr(), table.data_ptr()
-    heads, q_ptr, out_ptr, qs, qos = 0, None, None, (0, 0), (0, 0)
-    if q is not None:
-        qs, qshape = q.stride(), q.shape
-        if len(qshape) != 3 or q.dtype != k.dtype or qshape[0] != tokens or qshape[2] != dim or qs[2] != 1:
-            raise ValueError("q is [tokens, heads, dim] of k's type, with the dimension contiguous")
-        if q_out is None:
-            q_out = torch.empty_like(q)
-        elif q_out.shape != qshape or q_out.dtype != q.dtype or q_out.stride(2) != 1:
-            raise ValueError("q_out has q's shape and type, with the dimension contiguous")
-        heads, qos, q_ptr, out_ptr = qshape[1], q_out.stride(), q.data_ptr(), q_out.data_ptr()
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    _same_device(k.get_device(), (v, slots, positions, table, q, q_out, *cache))
-    check(_lib.load().up_sm100_kv4_append(
-        q_ptr, k.data_ptr(), v.data_ptr(), kind, tokens, heads, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], pos_ptr,
-        pos_kind, table_ptr, n_pos, rot, _LAYOUTS[layout], slots.data_ptr(), slot_kind, ctypes.byref(c), out_ptr, qos[0],
-        qos[1], _stream(k)), "kv4_append")
-    return q_out
-
-
-@functools.lru_cache(maxsize=1024)
-def _kv4_workspace_bytes(device, *sizes) -> int:
-    return _lib.load().up_sm100_kv4_attention_workspace_bytes(*sizes)
+    return _calls().kv4_append(k, v, cache, slots, positions, table, q, layout, q_out)
 
 
 def kv4_attention(q: torch.Tensor, cache: tuple, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -554,48 +460,9 @@ def kv4_attention(q: torch.Tensor, cache: tuple, block_table: torch.Tensor, seq_
     block_table int32 [batch, width]: its pages. cu_q int32 [batch + 1]: where each sequence's query tokens begin in q;
     None: one token a sequence. The query tokens are the last of their sequence: each sees the cached tokens up to its own
     (`causal`), and of these the last `window` where window > 0. A query that sees nothing gives 0 (and -inf)."""
-    _cuda(q, "q")
-    c, kv_heads, head_dim = _kv4(cache, "kv4_attention")
-    kind, shape, qs = _KV4_EK.get(q.dtype), q.shape, q.stride()
-    if kind is None or len(shape) != 3 or shape[2] != head_dim or qs[2] != 1:
-        raise ValueError("q is bfloat16 or float16 [tokens, heads, dim] of the cache's dim, with the dimension contiguous")
-    tokens, heads, dim = shape
-    if kv_heads == 0 or heads % kv_heads:
-        raise ValueError("q's heads are a multiple of the cache's")
-    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or not seq_lens.is_contiguous():
-        raise ValueError("seq_lens is contiguous int32 [batch]")
-    batch, pages, ps = seq_lens.shape[0], block_table.shape, block_table.stride()
-    if block_table.dtype != torch.int32 or len(pages) != 2 or pages[0] != batch or (ps[1] != 1 and pages[1] > 1):
-        raise ValueError("block_table is int32 [batch, width] with contiguous rows")
-    if cu_q is None:
-        if tokens != batch:
-            raise ValueError("without cu_q there is one query token a sequence")
-        cu_ptr = None
-    else:
-        if cu_q.dtype != torch.int32 or cu_q.shape != (batch + 1,) or not cu_q.is_contiguous():
-            raise ValueError("cu_q is contiguous int32 [batch + 1]")
-        cu_ptr = cu_q.data_ptr()
-    if window < 0:
-        raise ValueError("window is not negative")
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.shape != shape or out.dtype != q.dtype or out.stride(2) != 1:
-        raise ValueError("out has q's shape and type, with the dimension contiguous")
-    dev = q.get_device()
-    _same_device(dev, (block_table, seq_lens, cu_q, out, *cache))
-    lse, lse_ptr = None, None
-    if want_lse:
-        lse = q.new_empty((tokens, heads), dtype=torch.float32)
-        lse_ptr = lse.data_ptr()
-    L = _lib.load()
-    if ws is None:
-        ws = workspace("kv4", _kv4_workspace_bytes(dev, tokens, heads, batch, kv_heads, dim), q.device)
-    os = out.stride()
-    check(L.up_sm100_kv4_attention(
-        q.data_ptr(), kind, tokens, heads, qs[0], qs[1], ctypes.byref(c), block_table.data_ptr(), ps[0], pages[1],
-        seq_lens.data_ptr(), cu_ptr, batch, causal, window, dim ** -0.5 if scale is None else scale, out.data_ptr(), os[0],
-        os[1], lse_ptr, heads, ws.data_ptr(), ws.numel(), _stream(q)), "kv4_attention")
-    return (out, lse) if want_lse else out
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    return _calls().kv4_attention(q, cache, block_table, seq_lens, cu_q, causal, window, scale, out, want_lse, ws)
 
 
 def launch_count() -> int:
