@@ -1,9 +1,9 @@
 // bind.cpp — the Python side of the calls that a decode step makes for every layer (rotary positions, the 4-bit cache's
-// append, the attention over it): the tensors' checks, the outputs' allocation and the C call.
+// append and reading, the attention over it): the tensors' checks, the outputs' allocation and the C call.
 //
 // Why not in Python over ctypes as elsewhere: these kernels take 2 to 10 us for one token, and there the same checks took
-// 5 us, the arguments' conversion 2 and the outputs 1.4 to 2.4 each: 11.3 us for a rotation, 15.3 for an append, 18.6 for
-// an attention, the launch's own 4 us among them. The entry points of ops.py are the names and the documentation.
+// 5 us, the arguments' conversion 2 and the outputs 1.4 to 2.4 each. One token's rotation takes 5.6 us a call here and took
+// 11.4, an append 5.2 and 15.3, an attention 7.6 and 18.6. The entry points of ops.py are the names and the documentation.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -350,6 +350,34 @@ PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// dequant_i4(w, scale, group, out): the cache's rows as values, among others
+PyObject* dequant_i4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 4);
+    const at::Tensor &w = cuda_tensor(a[0], "w"), &scale = cuda_tensor(a[1], "scale");
+    need(w.dim() == 2, "w is [n, k / 2]");
+    const int64_t rows = w.size(0), k = 2 * w.size(1), group = PyLong_AsLongLong(a[2]);
+    if (group == -1 && PyErr_Occurred()) throw Raised();
+    at::Tensor out;
+    if (given(a[3])) {
+      out = tensor(a[3], "out");
+    } else {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      out = at::empty({rows, k}, w.options().dtype(at::kBFloat16));
+    }
+    check(unlocked([&] {
+            return up_sm100_dequant_i4_bf16(static_cast<const uint8_t*>(w.data_ptr()), static_cast<const uint16_t*>(scale.data_ptr()),
+                                            rows, k, group, static_cast<uint16_t*>(out.data_ptr()), stream_of(w.get_device()));
+          }),
+          "dequant_i4");
+    if (given(a[3])) {
+      Py_INCREF(a[3]);
+      return a[3];
+    }
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 // init(check, workspace, workspaces)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -366,6 +394,7 @@ PyMethodDef methods[] = {
     {"init", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(init)), METH_FASTCALL, nullptr},
     {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rope)), METH_FASTCALL, nullptr},
     {"kv4_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_append)), METH_FASTCALL, nullptr},
+    {"dequant_i4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequant_i4)), METH_FASTCALL, nullptr},
     {"kv4_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_attention)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -64,6 +64,20 @@ def check_workspace(kind: str, device: torch.device):
         check(workspace_status(ws), f"{kind} device wait")
 
 
+_bound = None
+
+
+def _calls():
+    """The calls of csrc/bind.cpp; like the library, there is no substitute for them."""
+    global _bound
+    if _bound is None:
+        from . import _bind
+
+        _bind.init(check, workspace, _ws_cache)
+        _bound = _bind
+    return _bound
+
+
 # ---- row sum ----
 def row_sum(x: torch.Tensor, accum: str = "f32", block: int = 256, out: torch.Tensor | None = None) -> torch.Tensor:
     """Sum of each row of a 2-D f32 tensor (last axis). accum='f32' (fixed-order f32 tree) or 'auto' (f64 in
@@ -347,15 +361,7 @@ def gather_rows(table: torch.Tensor, ids: torch.Tensor, oob: str = "skip",
 # ---- int4 dequant and W4A16 ----
 def dequant_i4(w_packed: torch.Tensor, scale: torch.Tensor, group: int, out: torch.Tensor | None = None):
     """bf16 [N, K] from int4 [N, K] packed two per byte ([N, K/2] uint8) and f16 scales [N, K/group]."""
-    _cuda(w_packed, "w")
-    _cuda(scale, "scale")
-    n, kh = w_packed.shape
-    k = 2 * kh
-    if out is None:
-        out = w_packed.new_empty((n, k), dtype=torch.bfloat16)
-    check(_lib.load().up_sm100_dequant_i4_bf16(w_packed.data_ptr(), scale.data_ptr(), n, k, group, out.data_ptr(),
-                                               _stream(w_packed)), "dequant_i4")
-    return out
+    return _calls().dequant_i4(w_packed, scale, group, out)
 
 
 def w4a16(w_packed: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, group: int,
@@ -393,20 +399,6 @@ def rope_table(n_pos: int, rot: int, base: float = 10000.0, scaling: tuple | Non
     check(_lib.load().up_sm100_rope_table(out.data_ptr(), n_pos, rot, base, ROPE_SCALING[kind.upper()], factor, low,
                                           high, orig, gain, _stream(out)), "rope_table")
     return out
-
-
-_bound = None
-
-
-def _calls():
-    """The serving operators' calls (csrc/bind.cpp); like the library, there is no substitute for them."""
-    global _bound
-    if _bound is None:
-        from . import _bind
-
-        _bind.init(check, workspace, _ws_cache)
-        _bound = _bind
-    return _bound
 
 
 def rope(x: torch.Tensor, positions: torch.Tensor | None, table: torch.Tensor, layout: str = "half",
