@@ -196,3 +196,19 @@ def test_the_split_gives_every_unit_to_one_cta_and_every_part_its_counter():
         assert all(s == list(range(n)) for s, n in zip(seen, tiles))
         for users in arrivals.values():  # one tile a counter, and it is met exactly as often as it is waited for
             assert len({i for i, _ in users}) == 1 and all(of == len(users) for _, of in users)
+
+
+def test_the_calls_refuse_tensors_that_are_not_on_a_gpu():
+    torch = pytest.importorskip("torch")
+    from unpopped_b200 import ops
+
+    x = torch.zeros(2, 2, 64)
+    cache = tuple(torch.zeros(2, 2, 16, n, dtype=t) for n, t in ((32, torch.uint8), (32, torch.uint8), (2, torch.float16),
+                                                                   (2, torch.float16)))
+    lens = torch.zeros(2, dtype=torch.int32)
+    for bad in (lambda: ops.rope(x, None, torch.zeros(4, 64)), lambda: ops.rope("x", None, torch.zeros(4, 64)),
+                lambda: ops.rope_backward(x, None, torch.zeros(4, 64)), lambda: ops.kv4_append(x, x, cache, lens),
+                lambda: ops.kv4_attention(x, cache, lens.view(2, 1), lens),
+                lambda: ops.dequant_i4(cache[0].view(64, 32), cache[2].view(64, 2), 32)):
+        with pytest.raises(TypeError):
+            bad()
