@@ -8,7 +8,7 @@
 // values: it reads back as NaN. The clamp is met only where f16 rounds a tiny scale down.
 //
 // What bounds it: HBM. q, k and v are read once, q is written once, and a cached row takes dim / 2 + 2 dim / group bytes.
-// 16001 tokens of 64 and 8 heads of 128, f16: 128 us (612 MB: 4.8 TB/s, the slots' scattered rows in 64-byte pieces among
+// 16001 tokens of 64 and 8 heads of 128, f16: 112 us (612 MB: 5.5 TB/s, the slots' scattered rows in 64-byte pieces among
 // them); one token 2.8 us, the launch's own time.
 //
 // Some blocks turn the queries as rope.cu does, the others take the rows of keys and values; they alternate over the grid,
@@ -17,6 +17,8 @@
 // chunks (8 dimensions each) of its row, so that each rotated pair is in one thread: chunks j and rot / 16 + j of the half
 // layout, two neighbours otherwise. A chunk's magnitude goes through shared memory: groups need not fall on a warp's lanes
 // (dim 96 has 6 threads a row), and a group's maximum is then group / 32 16-byte reads.
+// Four blocks an SM hide the rows' lookups best: 112 us for the 16001 tokens, with 64 registers a thread, against 128 for
+// the three that 72 registers leave and 157 for five, which spill.
 // Four rows a thread, loaded together, measured slower (231 us against 159 us for 16001 tokens of 64 and 8 heads, both with
 // an earlier form of the queries' part): the registers that they take halve the queries' blocks on an SM.
 #include "kv4.cuh"
@@ -90,7 +92,7 @@ __device__ __forceinline__ uint32_t magnitude8(const float (&f)[8]) {  // as bit
 // VEC: blocks of queries (items of rope_item, HEADS heads each) and of rows. Else (rows or rotations that are not whole
 // 16-byte chunks) every block takes rows, and the queries are rows like the others.
 template <typename T, bool VEC, int HEADS>
-__global__ void __launch_bounds__(kThreads) kv4_append_kernel(const T* q, const T* __restrict__ k,
+__global__ void __launch_bounds__(kThreads, 4) kv4_append_kernel(const T* q, const T* __restrict__ k,
                                                               const T* __restrict__ v, T* q_out, const Append a,
                                                               const Geometry g, const Mix mix,
                                                               const Items<Divide32> n) {
