@@ -209,14 +209,14 @@ inline int split_rows(int64_t rows_a_sequence, int64_t dim) {
 // Whether the kernel for many query rows (head sizes 64 and 128; 256 rows a CTA, one CTA an SM) takes less time than the
 // split one, given `rows` query rows for each of `pairs` (sequence, key/value head): the first in as many turns as its
 // CTAs fill the SMs, the second in 16-row tiles that are spread evenly. Against as many cached tokens a 256-row tile takes
-// an SM as long as five 16-row ones at head size 128 and seven at 64 (2.75 and 2.4 us a 128 tokens). Measured over one
-// sequence of 32768 tokens to 32 of 2048, 8 key/value heads, 8 to 1024 rows each, the faster one is taken but within 4 %:
-// 12 sequences of 4096 at size 128, 96 rows 99 us split and 116 not, 128 rows 127 and 114; 4 of them, 256 rows 90 and 102,
-// 384 rows 128 and 113; at size 64, 12 of them, 128 rows 82 and 107, 192 rows 116 and 102.
+// an SM as long as four 16-row ones at head size 128 and six at 64. Measured from one sequence of 4096 tokens to 32 of
+// 2048, 8 key/value heads, 32 to 1024 rows each, the faster one is taken but within 4 %: 12 sequences of 4096 at size 128,
+// 96 rows 102 us split and 118 not, 128 rows 129 and 116; 4 of them, 256 rows 90 and 102, 384 rows 127 and 114; at size
+// 64, 12 of them, 128 rows 84 and 108, 192 rows 119 and 106.
 inline bool many_rows(int64_t rows, int64_t pairs, int64_t dim, int64_t sms) {
   if (dim != 64 && dim != 128) return false;
   const int64_t turns = (pairs * ((rows + 255) / 256) + sms - 1) / sms;
-  return turns * sms * (dim == 64 ? 7 : 5) < pairs * ((rows + 15) / 16);
+  return turns * sms * (dim == 64 ? 6 : 4) < pairs * ((rows + 15) / 16);
 }
 int prompt_attention(const Args& a, int dim, cudaStream_t s);
 
