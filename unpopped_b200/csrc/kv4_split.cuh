@@ -32,7 +32,7 @@
 //
 // What bounds it: HBM where contexts are long; while the loop runs it reads 6.0 to 6.4 TB/s, with about 560 instructions a
 // warp and 32 tokens of size 128 (the schedulers issue in 59 % of their cycles). 64 query over 8 key/value heads of 128,
-// bf16: 32 contexts of 8000 to 16384 tokens 91 us (412 MB: 4.5 TB/s), one of 131071 tokens 42 us (143 MB: 3.4 TB/s), one of
+// bf16: 32 contexts of 8000 to 16384 tokens 89 us (412 MB: 4.6 TB/s), one of 131071 tokens 42 us (143 MB: 3.4 TB/s), one of
 // 777 tokens 9.5 us. What is beside the loop, and all that short contexts cost: lengths, then pages, then the first data
 // (3 to 5 us), the parts' merge (2 to 5 us), and CTAs that share an SM with slower ones.
 #pragma once
@@ -118,7 +118,7 @@ __device__ __forceinline__ int64_t seq_units(const Args& a, int b, bool any) {
     const Seq w{__shfl_sync(0xffffffffu, s.len, src), __shfl_sync(0xffffffffu, s.nq, src), 0};
     int64_t sum = 0;
     for (int i = lane; i < of; i += 32) sum += kTileCost + tile_units<ROWS>(a, w, i, unit0);
-#pragma unroll
+#pragma unroll 1
     for (int d = 1; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == src) n = sum;
   }
@@ -208,28 +208,24 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
         off -= size;
         ++tile;
         while (tile < tiles) {  // 32 tiles at a time
-          int my_first = 0, my_units = 0;
-          int64_t my_size = 0;
-          if (tile + lane < tiles) {
-            my_units = tile_units<ROWS>(a, seq, tile + lane, my_first);
-            my_size = (int64_t)(my_units + kTileCost) * a.kv_heads;
-          }
-          int64_t end = my_size;
-#pragma unroll
+          int my_first = 0, my_units = -kTileCost;
+          if (tile + lane < tiles) my_units = tile_units<ROWS>(a, seq, tile + lane, my_first);
+          int end = my_units + kTileCost;  // of one head: 32 tiles of at most 2^23 units
+#pragma unroll 1  // unrolled, the registers of the main loop suffer (91.2 against 89.1 us for the 32 long contexts)
           for (int d = 1; d < 32; d <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, end, d);
+            const int v = __shfl_up_sync(0xffffffffu, end, d);
             if (lane >= d) end += v;
           }
-          const uint32_t past = __ballot_sync(0xffffffffu, off < end);
+          const uint32_t past = __ballot_sync(0xffffffffu, off < (int64_t)end * a.kv_heads);
           if (past) {
             const int at = __ffs(past) - 1;
-            off -= __shfl_sync(0xffffffffu, end - my_size, at);
             n_units = __shfl_sync(0xffffffffu, my_units, at);
+            off -= (int64_t)(__shfl_sync(0xffffffffu, end, at) - n_units - kTileCost) * a.kv_heads;
             unit0 = __shfl_sync(0xffffffffu, my_first, at);
             tile += at;
             break;
           }
-          off -= __shfl_sync(0xffffffffu, end, 31);
+          off -= (int64_t)__shfl_sync(0xffffffffu, end, 31) * a.kv_heads;
           tile = min(tile + 32, tiles);
         }
       }
