@@ -65,7 +65,7 @@ extern "C" int up_sm100_kv4_attention(const void* q, int dtype, int64_t tokens, 
   a.tokens = tokens;
   a.k4 = static_cast<const uint8_t*>(cache->k), a.v4 = static_cast<const uint8_t*>(cache->v);
   a.k_scale = static_cast<const __half*>(cache->k_scale), a.v_scale = static_cast<const __half*>(cache->v_scale);
-  if (cache->pages == 0) {  // every token is left out; copies of no bytes still name an address
+  if (cache->pages == 0) {  // every token is left out and nothing is read; copies of no bytes still name an address
     a.k4 = a.v4 = static_cast<const uint8_t*>(q);
     a.k_scale = a.v_scale = static_cast<const __half*>(q);
   }

@@ -450,15 +450,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     uint4 raw[CH];
     uint16_t sk[CH];  // this thread's token's scales (one a group)
     const uint32_t page_lines = (uint32_t)a.kv_heads << a.page_log2, head_line = (uint32_t)head << a.page_log2;
-    // a token that does not exist reads line 0's bytes: its scales are zero
+    // a run of 8 is on one page; one whose first token has no page is not read, as there may be no page at all
     auto fetch = [&](int t, int page) {
-      const int pg = max(page, 0), at = (tok0 + t * kTok + 32 * w) & in_page;  // a run of 8 is on one page
+      const int at = (tok0 + t * kTok + 32 * w) & in_page;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int u = (lane >> 3) + 4 * i, run = u / CH, c = u - run * CH;
-        const int64_t ln = (int64_t)(uint32_t)__shfl_sync(0xffffffffu, pg, 8 * run) * page_lines +
-                           (head_line + ((at + 8 * run) & in_page) + (lane & 7));
-        raw[i] = ld_nc_na_v4(nibbles + ln * (D / 2) + 16 * c);
+        const int pg = __shfl_sync(0xffffffffu, page, 8 * run);
+        const int64_t ln = (int64_t)(uint32_t)pg * page_lines + (head_line + ((at + 8 * run) & in_page) + (lane & 7));
+        raw[i] = pg >= 0 ? ld_nc_na_v4(nibbles + ln * (D / 2) + 16 * c) : make_uint4(0, 0, 0, 0);
       }
     };
     auto fetch_scales = [&](int t, int page) {
