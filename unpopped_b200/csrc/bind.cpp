@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -311,6 +312,12 @@ PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (given(a[10])) {
       ws = tensor(a[10], "ws");
       beside(dev, ws);
+    } else if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+      // A graph has a workspace of its own, as ops.workspace's have; of this kind only the counters need be zero (the
+      // fill of all of it takes 2 us).
+      ws = at::empty({(int64_t)up_sm100_kv4_attention_workspace_bytes(tokens, heads, batch, c.kv_heads, c.dim)},
+                     q.options().dtype(at::kByte));
+      ws.narrow(0, 0, (int64_t)up_sm100_kv4_attention_workspace_bytes(0, heads, batch, c.kv_heads, c.dim)).zero_();
     } else {
       const size_t bytes = up_sm100_kv4_attention_workspace_bytes(tokens, heads, batch, c.kv_heads, c.dim);
       PyObject* key = Py_BuildValue("siK", "kv4", dev, (unsigned long long)reinterpret_cast<uintptr_t>(stream));

@@ -43,7 +43,11 @@ _ws_cache: dict = {}
 
 
 def workspace(kind: str, nbytes: int, device: torch.device) -> torch.Tensor:
-    """A zero-filled device workspace for `kind`, reused by later calls on the same stream."""
+    """A zero-filled device workspace for `kind`, reused by later calls on the same stream. While a CUDA graph is being
+    captured, a new one for this call alone: its zero fill is then a part of the graph and its memory the graph's own, so
+    replays depend neither on another graph nor on a buffer that a later call may outgrow."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
     key = (kind, device.index, _raw_stream(device.index))
     with _ws_lock:
         ws = _ws_cache.get(key)
