@@ -30,3 +30,24 @@ def test_a_capture_has_workspaces_of_its_own(fake):
     # what a graph holds is not what an eager call takes, nor what one outgrows
     assert ops.workspace("u", 100, on).data_ptr() != first.data_ptr()
     assert ops.workspace("t", 4096, on).data_ptr() != two.data_ptr()
+
+
+def test_a_device_without_an_index_is_the_current_one(fake, monkeypatch):
+    def stream_of(index):
+        if not isinstance(index, int):
+            raise RuntimeError("a device's index is a number")
+        return {0: 7, 1: 8}[index]
+
+    monkeypatch.setattr(ops, "_raw_stream", stream_of)
+    plain = ops.workspace("t", 64, torch.device("cpu"))
+    assert ops.workspace("t", 64, torch.device("cpu", 0)) is plain
+    fake["device"] = 1
+    assert ops.workspace("t", 64, torch.device("cpu")) is not plain
+    assert set(ops._ws_cache) == {("t", 0, 7), ("t", 1, 8)}
+    asked = []
+    monkeypatch.setattr(ops, "workspace_status", lambda ws: asked.append(ws) or 0)
+    ops.check_workspace("t", torch.device("cpu", 0))
+    fake["device"] = 0
+    ops.check_workspace("t", torch.device("cpu"))
+    ops.check_workspace("none", torch.device("cpu"))
+    assert len(asked) == 2 and all(a is plain for a in asked)

@@ -42,13 +42,19 @@ _ws_lock = threading.Lock()
 _ws_cache: dict = {}
 
 
+def _ws_key(kind: str, device: torch.device):
+    """Of the device's current stream; a device without an index is the current one."""
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return kind, index, _raw_stream(index)
+
+
 def workspace(kind: str, nbytes: int, device: torch.device) -> torch.Tensor:
     """A zero-filled device workspace for `kind`, reused by later calls on the same stream. While a CUDA graph is being
     captured, a new one for this call alone: its zero fill is then a part of the graph and its memory the graph's own, so
     replays depend neither on another graph nor on a buffer that a later call may outgrow."""
     if torch.cuda.is_current_stream_capturing():
         return torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
-    key = (kind, device.index, _raw_stream(device.index))
+    key = _ws_key(kind, device)
     with _ws_lock:
         ws = _ws_cache.get(key)
         if ws is None or ws.numel() < nbytes:
@@ -63,7 +69,7 @@ def workspace_status(ws: torch.Tensor) -> int:
 
 
 def check_workspace(kind: str, device: torch.device):
-    ws = _ws_cache.get((kind, device.index, torch.cuda.current_stream(device).cuda_stream))
+    ws = _ws_cache.get(_ws_key(kind, device))
     if ws is not None:
         check(workspace_status(ws), f"{kind} device wait")
 
