@@ -302,7 +302,8 @@ PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     } else {
       out = new_like(q);
     }
-    const bool want_lse = a[9] == Py_True;
+    const int want_lse = PyObject_IsTrue(a[9]);
+    if (want_lse < 0) throw Raised();
     if (want_lse) {
       at::AutoDispatchBelowADInplaceOrView guard;
       lse = at::empty({tokens, heads}, q.options().dtype(at::kFloat));
