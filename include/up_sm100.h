@@ -492,7 +492,9 @@ UP_API int up_sm100_kv4_append(const void* q, const void* k, const void* v, int 
  * and only j > position - window where window > 0.
  *   out[i] = sum_j softmax_j(scale * q_i . k_j) v_j,   lse[i] = log sum_j exp(scale * q_i . k_j)  (f32, or NULL)
  * over the visible tokens, accumulated in f32, rounded once to q's type. A query that sees nothing gives 0 and -inf.
- * What a masked token's page or slot holds (a NaN scale included) has no effect. seq_lens beyond table_width * page count
+ * What a masked token's page or slot holds (a NaN scale included) has no effect beyond the last bits of f32 and f16
+ * roundings; but where many query rows share a tile, scales below 2^-11 are held to 2^-22 if one of the 128 cached tokens
+ * around them, masked or not, has a scale of 8192 or more. seq_lens beyond table_width * page count
  * as that much; cached tokens on a page outside [0, pages) are left out; query tokens that no sequence names are not
  * written. A NaN in a visible cached value (an infinite scale's are) reaches the outputs that it multiplies, or all of the
  * row's (where many query rows share a tile); one in a key reaches the whole row. `workspace` from

@@ -23,9 +23,12 @@
 //    q is stored in the same order and the output's columns are read in it.
 //  * warps 16 and 17 (products): each issues the tcgen05.mma of one query tile, so neither tile's products wait for the
 //    other's probabilities.
-// Scales. A tile's scales are divided by the power of two of the largest (separately for K and V), so nibble * scale
-// keeps f16's range whatever their size; the logits take K's power, the probabilities V's, relative to the largest one
-// met (O is scaled when a larger one comes). The logits are exact up to their f32 sums, as a row's logsumexp is in f32:
+// Scales. A tile's scales are multiplied by a power of two (separately for K and V) that takes the largest to 2^12 .. 2^13,
+// so nibble * scale ends just inside f16's range; the logits take K's power, the probabilities V's, relative to the one that
+// O has (O is scaled when a tile's is above it, or below a quarter of it). That leaves 2^26 below the largest scale in which
+// a scale keeps all of its bits, so a row's precision does not hang on tokens that it does not see: an f16 scale loses bits
+// only below 2^-11 and only beside one of 8192 or more in its 128 tokens (then it is off by at most 2^-22).
+// The logits are exact up to their f32 sums, as a row's logsumexp is in f32:
 // each of K's scales is split into its first 8 bits and the rest, a nibble times either is exact in f16, and both
 // products are added in one S (with one scale a token, multiplying the columns of S by it in the softmax instead took 381
 // us where this took 320). So is V for f16 outputs. For bf16 ones, which round to 8 bits, nibble * scale is rounded to f16:
@@ -47,6 +50,7 @@ namespace {
 
 constexpr int kRowsCta = 256, kTok = 128, kHalf = kTok / 2;
 constexpr int kThreads = 32 * 18, kCacheWarp = 8, kMmaWarp = 16;
+constexpr int kTop = 12, kLeastExp = -24 - kTop;  // the largest scale of a tile becomes 2^kTop .. 2^(kTop + 1): times -8, -65504
 constexpr int kBlockBytes = kTok * 128;       // 128 query rows of 64 dimensions (128 bytes), swizzled
 constexpr int kHalfBlockBytes = kHalf * 128;  // 64 tokens of 64 dimensions
 
@@ -63,7 +67,7 @@ struct Cfg {
 };
 
 struct Meta {          // what the cache warps say of a tile of tokens
-  int k_exp, v_exp;    // its scales were divided by 2^these
+  int k_exp, v_exp;    // its scales were multiplied by 2^-these
   uint32_t valid[4];   // tokens that exist
   uint32_t bad[4];     // of these, the ones with an infinite or NaN v_scale
 };
@@ -283,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     const int last = r >= live ? -1 : a.causal ? min(pos, seq.len - 1) : seq.len - 1;
     const int past = a.window > 0 ? max(pos - a.window, -1) : -1;
     float mx = kNoMax, sum = 0.f;
-    int vexp = -24;
+    int vexp = kLeastExp;  // O is in units of 2^vexp
     bool ok = true;
     const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (uint64_t)(2 * (a.os | a.oh))) & 15) == 0;  // 16-byte stores
     auto wait = [&](uint64_t* bar, int parity) {
@@ -331,12 +335,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         m = fmaxf(m, m1);
       }
       m = fmaxf(mx, m * c);  // c is not negative; where nothing is seen, -infinity or (c = 0) NaN
-      if (__any_sync(0xffffffffu, m > mx + 8.f || ve > vexp)) {
-        const int e = max(vexp, ve);
-        const float f = exp2_approx(mx - m), fo = f * pow2f(vexp - e);
-        sum *= f;
-        mx = m;
-        vexp = e;
+      const bool rise = __any_sync(0xffffffffu, m > mx + 8.f), move = ve > vexp || ve < vexp - 2;
+      if (rise || move) {
+        float fo = 1.f;
+        if (rise) {
+          fo = exp2_approx(mx - m);
+          sum *= fo;
+          mx = m;
+        }
+        if (move) {
+          fo *= pow2f(vexp - ve);
+          vexp = ve;
+        }
         if (u > 0) {
           // Phases are told apart by parity. PV of half u - 2 is done (S of half u was issued after it) and PV of half u
           // waits for this warp, so the barrier is in the phase asked for or just past it.
@@ -526,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       }
       cache_sync(z);  // also: every warp is done with the last tile's scales
       big = max(max(sh.big[z][0], sh.big[z][1]), max(sh.big[z][2], sh.big[z][3]));
-      const int e = big ? (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)big))) >> 23) - 127 : -24;
+      const int e = big ? (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)big))) >> 23) - 127 - kTop : kLeastExp;
 #pragma unroll
       for (int g = 0; g < CH; ++g) {
         if (g >= groups) continue;
