@@ -497,7 +497,7 @@ UP_API int up_sm100_kv4_append(const void* q, const void* k, const void* v, int 
  * around them, masked or not, has a scale of 8192 or more. seq_lens beyond table_width * page count
  * as that much; cached tokens on a page outside [0, pages) are left out; query tokens that no sequence names are not
  * written. A NaN in a visible cached value (an infinite scale's are) reaches the outputs that it multiplies, or all of the
- * row's (where many query rows share a tile); one in a key reaches the whole row. `workspace` from
+ * row's (where many query rows share a tile), but not lse; one in a key reaches the whole row and its lse. `workspace` from
  * up_sm100_kv4_attention_workspace_bytes, 256-byte aligned, zero-filled before its first use (of it the bytes that are
  * returned for 0 tokens; the rest may hold anything); launches leave it ready for the next one, of any shape that needs no
  * more bytes. A captured launch keeps its address: the buffer lives as long as the graph. The result does not depend on the

@@ -57,3 +57,32 @@ def hidden(dim, group, ratio, nq, which, kind, many):
 @pytest.mark.parametrize("dim,group,ratio,nq", MANY)
 def test_many_rows_keep_their_precision_beside_a_hidden_token(dim, group, ratio, nq, which, kind):
     hidden(dim, group, ratio, nq, which, kind, True)
+
+
+def not_finite(dim, group, ratio, nq, bad, many):
+    """The logsumexp does not depend on the values; outputs that the value does not multiply keep their precision where few
+    query rows share a tile, and are NaN where many do."""
+    n, j = 260, 200
+    assert many_rows(nq, 1, ratio, 1, dim) == many
+    cache, table = cache_of(tokens_of(n, 1, dim, dim + group), 16, group)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    q = torch.randn(nq, ratio, dim, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").bfloat16()
+    cu = cu_of(nq)
+    want, want_lse, tol, tol_lse = exact(q, cache, table, lens, cu)
+    cache[3][int(table[0, j // 16]), 0, j % 16, 0] = bad
+    out, lse = ops.kv4_attention(q, cache, table, lens, cu_q=cu, want_lse=True)
+    assert within(lse, want_lse, tol_lse)[0]
+    sees = n - nq + torch.arange(nq, device="cuda") >= j
+    assert within(out, want, tol, ~sees)[0] if bool((~sees).any()) else True
+    assert not bool(torch.isfinite(out[sees][..., :group]).any())
+    if many:
+        assert bool(out[sees].isnan().all())
+    elif group < dim:
+        rest = (sees.nonzero()[:, 0], slice(None), slice(group, None))
+        assert within(out, want, tol, rest)[0], within(out, want, tol, rest)[1]
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dim,group,ratio,nq", MANY)
+def test_many_rows_keep_the_logsumexp_of_a_value_that_is_not_finite(dim, group, ratio, nq, bad):
+    not_finite(dim, group, ratio, nq, bad, True)

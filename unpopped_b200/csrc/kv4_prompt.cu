@@ -35,7 +35,7 @@
 // that is one product, and the second part's memory is a second stage (310 us against 362). p is rounded to f16. All sums
 // are f32.
 // A token with an infinite or NaN v_scale is left out of the products (its rows would reach queries that do not see it)
-// and the queries that do see it become NaN.
+// and the outputs of the queries that do see it become NaN; their logsumexp, which no value is part of, stays.
 // Every wait is bounded; one that runs out sets the workspace's error word and the CTA unwinds.
 //
 // The tile of 2 x 128 rows is what 512 columns of tensor memory hold (S and O of both tiles at dim 128) and 227 KB of
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     const int past = a.window > 0 ? max(pos - a.window, -1) : -1;
     float mx = kNoMax, sum = 0.f;
     int vexp = kLeastExp;  // O is in units of 2^vexp
-    bool ok = true;
+    bool ok = true, not_finite = false;  // whether a value that the row sees is not
     const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (uint64_t)(2 * (a.os | a.oh))) & 15) == 0;  // 16-byte stores
     auto wait = [&](uint64_t* bar, int parity) {
       return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity & 1, wait_ns, abort_flag)) != 0;
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
       }
       sum = fmaf(s0 + s1, pow2f(vexp - ve), sum);
       const uint32_t bad0 = meta.bad[2 * h], bad1 = meta.bad[2 * h + 1];
-      if ((bad0 | bad1) && ((seen(0) & bad0) | (seen(1) & bad1))) sum = __int_as_float(0x7fffffff);
+      if (bad0 | bad1) not_finite |= ((seen(0) & bad0) | (seen(1) & bad1)) != 0;
       tc::wait_st();
       tc::fence_before_sync();
       __syncwarp();
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     } else {
       tc::fence_after_sync();
       // the row, rounded, into the warp's part of the query tile (its products are done), then out in whole rows
-      const float scale = sum == 0.f ? 0.f : pow2f(vexp) / sum;  // O is 0 where the sum is
+      const float scale = not_finite ? __int_as_float(0x7fffffff) : sum == 0.f ? 0.f : pow2f(vexp) / sum;  // O is 0 where the sum is
 #pragma unroll 1
       for (int g = 0; g < D / 32; ++g) {
         uint32_t v[32] = {};
