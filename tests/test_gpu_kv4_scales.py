@@ -86,3 +86,52 @@ def not_finite(dim, group, ratio, nq, bad, many):
 @pytest.mark.parametrize("dim,group,ratio,nq", MANY)
 def test_many_rows_keep_the_logsumexp_of_a_value_that_is_not_finite(dim, group, ratio, nq, bad):
     not_finite(dim, group, ratio, nq, bad, True)
+
+
+@pytest.mark.parametrize("dim,ratio,nq", [(128, 64, 150), (64, 115, 150)])
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+def test_many_rows_keep_many_small_weights(dim, ratio, nq, kind):
+    """One token with a value of 0 takes nearly all of the weight; 65536 others with weights of 2^-25.6 hold 2^-9.6 of it
+    between them, which is all of the output."""
+    n = 65537
+    assert many_rows(nq, 1, ratio, 1, dim)
+    pages = -(-n // 4096)
+    cache = ops.kv4_cache(pages, 1, dim, 4096, dim)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    cache[0].fill_(0x99), cache[1].fill_(0x77)  # -7 and 7 throughout
+    cache[2].fill_(25.6 * 0.6931471805599453 / (7 * dim)), cache[3].fill_(1.0 / 7)
+    cache[2][0, 0, 5] = cache[3][0, 0, 5] = 0.0
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    q = torch.ones(nq, ratio, dim, device="cuda").to(kind)
+    cu = cu_of(nq)
+    out, lse = ops.kv4_attention(q, cache, table, lens, cu_q=cu, causal=False, scale=1.0, want_lse=True)
+    want, want_lse, tol, tol_lse = exact(q[:1, :1], cache, table, lens, cu_of(1), causal=False, scale=1.0)
+    assert 2.0 ** -10 < float(want.min()) < 2.0 ** -9
+    off = (out.double() - want).abs().max()
+    assert float(off) <= float(tol.min()), (float(off), float(tol.min()))
+    assert float((lse.double() - want_lse).abs().max()) <= float(tol_lse.min())
+
+
+def grow_and_shrink(dim, group, ratio, nq, kind, many):
+    """Values between 2^-12 and 2^12 of the first ones, up and down again, and keys that grow: against 64 bits."""
+    n = 700
+    assert many_rows(nq, 1, ratio, 1, dim) == many
+    x = tokens_of(n, 1, dim, dim)
+    j = torch.arange(n, device="cuda")
+    x[0] *= (0.1 + j / 300)[:, None, None]
+    x[1] *= torch.exp2(12 * torch.sin(j / 50.0))[:, None, None]
+    cache, table = cache_of(x, 16, group)
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    q = torch.randn(nq, ratio, dim, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(kind)
+    for window in (0, 50):
+        cu = cu_of(nq)
+        out, lse = ops.kv4_attention(q, cache, table, lens, cu_q=cu, window=window, want_lse=True)
+        want, want_lse, tol, tol_lse = exact(q, cache, table, lens, cu, window=window)
+        assert within(out, want, tol)[0], within(out, want, tol)[1]
+        assert within(lse, want_lse, tol_lse)[0], within(lse, want_lse, tol_lse)[1]
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,group,ratio,nq", MANY)
+def test_many_rows_over_values_that_grow_and_shrink(dim, group, ratio, nq, kind):
+    grow_and_shrink(dim, group, ratio, nq, kind, True)

@@ -14,8 +14,9 @@
 // each with an S of its own, so that a query tile's probabilities of one half are computed while the tensor cores work
 // on the other.
 //  * warp groups 0 and 1 (probabilities): group w holds query tile w, a thread a row. A thread reads its row of S twice,
-//    for the largest logit and for p = 2^(logit - ref), and writes P as f16 over it: the A operand of the second product.
-//    ref moves only when a logit is more than 2^8 above it; then the thread scales its row of O.
+//    for the largest logit and for p = 2^(logit - ref + 7), and writes P as f16 over it: the A operand of the second product.
+//    ref moves only when a logit is more than 8 above it; then the thread scales its row of O. So p ends at 2^15, and f16
+//    takes weights down to 2^-30 of the largest (without the 7, 65536 weights of 2^-26, a thousandth together, were lost).
 //  * warp groups 2 and 3 (cache, K and V): read 128 tokens' nibbles and scales, a tile ahead in registers, and write
 //    them as f16 into 128-byte swizzled shared memory, a place a half, free again when the half's products are done. Both
 //    have a row a token: K is the B operand with its contraction (the dimensions) contiguous, V
@@ -51,6 +52,7 @@ namespace {
 constexpr int kRowsCta = 256, kTok = 128, kHalf = kTok / 2;
 constexpr int kThreads = 32 * 18, kCacheWarp = 8, kMmaWarp = 16;
 constexpr int kTop = 12, kLeastExp = -24 - kTop;  // the largest scale of a tile becomes 2^kTop .. 2^(kTop + 1): times -8, -65504
+constexpr int kLift = 7;  // p = 2^kLift where a logit is at the reference
 constexpr int kBlockBytes = kTok * 128;       // 128 query rows of 64 dimensions (128 bytes), swizzled
 constexpr int kHalfBlockBytes = kHalf * 128;  // 64 tokens of 64 dimensions
 
@@ -364,8 +366,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
           }
         }
       }
-      // p = 2^(c S - ref), as f16 over columns that were read, and their sum
-      const float add = (float)(ve - vexp) - mx;
+      // p = 2^(c S - ref + kLift), in units of O, as f16 over columns that were read, and their sum
+      const float add = (float)(ve - vexp + kLift) - mx;
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll 1
       for (int g = 0; g < 2; ++g) {
@@ -387,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
         }
         tc::st_32x32b_x16(th + 16 * g, p);
       }
-      sum = fmaf(s0 + s1, pow2f(vexp - ve), sum);
+      sum = fmaf(s0 + s1, pow2f(vexp - ve - kLift), sum);
       const uint32_t bad0 = meta.bad[2 * h], bad1 = meta.bad[2 * h + 1];
       if (bad0 | bad1) not_finite |= ((seen(0) & bad0) | (seen(1) & bad1)) != 0;
       tc::wait_st();
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prompt_kernel(const Args a, c
     } else {
       tc::fence_after_sync();
       // the row, rounded, into the warp's part of the query tile (its products are done), then out in whole rows
-      const float scale = not_finite ? __int_as_float(0x7fffffff) : sum == 0.f ? 0.f : pow2f(vexp) / sum;  // O is 0 where the sum is
+      const float scale = not_finite ? __int_as_float(0x7fffffff) : sum == 0.f ? 0.f : pow2f(vexp - kLift) / sum;  // O is 0 where the sum is
 #pragma unroll 1
       for (int g = 0; g < D / 32; ++g) {
         uint32_t v[32] = {};
