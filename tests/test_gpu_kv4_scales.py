@@ -135,3 +135,16 @@ def grow_and_shrink(dim, group, ratio, nq, kind, many):
 @pytest.mark.parametrize("dim,group,ratio,nq", MANY)
 def test_many_rows_over_values_that_grow_and_shrink(dim, group, ratio, nq, kind):
     grow_and_shrink(dim, group, ratio, nq, kind, True)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("dim,group,ratio,nq", FEW)
+def test_few_rows_keep_their_precision_beside_a_hidden_token(dim, group, ratio, nq, which, kind):
+    hidden(dim, group, ratio, nq, which, kind, False)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dim,group,ratio,nq", FEW)
+def test_few_rows_keep_the_others_precision_beside_a_value_that_is_not_finite(dim, group, ratio, nq, bad):
+    not_finite(dim, group, ratio, nq, bad, False)

@@ -16,8 +16,9 @@
 //    in the two halves of a word, which is the A fragment of V transposed after the same conversion.
 //  * Probabilities: the score fragment times v_scale, rounded to f16, transposed by movmatrix, is the B fragment.
 // q is scaled by a power of two a row to fit f16 (exactly, where it is within 2^-24 of the row's largest); the
-// probabilities by a power of two a warp, the largest exponent of the v_scale seen, so that p * v_scale fits f16 with
-// 2^-24 of range below its largest value. p * v_scale is rounded to f16; every sum is f32.
+// probabilities by a power of two a warp and row, the largest exponent of the v_scale that the row has seen, so that p *
+// v_scale fits f16 with 2^-24 of range below its largest value, whatever the tokens hold that it does not see. p * v_scale is
+// rounded to f16; every sum is f32.
 // The running maximum moves only when a step's probabilities sum to more than 2^9 (f32 sums and the f16 range above hold
 // that), so most steps need one vote, no reduction across lanes and no rescaling.
 //
@@ -65,6 +66,10 @@ __device__ __forceinline__ int swizzle(int r) {
   constexpr int n = D / 32, z = n % 8 == 0 ? 8 : n % 4 == 0 ? 4 : n % 2 == 0 ? 2 : 1;
   return (r / (8 / z)) & (z - 1);
 }
+
+// A column's threshold and the exponent of v_scale that it stands for.
+__device__ __forceinline__ float exp_to_lim(int vexp) { return __uint_as_float((uint32_t)(136 - vexp) << 23); }
+__device__ __forceinline__ int lim_to_exp(float lim) { return 136 - (int)(__float_as_uint(lim) >> 23); }
 
 // a / b for a >= 0, b > 0, in 32 bits where both fit (a 64-bit division is a long sequence).
 __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
@@ -381,15 +386,18 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
     const int all_past = a.window > 0 ? seq.len - seq.nq + i1 - a.window : -1;
 
     float O[CH][2][NT][4];
-    // p = 2^(logit - ref) with ref = mx + vexp: mx a recent maximum of the row's logits, vexp of the exponents of v_scale
-    float ref[NT][2], sum[NT][2], mx[NT][2];
-    int vexp = -24;  // the smallest exponent of an f16
-    uint32_t vbits = 0x0002u;  // the f16 2^(vexp + 1): scales from here on raise vexp
-    float most = 0x1p33f;      // 2^(9 - vexp): a step's sum from here on raises mx
+    // p = 2^(logit - ref) with ref = mx + vexp: mx a recent maximum of the row's logits, vexp of the exponents of the v_scale
+    // that it has seen, which its lim = 2^(9 - vexp) holds: a step's sum from there on raises mx. A column of no row has the
+    // largest vexp, so that it asks for nothing.
+    float ref[NT][2], sum[NT][2], lim[NT][2];
+    uint32_t vbits = 0x0002u;  // the f16 2^(vexp + 1) of the least vexp: scales from here on may raise one
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) ref[nt][j] = mx[nt][j] = kNoMax, sum[nt][j] = 0.f;  // (-3e38 + vexp is -3e38)
+      for (int j = 0; j < 2; ++j) {
+        ref[nt][j] = kNoMax, sum[nt][j] = 0.f;  // (-3e38 + vexp is -3e38)
+        lim[nt][j] = exp_to_lim(tile * ROWS + nt * 8 + 2 * t + j < rows ? -24 : 15);  // -24: the smallest exponent of an f16
+      }
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -484,7 +492,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
             }
       }
       // ---- probabilities, against the running reference ----
-      // this lane's token: the largest of its v_scale, as bits. What is masked, or not finite there, does not count.
+      // this lane's token: the largest of its v_scale, as bits, where it exists
       uint32_t vb = 0;
       if constexpr (!MASKED && EXACT && GT % 2 == 0) {
 #pragma unroll
@@ -518,27 +526,50 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
       weigh();
       bool over = vb >= vbits;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) over |= part[nt][0] > most || part[nt][1] > most;
+      for (int nt = 0; nt < NT; ++nt) over |= part[nt][0] > lim[nt][0] || part[nt][1] > lim[nt][1];
       if (__any_sync(0xffffffffu, over)) {
-        vb = __reduce_max_sync(0xffffffffu, vb);
-        if (vb >= vbits) {
-          vexp = (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)vb))) >> 23) - 127;
-          vbits = vexp >= 15 ? 0x8000u : __half_as_ushort(__float2half_rn(__uint_as_float((uint32_t)(vexp + 128) << 23)));
-          most = __uint_as_float((uint32_t)(136 - vexp) << 23);
+        // each column's largest logit and, where scales have grown, the largest finite v_scale of the tokens that it sees
+        auto finite_scale = [&](int tok) {  // of a token, as bits
+          uint32_t most = 0;
+          for (int z = 0; z < groups; ++z) {
+            const uint32_t w = __half_as_ushort(vs[tok * groups + z]) & 0x7fffu;
+            most = max(most, w < 0x7c00u ? w : 0u);
+          }
+          return most;
+        };
+        const bool grown = __any_sync(0xffffffffu, vb >= vbits);
+        uint32_t all = 0, own[4] = {0, 0, 0, 0};  // own: of this lane's tokens g, g + 8, g + 16, g + 24
+        if (!MASKED) {
+          all = __reduce_max_sync(0xffffffffu, finite_scale(lane));
+        } else if (grown) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) own[i] = finite_scale(g + 8 * i);
         }
+        vbits = 0x8000u;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float m = mx[nt][j];
+            int vexp = lim_to_exp(lim[nt][j]);
+            float m = ref[nt][j] - (float)vexp;
+            uint32_t most = all;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int i = j; i < 4; i += 2) m = fmaxf(m, MASKED ? S[h][nt][i] : S[h][nt][i] * qs[nt][j]);
+              for (int i = j; i < 4; i += 2) {
+                m = fmaxf(m, MASKED ? S[h][nt][i] : S[h][nt][i] * qs[nt][j]);
+                if (MASKED && S[h][nt][i] != -INFINITY) most = max(most, own[2 * h + i / 2]);
+              }
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            if (MASKED && grown) {
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+            }
+            if (most) vexp = max(vexp, (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)most))) >> 23) - 127);
+            lim[nt][j] = exp_to_lim(vexp);
+            if (vexp < 15) vbits = min(vbits, (uint32_t)__half_as_ushort(__float2half_rn(__uint_as_float((uint32_t)(vexp + 128) << 23))));
             const float now = m + (float)vexp, f = exp2_approx(ref[nt][j] - now);
-            mx[nt][j] = m;
             ref[nt][j] = now;
             sum[nt][j] *= f;
 #pragma unroll
@@ -546,6 +577,8 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
 #pragma unroll
               for (int z = 0; z < 2; ++z) O[c][z][nt][j] *= f, O[c][z][nt][2 + j] *= f;
           }
+        vbits = min(vbits, __shfl_xor_sync(0xffffffffu, vbits, 1));
+        vbits = min(vbits, __shfl_xor_sync(0xffffffffu, vbits, 2));
         weigh();
       }
 #pragma unroll
