@@ -148,3 +148,31 @@ def test_few_rows_keep_their_precision_beside_a_hidden_token(dim, group, ratio, 
 @pytest.mark.parametrize("dim,group,ratio,nq", FEW)
 def test_few_rows_keep_the_others_precision_beside_a_value_that_is_not_finite(dim, group, ratio, nq, bad):
     not_finite(dim, group, ratio, nq, bad, False)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,group,ratio,nq", FEW)
+def test_few_rows_over_values_that_grow_and_shrink(dim, group, ratio, nq, kind):
+    grow_and_shrink(dim, group, ratio, nq, kind, False)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+def test_few_rows_keep_many_small_weights(dim, kind):
+    """The same with a heavy token for each of a block's four warps, and sequences (over the same pages) enough that each is
+    the work of few blocks."""
+    n, batch = 65537, 600
+    pages = -(-n // 4096)
+    cache = ops.kv4_cache(pages, 1, dim, 4096, dim)
+    cache[0].fill_(0x99), cache[1].fill_(0x77)
+    cache[2].fill_(25.6 * 0.6931471805599453 / (7 * dim)), cache[3].fill_(1.0 / 7)
+    for j in (5, 37, 69, 101):
+        cache[2][0, 0, j] = cache[3][0, 0, j] = 0.0
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(batch, pages).contiguous()
+    lens = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    q = torch.ones(batch, 2, dim, device="cuda").to(kind)
+    assert not many_rows(batch, batch, 2, 1, dim)
+    out, lse = ops.kv4_attention(q, cache, table, lens, scale=1.0, want_lse=True)
+    want, want_lse, tol, tol_lse = exact(q[:1], cache, table[:1], lens[:1], scale=1.0)
+    assert float((out.double() - want).abs().max()) <= float(tol.min()) < float(want.min()) / 4
+    assert float((lse.double() - want_lse).abs().max()) <= float(tol_lse.min())

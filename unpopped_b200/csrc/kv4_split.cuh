@@ -16,11 +16,11 @@
 //    in the two halves of a word, which is the A fragment of V transposed after the same conversion.
 //  * Probabilities: the score fragment times v_scale, rounded to f16, transposed by movmatrix, is the B fragment.
 // q is scaled by a power of two a row to fit f16 (exactly, where it is within 2^-24 of the row's largest); the
-// probabilities by a power of two a warp and row, the largest exponent of the v_scale that the row has seen, so that p *
-// v_scale fits f16 with 2^-24 of range below its largest value, whatever the tokens hold that it does not see. p * v_scale is
-// rounded to f16; every sum is f32.
-// The running maximum moves only when a step's probabilities sum to more than 2^9 (f32 sums and the f16 range above hold
-// that), so most steps need one vote, no reduction across lanes and no rescaling.
+// probabilities by a power of two a warp and row, the largest exponent of the v_scale that the row has seen, less 5, so that
+// p * v_scale ends at 2^15 and f16 has 2^-30 of range below a weight of one, whatever the tokens hold that the row does not
+// see. p * v_scale is rounded to f16; every sum is f32.
+// The running maximum moves only when a lane's probabilities of a step sum to more than 2^9 (which the 2^15 above holds), so
+// most steps need one vote, no reduction across lanes and no rescaling.
 //
 // Work. Units of 128 cached tokens, over sequences, tiles and heads in order, are split evenly over the launch's CTAs
 // (each sequence's count comes from its length on the device: no host read, no launch bound by the longest sequence).
@@ -67,9 +67,11 @@ __device__ __forceinline__ int swizzle(int r) {
   return (r / (8 / z)) & (z - 1);
 }
 
-// A column's threshold and the exponent of v_scale that it stands for.
-__device__ __forceinline__ float exp_to_lim(int vexp) { return __uint_as_float((uint32_t)(136 - vexp) << 23); }
-__device__ __forceinline__ int lim_to_exp(float lim) { return 136 - (int)(__float_as_uint(lim) >> 23); }
+// A column's threshold and the exponent of v_scale that it stands for. p * v_scale is 2^kLift to 2^(kLift + 1) where a logit
+// is at the running maximum and the v_scale the largest.
+constexpr int kLift = 5;
+__device__ __forceinline__ float exp_to_lim(int vexp) { return __uint_as_float((uint32_t)(136 + kLift - vexp) << 23); }
+__device__ __forceinline__ int lim_to_exp(float lim) { return 136 + kLift - (int)(__float_as_uint(lim) >> 23); }
 
 // a / b for a >= 0, b > 0, in 32 bits where both fit (a 64-bit division is a long sequence).
 __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
@@ -386,16 +388,16 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
     const int all_past = a.window > 0 ? seq.len - seq.nq + i1 - a.window : -1;
 
     float O[CH][2][NT][4];
-    // p = 2^(logit - ref) with ref = mx + vexp: mx a recent maximum of the row's logits, vexp of the exponents of the v_scale
-    // that it has seen, which its lim = 2^(9 - vexp) holds: a step's sum from there on raises mx. A column of no row has the
-    // largest vexp, so that it asks for nothing.
+    // p = 2^(logit - ref) with ref = mx + vexp - kLift: mx a recent maximum of the row's logits, vexp of the exponents of the
+    // v_scale that it has seen, which its lim = 2^(9 + kLift - vexp) holds: a step's sum from there on raises mx. A column of
+    // no row has the largest vexp, so that it asks for nothing.
     float ref[NT][2], sum[NT][2], lim[NT][2];
     uint32_t vbits = 0x0002u;  // the f16 2^(vexp + 1) of the least vexp: scales from here on may raise one
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        ref[nt][j] = kNoMax, sum[nt][j] = 0.f;  // (-3e38 + vexp is -3e38)
+        ref[nt][j] = kNoMax, sum[nt][j] = 0.f;  // (-3e38 + vexp - kLift is -3e38)
         lim[nt][j] = exp_to_lim(tile * ROWS + nt * 8 + 2 * t + j < rows ? -24 : 15);  // -24: the smallest exponent of an f16
       }
 #pragma unroll
@@ -551,7 +553,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             int vexp = lim_to_exp(lim[nt][j]);
-            float m = ref[nt][j] - (float)vexp;
+            float m = ref[nt][j] - (float)(vexp - kLift);
             uint32_t most = all;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -569,7 +571,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<D, NT>::kOcc) kv4_spli
             if (most) vexp = max(vexp, (int)(__float_as_uint(__half2float(__ushort_as_half((unsigned short)most))) >> 23) - 127);
             lim[nt][j] = exp_to_lim(vexp);
             if (vexp < 15) vbits = min(vbits, (uint32_t)__half_as_ushort(__float2half_rn(__uint_as_float((uint32_t)(vexp + 128) << 23))));
-            const float now = m + (float)vexp, f = exp2_approx(ref[nt][j] - now);
+            const float now = m + (float)(vexp - kLift), f = exp2_approx(ref[nt][j] - now);
             ref[nt][j] = now;
             sum[nt][j] *= f;
 #pragma unroll
