@@ -502,8 +502,8 @@ UP_API int up_sm100_kv4_append(const void* q, const void* k, const void* v, int 
  * returned for 0 tokens; the rest may hold anything); launches leave it ready for the next one, of any shape that needs no
  * more bytes. A captured launch keeps its address: the buffer lives as long as the graph. The result does not depend on the
  * order in which the parts of a split sequence finish. q is 16-byte aligned with strides of whole 8 elements, out 8-byte
- * aligned with strides of whole 4 (UP_ERR_UNSUPPORTED else); at most 2^30 cached tokens a sequence and 2^30 query rows
- * (tokens * q_heads / kv_heads). The device-side waits of the kernel for many query rows are bounded:
+ * aligned with strides of whole 4 (UP_ERR_UNSUPPORTED else); at most 2^30 sequences, 2^30 cached tokens each and 2^30
+ * query rows (tokens * q_heads / kv_heads). The device-side waits of the kernel for many query rows are bounded:
  * up_sm100_workspace_status reports one that ran out. Launches that overlap on the GPU need separate workspaces. */
 UP_API int up_sm100_kv4_attention(const void* q, int dtype, int64_t tokens, int64_t q_heads, int64_t q_stride_t,
                                   int64_t q_stride_h, const up_kv4_cache* cache, const int32_t* block_table,

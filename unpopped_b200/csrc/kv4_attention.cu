@@ -41,7 +41,7 @@ extern "C" int up_sm100_kv4_attention(const void* q, int dtype, int64_t tokens, 
   UP_CHECK_ARG(tokens >= 0 && q_heads >= 0 && batch >= 0 && window >= 0 && table_width >= 0 && table_stride >= 0);
   UP_CHECK_ARG(q_stride_t >= 0 && q_stride_h >= 0);
   if (dtype != UP_EK_BF16 && dtype != UP_EK_F16) return UP_ERR_UNSUPPORTED;
-  if (q_heads % cache->kv_heads != 0 || batch > 0x7fffffff) return UP_ERR_UNSUPPORTED;
+  if (q_heads % cache->kv_heads != 0 || batch > kMaxTokens) return UP_ERR_UNSUPPORTED;
   UP_CHECK_ARG(cu_q != nullptr || tokens == batch);
   if (tokens == 0 || q_heads == 0 || batch == 0) return UP_OK;
   const int64_t ratio = q_heads / cache->kv_heads;

@@ -37,7 +37,7 @@ struct Args {
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kNoMax = -3.0e38f;     // a running maximum before anything was seen: below every logit, yet finite
 
-constexpr int64_t kMaxTokens = (int64_t)1 << 30;  // cached tokens a sequence, query rows a head, window: sums fit an int
+constexpr int64_t kMaxTokens = (int64_t)1 << 30;  // cached tokens a sequence, query rows a head, window, sequences: sums fit an int
 
 struct Seq {
   int len, nq;
