@@ -25,3 +25,14 @@ def test_want_lse_is_any_truth_value():
         assert torch.equal(ops.kv4_attention(*args, want_lse=no), out)
     with pytest.raises(RuntimeError):  # a tensor of several elements has no truth value
         ops.kv4_attention(*args, want_lse=torch.ones(2))
+
+
+def test_a_workspace_is_contiguous():
+    """Its size is that of its elements, which a view with other strides does not have behind it."""
+    args = one()
+    for ws in (torch.zeros(1, dtype=torch.uint8, device="cuda").expand(64 << 20),
+               torch.zeros(32 << 20, 2, dtype=torch.uint8, device="cuda")[:, 0]):
+        with pytest.raises(ValueError):
+            ops.kv4_attention(*args, ws=ws)
+    want = ops.kv4_attention(*args)
+    assert torch.equal(ops.kv4_attention(*args, ws=torch.zeros(4 << 20, dtype=torch.float32, device="cuda")), want)

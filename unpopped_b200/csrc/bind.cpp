@@ -313,6 +313,7 @@ PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (given(a[10])) {
       ws = tensor(a[10], "ws");
       beside(dev, ws);
+      need(ws.is_contiguous(), "ws is contiguous");
     } else if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
       // A graph has a workspace of its own, as ops.workspace's have; of this kind only the counters need be zero (the
       // fill of all of it takes 2 us).
