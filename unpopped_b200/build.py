@@ -4,12 +4,14 @@
 
 Sources: unpopped_b200/csrc/*.cu. Output: unpopped_b200/libunpopped_sm100.so, which the snapshot carries to
 the GPU box. Objects are compiled in parallel and relinked only when a source or header changed. Beside it stands
-unpopped_b200/_bind.so, the serving operators' Python calls (csrc/bind.cpp, host code against torch's headers).
+unpopped_b200/_bind.<Python's ABI>.so, the serving operators' Python calls (csrc/bind.cpp, host code against torch's
+headers); it is built anew when its source, torch or Python changes, and left out where there is no torch.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -21,7 +23,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libunpopped_sm100.so")
-BIND = os.path.join(HERE, "_bind.so")
+BIND = os.path.join(HERE, "_bind" + sysconfig.get_config_var("EXT_SUFFIX"))
+BIND_MADE_WITH = os.path.join(OBJ, "bind.txt")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -87,25 +90,54 @@ def build(verbose: bool = False, extra=()) -> str:
     return LIB
 
 
-def _build_bind():
-    src = os.path.join(CSRC, "bind.cpp")
-    if not _stale(BIND, [src, os.path.join(ROOT, "include", "up_sm100.h")]):
-        return
+def _bind_command() -> list | None:
+    """What compiles csrc/bind.cpp, without its output; None where there is no torch to compile it against."""
+    if importlib.util.find_spec("torch") is None:
+        return None
     import torch
 
     base = os.path.dirname(torch.__file__)
+    if not os.path.isdir(os.path.join(base, "include", "ATen")):
+        return None
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc()))), "include")
     includes = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
                 sysconfig.get_paths()["include"], cuda, os.path.join(ROOT, "include")]
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{d}" for d in includes] +
+            [os.path.join(CSRC, "bind.cpp"), "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+             "-lc10_cuda", "-L" + HERE, "-l:libunpopped_sm100.so", "-Wl,-rpath,$ORIGIN"])
+
+
+def _bind_made_with(cmd) -> str:
+    """The text that changes with whatever the binding's binary form depends on beside its source."""
+    import torch
+
+    return "\n".join([torch.__version__, sys.version, *cmd])
+
+
+def _bind_stale(cmd) -> bool:
+    if _stale(BIND, [os.path.join(CSRC, "bind.cpp"), os.path.join(ROOT, "include", "up_sm100.h")]):
+        return True
+    if not os.path.exists(BIND_MADE_WITH):
+        return True
+    with open(BIND_MADE_WITH) as f:
+        return f.read() != _bind_made_with(cmd)
+
+
+def _build_bind():
+    cmd = _bind_command()
+    if cmd is None:
+        print("no torch headers: the C library only, without the Python calls of the serving operators", file=sys.stderr)
+        return
+    if not _bind_stale(cmd):
+        return
     tmp = BIND + ".tmp"
-    cmd = (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + [f"-I{d}" for d in includes] +
-           [src, "-o", tmp, "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
-            "-L" + HERE, "-l:libunpopped_sm100.so", "-Wl,-rpath,$ORIGIN"])
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    r = subprocess.run(cmd + ["-o", tmp], capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on bind.cpp:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, BIND)
+    with open(BIND_MADE_WITH, "w") as f:
+        f.write(_bind_made_with(cmd))
 
 
 def ptxas_report(src_name: str) -> str:

@@ -81,8 +81,11 @@ def _calls():
     """The calls of csrc/bind.cpp; like the library, there is no substitute for them."""
     global _bound
     if _bound is None:
-        from . import _bind
-
+        try:
+            from . import _bind
+        except ImportError as e:
+            raise ImportError("the serving operators' calls are not built for this torch and Python: "
+                              "run python -m unpopped_b200.build") from e
         _bind.init(check, workspace, _ws_cache)
         _bound = _bind
     return _bound
@@ -371,7 +374,22 @@ def gather_rows(table: torch.Tensor, ids: torch.Tensor, oob: str = "skip",
 # ---- int4 dequant and W4A16 ----
 def dequant_i4(w_packed: torch.Tensor, scale: torch.Tensor, group: int, out: torch.Tensor | None = None):
     """bf16 [N, K] from int4 [N, K] packed two per byte ([N, K/2] uint8) and f16 scales [N, K/group]."""
-    return _calls().dequant_i4(w_packed, scale, group, out)
+    try:
+        call = _calls().dequant_i4
+    except ImportError:  # unlike the serving operators it needs the C library only, 3 us a call slower
+        call = _dequant_i4
+    return call(w_packed, scale, group, out)
+
+
+def _dequant_i4(w_packed, scale, group, out):
+    _cuda(w_packed, "w")
+    _cuda(scale, "scale")
+    n, kh = w_packed.shape
+    if out is None:
+        out = torch.empty((n, 2 * kh), dtype=torch.bfloat16, device=w_packed.device)
+    check(_lib.load().up_sm100_dequant_i4_bf16(w_packed.data_ptr(), scale.data_ptr(), n, 2 * kh, group, out.data_ptr(),
+                                               _stream(w_packed)), "dequant_i4")
+    return out
 
 
 def w4a16(w_packed: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, group: int,
