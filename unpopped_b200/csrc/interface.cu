@@ -95,7 +95,7 @@ static const char* interface_body(int id) {
     case UP_K_KV4_APPEND:
       return R"J({"entry_symbol":"up_sm100_kv4_append","params":[{"name":"q","role":"read","elem":"F16|BF16","rank":3},{"name":"k","role":"read","elem":"F16|BF16","rank":3},{"name":"v","role":"read","elem":"F16|BF16","rank":3},{"name":"positions","role":"read","elem":"I32|I64","rank":1},{"name":"table","role":"read","elem":"F32","rank":2},{"name":"slots","role":"read","elem":"I32|I64","rank":1},{"name":"cache","role":"readwrite","elem":"I4+F16","rank":4},{"name":"q_out","role":"write","elem":"F16|BF16","rank":3},{"name":"layout","role":"scalar","elem":"I32"}],"launch":{"block":[256,1,1],"grid":"blocks of query chunks and blocks of key and value rows, alternating","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":256,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["packed values and scales are the stated f32 operations bit for bit"],"workspace":null})J";
     case UP_K_KV4_ATTENTION:
-      return R"J({"entry_symbol":"up_sm100_kv4_attention","params":[{"name":"q","role":"read","elem":"F16|BF16","rank":3},{"name":"cache","role":"read","elem":"I4+F16","rank":4},{"name":"block_table","role":"read","elem":"I32","rank":2},{"name":"seq_lens","role":"read","elem":"I32","rank":1},{"name":"cu_q","role":"read","elem":"I32","rank":1},{"name":"out","role":"write","elem":"F16|BF16","rank":3},{"name":"lse","role":"write","elem":"F32","rank":2},{"name":"causal","role":"scalar","elem":"I32"},{"name":"window","role":"scalar","elem":"I64"},{"name":"scale","role":"scalar","elem":"F32"}],"launch":{"block":[128,1,1],"grid":"few query rows: two to four CTAs per SM over units of 128 cached tokens; prompts (block 576): a CTA per 256 query rows","cluster":null,"dynamic_shared_bytes":"up to 200704"},"launch_bounds":{"max_threads":576,"min_blocks":1},"cooperative":false,"requires":["sm_100a","cp.async","mma.sync","tcgen05","tensor_memory","mbarrier"],"fidelity_notes":["f32 sums; p * v_scale rounded to f16, and in prompts nibble * scale too","split tiles are added in order: deterministic"],"workspace":"counters and parts of split tiles: up_sm100_kv4_attention_workspace_bytes, zero-filled once"})J";
+      return R"J({"entry_symbol":"up_sm100_kv4_attention","params":[{"name":"q","role":"read","elem":"F16|BF16","rank":3},{"name":"cache","role":"read","elem":"I4+F16","rank":4},{"name":"block_table","role":"read","elem":"I32","rank":2},{"name":"seq_lens","role":"read","elem":"I32","rank":1},{"name":"cu_q","role":"read","elem":"I32","rank":1},{"name":"out","role":"write","elem":"F16|BF16","rank":3},{"name":"lse","role":"write","elem":"F32","rank":2},{"name":"causal","role":"scalar","elem":"I32"},{"name":"window","role":"scalar","elem":"I64"},{"name":"scale","role":"scalar","elem":"F32"}],"launch":{"block":[128,1,1],"grid":"few query rows: two to four CTAs per SM over units of 128 cached tokens; prompts (block 576): a CTA per 256 query rows","cluster":null,"dynamic_shared_bytes":"up to 201728"},"launch_bounds":{"max_threads":576,"min_blocks":1},"cooperative":false,"requires":["sm_100a","cp.async","mma.sync","tcgen05","tensor_memory","mbarrier"],"fidelity_notes":["f32 sums, exact logits up to them; few query rows: p * v_scale rounded to f16; many: p, and with bf16 outputs nibble * v_scale","split tiles are added in order: deterministic"],"workspace":"counters and parts of split tiles: up_sm100_kv4_attention_workspace_bytes, zero-filled once"})J";
     default: return nullptr;
   }
 }
