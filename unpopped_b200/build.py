@@ -13,6 +13,7 @@ import concurrent.futures as cf
 import glob
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -51,13 +52,47 @@ def _stale(target: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def revision_hash_of(data: bytes, h: int = 0xCBF29CE484222325) -> int:
+    for b in data:
+        h = ((h ^ b) * 0x100000001B3) & 0xFFFFFFFFFFFFFFFF
+    return h
+
+
 def revision_hash(path: str) -> int:
     """FNV-1a 64 over a source file's bytes: the reference's revision hash (crates/unpopped/src/revision.rs)."""
-    h = 0xCBF29CE484222325
     with open(path, "rb") as f:
-        for b in f.read():
-            h = ((h ^ b) * 0x100000001B3) & 0xFFFFFFFFFFFFFFFF
-    return h
+        return revision_hash_of(f.read())
+
+
+# A serving operator's kernels are in more files than the one that its revision hash is of. That one holds a line with the
+# hash of the others, so the revision changes with any of them.
+OPERATOR_SOURCES = {
+    "rope.cu": ("divide.cuh", "rope.cuh"),
+    "kv4_append.cu": ("divide.cuh", "kv4.cuh", "rope.cuh"),
+    "kv4_attention.cu": ("divide.cuh", "kv4.cuh", "kv4_attention.cuh", "kv4_prompt.cu", "kv4_split.cuh", "kv4_split_128.cu",
+                         "kv4_split_large.cu", "kv4_split_small.cu"),
+}
+
+
+def sources_line(name: str) -> str:
+    """The line of csrc/<name> that stands for the operator's other sources."""
+    h = 0xCBF29CE484222325
+    for other in OPERATOR_SOURCES[name]:
+        with open(os.path.join(CSRC, other), "rb") as f:
+            h = revision_hash_of(f.read(), h)
+    return f"// FNV-1a 64 of {', '.join(OPERATOR_SOURCES[name])}: {h:016x}\n"
+
+
+def write_sources_lines():
+    """Brings the operators' lines up to date (python -m unpopped_b200.build --sources), after any of their files changed."""
+    for name in OPERATOR_SOURCES:
+        path = os.path.join(CSRC, name)
+        with open(path) as f:
+            text = f.read()
+        new = re.sub(r"// FNV-1a 64 of .*\n", lambda m: sources_line(name), text, count=1)
+        if new != text:
+            with open(path, "w") as f:
+                f.write(new)
 
 
 def _compile(src: str, extra) -> str:
@@ -152,5 +187,7 @@ if __name__ == "__main__":
     if len(sys.argv) > 1 and sys.argv[1] == "--ptxas":
         for name in sys.argv[2:]:
             print(ptxas_report(name))
+    elif sys.argv[1:] == ["--sources"]:
+        write_sources_lines()
     else:
         build(verbose=True)

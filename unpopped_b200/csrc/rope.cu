@@ -7,6 +7,8 @@
 // A thread owns two 16-byte chunks whose pairs are complete: in the half layout chunk j of the first half and chunk j of
 // the second, in the interleaved one two neighbours. So a pair is rotated in one thread, nothing is exchanged, and a row
 // may be rotated in place. Consecutive threads take consecutive chunks of a head, then heads, then tokens.
+// The operator's other sources, which its revision hash covers through this line (build.py --sources):
+// FNV-1a 64 of divide.cuh, rope.cuh: 7c239956395924fd
 #include "rope.cuh"
 
 #include <type_traits>
