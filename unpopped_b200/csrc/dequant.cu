@@ -101,11 +101,12 @@ __global__ void __launch_bounds__(256) dequant_i4_rows_kernel(const uint32_t* __
 }
 
 // Rows of at most 768 words (k <= 6144), which leave threads of the kernel above idle (a 128-wide cache row has 16 words), where
-// there are more than four a SM: rows and groups follow one another without a gap, so the array is walked as one line of
+// there are more than three a SM: rows and groups follow one another without a gap, so the array is walked as one line of
 // `words` words, 1024 to a CTA's turn, with the same software pipeline. Measured, this / a CTA a row, in us: 131072 rows
 // of 128 8.1 / 82.7, of 1024 56 / 122, of 4096 227 / 254, of 6144 340 / 344, of 8064 450 / 447; 800 rows of 64 2.1 / 2.4, of 4096
-// 2.9 / 3.4. With fewer rows the CTAs of the kernel above do not wait for one another and less is divided: 296 rows of 1024
-// 2.2 / 1.8, 16 rows of 512 2.2 / 1.7.
+// 2.9 / 3.4. With fewer rows the kernel above has a CTA for each at once and divides less: 296 rows of 1024 2.2 / 1.8, 16 rows
+// of 512 2.2 / 1.7. The two meet between three and four rows a SM: 444 rows of 128 2.04 / 1.89, 592 2.06 / 2.05, 444 rows of
+// 4096 2.6 / 2.4, 592 2.7 / 2.8. There calls that allocate their output take 3.8 / 4.5 us of the host's time.
 __global__ void __launch_bounds__(256) dequant_i4_line_kernel(const uint32_t* __restrict__ w,
                                                               const __half* __restrict__ scale, uint32_t words,
                                                               uint32_t wpg, uint4* __restrict__ out) {
@@ -169,7 +170,7 @@ extern "C" int up_sm100_dequant_i4_bf16(const uint8_t* w, const uint16_t* scale,
   const int sms = sm_count();
   const auto* sc = reinterpret_cast<const __half*>(scale);
   if (k % 8 == 0 && group % 8 == 0 && aligned(w, 4) && aligned(out, 16) && k / 8 <= 0x7fffffff) {
-    if (k <= 6144 && n > 4 * sms && n <= (int64_t)1 << 31 && n * (k / 8) <= (int64_t)1 << 31) {
+    if (k <= 6144 && n > 3 * sms && n <= (int64_t)1 << 31 && n * (k / 8) <= (int64_t)1 << 31) {
       const int64_t words = n * (k / 8), turns = (words + 1023) / 1024, most = (int64_t)sms * 32;
       dequant_i4_line_kernel<<<(int)(turns < most ? turns : most), 256, 0, s>>>(
           reinterpret_cast<const uint32_t*>(w), sc, (uint32_t)words, (uint32_t)(group / 8), reinterpret_cast<uint4*>(out));
