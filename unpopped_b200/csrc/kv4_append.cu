@@ -22,7 +22,7 @@
 // Four rows a thread, loaded together, measured slower (231 us against 159 us for 16001 tokens of 64 and 8 heads, both with
 // an earlier form of the queries' part): the registers that they take halve the queries' blocks on an SM.
 // The operator's other sources, which its revision hash covers through this line (build.py --sources):
-// FNV-1a 64 of divide.cuh, kv4.cuh, rope.cuh: cf33daadbd025db6
+// FNV-1a 64 of divide.cuh, kv4.cuh, rope.cuh: 96ec8a3a8dd401a2
 #include "kv4.cuh"
 #include "rope.cuh"
 

@@ -1,6 +1,6 @@
 // kv4_attention.cu — attention over the paged 4-bit cache: argument checks, workspace and the choice of kernel.
 // The operator's other sources, which its revision hash covers through this line (build.py --sources):
-// FNV-1a 64 of divide.cuh, kv4.cuh, kv4_attention.cuh, kv4_prompt.cu, kv4_split.cuh, kv4_split_128.cu, kv4_split_large.cu, kv4_split_small.cu: 3d85f77e792155d1
+// FNV-1a 64 of divide.cuh, kv4.cuh, kv4_attention.cuh, kv4_prompt.cu, kv4_split.cuh, kv4_split_128.cu, kv4_split_large.cu, kv4_split_small.cu: 68c4624a8b9ca682
 #include "kv4_attention.cuh"
 
 namespace up {

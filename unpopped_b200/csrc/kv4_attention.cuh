@@ -199,9 +199,10 @@ constexpr int kGroup = 16;                     // parts of a split tile that are
 constexpr size_t kHeaderBytes = 256, kCounterBytes = kHeaderBytes + 3 * kMaxCtas * sizeof(uint32_t);
 
 // Query rows a tile has in the split kernel: 8 a column group, a second one where the head size leaves registers (not
-// above 128) and the rows of a sequence and key/value head need it. Measured with 64 sequences of 2048 tokens, 8 key/value
-// heads of 128: 8 rows 41 us in tiles of 8 and 53 of 16, 12 rows 68 and 55, 32 rows 123 and 97; one sequence of 2048, where
-// little but the start counts: 8 rows 10.1 and 11.7, 32 rows 12.5 and 15.4.
+// above 128) and the rows of a sequence and key/value head need it on average: the host knows the batch's rows, not each
+// sequence's, and a sequence of fewer rows then computes an empty group. Measured with 64 sequences of 2048 tokens, all of the
+// same rows, 8 key/value heads of 128: 8 rows 41 us in tiles of 8 and 53 of 16, 12 rows 68 and 55, 32 rows 123 and 97; one
+// sequence of 2048, where little but the start counts: 8 rows 10.1 and 11.7, 32 rows 12.5 and 15.4.
 inline int split_rows(int64_t rows_a_sequence, int64_t dim) {
   return rows_a_sequence > 8 && (dim == 64 || dim == 96 || dim == 128) ? 16 : 8;
 }
@@ -209,10 +210,12 @@ inline int split_rows(int64_t rows_a_sequence, int64_t dim) {
 // Whether the kernel for many query rows (head sizes 64 and 128; 256 rows a CTA, one CTA an SM) takes less time than the
 // split one, given `rows` query rows for each of `pairs` (sequence, key/value head): the first in as many turns as its
 // CTAs fill the SMs, the second in 16-row tiles that are spread evenly. Against as many cached tokens a 256-row tile takes
-// an SM as long as four 16-row ones at head size 128 and six at 64. Measured from one sequence of 4096 tokens to 32 of
-// 2048, 8 key/value heads, 32 to 1024 rows each, the faster one is taken but within 4 %: 12 sequences of 4096 at size 128,
-// 96 rows 102 us split and 118 not, 128 rows 129 and 116; 4 of them, 256 rows 90 and 102, 384 rows 127 and 114; at size
-// 64, 12 of them, 128 rows 84 and 108, 192 rows 119 and 106.
+// an SM as long as four 16-row ones at head size 128 and six at 64. `rows` is the batch's mean and the measurements are of
+// equal sequences; a batch of unequal ones goes to one kernel whole (a prompt of 2048 and 63 single tokens, 4096 cached
+// tokens each, 32 heads over 8: 617 us, as two calls 152 and 67). From one sequence of 4096 tokens to 32 of 2048, 8 key/value
+// heads, 32 to 1024 rows each, the faster one is taken but within 4 %: 12 sequences of 4096 at size 128, 96 rows 102 us split
+// and 118 not, 128 rows 129 and 116; 4 of them, 256 rows 90 and 102, 384 rows 127 and 114; at size 64, 12 of them, 128 rows
+// 84 and 108, 192 rows 119 and 106.
 inline bool many_rows(int64_t rows, int64_t pairs, int64_t dim, int64_t sms) {
   if (dim != 64 && dim != 128) return false;
   const int64_t turns = (pairs * ((rows + 255) / 256) + sms - 1) / sms;

@@ -6,7 +6,7 @@
 // memory again), the exponentials 2050 (16 a clock and SM), and the schedulers issue in half. Leaving out half of the
 // products, the exponentials or the conversion of the cache gains 6, 1 and 5 % each: the chain from S to P to the next S
 // is what takes the time. Starting and ending a CTA takes 14000 cycles more. Three sequences of 1500 to 2048 query
-// tokens, 32 heads over 8, dim 128: bf16 310 us (198 GFLOP, 638 TFLOP/s; the second products of the parts not counted).
+// tokens, 32 heads over 8, dim 128: bf16 311 us (198 GFLOP, 636 TFLOP/s; the second products of the parts not counted).
 //
 // A CTA takes 256 query rows (query token x head of the group) of one sequence and key/value head as two tiles of 128,
 // and walks the cached tokens that any of them sees, 128 at a time. Per tile of tokens, S = Q K^T (128 x 128) and
@@ -33,7 +33,7 @@
 // each of K's scales is split into its first 8 bits and the rest, a nibble times either is exact in f16, and both
 // products are added in one S (with one scale a token, multiplying the columns of S by it in the softmax instead took 381
 // us where this took 320). So is V for f16 outputs. For bf16 ones, which round to 8 bits, nibble * scale is rounded to f16:
-// that is one product, and the second part's memory is a second stage (310 us against 362). p is rounded to f16. All sums
+// that is one product, and the second part's memory is a second stage (311 us against 367). p is rounded to f16. All sums
 // are f32.
 // A token with an infinite or NaN v_scale is left out of the products (its rows would reach queries that do not see it)
 // and the outputs of the queries that do see it become NaN; their logsumexp, which no value is part of, stays.

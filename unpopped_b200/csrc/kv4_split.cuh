@@ -32,9 +32,9 @@
 // finishes last adds them in order. No CTA waits for another.
 //
 // What bounds it: HBM where contexts are long; while the loop runs it reads 6.0 to 6.4 TB/s, with about 560 instructions a
-// warp and 32 tokens of size 128 (the schedulers issue in 59 % of their cycles). 64 query over 8 key/value heads of 128,
+// warp and 32 tokens of size 128 (the schedulers issue in 60 % of their cycles). 64 query over 8 key/value heads of 128,
 // bf16: 32 contexts of 8000 to 16384 tokens 89 us (412 MB: 4.6 TB/s), one of 131071 tokens 42 us (143 MB: 3.4 TB/s), one of
-// 777 tokens 9.5 us. What is beside the loop, and all that short contexts cost: lengths, then pages, then the first data
+// 777 tokens 9.2 us. What is beside the loop, and all that short contexts cost: lengths, then pages, then the first data
 // (3 to 5 us), the parts' merge (2 to 5 us), and CTAs that share an SM with slower ones.
 #pragma once
 

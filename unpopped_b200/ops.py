@@ -434,13 +434,15 @@ def rope(x: torch.Tensor, positions: torch.Tensor | None, table: torch.Tensor, l
     """Rotary positions: x [tokens, heads, dim] or [batch, seq, heads, dim] (float32, float16, bfloat16; any strides with
     the dimension contiguous) with the first table.shape[1] dimensions of each head turned by the token's position.
     layout "half" pairs dimensions (i, i + rot/2), "interleaved" (2i, 2i + 1). positions: int32 or int64, one a token
-    ([seq] serves every sequence of a batch), None counts from 0; one outside the table gives NaN. out may be x."""
+    ([seq] serves every sequence of a batch), None counts from 0; one outside the table gives NaN. out may be x.
+    Like every function here it is no part of autograd: the result requires no gradient, `rope_backward` gives it."""
     return _calls().rope(x, positions, table, layout, out, False)
 
 
 def rope_backward(grad: torch.Tensor, positions: torch.Tensor | None, table: torch.Tensor, layout: str = "half",
                   out: torch.Tensor | None = None) -> torch.Tensor:
-    """The gradient of `rope` with respect to its input, from the gradient of its output."""
+    """The gradient of `rope` with respect to its input, from the gradient of its output (what a torch.autograd.Function
+    around `rope` returns from its backward)."""
     return _calls().rope(grad, positions, table, layout, out, True)
 
 
@@ -479,7 +481,9 @@ def kv4_attention(q: torch.Tensor, cache: tuple, block_table: torch.Tensor, seq_
     key/value head h // (heads // kv_heads). seq_lens int32 [batch]: a sequence's cached tokens, the new ones included;
     block_table int32 [batch, width]: its pages. cu_q int32 [batch + 1]: where each sequence's query tokens begin in q;
     None: one token a sequence. The query tokens are the last of their sequence: each sees the cached tokens up to its own
-    (`causal`), and of these the last `window` where window > 0. A query that sees nothing gives 0 (and -inf)."""
+    (`causal`), and of these the last `window` where window > 0. A query that sees nothing gives 0 (and -inf).
+    ws: a workspace of the caller's, contiguous and zero-filled once; without one the stream's is used, or a captured graph's
+    own. A batch of long prompts and single tokens takes less time as two calls."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     return _calls().kv4_attention(q, cache, block_table, seq_lens, cu_q, causal, window, scale, out, want_lse, ws)
