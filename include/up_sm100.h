@@ -119,7 +119,11 @@ typedef enum up_kernel_id {
    * them; their typed entry points are below. */
   UP_K_ROPE = 17,
   UP_K_KV4_APPEND = 18,
-  UP_K_KV4_ATTENTION = 19
+  UP_K_KV4_ATTENTION = 19,
+  UP_K_F8_QUANTISE = 20,
+  UP_K_F8_MATMUL = 21,
+  UP_K_EXPERT_ROUTE = 22,
+  UP_K_EXPERT_COMBINE = 23
 } up_kernel_id;
 
 /* A buffer argument: the reference's TypedBuffer / OperandDesc. `base` and `stride` count elements
@@ -513,6 +517,71 @@ UP_API int up_sm100_kv4_attention(const void* q, int dtype, int64_t tokens, int6
                                   void* workspace, size_t workspace_bytes, void* stream);
 UP_API size_t up_sm100_kv4_attention_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t batch, int64_t kv_heads,
                                                      int64_t dim);
+
+/* ---- Serving operators: 8-bit products with a scale for each block of 128, and experts --------------------
+ *
+ * No counterpart in the reference. up_sm100_w4a16_gemm serves at most 16 rows; these serve prompts too, and layers whose
+ * tokens go to a few of many experts. 8-bit values are e4m3 (UP_EK_FP8_E4M3FN, largest 448, no infinities). Activations
+ * have one f32 scale for each 128 values of a row, weights one for each 128 x 128 block; a last block may be shorter. */
+
+/* Rows of x as 8-bit values. Row r of the result is y = x[rows[r]] (rows NULL: x[r], and n_rows = tokens), or with
+ * `gate` != 0, where x holds 2k values a row, y[i] = x[i] / (1 + exp(-x[i])) * x[k + i]. For each 128 values of y, with a
+ * the largest magnitude of its finite ones: scale = a * f32(1/448), q = e4m3(y * (1/scale)), in f32. Where that scale is below 2^-126 it is
+ * 0, and so is q. An infinity or a NaN gives the NaN code in its place. A row whose rows[r] is outside [0, tokens) gives
+ * zeros, scales too. x [tokens, k] is F32, F16 or BF16, 16-byte aligned with rows of whole 16 bytes, k a multiple of 16
+ * (UP_ERR_UNSUPPORTED else); q [n_rows, k] is dense and 16-byte aligned; scale [n_rows, ceil(k / 128)] has the strides given. */
+UP_API int up_sm100_f8_quantise(const void* x, int dtype, int64_t tokens, int64_t x_stride, const int32_t* rows,
+                                int64_t n_rows, int64_t k, int gate, uint8_t* q, float* scale, int64_t scale_stride_r,
+                                int64_t scale_stride_b, void* stream);
+
+/* Weights as 8-bit values: w [experts, n, k] (strides in elements, k contiguous) to q, dense, with one scale for each
+ * 128 x 128 block: scale [experts, ceil(n / 128), ceil(k / 128)], dense. The same formula, types and limits. */
+UP_API int up_sm100_f8_quantise_weight(const void* w, int dtype, int64_t experts, int64_t n, int64_t k,
+                                       int64_t w_stride_e, int64_t w_stride_n, uint8_t* q, float* scale, void* stream);
+
+/* out[m][j] = sum over blocks b of 128: x_scale[m][b] * w_scale[e][j / 128][b] * (sum over k in b: x[m][k] w[e][j][k]),
+ * each block's sum and the sum over blocks in f32 (tcgen05, block by block), rounded once to out_dtype (F32, F16 or BF16).
+ * offsets NULL: one matrix (experts 1) for all rows. Otherwise (I32, experts + 1 entries, on the device) rows
+ * [offsets[e], offsets[e + 1]) take matrix e; entries are held to [0, m] and to their predecessors, and rows that no
+ * expert has are left as they were. x [m, k] e4m3, rows `x_stride` bytes apart; w [experts, n, k] e4m3, dense; both 16-byte
+ * aligned, k and x_stride multiples of 16 (UP_ERR_UNSUPPORTED else). x_scale [m, ceil(k / 128)] f32 has the strides given (as
+ * up_sm100_f8_quantise leaves them, one block's scales of all rows beside one another, is fastest); w_scale [experts,
+ * ceil(n / 128), ceil(k / 128)] f32, dense. out's rows are out_stride elements apart. At most 1024 experts. `workspace` from
+ * up_sm100_f8_matmul_workspace_bytes, 256-byte aligned, its first UP_F8_COUNTER_BYTES zero-filled before its first use; a
+ * launch leaves it ready for the next, of any shape. The result does not depend on the order in which parts of a split
+ * tile finish. The waits inside are bounded: up_sm100_workspace_status reports one that ran out. Launches that overlap
+ * on the GPU need separate workspaces. */
+#define UP_F8_COUNTER_BYTES 8192
+UP_API int up_sm100_f8_matmul(const uint8_t* x, int64_t m, int64_t x_stride, const float* x_scale, int64_t xs_stride_m,
+                              int64_t xs_stride_b, const uint8_t* w, const float* w_scale, int64_t experts, int64_t n,
+                              int64_t k, const int32_t* offsets, void* out, int out_dtype, int64_t out_stride,
+                              void* workspace, size_t workspace_bytes, void* stream);
+UP_API size_t up_sm100_f8_matmul_workspace_bytes(int64_t m, int64_t experts, int64_t n, int64_t k);
+
+/* How a token's logits become weights: exp(l - max) / sum over the experts, or 1 / (1 + exp(-l)). */
+typedef enum up_expert_score { UP_EXPERT_SOFTMAX = 0, UP_EXPERT_SIGMOID = 1 } up_expert_score;
+
+/* Routes tokens to experts and lays the pairs out by expert. Of each row of logits [tokens, experts] (F32, F16 or BF16) the
+ * k largest are taken, largest first, the lower expert of equal ones, a NaN before all others; an expert whose logit is
+ * -inf is never taken. ids[t][j] is the expert (-1 where none is left), weights[t][j] its score in f32 (0 there), divided by
+ * the chosen ones' sum with `renormalise` != 0 (0 where that sum is 0), times gain. The pairs that were taken, in the order
+ * of their expert and then of their token, have the places 0, 1, ...: slots[t][j] is a pair's place (-1 for none), rows[place] its
+ * token (-1 behind the last), offsets[e] the first place of expert e and offsets[experts] the number of pairs. At most
+ * 1024 experts, k at most 32 and at most experts, tokens * k below 2^31. `workspace` from
+ * up_sm100_expert_route_workspace_bytes, 256-byte aligned; what it holds does not matter. Launches that overlap on the
+ * GPU need separate workspaces. */
+UP_API int up_sm100_expert_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t stride, int64_t k,
+                                 int score, int renormalise, float gain, int32_t* ids, float* weights, int32_t* rows,
+                                 int32_t* slots, int32_t* offsets, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+UP_API size_t up_sm100_expert_route_workspace_bytes(int64_t tokens, int64_t experts);
+
+/* out[t] = add[t] + sum over j in order: weights[t][j] * y[slots[t][j]], in f32, rounded once; a slot outside [0, rows) adds
+ * nothing, add NULL is zeros. y [rows, n], add and out [tokens, n] have one type (F32, F16 or BF16) and contiguous rows,
+ * strides in elements; slots and weights [tokens, k] are dense. out may be add. */
+UP_API int up_sm100_expert_combine(const void* y, int dtype, int64_t rows, int64_t y_stride, int64_t n,
+                                   const int32_t* slots, const float* weights, int64_t tokens, int64_t k,
+                                   const void* add, int64_t add_stride, void* out, int64_t out_stride, void* stream);
 
 /* ---- Several GPUs of one node ------------------------------------------------------------------------
  *

@@ -31,10 +31,12 @@ KERNEL = dict(NONE=-1, ROW_SUM_F32=1, ROW_MAX_ARGMAX_BF16=2, SCAN_I32=3, GATHER_
               W4A16_GEMM=6, REDUCE2D_F32=7, REDUCE2D_I32=8, SCATTER=9, BINCOUNT=10, REDUCE_F32=11, REDUCE_I32=12,
               ROW_REDUCE_F32=13, COL_SUM_SPLITK=14, WINDOW=15, IM2COL=16)
 # The serving operators' ids, for their interface artifacts: no plan lowers to them
-SERVING_KERNEL = dict(ROPE=17, KV4_APPEND=18, KV4_ATTENTION=19)
+SERVING_KERNEL = dict(ROPE=17, KV4_APPEND=18, KV4_ATTENTION=19, F8_QUANTISE=20, F8_MATMUL=21, EXPERT_ROUTE=22,
+                      EXPERT_COMBINE=23)
 ROW_REDUCE_FORM = dict(NONE=0, SOFTMAX=1, RMS_NORM=2, CENTRED=3)
 # up_rope_layout, up_rope_scaling
 ROPE_LAYOUT = dict(HALF=0, INTERLEAVED=1)
+EXPERT_SCORE = dict(SOFTMAX=0, SIGMOID=1)  # up_expert_score
 ROPE_SCALING = dict(NONE=0, LINEAR=1, BASE=2, WAVELENGTH=3, RAMP=4)
 # WriteCombine ordinals (crates/unpopped/src/ir.rs:2723-2732)
 COMBINE = dict(ASSIGN=0, ADD=1, MAX=2, MIN=3)
@@ -130,6 +132,13 @@ SIGNATURES = {
     "up_sm100_kv4_attention": ([_P, _I, _I64, _I64, _I64, _I64, _KV4, _P, _I64, _I64, _P, _P, _I64, _I, _I64, _F32, _P,
                                 _I64, _I64, _P, _I64, _P, _SZ, _P], _I),
     "up_sm100_kv4_attention_workspace_bytes": ([_I64, _I64, _I64, _I64, _I64], _SZ),
+    "up_sm100_f8_quantise": ([_P, _I, _I64, _I64, _P, _I64, _I64, _I, _P, _P, _I64, _I64, _P], _I),
+    "up_sm100_f8_quantise_weight": ([_P, _I, _I64, _I64, _I64, _I64, _I64, _P, _P, _P], _I),
+    "up_sm100_f8_matmul": ([_P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _P, _I, _I64, _P, _SZ, _P], _I),
+    "up_sm100_f8_matmul_workspace_bytes": ([_I64, _I64, _I64, _I64], _SZ),
+    "up_sm100_expert_route": ([_P, _I, _I64, _I64, _I64, _I64, _I, _I, _F32, _P, _P, _P, _P, _P, _P, _SZ, _P], _I),
+    "up_sm100_expert_route_workspace_bytes": ([_I64, _I64], _SZ),
+    "up_sm100_expert_combine": ([_P, _I, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _P], _I),
     "up_sm100_set_wait_limit_ns": ([_U64], None),
     "up_sm100_set_test_withhold_flag": ([_I], None),
     "up_sm100_set_test_scan_epoch": ([_U64], None),

@@ -11,9 +11,11 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <exception>
+#include <initializer_list>
 
 #include "up_sm100.h"
 
@@ -387,6 +389,260 @@ PyObject* dequant_i4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- 8-bit products and experts ----
+int float_kind(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? (int)UP_EK_F32 : half_kind(t); }
+
+at::Tensor empty(at::IntArrayRef sizes, const at::Tensor& beside_it, at::ScalarType type) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return at::empty(sizes, beside_it.options().dtype(type));
+}
+
+// The stream's workspace of this kind (ops.workspace's), or a captured graph's own, of which the first `counters` bytes are
+// zero-filled within the graph.
+at::Tensor workspace_of(const char* kind, PyObject* beside_it, int dev, void* stream, size_t bytes, size_t counters) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+    at::Tensor ws = empty({(int64_t)bytes}, THPVariable_Unpack(beside_it), at::kByte);
+    if (counters > 0) ws.narrow(0, 0, (int64_t)counters).zero_();
+    return ws;
+  }
+  PyObject* key = Py_BuildValue("siK", kind, dev, (unsigned long long)reinterpret_cast<uintptr_t>(stream));
+  if (!key) throw Raised();
+  PyObject* held = PyDict_GetItemWithError(g_cache, key);
+  Py_DECREF(key);
+  if (held && (size_t)tensor(held, "workspace").nbytes() >= bytes) return tensor(held, "workspace");
+  if (PyErr_Occurred()) throw Raised();
+  PyObject* device = PyObject_GetAttrString(beside_it, "device");
+  PyObject* made = device ? PyObject_CallFunction(g_workspace, "snO", kind, (Py_ssize_t)bytes, device) : nullptr;
+  Py_XDECREF(device);
+  if (!made) throw Raised();
+  at::Tensor ws = tensor(made, "workspace");
+  Py_DECREF(made);
+  return ws;
+}
+
+PyObject* tuple_of(std::initializer_list<at::Tensor*> items) {
+  PyObject* all = PyTuple_New((Py_ssize_t)items.size());
+  if (!all) throw Raised();
+  Py_ssize_t i = 0;
+  for (at::Tensor* t : items) {
+    PyObject* o = THPVariable_Wrap(std::move(*t));
+    if (!o) {
+      Py_DECREF(all);
+      throw Raised();
+    }
+    PyTuple_SET_ITEM(all, i++, o);
+  }
+  return all;
+}
+
+// f8_quantise(x, rows, gate)
+PyObject* f8_quantise(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 3);
+    const at::Tensor& x = cuda_tensor(a[0], "x");
+    const int kind = float_kind(x);
+    need(kind >= 0 && x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1),
+         "x is float32, float16 or bfloat16 [tokens, k] with contiguous rows");
+    const int dev = current_device_of(x);
+    const int gate = PyObject_IsTrue(a[2]);
+    if (gate < 0) throw Raised();
+    need(!gate || x.size(1) % 2 == 0, "with a gate, x holds 2k values a row");
+    const int64_t k = gate ? x.size(1) / 2 : x.size(1);
+    const int32_t* rows = nullptr;
+    int64_t n_rows = x.size(0);
+    if (given(a[1])) {
+      const at::Tensor& r = tensor(a[1], "rows");
+      need(r.scalar_type() == at::kInt && r.dim() == 1 && r.is_contiguous(), "rows is contiguous int32 [n]");
+      beside(dev, r);
+      rows = r.data_ptr<int32_t>(), n_rows = r.size(0);
+    }
+    const int64_t blocks = (k + 127) / 128;
+    at::Tensor q = empty({n_rows, k}, x, at::kFloat8_e4m3fn), scale;
+    {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      scale = at::empty_strided({n_rows, blocks}, {1, n_rows}, x.options().dtype(at::kFloat));
+    }
+    check(unlocked([&] {
+            return up_sm100_f8_quantise(x.data_ptr(), kind, x.size(0), x.stride(0), rows, n_rows, k, gate,
+                                        static_cast<uint8_t*>(q.data_ptr()), scale.data_ptr<float>(), 1, n_rows, stream_of(dev));
+          }),
+          "f8_quantise");
+    return tuple_of({&q, &scale});
+  });
+}
+
+// f8_quantise_weight(w)
+PyObject* f8_quantise_weight(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 1);
+    const at::Tensor& w = cuda_tensor(a[0], "w");
+    const int kind = float_kind(w);
+    const bool many = w.dim() == 3;
+    need(kind >= 0 && (many || w.dim() == 2) && (w.stride(-1) == 1 || w.size(-1) <= 1),
+         "w is float32, float16 or bfloat16 [n, k] or [experts, n, k] with contiguous rows");
+    const int dev = current_device_of(w);
+    const int64_t experts = many ? w.size(0) : 1, rows = w.size(-2), k = w.size(-1), bn = (rows + 127) / 128, bk = (k + 127) / 128;
+    at::Tensor q, scale;
+    if (many)
+      q = empty({experts, rows, k}, w, at::kFloat8_e4m3fn), scale = empty({experts, bn, bk}, w, at::kFloat);
+    else
+      q = empty({rows, k}, w, at::kFloat8_e4m3fn), scale = empty({bn, bk}, w, at::kFloat);
+    check(unlocked([&] {
+            return up_sm100_f8_quantise_weight(w.data_ptr(), kind, experts, rows, k, many ? w.stride(0) : 0, w.stride(-2),
+                                               static_cast<uint8_t*>(q.data_ptr()), scale.data_ptr<float>(), stream_of(dev));
+          }),
+          "f8_quantise_weight");
+    return tuple_of({&q, &scale});
+  });
+}
+
+// f8_matmul(x, x_scale, w, w_scale, offsets, dtype, out, ws): offsets None for one matrix
+PyObject* f8_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 8);
+    const bool many = given(a[4]);
+    const char* name = many ? "f8_expert_matmul" : "f8_matmul";
+    const at::Tensor &x = cuda_tensor(a[0], "x"), &xs = tensor(a[1], "x_scale"), &w = tensor(a[2], "w"), &ws = tensor(a[3], "w_scale");
+    const int dev = current_device_of(x);
+    need(x.scalar_type() == at::kFloat8_e4m3fn && x.dim() == 2 && (x.stride(1) == 1 || x.size(1) <= 1),
+         "x is float8_e4m3fn [rows, k] with contiguous rows");
+    const int64_t m = x.size(0), k = x.size(1), kb = (k + 127) / 128;
+    need(w.scalar_type() == at::kFloat8_e4m3fn && w.dim() == (many ? 3 : 2) && w.size(-1) == k && w.is_contiguous(),
+         many ? "w is float8_e4m3fn [experts, n, k] of x's k, contiguous" : "w is float8_e4m3fn [n, k] of x's k, contiguous");
+    const int64_t experts = many ? w.size(0) : 1, cols = w.size(-2), nb = (cols + 127) / 128;
+    need(xs.scalar_type() == at::kFloat && xs.dim() == 2 && xs.size(0) == m && xs.size(1) == kb,
+         "x_scale is float32 [rows, ceil(k / 128)]");
+    need(ws.scalar_type() == at::kFloat && ws.dim() == w.dim() && ws.size(-2) == nb && ws.size(-1) == kb &&
+             (!many || ws.size(0) == experts) && ws.is_contiguous(),
+         "w_scale is float32 [ceil(n / 128), ceil(k / 128)], for each expert, contiguous");
+    beside(dev, xs), beside(dev, w), beside(dev, ws);
+    const int32_t* offsets = nullptr;
+    if (many) {
+      const at::Tensor& o = tensor(a[4], "offsets");
+      need(o.scalar_type() == at::kInt && o.dim() == 1 && o.size(0) == experts + 1 && o.is_contiguous(),
+           "offsets is contiguous int32 [experts + 1]");
+      beside(dev, o);
+      offsets = o.data_ptr<int32_t>();
+    }
+    at::Tensor out;
+    if (given(a[6])) {
+      out = tensor(a[6], "out");
+      need(out.dim() == 2 && out.size(0) == m && out.size(1) == cols && (out.stride(1) == 1 || cols <= 1),
+           "out is [rows, n] with contiguous rows");
+      beside(dev, out);
+    } else {
+      need(THPDtype_Check(a[5]), "dtype is a torch dtype");
+      const at::ScalarType type = reinterpret_cast<THPDtype*>(a[5])->scalar_type;
+      need(type == at::kFloat || type == at::kHalf || type == at::kBFloat16, "dtype is float32, float16 or bfloat16");
+      out = empty({m, cols}, x, type);
+    }
+    const int kind = float_kind(out);
+    need(kind >= 0, "out is float32, float16 or bfloat16");
+    void* stream = stream_of(dev);
+    at::Tensor space;
+    if (given(a[7])) {
+      space = tensor(a[7], "ws");
+      beside(dev, space);
+      need(space.is_contiguous(), "ws is contiguous");
+    } else {
+      space = workspace_of("f8", a[0], dev, stream, up_sm100_f8_matmul_workspace_bytes(m, experts, cols, k), UP_F8_COUNTER_BYTES);
+    }
+    check(unlocked([&] {
+            return up_sm100_f8_matmul(static_cast<const uint8_t*>(x.data_ptr()), m, x.stride(0), xs.data_ptr<float>(), xs.stride(0),
+                                      xs.stride(1), static_cast<const uint8_t*>(w.data_ptr()), ws.data_ptr<float>(), experts, cols, k,
+                                      offsets, out.data_ptr(), kind, out.stride(0), space.data_ptr(), space.nbytes(), stream);
+          }),
+          name);
+    if (given(a[6])) {
+      Py_INCREF(a[6]);
+      return a[6];
+    }
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// expert_route(logits, k, score, renormalise, gain)
+PyObject* expert_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 5);
+    const at::Tensor& l = cuda_tensor(a[0], "logits");
+    const int kind = float_kind(l);
+    need(kind >= 0 && l.dim() == 2 && (l.stride(1) == 1 || l.size(1) <= 1),
+         "logits is float32, float16 or bfloat16 [tokens, experts] with contiguous rows");
+    const int dev = current_device_of(l);
+    const int64_t tokens = l.size(0), experts = l.size(1), k = PyLong_AsLongLong(a[1]);
+    if (k == -1 && PyErr_Occurred()) throw Raised();
+    need(k >= 1 && k <= experts, "k is from 1 to the number of experts");
+    int score = -1;
+    if (PyUnicode_Check(a[2])) {
+      if (PyUnicode_CompareWithASCIIString(a[2], "softmax") == 0) score = UP_EXPERT_SOFTMAX;
+      if (PyUnicode_CompareWithASCIIString(a[2], "sigmoid") == 0) score = UP_EXPERT_SIGMOID;
+    }
+    need(score >= 0, "score is \"softmax\" or \"sigmoid\"");
+    const int renormalise = PyObject_IsTrue(a[3]);
+    if (renormalise < 0) throw Raised();
+    const double gain = PyFloat_AsDouble(a[4]);
+    if (gain == -1.0 && PyErr_Occurred()) throw Raised();
+    at::Tensor ids = empty({tokens, k}, l, at::kInt), weights = empty({tokens, k}, l, at::kFloat), rows = empty({tokens * k}, l, at::kInt),
+               slots = empty({tokens, k}, l, at::kInt), offsets = empty({experts + 1}, l, at::kInt);
+    void* stream = stream_of(dev);
+    const at::Tensor ws = workspace_of("route", a[0], dev, stream, up_sm100_expert_route_workspace_bytes(tokens, experts), 0);
+    check(unlocked([&] {
+            return up_sm100_expert_route(l.data_ptr(), kind, tokens, experts, l.stride(0), k, score, renormalise, (float)gain,
+                                         ids.data_ptr<int32_t>(), weights.data_ptr<float>(), rows.data_ptr<int32_t>(),
+                                         slots.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(), ws.data_ptr(), ws.nbytes(), stream);
+          }),
+          "expert_route");
+    return tuple_of({&ids, &weights, &rows, &slots, &offsets});
+  });
+}
+
+// expert_combine(y, slots, weights, add, out)
+PyObject* expert_combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    count(n, 5);
+    const at::Tensor &y = cuda_tensor(a[0], "y"), &slots = tensor(a[1], "slots"), &weights = tensor(a[2], "weights");
+    const int kind = float_kind(y);
+    need(kind >= 0 && y.dim() == 2 && (y.stride(1) == 1 || y.size(1) <= 1), "y is float32, float16 or bfloat16 [rows, n] with contiguous rows");
+    const int dev = current_device_of(y);
+    need(slots.scalar_type() == at::kInt && slots.dim() == 2 && slots.is_contiguous(), "slots is contiguous int32 [tokens, k]");
+    need(weights.scalar_type() == at::kFloat && weights.sizes() == slots.sizes() && weights.is_contiguous(),
+         "weights is contiguous float32 of slots' shape");
+    beside(dev, slots), beside(dev, weights);
+    const int64_t tokens = slots.size(0), cols = y.size(1);
+    const void* add = nullptr;
+    int64_t add_stride = 0;
+    if (given(a[3])) {
+      const at::Tensor& t = tensor(a[3], "add");
+      need(t.dim() == 2 && t.size(0) == tokens && t.size(1) == cols && t.scalar_type() == y.scalar_type() && (t.stride(1) == 1 || cols <= 1),
+           "add is [tokens, n] of y's type with contiguous rows");
+      beside(dev, t);
+      add = t.data_ptr(), add_stride = t.stride(0);
+    }
+    at::Tensor out;
+    if (given(a[4])) {
+      out = tensor(a[4], "out");
+      need(out.dim() == 2 && out.size(0) == tokens && out.size(1) == cols && out.scalar_type() == y.scalar_type() &&
+               (out.stride(1) == 1 || cols <= 1),
+           "out is [tokens, n] of y's type with contiguous rows");
+      beside(dev, out);
+    } else {
+      out = empty({tokens, cols}, y, y.scalar_type());
+    }
+    check(unlocked([&] {
+            return up_sm100_expert_combine(y.data_ptr(), kind, y.size(0), y.stride(0), cols, slots.data_ptr<int32_t>(),
+                                           weights.data_ptr<float>(), tokens, slots.size(1), add, add_stride, out.data_ptr(),
+                                           out.stride(0), stream_of(dev));
+          }),
+          "expert_combine");
+    if (given(a[4])) {
+      Py_INCREF(a[4]);
+      return a[4];
+    }
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 // init(check, workspace, workspaces)
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -405,6 +661,11 @@ PyMethodDef methods[] = {
     {"kv4_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_append)), METH_FASTCALL, nullptr},
     {"dequant_i4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dequant_i4)), METH_FASTCALL, nullptr},
     {"kv4_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kv4_attention)), METH_FASTCALL, nullptr},
+    {"f8_quantise", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f8_quantise)), METH_FASTCALL, nullptr},
+    {"f8_quantise_weight", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f8_quantise_weight)), METH_FASTCALL, nullptr},
+    {"f8_matmul", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f8_matmul)), METH_FASTCALL, nullptr},
+    {"expert_route", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(expert_route)), METH_FASTCALL, nullptr},
+    {"expert_combine", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(expert_combine)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

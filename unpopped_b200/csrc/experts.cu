@@ -1,0 +1,481 @@
+// experts.cu — routing of tokens to experts, and the weighted sum of the experts' rows.
+//
+// Routing: a warp takes a token's k largest logits by k rounds of a warp maximum over order-preserving 32-bit keys, then
+// the pairs are counted and placed by expert. A pair's place is the number of pairs of lower experts plus that of the same
+// expert's earlier tokens, so it does not depend on the order in which anything runs: within 128 tokens the earlier
+// ones are the lower bits of a mask that each expert has (set by atomicOr, which commutes), before them the counts of earlier blocks.
+#include "common.cuh"
+#include "divide.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace up {
+namespace experts {
+
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxK = 32;
+constexpr int kTile = 128;            // tokens a tile: four words of mask an expert
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxBlocks = 256;       // each block of the placing kernel reads every block's counts
+
+struct Route {
+  const void* logits;
+  int64_t stride;
+  int tokens, experts, k, score, renormalise;
+  int per;                            // tiles a block
+  float gain;
+  int32_t *ids, *rows, *slots, *offsets;
+  float* weights;
+  uint32_t* counts;                   // [blocks][experts]
+};
+
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Order-preserving key: larger logits have larger keys, a NaN the largest, -inf 0 (never taken), -0 that of 0.
+__device__ __forceinline__ uint32_t key_of(float v) {
+  if (v != v) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(v + 0.f);
+  if (u == 0xff800000u) return 0u;
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? (key == 0xffffffffu ? 0x7fc00000u : key & 0x7fffffffu) : ~key);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// One token's choice by one warp: lane j < k gets the j-th expert (or -1) and its weight. Lane l holds experts l, l + 32, ...
+template <int PER>
+__device__ __forceinline__ void choose(const uint32_t (&key)[PER], const Route& a, int lane, int& id, float& weight) {
+  uint32_t left[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) left[i] = key[i];
+  uint32_t mine = 0, top = 0;
+  id = -1;
+  for (int j = 0; j < a.k; ++j) {
+    uint32_t best = left[0];
+    int at = lane;
+#pragma unroll
+    for (int i = 1; i < PER; ++i)
+      if (left[i] > best) best = left[i], at = i * 32 + lane;
+    const uint32_t high = __reduce_max_sync(0xffffffffu, best);
+    if (high == 0) break;  // the others are masked
+    const int e = (int)__reduce_min_sync(0xffffffffu, best == high ? (unsigned)at : 0x7fffffffu);
+    if (j == 0) top = high;
+    if (lane == j) mine = high, id = e;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (e == i * 32 + lane) left[i] = 0;
+  }
+  const float l = value_of(mine);
+  float w = 0.f, total = 1.f;
+  if (a.score == UP_EXPERT_SOFTMAX) {
+    const float m = value_of(top);
+    if (id >= 0) w = expf(l - m);
+    if (!a.renormalise) {
+      total = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (key[i] != 0) total += expf(value_of(key[i]) - m);
+      total = warp_sum(total);
+    }
+  } else if (id >= 0) {
+    w = 1.f / (1.f + expf(-l));
+  }
+  if (a.renormalise) total = warp_sum(w);
+  weight = (id >= 0 && !(total == 0.f)) ? w / total * a.gain : 0.f;
+}
+
+// Chooses for the tile's tokens; marks them in the experts' masks.
+template <int PER, typename T>
+__device__ __forceinline__ void choose_tile(const Route& a, int first, uint32_t (*mask)[kTile / 32], int32_t* held) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int end = min(first + kTile, a.tokens);
+  for (int t = first + warp; t < end; t += kWarps) {
+    const T* row = static_cast<const T*>(a.logits) + (int64_t)t * a.stride;
+    uint32_t key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = i * 32 + lane < a.experts ? key_of(as_float(row[i * 32 + lane])) : 0u;
+    int id;
+    float w;
+    choose<PER>(key, a, lane, id, w);
+    if (lane < a.k) {
+      const int64_t at = (int64_t)t * a.k + lane;
+      a.ids[at] = id;
+      a.weights[at] = w;
+      const int in = t - first;
+      if (held) held[in * a.k + lane] = id;
+      if (id >= 0) atomicOr(&mask[id][in >> 5], 1u << (in & 31));
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t count_of(const uint32_t (&m)[kTile / 32]) {
+  uint32_t n = 0;
+#pragma unroll
+  for (int i = 0; i < kTile / 32; ++i) n += __popc(m[i]);
+  return n;
+}
+
+__device__ __forceinline__ void clear(uint32_t (*mask)[kTile / 32], int experts) {
+  for (int i = threadIdx.x; i < experts * (kTile / 32); i += kThreads) (&mask[0][0])[i] = 0;
+}
+
+// total[e] (all counts) to offsets, by warp 0: start[e] becomes the sum of the totals before e; returns the sum of all.
+__device__ __forceinline__ uint32_t scan_experts(const uint32_t* total, uint32_t* start, int experts, int lane) {
+  uint32_t run = 0;
+  for (int e0 = 0; e0 < experts; e0 += 32) {
+    const uint32_t n = e0 + lane < experts ? total[e0 + lane] : 0u;
+    uint32_t s = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += v;
+    }
+    if (e0 + lane < experts) start[e0 + lane] = run + s - n;
+    run += __shfl_sync(0xffffffffu, s, 31);
+  }
+  return run;
+}
+
+// Places the tile's pairs: next[e] is the place of expert e's first pair in it.
+__device__ __forceinline__ void place_tile(const Route& a, int first, const uint32_t (*mask)[kTile / 32], const uint32_t* next,
+                                           const int32_t* held) {
+  const int pairs = (min(first + kTile, a.tokens) - first) * a.k;
+  for (int p = threadIdx.x; p < pairs; p += kThreads) {
+    const int in = p / a.k, id = held[p];
+    int slot = -1;
+    if (id >= 0) {
+      uint32_t before = __popc(mask[id][in >> 5] & ((1u << (in & 31)) - 1u));
+      for (int i = 0; i < (in >> 5); ++i) before += __popc(mask[id][i]);
+      slot = (int)(next[id] + before);
+      a.rows[slot] = first + in;
+    }
+    a.slots[(int64_t)first * a.k + p] = slot;
+  }
+}
+
+// All of it in one block, for at most kTile tokens.
+template <int PER, typename T>
+__global__ void __launch_bounds__(kThreads) route_one_kernel(const Route a) {
+  __shared__ uint32_t mask[PER * 32][kTile / 32];
+  __shared__ uint32_t total[PER * 32], start[PER * 32];
+  __shared__ uint32_t all;
+  __shared__ int32_t held[kTile * kMaxK];
+  clear(mask, a.experts);
+  __syncthreads();
+  choose_tile<PER, T>(a, 0, mask, held);
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.experts; e += kThreads) total[e] = count_of(mask[e]);
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const uint32_t n = scan_experts(total, start, a.experts, threadIdx.x);
+    if (threadIdx.x == 0) all = n;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e <= a.experts; e += kThreads) a.offsets[e] = (int32_t)(e < a.experts ? start[e] : all);
+  place_tile(a, 0, mask, start, held);
+  for (int i = (int)all + threadIdx.x; i < a.tokens * a.k; i += kThreads) a.rows[i] = -1;
+}
+
+// First of two launches: choice, and each block's counts.
+template <int PER, typename T>
+__global__ void __launch_bounds__(kThreads) choose_kernel(const Route a) {
+  __shared__ uint32_t mask[PER * 32][kTile / 32];
+  __shared__ uint32_t total[PER * 32];
+  for (int e = threadIdx.x; e < a.experts; e += kThreads) total[e] = 0;
+  for (int i = 0; i < a.per; ++i) {
+    const int first = (blockIdx.x * a.per + i) * kTile;
+    if (first >= a.tokens) break;
+    clear(mask, a.experts);
+    __syncthreads();
+    choose_tile<PER, T>(a, first, mask, nullptr);
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.experts; e += kThreads) total[e] += count_of(mask[e]);
+    __syncthreads();
+  }
+  for (int e = threadIdx.x; e < a.experts; e += kThreads) a.counts[(int64_t)blockIdx.x * a.experts + e] = total[e];
+}
+
+// Second: where each block's pairs begin, and the places.
+__global__ void __launch_bounds__(kThreads) place_kernel(const Route a) {
+  __shared__ uint32_t mask[kMaxExperts][kTile / 32];
+  __shared__ uint32_t total[kMaxExperts], next[kMaxExperts], before[kMaxExperts];
+  __shared__ uint32_t all;
+  __shared__ int32_t held[kTile * kMaxK];
+  for (int e = threadIdx.x; e < a.experts; e += kThreads) total[e] = before[e] = 0;
+  __syncthreads();
+  // a column of threads for each 32 experts' warp: warps take blocks in turn
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wide = (a.experts + 31) / 32;
+  for (int c = warp % wide; c < wide; c += kWarps) {
+    const int e = c * 32 + lane;
+    const int parts = wide < kWarps ? (kWarps - c + wide - 1) / wide : 1;  // warps that share column c
+    uint32_t n = 0, m = 0;
+    if (e < a.experts) {
+#pragma unroll 8
+      for (int b = warp / wide; b < (int)gridDim.x; b += parts) {
+        const uint32_t v = a.counts[(int64_t)b * a.experts + e];
+        n += v;
+        if (b < (int)blockIdx.x) m += v;
+      }
+      atomicAdd(&total[e], n);
+      atomicAdd(&before[e], m);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const uint32_t n = scan_experts(total, next, a.experts, lane);
+    if (lane == 0) all = n;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= a.experts; e += kThreads) a.offsets[e] = (int32_t)(e < a.experts ? next[e] : all);
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.experts; e += kThreads) next[e] += before[e];
+  for (int i = 0; i < a.per; ++i) {
+    const int first = (blockIdx.x * a.per + i) * kTile;
+    if (first >= a.tokens) break;
+    clear(mask, a.experts);
+    const int pairs = (min(first + kTile, a.tokens) - first) * a.k;
+    for (int p = threadIdx.x; p < pairs; p += kThreads) held[p] = a.ids[(int64_t)first * a.k + p];
+    __syncthreads();
+    for (int p = threadIdx.x; p < pairs; p += kThreads) {
+      const int in = p / a.k;
+      if (held[p] >= 0) atomicOr(&mask[held[p]][in >> 5], 1u << (in & 31));
+    }
+    __syncthreads();
+    place_tile(a, first, mask, next, held);
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.experts; e += kThreads) next[e] += count_of(mask[e]);
+    __syncthreads();
+  }
+  const int64_t pairs = (int64_t)a.tokens * a.k;
+  for (int64_t i = (int64_t)all + blockIdx.x * kThreads + threadIdx.x; i < pairs; i += (int64_t)gridDim.x * kThreads)
+    a.rows[i] = -1;
+}
+
+static int blocks_of(int64_t tokens, int* per) {
+  const int64_t tiles = (tokens + kTile - 1) / kTile;
+  *per = (int)((tiles + kMaxBlocks - 1) / kMaxBlocks);
+  if (*per < 1) *per = 1;
+  return (int)((tiles + *per - 1) / *per);
+}
+
+template <int PER, typename T>
+int route(Route& a, cudaStream_t s) {
+  if (a.tokens <= kTile) {
+    route_one_kernel<PER, T><<<1, kThreads, 0, s>>>(a);
+    note_launch();
+    return check_launch();
+  }
+  const int blocks = blocks_of(a.tokens, &a.per);
+  choose_kernel<PER, T><<<blocks, kThreads, 0, s>>>(a);
+  note_launch();
+  const int ok = check_launch();
+  if (ok != UP_OK) return ok;
+  place_kernel<<<blocks, kThreads, 0, s>>>(a);
+  note_launch();
+  return check_launch();
+}
+template <typename T>
+int route_sized(Route& a, cudaStream_t s) {
+  const int per = (a.experts + 31) / 32;
+  if (per <= 1) return route<1, T>(a, s);
+  if (per <= 2) return route<2, T>(a, s);
+  if (per <= 4) return route<4, T>(a, s);
+  if (per <= 8) return route<8, T>(a, s);
+  if (per <= 16) return route<16, T>(a, s);
+  return route<32, T>(a, s);
+}
+
+// ---- the weighted sum ----
+constexpr int kSumThreads = 256;
+constexpr int kAtOnce = 8;  // rows in flight a thread
+
+template <typename T, int V>
+struct Vec;
+template <>
+struct Vec<float, 4> {
+  using Raw = uint4;
+  static __device__ __forceinline__ void widen(const Raw& r, float (&f)[4]) {
+    f[0] = __uint_as_float(r.x), f[1] = __uint_as_float(r.y), f[2] = __uint_as_float(r.z), f[3] = __uint_as_float(r.w);
+  }
+  static __device__ __forceinline__ Raw narrow(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <>
+struct Vec<__half, 8> {
+  using Raw = uint4;
+  static __device__ __forceinline__ void widen(const Raw& r, float (&f)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = v.x, f[2 * i + 1] = v.y;
+    }
+  }
+  static __device__ __forceinline__ Raw narrow(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <>
+struct Vec<__nv_bfloat16, 8> {
+  using Raw = uint4;
+  static __device__ __forceinline__ void widen(const Raw& r, float (&f)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  static __device__ __forceinline__ Raw narrow(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <typename T>
+struct Vec<T, 1> {
+  using Raw = T;
+  static __device__ __forceinline__ void widen(const T& r, float (&f)[1]) { f[0] = as_float(r); }
+  static __device__ __forceinline__ T narrow(const float (&f)[1]);
+};
+template <>
+__device__ __forceinline__ float Vec<float, 1>::narrow(const float (&f)[1]) { return f[0]; }
+template <>
+__device__ __forceinline__ __half Vec<__half, 1>::narrow(const float (&f)[1]) { return __float2half_rn(f[0]); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 Vec<__nv_bfloat16, 1>::narrow(const float (&f)[1]) { return __float2bfloat16_rn(f[0]); }
+
+// A thread sums one piece of V values (16 bytes) of one token over the token's slots. Bound by HBM: every chosen row once.
+template <typename T, int V, typename Div>
+__global__ void __launch_bounds__(kSumThreads)
+    combine_kernel(const T* __restrict__ y, int64_t rows, int64_t ys, const int32_t* __restrict__ slots,
+                   const float* __restrict__ weights, int k, const T* add, int64_t as, T* out, int64_t os,
+                   typename Div::Int pieces, typename Div::Int row_pieces, Div by_row) {
+  using Int = typename Div::Int;
+  using W = Vec<T, V>;
+  const Int p = (Int)blockIdx.x * kSumThreads + threadIdx.x;
+  if (p >= pieces) return;
+  const Int t = by_row(p);
+  const int64_t at = (int64_t)(p - t * row_pieces) * V;
+  float sum[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum[i] = 0.f;
+  if (add) W::widen(*reinterpret_cast<const typename W::Raw*>(add + (int64_t)t * as + at), sum);
+  for (int j0 = 0; j0 < k; j0 += kAtOnce) {
+    typename W::Raw raw[kAtOnce];
+    float w[kAtOnce];
+    bool there[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int64_t s = j0 + j < k ? (int64_t)slots[(int64_t)t * k + j0 + j] : -1;
+      there[j] = (uint64_t)s < (uint64_t)rows;
+      w[j] = there[j] ? weights[(int64_t)t * k + j0 + j] : 0.f;
+      if (there[j]) raw[j] = *reinterpret_cast<const typename W::Raw*>(y + s * ys + at);
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j)
+      if (there[j]) {
+        float f[V];
+        W::widen(raw[j], f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] = fmaf(w[j], f[i], sum[i]);
+      }
+  }
+  *reinterpret_cast<typename W::Raw*>(out + (int64_t)t * os + at) = W::narrow(sum);
+}
+
+template <typename T, int V>
+int combine(const void* y, int64_t rows, int64_t ys, int64_t n, const int32_t* slots, const float* weights, int64_t tokens,
+            int64_t k, const void* add, int64_t as, void* out, int64_t os, cudaStream_t s) {
+  const int64_t row_pieces = n / V, pieces = tokens * row_pieces;
+  const int64_t ctas = (pieces + kSumThreads - 1) / kSumThreads;
+  if (ctas > 0x7fffffff) return UP_ERR_UNSUPPORTED;
+  const T *from = static_cast<const T*>(y), *more = static_cast<const T*>(add);
+  if (pieces < ((int64_t)1 << 31) - kSumThreads)
+    combine_kernel<T, V, Divide32><<<(unsigned)ctas, kSumThreads, 0, s>>>(from, rows, ys, slots, weights, (int)k, more, as,
+        static_cast<T*>(out), os, (uint32_t)pieces, (uint32_t)row_pieces, Divide32(row_pieces));
+  else
+    combine_kernel<T, V, Divide64><<<(unsigned)ctas, kSumThreads, 0, s>>>(from, rows, ys, slots, weights, (int)k, more, as,
+        static_cast<T*>(out), os, (uint64_t)pieces, (uint64_t)row_pieces, Divide64(row_pieces));
+  note_launch();
+  return check_launch();
+}
+
+}  // namespace experts
+}  // namespace up
+
+using namespace up;
+using namespace up::experts;
+
+extern "C" size_t up_sm100_expert_route_workspace_bytes(int64_t tokens, int64_t experts) {
+  if (tokens <= kTile || experts <= 0 || experts > kMaxExperts) return 256;
+  int per;
+  return (size_t)blocks_of(tokens, &per) * experts * sizeof(uint32_t);
+}
+
+extern "C" int up_sm100_expert_route(const void* logits, int dtype, int64_t tokens, int64_t n_experts, int64_t stride,
+                                     int64_t k, int score, int renormalise, float gain, int32_t* ids, float* weights,
+                                     int32_t* rows, int32_t* slots, int32_t* offsets, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  UP_CHECK_ARG(tokens >= 0 && n_experts >= 1 && k >= 1 && k <= n_experts && stride >= 0);
+  UP_CHECK_ARG(score == UP_EXPERT_SOFTMAX || score == UP_EXPERT_SIGMOID);
+  if (dtype != UP_EK_F32 && dtype != UP_EK_F16 && dtype != UP_EK_BF16) return UP_ERR_UNSUPPORTED;
+  if (n_experts > kMaxExperts || k > kMaxK || tokens > (0x7fffffff - kTile) / k) return UP_ERR_UNSUPPORTED;
+  UP_CHECK_ARG(offsets != nullptr);
+  UP_CHECK_ARG(tokens == 0 || (logits && ids && weights && rows && slots && workspace));
+  UP_CHECK_ARG(tokens <= 1 || stride >= n_experts);
+  UP_CHECK_ARG(aligned(workspace, 256) && (tokens == 0 || workspace_bytes >= up_sm100_expert_route_workspace_bytes(tokens, n_experts)));
+  Route a{};
+  a.logits = logits, a.stride = stride, a.tokens = (int)tokens, a.experts = (int)n_experts, a.k = (int)k, a.score = score;
+  a.renormalise = renormalise != 0, a.gain = gain, a.ids = ids, a.rows = rows, a.slots = slots, a.offsets = offsets;
+  a.weights = weights, a.counts = static_cast<uint32_t*>(workspace), a.per = 1;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == UP_EK_F32) return route_sized<float>(a, s);
+  if (dtype == UP_EK_F16) return route_sized<__half>(a, s);
+  return route_sized<__nv_bfloat16>(a, s);
+}
+
+extern "C" int up_sm100_expert_combine(const void* y, int dtype, int64_t rows, int64_t y_stride, int64_t n,
+                                       const int32_t* slots, const float* weights, int64_t tokens, int64_t k,
+                                       const void* add, int64_t add_stride, void* out, int64_t out_stride, void* stream) {
+  UP_CHECK_ARG(rows >= 0 && n >= 0 && tokens >= 0 && k >= 0 && y_stride >= 0 && add_stride >= 0 && out_stride >= 0);
+  if (dtype != UP_EK_F32 && dtype != UP_EK_F16 && dtype != UP_EK_BF16) return UP_ERR_UNSUPPORTED;
+  if (k > 0x7fffffff || n > ((int64_t)1 << 31) || tokens > ((int64_t)1 << 31)) return UP_ERR_UNSUPPORTED;
+  if (tokens == 0 || n == 0) return UP_OK;
+  UP_CHECK_ARG(out != nullptr && (y != nullptr || rows == 0) && (k == 0 || (slots && weights)));
+  UP_CHECK_ARG((rows <= 1 || y_stride >= n) && (tokens <= 1 || (out_stride >= n && (!add || add_stride >= n))));
+  if (rows <= 1) y_stride = 0;
+  if (tokens == 1) add_stride = out_stride = 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int v = dtype == UP_EK_F32 ? 4 : 8;
+  // 16 bytes a thread where every row starts on 16 bytes, single values else
+  const bool wide = n % v == 0 && y_stride % v == 0 && out_stride % v == 0 && add_stride % v == 0 && aligned(y, 16) &&
+                    aligned(out, 16) && aligned(add, 16);
+#define UP_SUM(T, V) combine<T, V>(y, rows, y_stride, n, slots, weights, tokens, k, add, add_stride, out, out_stride, s)
+  if (dtype == UP_EK_F32) return wide ? UP_SUM(float, 4) : UP_SUM(float, 1);
+  if (dtype == UP_EK_F16) return wide ? UP_SUM(__half, 8) : UP_SUM(__half, 1);
+  return wide ? UP_SUM(__nv_bfloat16, 8) : UP_SUM(__nv_bfloat16, 1);
+#undef UP_SUM
+}
+
+UP_DEFINE_REVISION(experts)

@@ -489,5 +489,61 @@ def kv4_attention(q: torch.Tensor, cache: tuple, block_table: torch.Tensor, seq_
     return _calls().kv4_attention(q, cache, block_table, seq_lens, cu_q, causal, window, scale, out, want_lse, ws)
 
 
+# ---- 8-bit products with a scale for each block of 128, and experts ----
+def f8_quantise(x: torch.Tensor, rows: torch.Tensor | None = None, gate: bool = False):
+    """(q, scale): the rows of x [tokens, k] (float32, float16, bfloat16; rows of whole 16 bytes, k a multiple of 16) as
+    float8_e4m3fn [n, k] with one f32 scale for each 128 values of a row, [n, ceil(k / 128)] (a block's scales lie beside one
+    another in memory, as `f8_matmul` reads them fastest). rows (int32 [n]): row r is x[rows[r]], and zeros where that is no row of
+    x (`expert_route`'s rows). gate: x holds 2k values a row, and y = silu(x[:, :k]) * x[:, k:] is quantised, in f32.
+    scale = max|y| / 448 over a block's finite values; an infinity or a NaN reads back as NaN."""
+    return _calls().f8_quantise(x, rows, gate)
+
+
+def f8_quantise_weight(w: torch.Tensor):
+    """(q, scale): weights [n, k] or [experts, n, k] as float8_e4m3fn with one f32 scale for each block of 128 x 128,
+    [(experts,) ceil(n / 128), ceil(k / 128)]: what `f8_matmul` and `f8_expert_matmul` take. Types and sizes as `f8_quantise`."""
+    return _calls().f8_quantise_weight(w)
+
+
+def f8_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, dtype=torch.bfloat16,
+              out: torch.Tensor | None = None, ws: torch.Tensor | None = None) -> torch.Tensor:
+    """[rows, n] = x [rows, k] times w [n, k], both float8_e4m3fn with their scales (`f8_quantise`, `f8_quantise_weight`):
+    tcgen05 products of each block of 128, scaled and summed in f32, rounded once to `dtype` (bfloat16, float16 or float32;
+    out's where it is given). Any number of rows and columns; k a multiple of 16. x's and out's rows may be views.
+    ws: a workspace of the caller's, contiguous, its first 8192 bytes zero-filled once; without one the stream's is used, or
+    a captured graph's own. Like `w4a16` it is no part of autograd."""
+    return _calls().f8_matmul(x, x_scale, w, w_scale, None, dtype, out, ws)
+
+
+def f8_expert_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor,
+                     dtype=torch.bfloat16, out: torch.Tensor | None = None, ws: torch.Tensor | None = None) -> torch.Tensor:
+    """`f8_matmul` by expert: rows offsets[e] to offsets[e + 1] of x (int32 [experts + 1], on the device; `expert_route`'s) take
+    the matrix w[e] of [experts, n, k]. Groups are of any size, none included. Rows that no expert has are left as
+    they were (undefined in a new out)."""
+    if offsets is None:
+        raise TypeError("offsets must be a tensor")
+    return _calls().f8_matmul(x, x_scale, w, w_scale, offsets, dtype, out, ws)
+
+
+def expert_route(logits: torch.Tensor, k: int, score: str = "softmax", renormalise: bool = True, gain: float = 1.0):
+    """(ids, weights, rows, slots, offsets): each token's k experts of logits [tokens, experts] (float32, float16, bfloat16; at
+    most 1024 experts and k of 32) and their pairs' places, laid out by expert and in each by token.
+
+    ids int32 [tokens, k]: the experts of the largest logits, the lower of equal ones first; an expert whose logit is -inf is
+    never taken, and -1 stands where none is left (a padded token has -inf everywhere). weights float32 [tokens, k]: their
+    "softmax" over all experts or "sigmoid", divided by the chosen ones' sum (renormalise), times gain; 0 for -1. rows int32
+    [tokens * k]: the token at each place, -1 behind the last (`f8_quantise` gathers by it). slots int32 [tokens, k]: each
+    pair's place, or -1 (`expert_combine` reads it). offsets int32 [experts + 1]: where each expert's places begin
+    (`f8_expert_matmul` takes it). One launch up to 128 tokens, two above; nothing comes to the host."""
+    return _calls().expert_route(logits, k, score, renormalise, gain)
+
+
+def expert_combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, add: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """[tokens, n] of y's type: add (a residual, or a shared expert's output) plus the sum of weights[t, j] * y[slots[t, j]] over j, in
+    f32, rounded once. y [rows, n] float32, float16 or bfloat16; a slot that is no row of y adds nothing. out may be add."""
+    return _calls().expert_combine(y, slots, weights, add, out)
+
+
 def launch_count() -> int:
     return int(_lib.load().up_sm100_launch_count())
