@@ -1,7 +1,7 @@
 // experts.cu — routing of tokens to experts, and the weighted sum of the experts' rows.
 //
-// Routing: a warp takes a token's k largest logits by k rounds of a warp maximum over order-preserving 32-bit keys, then
-// the pairs are counted and placed by expert. A pair's place is the number of pairs of lower experts plus that of the same
+// Routing: a warp takes a token's k largest logits by k rounds of a warp maximum over order-preserving 32-bit keys, each lane's
+// sorted before, so that a round looks at their heads only. Then the pairs are counted and placed by expert. A pair's place is the number of pairs of lower experts plus that of the same
 // expert's earlier tokens, so it does not depend on the order in which anything runs: within 128 tokens the earlier
 // ones are the lower bits of a mask that each expert has (set by atomicOr, which commutes), before them the counts of earlier blocks.
 #include "common.cuh"
@@ -16,7 +16,7 @@ namespace experts {
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxK = 32;
 constexpr int kTile = 128;            // tokens a tile: four words of mask an expert
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxBlocks = 256;       // each block of the placing kernel reads every block's counts
 
@@ -35,15 +35,15 @@ __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Order-preserving key: larger logits have larger keys, a NaN the largest, -inf 0 (never taken), -0 that of 0.
+// Order-preserving key: larger logits have larger keys. Adding 0 makes every NaN the canonical one, whose key is the largest, and -0 equal to 0.
+// Keys up to that of -inf are never taken.
+constexpr uint32_t kMasked = 0x007fffffu;
 __device__ __forceinline__ uint32_t key_of(float v) {
-  if (v != v) return 0xffffffffu;
   const uint32_t u = __float_as_uint(v + 0.f);
-  if (u == 0xff800000u) return 0u;
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
-  return __uint_as_float((key & 0x80000000u) ? (key == 0xffffffffu ? 0x7fc00000u : key & 0x7fffffffu) : ~key);
+  return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -52,68 +52,119 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// Sorts a lane's keys, largest first, the lower expert of equal ones: Batcher's odd-even merge sort ("Sorting networks and their
+// applications", 1968) for a power of two of them.
+template <int PER>
+__device__ __forceinline__ void sort_keys(uint32_t (&key)[PER], int (&at)[PER]) {
+#pragma unroll
+  for (int p = 1; p < PER; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < PER; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < PER && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const int a = i + j, b = i + j + k;
+            const bool swap = key[b] > key[a] || (key[b] == key[a] && at[b] < at[a]);
+            const uint32_t ka = key[a], kb = key[b];
+            const int ia = at[a], ib = at[b];
+            key[a] = swap ? kb : ka, key[b] = swap ? ka : kb;
+            at[a] = swap ? ib : ia, at[b] = swap ? ia : ib;
+          }
+}
+
 // One token's choice by one warp: lane j < k gets the j-th expert (or -1) and its weight. Lane l holds experts l, l + 32, ...
 template <int PER>
-__device__ __forceinline__ void choose(const uint32_t (&key)[PER], const Route& a, int lane, int& id, float& weight) {
-  uint32_t left[PER];
+__device__ __forceinline__ void choose(uint32_t (&key)[PER], const Route& a, int lane, int& id, float& weight) {
+  constexpr bool kSorted = PER <= 8;  // 19 exchanges for 8 keys; 63 for 16 would cost more than the rounds save
+  int at[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) left[i] = key[i];
+  for (int i = 0; i < PER; ++i) at[i] = i * 32 + lane;
+  float all = 1.f;
+  if (a.score == UP_EXPERT_SOFTMAX && !a.renormalise) {
+    uint32_t high = key[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) high = max(high, key[i]);
+    const float m = value_of(__reduce_max_sync(0xffffffffu, high));
+    all = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] > kMasked) all += expf(value_of(key[i]) - m);
+    all = warp_sum(all);
+  }
+  if (kSorted) sort_keys<PER>(key, at);
   uint32_t mine = 0, top = 0;
   id = -1;
   for (int j = 0; j < a.k; ++j) {
-    uint32_t best = left[0];
-    int at = lane;
+    uint32_t best = key[0];
+    int e = at[0];
+    if (!kSorted) {
 #pragma unroll
-    for (int i = 1; i < PER; ++i)
-      if (left[i] > best) best = left[i], at = i * 32 + lane;
+      for (int i = 1; i < PER; ++i)
+        if (key[i] > best) best = key[i], e = at[i];
+    }
     const uint32_t high = __reduce_max_sync(0xffffffffu, best);
-    if (high == 0) break;  // the others are masked
-    const int e = (int)__reduce_min_sync(0xffffffffu, best == high ? (unsigned)at : 0x7fffffffu);
+    if (high <= kMasked) break;  // the others are masked
+    const unsigned same = __ballot_sync(0xffffffffu, best == high);
+    if (same & (same - 1))  // several lanes' heads are equal: the lowest expert
+      e = (int)__reduce_min_sync(0xffffffffu, best == high ? (unsigned)e : 0x7fffffffu);
+    else
+      e = __shfl_sync(0xffffffffu, e, __ffs(same) - 1);
     if (j == 0) top = high;
     if (lane == j) mine = high, id = e;
+    if (kSorted) {
+      if (lane == (e & 31)) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (e == i * 32 + lane) left[i] = 0;
-  }
-  const float l = value_of(mine);
-  float w = 0.f, total = 1.f;
-  if (a.score == UP_EXPERT_SOFTMAX) {
-    const float m = value_of(top);
-    if (id >= 0) w = expf(l - m);
-    if (!a.renormalise) {
-      total = 0.f;
+        for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1], at[i] = at[i + 1];
+        key[PER - 1] = 0;
+      }
+    } else {
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        if (key[i] != 0) total += expf(value_of(key[i]) - m);
-      total = warp_sum(total);
+        if (e == at[i]) key[i] = 0;
     }
-  } else if (id >= 0) {
-    w = 1.f / (1.f + expf(-l));
   }
-  if (a.renormalise) total = warp_sum(w);
+  const float l = value_of(mine);
+  float w = 0.f;
+  if (id >= 0) w = a.score == UP_EXPERT_SOFTMAX ? expf(l - value_of(top)) : 1.f / (1.f + expf(-l));
+  const float total = a.renormalise ? warp_sum(w) : all;
   weight = (id >= 0 && !(total == 0.f)) ? w / total * a.gain : 0.f;
 }
 
-// Chooses for the tile's tokens; marks them in the experts' masks.
+// Chooses for the tile's tokens; marks them in the experts' masks. A warp's tokens' logits are all on their way at once where
+// they leave it the registers.
 template <int PER, typename T>
 __device__ __forceinline__ void choose_tile(const Route& a, int first, uint32_t (*mask)[kTile / 32], int32_t* held) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int end = min(first + kTile, a.tokens);
-  for (int t = first + warp; t < end; t += kWarps) {
-    const T* row = static_cast<const T*>(a.logits) + (int64_t)t * a.stride;
-    uint32_t key[PER];
+  constexpr int kEach = kTile / kWarps, kAtOnce = PER <= 4 ? kEach : PER <= 8 ? 2 : 1;
+#pragma unroll 1
+  for (int t0 = first + warp; t0 < end; t0 += kAtOnce * kWarps) {
+    uint32_t key[kAtOnce][PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) key[i] = i * 32 + lane < a.experts ? key_of(as_float(row[i * 32 + lane])) : 0u;
-    int id;
-    float w;
-    choose<PER>(key, a, lane, id, w);
-    if (lane < a.k) {
-      const int64_t at = (int64_t)t * a.k + lane;
-      a.ids[at] = id;
-      a.weights[at] = w;
-      const int in = t - first;
-      if (held) held[in * a.k + lane] = id;
-      if (id >= 0) atomicOr(&mask[id][in >> 5], 1u << (in & 31));
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int t = t0 + u * kWarps;
+      const T* row = static_cast<const T*>(a.logits) + (int64_t)t * a.stride;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        key[u][i] = t < end && i * 32 + lane < a.experts ? key_of(as_float(row[i * 32 + lane])) : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int t = t0 + u * kWarps;
+      if (t >= end) break;
+      int id;
+      float w;
+      choose<PER>(key[u], a, lane, id, w);
+      if (lane < a.k) {
+        const int64_t at = (int64_t)t * a.k + lane;
+        a.ids[at] = id;
+        a.weights[at] = w;
+        const int in = t - first;
+        if (held) held[in * a.k + lane] = id;
+        if (id >= 0) atomicOr(&mask[id][in >> 5], 1u << (in & 31));
+      }
     }
   }
 }
@@ -221,7 +272,7 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const Route a) {
     const int parts = wide < kWarps ? (kWarps - c + wide - 1) / wide : 1;  // warps that share column c
     uint32_t n = 0, m = 0;
     if (e < a.experts) {
-#pragma unroll 8
+#pragma unroll 16
       for (int b = warp / wide; b < (int)gridDim.x; b += parts) {
         const uint32_t v = a.counts[(int64_t)b * a.experts + e];
         n += v;
@@ -299,7 +350,6 @@ int route_sized(Route& a, cudaStream_t s) {
 
 // ---- the weighted sum ----
 constexpr int kSumThreads = 256;
-constexpr int kAtOnce = 8;  // rows in flight a thread
 
 template <typename T, int V>
 struct Vec;
@@ -365,60 +415,84 @@ __device__ __forceinline__ __half Vec<__half, 1>::narrow(const float (&f)[1]) { 
 template <>
 __device__ __forceinline__ __nv_bfloat16 Vec<__nv_bfloat16, 1>::narrow(const float (&f)[1]) { return __float2bfloat16_rn(f[0]); }
 
-// A thread sums one piece of V values (16 bytes) of one token over the token's slots. Bound by HBM: every chosen row once.
-template <typename T, int V, typename Div>
+// A thread sums U pieces of V values (16 bytes each) over their token's slots. Bound by HBM: every chosen row once. With U pieces of up to
+// kAtOnce slots about 8 loads are on their way a thread.
+template <typename T, int V, int U, typename Div>
 __global__ void __launch_bounds__(kSumThreads)
     combine_kernel(const T* __restrict__ y, int64_t rows, int64_t ys, const int32_t* __restrict__ slots,
                    const float* __restrict__ weights, int k, const T* add, int64_t as, T* out, int64_t os,
                    typename Div::Int pieces, typename Div::Int row_pieces, Div by_row) {
   using Int = typename Div::Int;
   using W = Vec<T, V>;
-  const Int p = (Int)blockIdx.x * kSumThreads + threadIdx.x;
-  if (p >= pieces) return;
-  const Int t = by_row(p);
-  const int64_t at = (int64_t)(p - t * row_pieces) * V;
-  float sum[V];
+  constexpr int kAtOnce = 8 / U;
+  const Int p0 = (Int)blockIdx.x * (kSumThreads * U) + threadIdx.x;
+  float sum[U][V];
+  int64_t at[U], tk[U], out_at[U];
+  bool in[U];
 #pragma unroll
-  for (int i = 0; i < V; ++i) sum[i] = 0.f;
-  if (add) W::widen(*reinterpret_cast<const typename W::Raw*>(add + (int64_t)t * as + at), sum);
-  for (int j0 = 0; j0 < k; j0 += kAtOnce) {
-    typename W::Raw raw[kAtOnce];
-    float w[kAtOnce];
-    bool there[kAtOnce];
+  for (int u = 0; u < U; ++u) {
+    const Int p = p0 + u * kSumThreads;
+    in[u] = p < pieces;
+    const Int t = in[u] ? by_row(p) : 0;
+    at[u] = in[u] ? (int64_t)(p - t * row_pieces) * V : 0;
+    tk[u] = (int64_t)t * k, out_at[u] = (int64_t)t * os + at[u];
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      const int64_t s = j0 + j < k ? (int64_t)slots[(int64_t)t * k + j0 + j] : -1;
-      there[j] = (uint64_t)s < (uint64_t)rows;
-      w[j] = there[j] ? weights[(int64_t)t * k + j0 + j] : 0.f;
-      if (there[j]) raw[j] = *reinterpret_cast<const typename W::Raw*>(y + s * ys + at);
-    }
-#pragma unroll
-    for (int j = 0; j < kAtOnce; ++j)
-      if (there[j]) {
-        float f[V];
-        W::widen(raw[j], f);
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] = fmaf(w[j], f[i], sum[i]);
-      }
+    for (int i = 0; i < V; ++i) sum[u][i] = 0.f;
+    if (add && in[u]) W::widen(*reinterpret_cast<const typename W::Raw*>(add + (int64_t)t * as + at[u]), sum[u]);
   }
-  *reinterpret_cast<typename W::Raw*>(out + (int64_t)t * os + at) = W::narrow(sum);
+  for (int j0 = 0; j0 < k; j0 += kAtOnce) {
+    typename W::Raw raw[U][kAtOnce];
+    float w[U][kAtOnce];
+    bool there[U][kAtOnce];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int64_t s = in[u] && j0 + j < k ? (int64_t)slots[tk[u] + j0 + j] : -1;
+        there[u][j] = (uint64_t)s < (uint64_t)rows;
+        w[u][j] = there[u][j] ? weights[tk[u] + j0 + j] : 0.f;
+        if (there[u][j]) raw[u][j] = *reinterpret_cast<const typename W::Raw*>(y + s * ys + at[u]);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        if (there[u][j]) {
+          float f[V];
+          W::widen(raw[u][j], f);
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum[u][i] = fmaf(w[u][j], f[i], sum[u][i]);
+        }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (in[u]) *reinterpret_cast<typename W::Raw*>(out + out_at[u]) = W::narrow(sum[u]);
 }
 
-template <typename T, int V>
-int combine(const void* y, int64_t rows, int64_t ys, int64_t n, const int32_t* slots, const float* weights, int64_t tokens,
-            int64_t k, const void* add, int64_t as, void* out, int64_t os, cudaStream_t s) {
+template <typename T, int V, int U>
+int combine_by(const void* y, int64_t rows, int64_t ys, int64_t n, const int32_t* slots, const float* weights, int64_t tokens,
+               int64_t k, const void* add, int64_t as, void* out, int64_t os, cudaStream_t s) {
   const int64_t row_pieces = n / V, pieces = tokens * row_pieces;
-  const int64_t ctas = (pieces + kSumThreads - 1) / kSumThreads;
+  const int64_t ctas = (pieces + kSumThreads * U - 1) / (kSumThreads * U);
   if (ctas > 0x7fffffff) return UP_ERR_UNSUPPORTED;
   const T *from = static_cast<const T*>(y), *more = static_cast<const T*>(add);
-  if (pieces < ((int64_t)1 << 31) - kSumThreads)
-    combine_kernel<T, V, Divide32><<<(unsigned)ctas, kSumThreads, 0, s>>>(from, rows, ys, slots, weights, (int)k, more, as,
+  if (pieces < ((int64_t)1 << 31) - kSumThreads * U)
+    combine_kernel<T, V, U, Divide32><<<(unsigned)ctas, kSumThreads, 0, s>>>(from, rows, ys, slots, weights, (int)k, more, as,
         static_cast<T*>(out), os, (uint32_t)pieces, (uint32_t)row_pieces, Divide32(row_pieces));
   else
-    combine_kernel<T, V, Divide64><<<(unsigned)ctas, kSumThreads, 0, s>>>(from, rows, ys, slots, weights, (int)k, more, as,
+    combine_kernel<T, V, U, Divide64><<<(unsigned)ctas, kSumThreads, 0, s>>>(from, rows, ys, slots, weights, (int)k, more, as,
         static_cast<T*>(out), os, (uint64_t)pieces, (uint64_t)row_pieces, Divide64(row_pieces));
   note_launch();
   return check_launch();
+}
+template <typename T, int V>
+int combine(const void* y, int64_t rows, int64_t ys, int64_t n, const int32_t* slots, const float* weights, int64_t tokens,
+            int64_t k, const void* add, int64_t as, void* out, int64_t os, cudaStream_t s) {
+  // several pieces a thread where one has few slots and the GPU is full all the same
+  const bool full = tokens * (n / V) > (int64_t)sm_count() * 2048 * 4;
+  if (full && k <= 2) return combine_by<T, V, 4>(y, rows, ys, n, slots, weights, tokens, k, add, as, out, os, s);
+  if (full && k <= 4) return combine_by<T, V, 2>(y, rows, ys, n, slots, weights, tokens, k, add, as, out, os, s);
+  return combine_by<T, V, 1>(y, rows, ys, n, slots, weights, tokens, k, add, as, out, os, s);
 }
 
 }  // namespace experts

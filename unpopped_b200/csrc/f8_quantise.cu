@@ -20,153 +20,242 @@ constexpr int kBlock = 128;           // values a scale
 constexpr float kMax = 448.f;         // e4m3's largest
 constexpr float kSmallest = 1.17549435e-38f;  // 2^-126: a smaller scale has no finite 1/scale to rely on
 
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const float4 a = ld_nc_na_f4(p), b = ld_nc_na_f4(p + 4);
-  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+// Sixteen values as they lie in memory (8 words of two, or 16), by loads of 32 bytes where they lie on such borders.
+template <typename T>
+struct Raw {
+  uint32_t w[8];
+};
+template <>
+struct Raw<float> {
+  uint32_t w[16];
+};
+__device__ __forceinline__ void load32(const void* p, uint32_t* w, bool wide) {
+  if (wide) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p));
+  } else {
+    const uint4 a = ld_nc_na_v4(p), b = ld_nc_na_v4(static_cast<const char*>(p) + 16);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+  }
 }
-__device__ __forceinline__ void load8(const __half* p, float (&v)[8]) {
-  const uint4 u = ld_nc_na_v4(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+template <typename T>
+__device__ __forceinline__ void load(const T* p, Raw<T>& r, bool wide) {
+  load32(p, r.w, wide);
+  if (sizeof(T) == 4) load32(reinterpret_cast<const char*>(p) + 32, r.w + (sizeof(T) == 4 ? 8 : 0), wide);
+}
+template <typename T>
+__device__ __forceinline__ void clear(Raw<T>& r) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+  for (int i = 0; i < (int)(sizeof(r) / 4); ++i) r.w[i] = 0;
+}
+__device__ __forceinline__ void widen(const Raw<float>& r, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r.w[i]);
+}
+__device__ __forceinline__ void widen(const Raw<__half>& r, float (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
     v[2 * i] = f.x, v[2 * i + 1] = f.y;
   }
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 u = ld_nc_na_v4(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void widen(const Raw<__nv_bfloat16>& r, float (&v)[16]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  for (int i = 0; i < 8; ++i) v[2 * i] = __uint_as_float(r.w[i] << 16), v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
 }
 
-__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __int_as_float(0x7f800000); }
-
-__device__ __forceinline__ float largest(const float (&v)[8]) {
-  float a = 0.f;
+// Magnitudes compare as their bits do; those from kInfinity on are not finite.
+constexpr uint32_t kInfinity = 0x7f800000u;
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t largest(const float (&v)[16]) {
+  uint32_t a = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = fmaxf(a, finite(v[i]) ? fabsf(v[i]) : 0.f);
+  for (int i = 0; i < 16; ++i) a = max(a, magnitude(v[i]));
+  return a;
+}
+__device__ __forceinline__ uint32_t largest_finite(const float (&v)[16]) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) a = max(a, magnitude(v[i]) < kInfinity ? magnitude(v[i]) : 0u);
   return a;
 }
 
-__device__ __forceinline__ float scale_of(float a) {
-  const float s = a * (1.f / kMax);
+__device__ __forceinline__ float scale_of(uint32_t a) {
+  const float s = __uint_as_float(a) * (1.f / kMax);
   return s >= kSmallest ? s : 0.f;
 }
 
-// Eight values as e4m3 bytes. |y * inv| is at most 448 (1 + 2^-22), so only values that are not finite need a care.
-__device__ __forceinline__ uint2 codes(const float (&v)[8], float inv) {
-  uint32_t w[2] = {0, 0};
+// Sixteen values as e4m3 bytes; |v * inv| is at most 448 (1 + 2^-22). CHECK: some may not be finite.
+template <bool CHECK>
+__device__ __forceinline__ uint4 codes(const float (&v)[16], float inv) {
+  uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float2 f;
-    f.x = finite(v[2 * i]) ? v[2 * i] * inv : __int_as_float(0x7fc00000);
-    f.y = finite(v[2 * i + 1]) ? v[2 * i + 1] * inv : __int_as_float(0x7fc00000);
-    w[i >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3) << (16 * (i & 1));
+    uint32_t two[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float a = v[4 * i + 2 * h], b = v[4 * i + 2 * h + 1];
+      float2 f = make_float2(a * inv, b * inv);
+      if (CHECK && magnitude(a) >= kInfinity) f.x = __int_as_float(0x7fc00000);
+      if (CHECK && magnitude(b) >= kInfinity) f.y = __int_as_float(0x7fc00000);
+      two[h] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+    }
+    w[i] = __byte_perm(two[0], two[1], 0x5410);
   }
-  return make_uint2(w[0], w[1]);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A piece is 8 values; 16 pieces (half a warp) are a block. The last block of a row may have fewer.
-template <typename T, bool GATE, typename Div>
+// A piece is 16 values; 8 pieces (a quarter of a warp) are a block. The last block of a row may have fewer. A thread has U pieces, whose loads
+// are all on their way before the first is looked at. (With 8 values a piece the blocks' own instructions, 150 a piece, were the bound:
+// 8192 x 8192 bf16 values took 52 us.)
+template <typename T, bool GATE, int U, typename Div>
 __global__ void __launch_bounds__(kThreads)
     quantise_kernel(const T* __restrict__ x, int64_t tokens, int64_t x_stride, const int32_t* __restrict__ rows,
-                    typename Div::Int pieces, Div by_row, int k, uint2* __restrict__ q, float* __restrict__ scale, int64_t ss_r,
-                    int64_t ss_b) {
+                    typename Div::Int pieces, Div by_row, int k, bool wide, uint4* __restrict__ q, float* __restrict__ scale,
+                    int64_t ss_r, int64_t ss_b) {
   using Int = typename Div::Int;
-  const int row_pieces = (k + kBlock - 1) / kBlock * (kBlock / 8);
-  for (Int p = (Int)blockIdx.x * kThreads + threadIdx.x; p < pieces; p += (Int)gridDim.x * kThreads) {
-    // pieces is a multiple of 16 and so is the step: the 16 lanes of a block come here together
-    const Int r = by_row(p);
-    const int at = (int)(p - r * (Int)row_pieces) * 8;
-    const int64_t src = rows ? (int64_t)rows[r] : (int64_t)r;
-    float v[8];
+  const int row_pieces = (k + kBlock - 1) / kBlock * (kBlock / 16);
+  const Int p0 = (Int)blockIdx.x * (kThreads * U) + threadIdx.x;
+  const unsigned mask = 0xffu << (threadIdx.x & 24);
+  Raw<T> raw[U][GATE ? 2 : 1];
+  Int row[U];
+  int at[U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    if (at < k && (uint64_t)src < (uint64_t)tokens) {
-      const T* from = x + src * x_stride + at;
-      load8(from, v);
-      if (GATE) {
-        float u[8];
-        load8(from + k, u);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fdividef(v[i], 1.f + __expf(-v[i])) * u[i];
-      }
+  for (int u = 0; u < U; ++u) {
+    // pieces is a multiple of 8, as kThreads is: the 8 lanes of a block are there together or not at all
+    const Int p = p0 + u * kThreads;
+    row[u] = p < pieces ? by_row(p) : 0;
+    at[u] = p < pieces ? (int)(p - row[u] * (Int)row_pieces) * 16 : -1;
+    const int64_t src = at[u] < 0 || at[u] >= k ? -1 : rows ? (int64_t)rows[row[u]] : (int64_t)row[u];
+    if ((uint64_t)src < (uint64_t)tokens) {
+      const T* from = x + src * x_stride + at[u];
+      load(from, raw[u][0], wide);
+      if (GATE) load(from + k, raw[u][GATE], wide);
+    } else {
+      clear(raw[u][0]);
+      if (GATE) clear(raw[u][GATE]);
     }
-    float a = largest(v);
-    const unsigned mask = 0xffffu << (threadIdx.x & 16);
+  }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(mask, a, o));
+  for (int u = 0; u < U; ++u) {
+    if (at[u] < 0) break;
+    float v[16];
+    widen(raw[u][0], v);
+    if (GATE) {
+      float g[16];
+      widen(raw[u][GATE], g);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = __fdividef(v[i], 1.f + __expf(-v[i])) * g[i];
+    }
+    uint32_t a = largest(v);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(mask, a, o));
+    const bool fine = a < kInfinity;  // alike in the block's lanes
+    if (!fine) {
+      a = largest_finite(v);
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(mask, a, o));
+    }
     const float s = scale_of(a);
-    const float inv = s > 0.f ? 1.f / s : 0.f;
-    if (at < k) q[((int64_t)r * k + at) >> 3] = codes(v, inv);
-    if ((threadIdx.x & 15) == 0) scale[(int64_t)r * ss_r + (at / kBlock) * ss_b] = s;
+    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+    if (at[u] < k) q[((int64_t)row[u] * k + at[u]) >> 4] = fine ? codes<false>(v, inv) : codes<true>(v, inv);
+    if ((threadIdx.x & 7) == 0) scale[(int64_t)row[u] * ss_r + (at[u] / kBlock) * ss_b] = s;
   }
 }
 
 // One CTA a block of 128 x 128 weights: its values stay in registers between the maximum and the codes.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    weight_kernel(const T* __restrict__ w, int64_t n, int64_t k, int64_t stride_e, int64_t stride_n, int64_t blocks_k,
-                  int64_t blocks_n, uint2* __restrict__ q, float* __restrict__ scale) {
-  const int64_t bk = blockIdx.x % blocks_k, rest = blockIdx.x / blocks_k, bn = rest % blocks_n, e = rest / blocks_n;
-  const int piece = threadIdx.x & 15;
-  const int64_t col = bk * kBlock + piece * 8;
-  constexpr int kEach = kBlock / (kThreads / 16);  // rows a thread
-  float v[kEach][8];
-  float a = 0.f;
+    weight_kernel(const T* __restrict__ w, int64_t n, int64_t k, int64_t stride_e, int64_t stride_n, uint32_t blocks_k,
+                  uint32_t blocks_n, bool wide, uint4* __restrict__ q, float* __restrict__ scale) {
+  const uint32_t rest = blockIdx.x / blocks_k, e = rest / blocks_n;
+  const int64_t bk = blockIdx.x - rest * blocks_k, bn = rest - e * blocks_n;
+  const int64_t col = bk * kBlock + (threadIdx.x & 7) * 16;
+  constexpr int kApart = kThreads / 8, kEach = kBlock / kApart;  // rows from one to the next of a thread, and how many it has
+  const int64_t row0 = bn * kBlock + (threadIdx.x >> 3);
+  Raw<T> raw[kEach];
+  uint32_t a = 0;
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
-    const int64_t row = bn * kBlock + (threadIdx.x >> 4) + j * (kThreads / 16);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[j][i] = 0.f;
-    if (row < n && col < k) load8(w + e * stride_e + row * stride_n + col, v[j]);
+    clear(raw[j]);
+    if (row0 + j * kApart < n && col < k) load(w + e * stride_e + (row0 + j * kApart) * stride_n + col, raw[j], wide);
   }
+  float v[16];
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) a = fmaxf(a, largest(v[j]));
-  __shared__ float part[kThreads / 32];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
+  for (int j = 0; j < kEach; ++j) {
+    widen(raw[j], v);
+    a = max(a, largest(v));
+  }
+  __shared__ uint32_t part[2][kThreads / 32];
+  a = __reduce_max_sync(0xffffffffu, a);
+  if ((threadIdx.x & 31) == 0) part[0][threadIdx.x >> 5] = a;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) a = fmaxf(a, part[i]);
+  for (int i = 0; i < kThreads / 32; ++i) a = max(a, part[0][i]);
+  const bool fine = a < kInfinity;
+  if (!fine) {
+    a = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      widen(raw[j], v);
+      a = max(a, largest_finite(v));
+    }
+    a = __reduce_max_sync(0xffffffffu, a);
+    if ((threadIdx.x & 31) == 0) part[1][threadIdx.x >> 5] = a;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) a = max(a, part[1][i]);
+  }
   const float s = scale_of(a);
-  const float inv = s > 0.f ? 1.f / s : 0.f;
+  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
-    const int64_t row = bn * kBlock + (threadIdx.x >> 4) + j * (kThreads / 16);
-    if (row < n && col < k) q[((e * n + row) * k + col) >> 3] = codes(v[j], inv);
+    const int64_t row = row0 + j * kApart;
+    if (row < n && col < k) {
+      widen(raw[j], v);
+      q[((e * n + row) * k + col) >> 4] = fine ? codes<false>(v, inv) : codes<true>(v, inv);
+    }
   }
   if (threadIdx.x == 0) scale[blockIdx.x] = s;
 }
 
+template <typename T, bool GATE, int U>
+int quantise_by(const T* x, int64_t tokens, int64_t x_stride, const int32_t* rows, int64_t pieces, int64_t row_pieces, int64_t k,
+                uint4* q, float* scale, int64_t ss_r, int64_t ss_b, cudaStream_t s) {
+  const int64_t ctas = (pieces + kThreads * U - 1) / (kThreads * U);
+  if (ctas > 0x7fffffff) return UP_ERR_UNSUPPORTED;
+  // gated values of 16 bits lie 2k bytes on, of 32 bits 4k: k is a multiple of 16, so on such borders as x is
+  const bool wide = aligned(x, 32) && x_stride * sizeof(T) % 32 == 0;
+  if (pieces + kThreads * U < (int64_t)1 << 31)
+    quantise_kernel<T, GATE, U, Divide32><<<(unsigned)ctas, kThreads, 0, s>>>(x, tokens, x_stride, rows, (uint32_t)pieces,
+                                                                              Divide32(row_pieces), (int)k, wide, q, scale, ss_r, ss_b);
+  else
+    quantise_kernel<T, GATE, U, Divide64><<<(unsigned)ctas, kThreads, 0, s>>>(x, tokens, x_stride, rows, (uint64_t)pieces,
+                                                                              Divide64(row_pieces), (int)k, wide, q, scale, ss_r, ss_b);
+  note_launch();
+  return check_launch();
+}
 template <typename T, bool GATE>
 int quantise(const void* x, int64_t tokens, int64_t x_stride, const int32_t* rows, int64_t n_rows, int64_t k, uint8_t* q,
              float* scale, int64_t ss_r, int64_t ss_b, cudaStream_t s) {
-  const int64_t row_pieces = (k + kBlock - 1) / kBlock * (kBlock / 8);
-  const int64_t pieces = n_rows * row_pieces;
-  const int64_t ctas = (pieces + kThreads - 1) / kThreads;
-  const int64_t most = (int64_t)sm_count() * 64;
-  const unsigned grid = (unsigned)(ctas < most ? ctas : most);
+  const int64_t row_pieces = (k + kBlock - 1) / kBlock * (kBlock / 16), pieces = n_rows * row_pieces;
+  constexpr int kMany = sizeof(T) == 4 || GATE ? 1 : 2;  // 64 bytes a thread on their way
   const T* from = static_cast<const T*>(x);
-  uint2* to = reinterpret_cast<uint2*>(q);
-  if (pieces + most * kThreads < (int64_t)1 << 31)
-    quantise_kernel<T, GATE, Divide32><<<grid, kThreads, 0, s>>>(from, tokens, x_stride, rows, (uint32_t)pieces,
-                                                                 Divide32(row_pieces), (int)k, to, scale, ss_r, ss_b);
-  else
-    quantise_kernel<T, GATE, Divide64><<<grid, kThreads, 0, s>>>(from, tokens, x_stride, rows, (uint64_t)pieces,
-                                                                 Divide64(row_pieces), (int)k, to, scale, ss_r, ss_b);
-  note_launch();
-  return check_launch();
+  uint4* to = reinterpret_cast<uint4*>(q);
+  // one piece a thread until the SMs are full
+  if (pieces <= (int64_t)sm_count() * 2048)
+    return quantise_by<T, GATE, 1>(from, tokens, x_stride, rows, pieces, row_pieces, k, to, scale, ss_r, ss_b, s);
+  return quantise_by<T, GATE, kMany>(from, tokens, x_stride, rows, pieces, row_pieces, k, to, scale, ss_r, ss_b, s);
 }
 
 template <typename T>
 int quantise_weight(const void* w, int64_t experts, int64_t n, int64_t k, int64_t se, int64_t sn, uint8_t* q, float* scale,
                     cudaStream_t s) {
   const int64_t bk = (k + kBlock - 1) / kBlock, bn = (n + kBlock - 1) / kBlock;
-  weight_kernel<T><<<(unsigned)(experts * bn * bk), kThreads, 0, s>>>(static_cast<const T*>(w), n, k, se, sn, bk, bn,
-                                                                      reinterpret_cast<uint2*>(q), scale);
+  weight_kernel<T><<<(unsigned)(experts * bn * bk), kThreads, 0, s>>>(static_cast<const T*>(w), n, k, se, sn, (uint32_t)bk, (uint32_t)bn,
+                                                                      aligned(w, 32) && se * sizeof(T) % 32 == 0 && sn * sizeof(T) % 32 == 0,
+                                                                      reinterpret_cast<uint4*>(q), scale);
   note_launch();
   return check_launch();
 }
