@@ -969,4 +969,13 @@ extern "C" int up_sm100_f8_matmul(const uint8_t* x, int64_t m, int64_t x_stride,
   }
 }
 
+namespace up {
+size_t f8_matmul_smem_bytes() {  // for the kernel interface: the largest form's
+  size_t most = 0;
+  for (const size_t n : {(size_t)Of<Narrow<32>>::kSmem, (size_t)Of<Narrow<64>>::kSmem, (size_t)Of<Wide<1>>::kSmem, (size_t)Of<Wide<2>>::kSmem})
+    most = n > most ? n : most;
+  return most;
+}
+}  // namespace up
+
 UP_DEFINE_REVISION(f8_matmul)

@@ -14,6 +14,9 @@ namespace up {
 uint64_t revision_backend();
 uint64_t revision_colsplit();
 uint64_t revision_dequant();
+uint64_t revision_experts();
+uint64_t revision_f8_matmul();
+uint64_t revision_f8_quantise();
 uint64_t revision_gather();
 uint64_t revision_kv4_append();
 uint64_t revision_kv4_attention();
@@ -27,6 +30,7 @@ uint64_t revision_w4a16();
 uint64_t revision_window();
 size_t scan_persist_smem_bytes();
 size_t w4a16_smem_bytes();
+size_t f8_matmul_smem_bytes();
 }  // namespace up
 
 using namespace up;
@@ -52,6 +56,10 @@ extern "C" uint64_t up_sm100_revision_hash(int kernel_id) {
     case UP_K_ROPE: return revision_rope();
     case UP_K_KV4_APPEND: return revision_kv4_append();
     case UP_K_KV4_ATTENTION: return revision_kv4_attention();
+    case UP_K_F8_QUANTISE: return revision_f8_quantise();
+    case UP_K_F8_MATMUL: return revision_f8_matmul();
+    case UP_K_EXPERT_ROUTE:
+    case UP_K_EXPERT_COMBINE: return revision_experts();
     default: return 0;
   }
 }
@@ -96,6 +104,14 @@ static const char* interface_body(int id) {
       return R"J({"entry_symbol":"up_sm100_kv4_append","params":[{"name":"q","role":"read","elem":"F16|BF16","rank":3},{"name":"k","role":"read","elem":"F16|BF16","rank":3},{"name":"v","role":"read","elem":"F16|BF16","rank":3},{"name":"positions","role":"read","elem":"I32|I64","rank":1},{"name":"table","role":"read","elem":"F32","rank":2},{"name":"slots","role":"read","elem":"I32|I64","rank":1},{"name":"cache","role":"readwrite","elem":"I4+F16","rank":4},{"name":"q_out","role":"write","elem":"F16|BF16","rank":3},{"name":"layout","role":"scalar","elem":"I32"}],"launch":{"block":[256,1,1],"grid":"blocks of query chunks and blocks of key and value rows, alternating","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":256,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["packed values and scales are the stated f32 operations bit for bit"],"workspace":null})J";
     case UP_K_KV4_ATTENTION:
       return R"J({"entry_symbol":"up_sm100_kv4_attention","params":[{"name":"q","role":"read","elem":"F16|BF16","rank":3},{"name":"cache","role":"read","elem":"I4+F16","rank":4},{"name":"block_table","role":"read","elem":"I32","rank":2},{"name":"seq_lens","role":"read","elem":"I32","rank":1},{"name":"cu_q","role":"read","elem":"I32","rank":1},{"name":"out","role":"write","elem":"F16|BF16","rank":3},{"name":"lse","role":"write","elem":"F32","rank":2},{"name":"causal","role":"scalar","elem":"I32"},{"name":"window","role":"scalar","elem":"I64"},{"name":"scale","role":"scalar","elem":"F32"}],"launch":{"block":[128,1,1],"grid":"few query rows: two to four CTAs per SM over units of 128 cached tokens; prompts (block 576): a CTA per 256 query rows","cluster":null,"dynamic_shared_bytes":"up to 201728"},"launch_bounds":{"max_threads":576,"min_blocks":1},"cooperative":false,"requires":["sm_100a","cp.async","mma.sync","tcgen05","tensor_memory","mbarrier"],"fidelity_notes":["f32 sums, exact logits up to them; few query rows: p * v_scale rounded to f16; many: p, and with bf16 outputs nibble * v_scale","split tiles are added in order: deterministic"],"workspace":"counters and parts of split tiles: up_sm100_kv4_attention_workspace_bytes, zero-filled once"})J";
+    case UP_K_F8_QUANTISE:
+      return R"J({"entry_symbol":"up_sm100_f8_quantise","params":[{"name":"x","role":"read","elem":"F32|F16|BF16","rank":2},{"name":"rows","role":"read","elem":"I32","rank":1},{"name":"q","role":"write","elem":"FP8_E4M3FN","rank":2},{"name":"scale","role":"write","elem":"F32","rank":2},{"name":"gate","role":"scalar","elem":"I32"}],"launch":{"block":[256,1,1],"grid":"a thread per one or two pieces of 16 values","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":256,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["values and scales are the stated f32 operations bit for bit; with a gate, exp and the quotient are approximate (2^-19 of a value)"],"workspace":null})J";
+    case UP_K_F8_MATMUL:
+      return R"J({"entry_symbol":"up_sm100_f8_matmul","params":[{"name":"x","role":"read","elem":"FP8_E4M3FN","rank":2},{"name":"x_scale","role":"read","elem":"F32","rank":2},{"name":"w","role":"read","elem":"FP8_E4M3FN","rank":3},{"name":"w_scale","role":"read","elem":"F32","rank":3},{"name":"offsets","role":"read","elem":"I32","rank":1},{"name":"out","role":"write","elem":"F32|F16|BF16","rank":2}],"launch":{"block":[384,1,1],"grid":"persistent, one CTA per SM (blocks of 256 or 384 threads, pairs for many rows)","cluster":[2,1,1],"dynamic_shared_bytes":"up to %SMEM%"},"launch_bounds":{"max_threads":384,"min_blocks":1},"cooperative":false,"requires":["sm_100a","tcgen05","tensor_memory","tma","mbarrier","thread_block_clusters"],"fidelity_notes":["each block of 128 k summed in f32 by the tensor cores, the blocks times their scales in f32, one rounding to out","parts of split tiles are added in order: deterministic"],"workspace":"counters and parts of split tiles: up_sm100_f8_matmul_workspace_bytes, its first 8192 bytes zero-filled once"})J";
+    case UP_K_EXPERT_ROUTE:
+      return R"J({"entry_symbol":"up_sm100_expert_route","params":[{"name":"logits","role":"read","elem":"F32|F16|BF16","rank":2},{"name":"ids","role":"write","elem":"I32","rank":2},{"name":"weights","role":"write","elem":"F32","rank":2},{"name":"rows","role":"write","elem":"I32","rank":1},{"name":"slots","role":"write","elem":"I32","rank":2},{"name":"offsets","role":"write","elem":"I32","rank":1},{"name":"k","role":"scalar","elem":"I64"},{"name":"score","role":"scalar","elem":"I32"},{"name":"renormalise","role":"scalar","elem":"I32"},{"name":"gain","role":"scalar","elem":"F32"}],"launch":{"block":[1024,1,1],"grid":"one CTA up to 128 tokens; else two launches of a CTA per 128 tokens, at most 256","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":1024,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["whole numbers are exact: largest logits, the lower expert of equal ones; weights in f32"],"workspace":"each CTA's counts: up_sm100_expert_route_workspace_bytes"})J";
+    case UP_K_EXPERT_COMBINE:
+      return R"J({"entry_symbol":"up_sm100_expert_combine","params":[{"name":"y","role":"read","elem":"F32|F16|BF16","rank":2},{"name":"slots","role":"read","elem":"I32","rank":2},{"name":"weights","role":"read","elem":"F32","rank":2},{"name":"add","role":"read","elem":"F32|F16|BF16","rank":2},{"name":"out","role":"write","elem":"F32|F16|BF16","rank":2}],"launch":{"block":[256,1,1],"grid":"a thread per one to four 16-byte pieces of the output","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":256,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["fused multiply-adds in f32 in the slots' order, one rounding"],"workspace":null})J";
     default: return nullptr;
   }
 }
@@ -106,7 +122,9 @@ extern "C" int up_sm100_kernel_interface(int kernel_id, char* buf, size_t cap, s
   std::string text(body);
   const size_t at = text.find("%SMEM%");  // the persistent kernels' dynamic shared memory, from their constants
   if (at != std::string::npos) {
-    const size_t smem = kernel_id == UP_K_SCAN_I32 ? scan_persist_smem_bytes() : w4a16_smem_bytes();
+    const size_t smem = kernel_id == UP_K_SCAN_I32    ? scan_persist_smem_bytes()
+                        : kernel_id == UP_K_F8_MATMUL ? f8_matmul_smem_bytes()
+                                                      : w4a16_smem_bytes();
     text.replace(at, 6, std::to_string(smem));
   }
   if (kernel_id == UP_K_REDUCE_F32 || kernel_id == UP_K_REDUCE_I32) {  // the flattened-geometry entry
