@@ -14,6 +14,7 @@
 //    token, so a block's scales are one factor for all of its columns. (With tokens as columns every thread needs every token's
 //    factor: at 128 bytes a cycle shared memory gives those of 128 x 128 values in 512 cycles, in which the MMA takes 256.)
 #include "common.cuh"
+#include "divide.cuh"
 #include "tc.cuh"
 
 #include <cuda.h>
@@ -30,7 +31,6 @@ constexpr int kBlock = 128;               // k a scale, and weight rows a scale
 constexpr int kTile = 128 * kBlock;       // bytes of 128 rows of a block
 constexpr int kBox = 16;                  // tokens of a small TMA box
 constexpr int kMaxExperts = 1024;
-constexpr int kEpi0 = 4;                  // warps 0 to 3: loads, MMA, scales, tensor memory
 constexpr int kRuns = 4;                  // runs of blocks that the roles may be apart
 constexpr int kMaxCtas = (UP_F8_COUNTER_BYTES - 64) / 4;  // a counter each
 
@@ -41,6 +41,7 @@ struct Narrow {
   static constexpr int kGroup = 4;                                  // blocks of an accumulator slot
   static constexpr int kDBlock = TOKENS;                            // columns of tensor memory a block
   static constexpr int kBBytes = TOKENS * kBlock, kStages = TOKENS == 64 ? 8 : 10;
+  static constexpr int kRunsWarp = 4, kEpi0 = 5;                    // the warp that deals the runs, the first of the epilogue's
   static constexpr int kEpiWarps = TOKENS == 32 ? 4 : 8, kSums = TOKENS * 4 / kEpiWarps;  // sums a thread
   static constexpr int kMinBlocks = 8;                              // of an owner: fewer do not pay for joining the parts
   static constexpr int kScRing = 4, kScSlot = kGroup * TOKENS;  // tokens' scales in shared memory, a group a slot
@@ -52,6 +53,7 @@ struct Wide {
   static constexpr int kGroup = 1;
   static constexpr int kDBlock = 256;
   static constexpr int kBBytes = 256 / CTAS * kBlock, kStages = CTAS == 2 ? 6 : 4;
+  static constexpr int kRunsWarp = 2, kEpi0 = 4;
   static constexpr int kEpiWarps = 8, kSums = 128;
   static constexpr int kMinBlocks = 16;
   static constexpr int kScRing = 0, kScSlot = 0;
@@ -61,14 +63,14 @@ template <typename C>
 struct Of {
   static constexpr int kStage = kTile + C::kBBytes;
   static constexpr int kDSlot = C::kDBlock * C::kGroup, kDRing = 512 / kDSlot;  // accumulators in tensor memory
-  static constexpr int kEpiThreads = 32 * C::kEpiWarps, kThreads = 32 * kEpi0 + kEpiThreads;
+  static constexpr int kEpiThreads = 32 * C::kEpiWarps, kThreads = 32 * C::kEpi0 + kEpiThreads;
   static constexpr size_t kPart = (size_t)C::kSums * kEpiThreads;  // values of a CTA's part of a tile
-  // One thread issues the MMAs and commits of a block in some 500 cycles, so where a block has few more two threads take turns; the rings' even
-  // depths then give each slot to one of them, which sees all of its phases.
-  static constexpr int kIssuers = C::kWide ? 2 : 1;
-  static constexpr int kBars = 2 * C::kStages + 2 * kDRing + 2 * C::kScRing + 2 * kRuns + 3;
+  // One thread issues the MMAs and commits of a block in some 450 cycles, so two take the blocks in turn; the ring's even
+  // depth then gives each stage to one of them, which sees all of its phases.
+  static constexpr int kIssuers = 2;
+  static constexpr int kBars = 2 * C::kStages + 2 * kDRing + 2 * C::kScRing + 3 * kRuns + 3;
   static constexpr int kSmem = 1024 + C::kStages * kStage + C::kScRing * C::kScSlot * 4 + kRuns * 48 + kBars * 8 + 16 + (kMaxExperts + 1) * 2 * 4;
-  static_assert(C::kStages % 2 == 0 && kDRing % 2 == 0 && kSmem <= 232448, "rings, shared memory");
+  static_assert(C::kStages % 2 == 0 && (C::kGroup > 1 || kDRing % 2 == 0) && kSmem <= 232448, "rings, shared memory");
 };
 
 struct Header {
@@ -82,6 +84,7 @@ struct Args {
   int64_t xs_m, xs_b;
   int64_t m;
   int experts, n, kb, nb, tb, groups;     // kb: blocks of k, in `groups` groups; nb: of weight rows, in tb tiles
+  Divide32 by_owners = Divide32(1), by_groups = Divide32(1);
   const int32_t* offsets;
   void* out;
   int64_t out_stride;
@@ -135,7 +138,7 @@ struct Runs {
 struct Run {
   int t, g0, g1;                          // the tile, its groups from g0 to before g1; no groups: the end
   int e, tb, m0, n;                       // the tile's expert, place among the weight rows, first row and number of tokens
-  int c0, c1;                             // the first and last of the owners that share the tile
+  int c0, c1;                             // the first and last of the owners that share the tile (by a barrier of their own)
   int pad[3];
 };
 static_assert(sizeof(Run) == 48, "Run");
@@ -152,23 +155,24 @@ struct Walk {
   __device__ __forceinline__ int owner_of(int unit) const {
     return unit < more * (base + 1) ? unit / (base + 1) : more + (unit - more * (base + 1)) / base;
   }
-  __device__ __forceinline__ Walk(const int* start_, const int* begin_, int experts, int groups_, int owner, int owners_)
-      : start(start_), begin(begin_), groups(groups_), left(0), owners(owners_) {
-    const int tiles = start[experts];
-    int rest = tiles % owners;
+  __device__ __forceinline__ Walk(const Args& a, const int* start_, const int* begin_, int owner, int owners_)
+      : start(start_), begin(begin_), groups(a.groups), left(0), owners(owners_) {
+    const int tiles = start[a.experts];
+    const int rounds = (int)a.by_owners(tiles);
+    int rest = tiles - rounds * owners;
     if (10 * rest > 9 * owners) rest = 0;  // a last round that is nearly full: parts would cost more than they save
     const int units = rest * groups, most = units * C::kGroup / C::kMinBlocks, sharers = most < 1 ? 1 : most < owners ? most : owners;
-    base = units / sharers, more = units - base * sharers;
+    base = sharers == owners ? (int)a.by_owners(units) : units / sharers, more = units - base * sharers;
     r.e = 0, r.t = 0, r.g0 = 0;
     if (owner < sharers) {
       left = base + (owner < more ? 1 : 0);
-      r.t = first_unit(owner) / groups;
+      r.t = (int)a.by_groups(first_unit(owner));
       r.g0 = first_unit(owner) - r.t * groups;
     }
     whole_t = rest + owner;
-    whole_left = owner < tiles - rest ? (tiles - rest - owner + owners - 1) / owners : 0;
+    whole_left = rounds + (rest == 0 && owner < tiles - rounds * owners ? 1 : 0);
     const int first = left > 0 ? r.t : whole_t;
-    int hi = experts - 1;                 // the last expert that starts at or before the first tile
+    int hi = a.experts - 1;               // the last expert that starts at or before the first tile
     while (r.e < hi) {
       const int mid = (r.e + hi + 1) >> 1;
       if (start[mid] <= first) r.e = mid;
@@ -177,11 +181,9 @@ struct Walk {
   }
   // the next run; the one without groups at the end
   __device__ __forceinline__ bool next() {
-    r.c0 = r.c1 = 0;
     if (left > 0) {
       r.g1 = min(groups, r.g0 + left);
       left -= r.g1 - r.g0;
-      if (r.g0 > 0 || r.g1 < groups) r.c0 = owner_of(r.t * groups), r.c1 = owner_of(r.t * groups + groups - 1);
     } else if (whole_left > 0) {
       --whole_left;
       r.t = whole_t, r.g0 = 0, r.g1 = groups;
@@ -192,11 +194,14 @@ struct Walk {
     }
     while (r.t >= start[r.e + 1]) ++r.e;
     const int rows = begin[r.e + 1] - begin[r.e], wide = (rows + C::kTokens - 1) / C::kTokens, at = r.t - start[r.e];
-    r.tb = at / wide;
-    // the group's tokens in tiles of equal width; the last may have fewer, and has some: (wide - 1) * kTokens < rows
-    const int each = ((rows + wide - 1) / wide + C::kStep - 1) / C::kStep * C::kStep, first = (at - r.tb * wide) * each;
-    r.m0 = begin[r.e] + first;
-    r.n = min(each, rows - first);
+    r.tb = at, r.m0 = begin[r.e], r.n = rows;
+    if (wide > 1) {
+      // the group's tokens in tiles of equal width; the last may have fewer, and has some: (wide - 1) * kTokens < rows
+      r.tb = at / wide;
+      const int each = ((rows + wide - 1) / wide + C::kStep - 1) / C::kStep * C::kStep, first = (at - r.tb * wide) * each;
+      r.m0 += first;
+      r.n = min(each, rows - first);
+    }
     return true;
   }
   __device__ __forceinline__ void passed() {  // the run was taken over
@@ -397,8 +402,9 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
   uint64_t* drain = seg_out + 1;
   uint64_t* run_full = drain + 1;
   uint64_t* run_empty = run_full + kRuns;
+  uint64_t* run_owners = run_empty + kRuns;
   static_assert((kStages * O::kStage + kScRing * C::kScSlot * 4 + O::kBars * 8) % 8 == 0, "alignment");
-  Run* runs = reinterpret_cast<Run*>(run_empty + kRuns);
+  Run* runs = reinterpret_cast<Run*>(run_owners + kRuns);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(runs + kRuns);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile uint32_t* verdict = tmem_slot + 2;
@@ -410,11 +416,11 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
   if (warp == 0) {
     if (lane == 0) {
       for (int s = 0; s < kStages; ++s) tc::mbar_init(&full[s], 1), tc::mbar_init(&empty[s], 1);
-      for (int d = 0; d < kDRing; ++d) tc::mbar_init(&d_full[d], 1), tc::mbar_init(&d_empty[d], C::kEpiWarps * C::kCtas);
+      for (int d = 0; d < kDRing; ++d) tc::mbar_init(&d_full[d], kGroup > 1 ? O::kIssuers : 1), tc::mbar_init(&d_empty[d], C::kEpiWarps * C::kCtas);
       for (int q = 0; q < kScRing; ++q) tc::mbar_init(&sc_full[q], 1), tc::mbar_init(&sc_empty[q], C::kEpiWarps);
       // readers of the runs: the loads, the issuers (a pair's are the first CTA's), the scales, the epilogue's warps
       for (int i = 0; i < kRuns; ++i)
-        tc::mbar_init(&run_full[i], 1), tc::mbar_init(&run_empty[i], 1 + (rank == 0 ? O::kIssuers : 0) + (C::kWide ? 0 : 1) + C::kEpiWarps);
+        tc::mbar_init(&run_full[i], 1), tc::mbar_init(&run_owners[i], 1), tc::mbar_init(&run_empty[i], 1 + (rank == 0 ? O::kIssuers : 0) + (C::kWide ? 0 : 1) + C::kEpiWarps);
       tc::mbar_init(seg_in, C::kEpiWarps), tc::mbar_init(seg_out, 1), tc::mbar_init(drain, O::kIssuers);
       *abort_flag = 0;
       tc::mbar_fence_init();
@@ -441,7 +447,7 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
     return good && runs[at.at].g1 > runs[at.at].g0;
   };
 
-  if (warp < kEpi0) {
+  if (warp < C::kEpi0) {
     if (C::kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
       // ---------------- loads ----------------
@@ -485,10 +491,11 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
           for (int64_t j = issued > kStages ? issued - kStages : 0; j < issued; ++j)
             wait(&full[j % kStages], (uint32_t)((j / kStages) & 1), a, nullptr);
       }
-    } else if (warp == 1 || (warp == 3 && O::kIssuers == 2)) {
-      // ---------------- MMA: issuer h takes the groups h, h + kIssuers, ... ----------------
+    } else if (warp == 1 || warp == 3) {
+      // ---------------- MMA: the issuers take the blocks in turn; a group's accumulators are done when both have committed ----------------
       if (lane == 0 && rank == 0) {
-        int s = 0, d = 0, turn = warp >> 1;
+        int s = 0, d = 0;
+        bool mine = warp == 1;
         uint32_t ph = 0, dph = 1;
         bool good = true;
         for (Runs at; take(at, good); at.next()) {
@@ -497,10 +504,9 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
           const uint32_t id = C::kWide ? idesc_f8(128 * C::kCtas, 256) : idesc_f8(128, (w.n + 15) / 16 * 16);
           const int end = min(a.kb, w.g1 * kGroup);
           for (int kb = w.g0 * kGroup; kb < end && good; kb += kGroup) {
-            const bool mine = O::kIssuers == 1 || turn == 0;
-            if (mine) good = wait(&d_empty[d], dph, a, abort_flag);
+            if (kGroup > 1 || mine) good = wait(&d_empty[d], dph, a, abort_flag);
 #pragma unroll 1
-            for (int j = 0; j < kGroup && kb + j < end && good; ++j) {
+            for (int j = 0; j < kGroup && kb + j < end && good; ++j, mine = !mine) {
               if (mine) {
                 good = wait(&full[s], ph, a, abort_flag);
                 if (!good) break;
@@ -510,12 +516,12 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
 #pragma unroll
                 for (int i = 0; i < kBlock / 32; ++i) mma_f8<PAIR>(tmem + d * O::kDSlot + j * C::kDBlock, ad + 2 * i, bd + 2 * i, id, i > 0);
                 commit<PAIR>(&empty[s]);
+                if (kGroup == 1) commit<PAIR>(&d_full[d]);
               }
               if (++s == kStages) s = 0, ph ^= 1u;
             }
-            if (mine) commit<PAIR>(&d_full[d]);
+            if (kGroup > 1) commit<PAIR>(&d_full[d]);
             if (++d == kDRing) d = 0, dph ^= 1u;
-            turn ^= 1;
           }
         }
         if (!good) give_up();
@@ -581,10 +587,10 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
         store(1);
       }
       if (!good) give_up();
-    } else if (warp == (C::kWide ? 2 : 3)) {
+    } else if (warp == C::kRunsWarp) {
       // ---------------- runs ----------------
       if (lane == 0) {
-        Walk<C> w(start, begin, a.experts, a.groups, blockIdx.x / C::kCtas, gridDim.x / C::kCtas);
+        Walk<C> w(a, start, begin, blockIdx.x / C::kCtas, gridDim.x / C::kCtas);
         Runs at;
         bool good = true;
         for (bool more = true; more; at.next()) {
@@ -593,6 +599,11 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
           if (!good) break;
           runs[at.at] = w.r;
           tc::mbar_arrive(&run_full[at.at]);
+          if (w.r.g0 > 0 || w.r.g1 < a.groups) {  // who shares the tile is needed last
+            runs[at.at].c0 = w.owner_of(w.r.t * a.groups);
+            runs[at.at].c1 = w.owner_of(w.r.t * a.groups + a.groups - 1);
+          }
+          tc::mbar_arrive(&run_owners[at.at]);
           w.passed();
         }
         if (!good) give_up();
@@ -601,7 +612,7 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
   } else {
     // ---------------- sums: lanes 32 (warp % 4) .. of tensor memory ----------------
     if (C::kWide) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    const int quarter = warp & 3, part = (warp - kEpi0) >> 2, thread = threadIdx.x - 32 * kEpi0, row = quarter * 32 + lane;
+    const int quarter = warp & 3, part = (warp - C::kEpi0) >> 2, thread = threadIdx.x - 32 * C::kEpi0, row = quarter * 32 + lane;
     const uint32_t d_empty0 = PAIR ? in_leader(d_empty) : 0;
     const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + kSums * part;
     float sum[kSums];
@@ -722,6 +733,8 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
       bool write = true;
       if (w.g0 > 0 || w.g1 < a.groups) {
         // A part of a tile: published, and whichever owner comes last adds the parts in the order of the owners.
+        good = __all_sync(0xffffffffu, wait(&run_owners[at.at], at.phase, a, abort_flag));
+        if (!good) break;
         const int c0 = w.c0, c1 = w.c1, owner = blockIdx.x / C::kCtas;
         float* parts = a.partials + thread;
         float* to = parts + ((size_t)blockIdx.x * 2 + (c0 == owner ? 1 : 0)) * O::kPart;
@@ -731,7 +744,7 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
         const uint32_t jp = joined & 1u;
         ++joined;
         if (lane == 0) tc::mbar_arrive(seg_in);
-        if (warp == kEpi0 && lane == 0) {
+        if (warp == C::kEpi0 && lane == 0) {
           // one release for all warps' stores, which the barrier put before it
           good = wait(seg_in, jp, a, abort_flag);
           if (good) {
@@ -856,15 +869,16 @@ static int cta_count() { return sm_count() < kMaxCtas ? sm_count() : kMaxCtas; }
 enum Form { kNarrow32, kNarrow64, kWide, kPair };
 
 // The form that takes the least time by a model of what was measured: a fixed part (launch, first loads, joining of parts) and so many
-// microseconds a block of an owner's tile. 8192 x 8192 weights, us by Narrow<32>, Narrow<64>, Wide<1>, Wide<2>: 1 row 21, 23, 27, 37;
-// 64 rows 31, 24, 29, 36; 128 rows 50, 33, 29, 37; 256 rows 90, 54, 41, 38; 2048 rows 657, 358, 153, 144. 128 experts of 4096 x 2048: 512
-// rows 174, 185, 169, 266; 8192 rows 435, 305, 212, 329; 65536 rows 2840, 1573, 746, 783.
+// microseconds a block of an owner's tile, fitted to calls of 1 to 2048 rows by 1024 x 8192 to 28672 x 8192 weights. Measured, us,
+// Narrow<32>, Narrow<64>, Wide<1>, Wide<2>: by 8192 x 8192 weights 1 row 21, 23, 28, 37; 64 rows 27, 24, 29, 37; 128 rows 40, 31, 29, 37; 256
+// rows 72, 47, 40, 39; 2048 rows 501, 281, 151, 143. 128 experts of 4096 x 2048: 512 rows 162, 181, 171, 266; 8192 rows 439, 316, 213, 333;
+// 65536 rows 2327, 1685, 749, 784.
 static Form form_of(int64_t m, int64_t experts, int64_t n, int64_t kb) {
   struct Cost {
-    int tokens, weights, owners;  // of a tile; owners of the 148
+    int tokens, weights, ctas;  // of a tile
     double fixed, block;
   };
-  static const Cost cost[4] = {{32, 128, 148, 6, 0.38}, {64, 128, 148, 8, 0.42}, {128, 256, 148, 18, 0.72}, {256, 256, 74, 18, 0.65}};
+  static const Cost cost[4] = {{32, 128, 1, 10.5, 0.275}, {64, 128, 1, 13, 0.30}, {128, 256, 1, 20, 0.59}, {256, 256, 2, 20, 0.56}};
   const double used = (double)(m < experts ? m : experts), per = m / used;  // experts that have rows, at most; rows of each
   int best = 0;
   double least = 0;
@@ -872,7 +886,7 @@ static Form form_of(int64_t m, int64_t experts, int64_t n, int64_t kb) {
     const Cost& c = cost[i];
     // a ragged group's last tile is half full in the mean
     const double tiles = experts == 1 ? (double)((m + c.tokens - 1) / c.tokens) : per / c.tokens + 0.5 > 1 ? per / c.tokens + 0.5 : 1;
-    const double us = c.fixed + c.block * tiles * used * (double)((n + c.weights - 1) / c.weights) * (double)kb / c.owners;
+    const double us = c.fixed + c.block * tiles * used * (double)((n + c.weights - 1) / c.weights) * (double)kb * c.ctas / cta_count();
     if (i == 0 || us < least) best = i, least = us;
   }
   return (Form)best;
@@ -910,6 +924,7 @@ struct Operands {
 template <typename C, typename K>
 static int launch(K kernel, unsigned grid, Args& a, const Operands& o, cudaStream_t s) {
   a.groups = (a.kb + C::kGroup - 1) / C::kGroup;
+  a.by_groups = Divide32(a.groups), a.by_owners = Divide32(grid / C::kCtas);
   a.tb = (a.nb + C::kWeights / kBlock - 1) / (C::kWeights / kBlock);
   CUtensorMap wmap, xmap, xmap_full;
   if (!encode(&wmap, o.w, 3, o.k, o.n, o.experts, o.k, kBlock) || !encode(&xmap, o.x, 2, o.k, o.m, 1, o.x_stride, kBox) ||
