@@ -202,3 +202,20 @@ def test_a_layer_of_experts(tokens):
     static.copy_(other)
     graph.replay()
     assert torch.equal(out, layer(other, router, up, up_s, down, down_s, k, add=other))
+
+
+@pytest.mark.parametrize("experts,k", [(40, 8), (64, 6), (256, 8), (256, 32), (1000, 32)])
+def test_route_where_more_experts_than_a_warp_has_lanes_reach_the_bound(experts, k):
+    """Few distinct logits: hundreds of equal ones around the k-th, in one lane and in all of them."""
+    logits = torch.randint(0, 3, (150, experts), generator=gen(experts), device=DEV).float()
+    logits[0] = 0.0
+    logits[1] = -0.0
+    logits[2, :k - 1] = 5.0
+    logits[3] = torch.arange(experts, device=DEV) % 32  # a lane's keys are equal, the lanes' differ
+    logits[4] = torch.arange(experts, device=DEV) // 32
+    logits[5] = float("inf")
+    logits[6] = float("nan")
+    logits[7] = -float("inf")
+    logits[7, 3::7] = -1e30
+    check_route(logits, k, "sigmoid")
+    check_route(logits[:5], k, "softmax", False)

@@ -1,11 +1,14 @@
 // experts.cu — routing of tokens to experts, and the weighted sum of the experts' rows.
 //
-// Routing: a warp takes a token's k largest logits by k rounds of a warp maximum over order-preserving 32-bit keys, each lane's
-// sorted before, so that a round looks at their heads only. Then the pairs are counted and placed by expert. A pair's place is the number of pairs of lower experts plus that of the same
+// Routing: a warp holds a token's logits as order-preserving 32-bit keys. The k-th largest of the lanes' own maxima is a bound that at
+// least k keys reach, and few more; those that do are collected in the experts' order, and each counts how many come before it, which is its
+// rank. (k rounds of a maximum over all keys took some 650 instructions a token of 256 experts, this takes about 250.) Then the pairs
+// are counted and placed by expert. A pair's place is the number of pairs of lower experts plus that of the same
 // expert's earlier tokens, so it does not depend on the order in which anything runs: within 128 tokens the earlier
 // ones are the lower bits of a mask that each expert has (set by atomicOr, which commutes), before them the counts of earlier blocks.
 #include "common.cuh"
 #include "divide.cuh"
+#include "launch.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -52,90 +55,95 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Sorts a lane's keys, largest first, the lower expert of equal ones: Batcher's odd-even merge sort ("Sorting networks and their
-// applications", 1968) for a power of two of them.
+// One token's choice by one warp, lane l holding the keys of experts l, l + 32, ...: up to k of its lanes get a rank (below k), an expert
+// and its weight; the others' rank is kMaxK.
+struct Choice {
+  int rank, id;
+  float weight;
+};
+struct Candidate {
+  uint32_t key;
+  int id;
+};
 template <int PER>
-__device__ __forceinline__ void sort_keys(uint32_t (&key)[PER], int (&at)[PER]) {
+__device__ __forceinline__ Choice choose(const uint32_t (&key)[PER], const Route& a, int lane, Candidate* found) {
+  uint32_t own = key[0];
 #pragma unroll
-  for (int p = 1; p < PER; p *= 2)
-#pragma unroll
-    for (int k = p; k >= 1; k /= 2)
-#pragma unroll
-      for (int j = k % p; j + k < PER; j += 2 * k)
-#pragma unroll
-        for (int i = 0; i < k; ++i)
-          if (i + j + k < PER && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
-            const int a = i + j, b = i + j + k;
-            const bool swap = key[b] > key[a] || (key[b] == key[a] && at[b] < at[a]);
-            const uint32_t ka = key[a], kb = key[b];
-            const int ia = at[a], ib = at[b];
-            key[a] = swap ? kb : ka, key[b] = swap ? ka : kb;
-            at[a] = swap ? ib : ia, at[b] = swap ? ia : ib;
-          }
-}
-
-// One token's choice by one warp: lane j < k gets the j-th expert (or -1) and its weight. Lane l holds experts l, l + 32, ...
-template <int PER>
-__device__ __forceinline__ void choose(uint32_t (&key)[PER], const Route& a, int lane, int& id, float& weight) {
-  constexpr bool kSorted = PER <= 8;  // 19 exchanges for 8 keys; 63 for 16 would cost more than the rounds save
-  int at[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) at[i] = i * 32 + lane;
-  float all = 1.f;
-  if (a.score == UP_EXPERT_SOFTMAX && !a.renormalise) {
-    uint32_t high = key[0];
-#pragma unroll
-    for (int i = 1; i < PER; ++i) high = max(high, key[i]);
-    const float m = value_of(__reduce_max_sync(0xffffffffu, high));
-    all = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (key[i] > kMasked) all += expf(value_of(key[i]) - m);
-    all = warp_sum(all);
-  }
-  if (kSorted) sort_keys<PER>(key, at);
-  uint32_t mine = 0, top = 0;
-  id = -1;
+  for (int i = 1; i < PER; ++i) own = max(own, key[i]);
+  // after r rounds at least r lanes have a maximum that reaches the bound (equal ones leave together)
+  uint32_t left = own, top = 0, bound = 0;
   for (int j = 0; j < a.k; ++j) {
-    uint32_t best = key[0];
-    int e = at[0];
-    if (!kSorted) {
+    bound = __reduce_max_sync(0xffffffffu, left);
+    if (j == 0) top = bound;
+    if (left == bound) left = 0;
+  }
+  bound = max(bound, kMasked + 1);
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const bool is = key[i] >= bound;
+    const unsigned who = __ballot_sync(0xffffffffu, is);
+    const int at = n + __popc(who & ((1u << lane) - 1u));
+    if (is && at < 32) found[at] = Candidate{key[i], i * 32 + lane};
+    n += __popc(who);
+  }
+  Choice c{kMaxK, -1, 0.f};
+  uint32_t mine = 0;
+  if (n <= 32) {
+    __syncwarp();
+    if (lane < n) mine = found[lane].key, c.id = found[lane].id;
+    int before = 0;  // candidates stand in the order of their experts: of equal ones the earlier comes first
+    for (int j = 0; j < n; ++j) {
+      const uint32_t other = __shfl_sync(0xffffffffu, mine, j);
+      before += other > mine || (other == mine && j < lane) ? 1 : 0;
+    }
+    if (lane < n && before < a.k) c.rank = before;
+    __syncwarp();  // before the next token's are written
+  } else {
+    // many equal ones: a round for each, of the largest key left and the lowest expert that has it
+    uint32_t rest[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) rest[i] = key[i];
+    for (int j = 0; j < a.k; ++j) {
+      uint32_t best = rest[0];
+      int e = lane;
 #pragma unroll
       for (int i = 1; i < PER; ++i)
-        if (key[i] > best) best = key[i], e = at[i];
-    }
-    const uint32_t high = __reduce_max_sync(0xffffffffu, best);
-    if (high <= kMasked) break;  // the others are masked
-    const unsigned same = __ballot_sync(0xffffffffu, best == high);
-    if (same & (same - 1))  // several lanes' heads are equal: the lowest expert
+        if (rest[i] > best) best = rest[i], e = i * 32 + lane;
+      const uint32_t high = __reduce_max_sync(0xffffffffu, best);
+      if (high <= kMasked) break;
       e = (int)__reduce_min_sync(0xffffffffu, best == high ? (unsigned)e : 0x7fffffffu);
-    else
-      e = __shfl_sync(0xffffffffu, e, __ffs(same) - 1);
-    if (j == 0) top = high;
-    if (lane == j) mine = high, id = e;
-    if (kSorted) {
-      if (lane == (e & 31)) {
-#pragma unroll
-        for (int i = 0; i + 1 < PER; ++i) key[i] = key[i + 1], at[i] = at[i + 1];
-        key[PER - 1] = 0;
-      }
-    } else {
+      if (lane == j) mine = high, c.id = e, c.rank = j;
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        if (e == at[i]) key[i] = 0;
+        if (e == i * 32 + lane) rest[i] = 0;
     }
   }
+  const bool taken = c.rank < kMaxK;
   const float l = value_of(mine);
-  float w = 0.f;
-  if (id >= 0) w = a.score == UP_EXPERT_SOFTMAX ? expf(l - value_of(top)) : 1.f / (1.f + expf(-l));
-  const float total = a.renormalise ? warp_sum(w) : all;
-  weight = (id >= 0 && !(total == 0.f)) ? w / total * a.gain : 0.f;
+  float w = 0.f, total = 1.f;
+  if (a.score == UP_EXPERT_SOFTMAX) {
+    const float m = value_of(top);
+    if (taken) w = expf(l - m);
+    if (!a.renormalise) {
+      total = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (key[i] > kMasked) total += expf(value_of(key[i]) - m);
+      total = warp_sum(total);
+    }
+  } else if (taken) {
+    w = 1.f / (1.f + expf(-l));
+  }
+  if (a.renormalise) total = warp_sum(w);
+  c.weight = taken && !(total == 0.f) ? w / total * a.gain : 0.f;
+  return c;
 }
 
 // Chooses for the tile's tokens; marks them in the experts' masks. A warp's tokens' logits are all on their way at once where
 // they leave it the registers.
 template <int PER, typename T>
-__device__ __forceinline__ void choose_tile(const Route& a, int first, uint32_t (*mask)[kTile / 32], int32_t* held) {
+__device__ __forceinline__ void choose_tile(const Route& a, int first, uint32_t (*mask)[kTile / 32], int16_t* held, Candidate* found) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int end = min(first + kTile, a.tokens);
   constexpr int kEach = kTile / kWarps, kAtOnce = PER <= 4 ? kEach : PER <= 8 ? 2 : 1;
@@ -154,16 +162,19 @@ __device__ __forceinline__ void choose_tile(const Route& a, int first, uint32_t 
     for (int u = 0; u < kAtOnce; ++u) {
       const int t = t0 + u * kWarps;
       if (t >= end) break;
-      int id;
-      float w;
-      choose<PER>(key[u], a, lane, id, w);
-      if (lane < a.k) {
-        const int64_t at = (int64_t)t * a.k + lane;
-        a.ids[at] = id;
-        a.weights[at] = w;
-        const int in = t - first;
-        if (held) held[in * a.k + lane] = id;
-        if (id >= 0) atomicOr(&mask[id][in >> 5], 1u << (in & 31));
+      const Choice c = choose<PER>(key[u], a, lane, found + 32 * warp);
+      const int64_t at = (int64_t)t * a.k;
+      const int in = t - first, n = __popc(__ballot_sync(0xffffffffu, c.rank < kMaxK));
+      if (c.rank < kMaxK) {
+        a.ids[at + c.rank] = c.id;
+        a.weights[at + c.rank] = c.weight;
+        if (held) held[in * a.k + c.rank] = (int16_t)c.id;
+        atomicOr(&mask[c.id][in >> 5], 1u << (in & 31));
+      }
+      if (lane >= n && lane < a.k) {  // the ranks that no expert has
+        a.ids[at + lane] = -1;
+        a.weights[at + lane] = 0.f;
+        if (held) held[in * a.k + lane] = -1;
       }
     }
   }
@@ -199,7 +210,7 @@ __device__ __forceinline__ uint32_t scan_experts(const uint32_t* total, uint32_t
 
 // Places the tile's pairs: next[e] is the place of expert e's first pair in it.
 __device__ __forceinline__ void place_tile(const Route& a, int first, const uint32_t (*mask)[kTile / 32], const uint32_t* next,
-                                           const int32_t* held) {
+                                           const int16_t* held) {
   const int pairs = (min(first + kTile, a.tokens) - first) * a.k;
   for (int p = threadIdx.x; p < pairs; p += kThreads) {
     const int in = p / a.k, id = held[p];
@@ -220,10 +231,13 @@ __global__ void __launch_bounds__(kThreads) route_one_kernel(const Route a) {
   __shared__ uint32_t mask[PER * 32][kTile / 32];
   __shared__ uint32_t total[PER * 32], start[PER * 32];
   __shared__ uint32_t all;
-  __shared__ int32_t held[kTile * kMaxK];
+  __shared__ int16_t held[kTile * kMaxK];
+  __shared__ Candidate found[kThreads];
   clear(mask, a.experts);
+  after_previous();
+  let_next_begin();
   __syncthreads();
-  choose_tile<PER, T>(a, 0, mask, held);
+  choose_tile<PER, T>(a, 0, mask, held, found);
   __syncthreads();
   for (int e = threadIdx.x; e < a.experts; e += kThreads) total[e] = count_of(mask[e]);
   __syncthreads();
@@ -242,13 +256,16 @@ template <int PER, typename T>
 __global__ void __launch_bounds__(kThreads) choose_kernel(const Route a) {
   __shared__ uint32_t mask[PER * 32][kTile / 32];
   __shared__ uint32_t total[PER * 32];
+  __shared__ Candidate found[kThreads];
   for (int e = threadIdx.x; e < a.experts; e += kThreads) total[e] = 0;
+  after_previous();
+  let_next_begin();
   for (int i = 0; i < a.per; ++i) {
     const int first = (blockIdx.x * a.per + i) * kTile;
     if (first >= a.tokens) break;
     clear(mask, a.experts);
     __syncthreads();
-    choose_tile<PER, T>(a, first, mask, nullptr);
+    choose_tile<PER, T>(a, first, mask, nullptr, found);
     __syncthreads();
     for (int e = threadIdx.x; e < a.experts; e += kThreads) total[e] += count_of(mask[e]);
     __syncthreads();
@@ -261,8 +278,10 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const Route a) {
   __shared__ uint32_t mask[kMaxExperts][kTile / 32];
   __shared__ uint32_t total[kMaxExperts], next[kMaxExperts], before[kMaxExperts];
   __shared__ uint32_t all;
-  __shared__ int32_t held[kTile * kMaxK];
+  __shared__ int16_t held[kTile * kMaxK];
   for (int e = threadIdx.x; e < a.experts; e += kThreads) total[e] = before[e] = 0;
+  after_previous();
+  let_next_begin();
   __syncthreads();
   // a column of threads for each 32 experts' warp: warps take blocks in turn
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -297,7 +316,7 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const Route a) {
     if (first >= a.tokens) break;
     clear(mask, a.experts);
     const int pairs = (min(first + kTile, a.tokens) - first) * a.k;
-    for (int p = threadIdx.x; p < pairs; p += kThreads) held[p] = a.ids[(int64_t)first * a.k + p];
+    for (int p = threadIdx.x; p < pairs; p += kThreads) held[p] = (int16_t)a.ids[(int64_t)first * a.k + p];
     __syncthreads();
     for (int p = threadIdx.x; p < pairs; p += kThreads) {
       const int in = p / a.k;
@@ -324,17 +343,16 @@ static int blocks_of(int64_t tokens, int* per) {
 template <int PER, typename T>
 int route(Route& a, cudaStream_t s) {
   if (a.tokens <= kTile) {
-    route_one_kernel<PER, T><<<1, kThreads, 0, s>>>(a);
+    const cudaError_t e = launch_early(route_one_kernel<PER, T>, 1, kThreads, 0, s, a);
+    if (e != cudaSuccess) return cuda_status(e);
     note_launch();
     return check_launch();
   }
   const int blocks = blocks_of(a.tokens, &a.per);
-  choose_kernel<PER, T><<<blocks, kThreads, 0, s>>>(a);
-  note_launch();
-  const int ok = check_launch();
-  if (ok != UP_OK) return ok;
-  place_kernel<<<blocks, kThreads, 0, s>>>(a);
-  note_launch();
+  cudaError_t e = launch_early(choose_kernel<PER, T>, blocks, kThreads, 0, s, a);
+  if (e == cudaSuccess) e = launch_early(place_kernel, blocks, kThreads, 0, s, a);
+  if (e != cudaSuccess) return cuda_status(e);
+  note_launch(2);
   return check_launch();
 }
 template <typename T>
@@ -426,6 +444,8 @@ __global__ void __launch_bounds__(kSumThreads)
   using W = Vec<T, V>;
   constexpr int kAtOnce = 8 / U;
   const Int p0 = (Int)blockIdx.x * (kSumThreads * U) + threadIdx.x;
+  after_previous();
+  let_next_begin();
   float sum[U][V];
   int64_t at[U], tk[U], out_at[U];
   bool in[U];
@@ -476,12 +496,13 @@ int combine_by(const void* y, int64_t rows, int64_t ys, int64_t n, const int32_t
   const int64_t ctas = (pieces + kSumThreads * U - 1) / (kSumThreads * U);
   if (ctas > 0x7fffffff) return UP_ERR_UNSUPPORTED;
   const T *from = static_cast<const T*>(y), *more = static_cast<const T*>(add);
-  if (pieces < ((int64_t)1 << 31) - kSumThreads * U)
-    combine_kernel<T, V, U, Divide32><<<(unsigned)ctas, kSumThreads, 0, s>>>(from, rows, ys, slots, weights, (int)k, more, as,
-        static_cast<T*>(out), os, (uint32_t)pieces, (uint32_t)row_pieces, Divide32(row_pieces));
-  else
-    combine_kernel<T, V, U, Divide64><<<(unsigned)ctas, kSumThreads, 0, s>>>(from, rows, ys, slots, weights, (int)k, more, as,
-        static_cast<T*>(out), os, (uint64_t)pieces, (uint64_t)row_pieces, Divide64(row_pieces));
+  const cudaError_t e =
+      pieces < ((int64_t)1 << 31) - kSumThreads * U
+          ? launch_early(combine_kernel<T, V, U, Divide32>, (unsigned)ctas, kSumThreads, 0, s, from, rows, ys, slots, weights, (int)k,
+                         more, as, static_cast<T*>(out), os, (uint32_t)pieces, (uint32_t)row_pieces, Divide32(row_pieces))
+          : launch_early(combine_kernel<T, V, U, Divide64>, (unsigned)ctas, kSumThreads, 0, s, from, rows, ys, slots, weights, (int)k,
+                         more, as, static_cast<T*>(out), os, (uint64_t)pieces, (uint64_t)row_pieces, Divide64(row_pieces));
+  if (e != cudaSuccess) return cuda_status(e);
   note_launch();
   return check_launch();
 }

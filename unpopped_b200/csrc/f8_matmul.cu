@@ -15,6 +15,7 @@
 //    factor: at 128 bytes a cycle shared memory gives those of 128 x 128 values in 512 cycles, in which the MMA takes 256.)
 #include "common.cuh"
 #include "divide.cuh"
+#include "launch.cuh"
 #include "tc.cuh"
 
 #include <cuda.h>
@@ -429,8 +430,11 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
   } else if (warp == 1) {
     tmem_alloc<PAIR>(tmem_slot);
   } else if (warp == 2) {
+    after_previous();
     schedule<C>(a, start, begin, lane);
   }
+  after_previous();
+  let_next_begin();
   tc::fence_before_sync();
   __syncthreads();
   if (PAIR) cluster_sync();
@@ -932,7 +936,8 @@ static int launch(K kernel, unsigned grid, Args& a, const Operands& o, cudaStrea
     return fail_with(UP_ERR_CUDA, "cuTensorMapEncodeTiled refused an operand's tensor map");
   const cudaError_t e = ensure_smem_attr((const void*)kernel, Of<C>::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
-  kernel<<<grid, Of<C>::kThreads, Of<C>::kSmem, s>>>(wmap, xmap, xmap_full, a);
+  const cudaError_t l = launch_early(kernel, grid, Of<C>::kThreads, Of<C>::kSmem, s, wmap, xmap, xmap_full, a);
+  if (l != cudaSuccess) return cuda_status(l);
   note_launch();
   return check_launch();
 }

@@ -7,6 +7,7 @@
 // Bound by HBM: 2 (4, 8) bytes read and 1.03 written a value.
 #include "common.cuh"
 #include "divide.cuh"
+#include "launch.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -119,6 +120,8 @@ __global__ void __launch_bounds__(kThreads)
   const Int p0 = (Int)blockIdx.x * (kThreads * U) + threadIdx.x;
   const unsigned mask = 0xffu << (threadIdx.x & 24);
   Raw<T> raw[U][GATE ? 2 : 1];
+  after_previous();
+  let_next_begin();
   Int row[U];
   int at[U];
 #pragma unroll
@@ -176,6 +179,8 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t row0 = bn * kBlock + (threadIdx.x >> 3);
   Raw<T> raw[kEach];
   uint32_t a = 0;
+  after_previous();
+  let_next_begin();
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     clear(raw[j]);
@@ -227,12 +232,13 @@ int quantise_by(const T* x, int64_t tokens, int64_t x_stride, const int32_t* row
   if (ctas > 0x7fffffff) return UP_ERR_UNSUPPORTED;
   // gated values of 16 bits lie 2k bytes on, of 32 bits 4k: k is a multiple of 16, so on such borders as x is
   const bool wide = aligned(x, 32) && x_stride * sizeof(T) % 32 == 0;
-  if (pieces + kThreads * U < (int64_t)1 << 31)
-    quantise_kernel<T, GATE, U, Divide32><<<(unsigned)ctas, kThreads, 0, s>>>(x, tokens, x_stride, rows, (uint32_t)pieces,
-                                                                              Divide32(row_pieces), (int)k, wide, q, scale, ss_r, ss_b);
-  else
-    quantise_kernel<T, GATE, U, Divide64><<<(unsigned)ctas, kThreads, 0, s>>>(x, tokens, x_stride, rows, (uint64_t)pieces,
-                                                                              Divide64(row_pieces), (int)k, wide, q, scale, ss_r, ss_b);
+  const cudaError_t e =
+      pieces + kThreads * U < (int64_t)1 << 31
+          ? launch_early(quantise_kernel<T, GATE, U, Divide32>, (unsigned)ctas, kThreads, 0, s, x, tokens, x_stride, rows,
+                         (uint32_t)pieces, Divide32(row_pieces), (int)k, wide, q, scale, ss_r, ss_b)
+          : launch_early(quantise_kernel<T, GATE, U, Divide64>, (unsigned)ctas, kThreads, 0, s, x, tokens, x_stride, rows,
+                         (uint64_t)pieces, Divide64(row_pieces), (int)k, wide, q, scale, ss_r, ss_b);
+  if (e != cudaSuccess) return cuda_status(e);
   note_launch();
   return check_launch();
 }
@@ -253,9 +259,11 @@ template <typename T>
 int quantise_weight(const void* w, int64_t experts, int64_t n, int64_t k, int64_t se, int64_t sn, uint8_t* q, float* scale,
                     cudaStream_t s) {
   const int64_t bk = (k + kBlock - 1) / kBlock, bn = (n + kBlock - 1) / kBlock;
-  weight_kernel<T><<<(unsigned)(experts * bn * bk), kThreads, 0, s>>>(static_cast<const T*>(w), n, k, se, sn, (uint32_t)bk, (uint32_t)bn,
-                                                                      aligned(w, 32) && se * sizeof(T) % 32 == 0 && sn * sizeof(T) % 32 == 0,
-                                                                      reinterpret_cast<uint4*>(q), scale);
+  const cudaError_t e = launch_early(weight_kernel<T>, (unsigned)(experts * bn * bk), kThreads, 0, s, static_cast<const T*>(w), n, k, se,
+                                     sn, (uint32_t)bk, (uint32_t)bn,
+                                     aligned(w, 32) && se * sizeof(T) % 32 == 0 && sn * sizeof(T) % 32 == 0,
+                                     reinterpret_cast<uint4*>(q), scale);
+  if (e != cudaSuccess) return cuda_status(e);
   note_launch();
   return check_launch();
 }
