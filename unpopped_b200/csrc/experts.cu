@@ -191,22 +191,33 @@ __device__ __forceinline__ void clear(uint32_t (*mask)[kTile / 32], int experts)
   for (int i = threadIdx.x; i < experts * (kTile / 32); i += kThreads) (&mask[0][0])[i] = 0;
 }
 
-// total[e] (all counts) to offsets, by warp 0: start[e] becomes the sum of the totals before e; returns the sum of all.
-__device__ __forceinline__ uint32_t scan_experts(const uint32_t* total, uint32_t* start, int experts, int lane) {
-  uint32_t run = 0;
-  for (int e0 = 0; e0 < experts; e0 += 32) {
-    const uint32_t n = e0 + lane < experts ? total[e0 + lane] : 0u;
-    uint32_t s = n;
+// start[e] becomes the sum of the totals before e, by all warps: each scans 32 experts, then adds the warps before. Returns the sum of all.
+// Ends and begins with the block in step.
+__device__ __forceinline__ uint32_t scan_experts(const uint32_t* total, uint32_t* start, int experts) {
+  __shared__ uint32_t of_warp[kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = threadIdx.x;  // kMaxExperts threads
+  const uint32_t n = e < experts ? total[e] : 0u;
+  uint32_t s = n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += v;
-    }
-    if (e0 + lane < experts) start[e0 + lane] = run + s - n;
-    run += __shfl_sync(0xffffffffu, s, 31);
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += v;
   }
-  return run;
+  if (lane == 31) of_warp[warp] = s;
+  __syncthreads();
+  uint32_t w = of_warp[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += v;
+  }
+  const uint32_t all = __shfl_sync(0xffffffffu, w, 31);
+  const uint32_t before = warp > 0 ? __shfl_sync(0xffffffffu, w, warp - 1) : 0u;
+  if (e < experts) start[e] = before + s - n;
+  __syncthreads();
+  return all;
 }
+static_assert(kThreads == kMaxExperts && kWarps == 32, "a thread an expert, a lane a warp");
 
 // Places the tile's pairs: next[e] is the place of expert e's first pair in it.
 __device__ __forceinline__ void place_tile(const Route& a, int first, const uint32_t (*mask)[kTile / 32], const uint32_t* next,
@@ -230,7 +241,6 @@ template <int PER, typename T>
 __global__ void __launch_bounds__(kThreads) route_one_kernel(const Route a) {
   __shared__ uint32_t mask[PER * 32][kTile / 32];
   __shared__ uint32_t total[PER * 32], start[PER * 32];
-  __shared__ uint32_t all;
   __shared__ int16_t held[kTile * kMaxK];
   __shared__ Candidate found[kThreads];
   clear(mask, a.experts);
@@ -241,11 +251,7 @@ __global__ void __launch_bounds__(kThreads) route_one_kernel(const Route a) {
   __syncthreads();
   for (int e = threadIdx.x; e < a.experts; e += kThreads) total[e] = count_of(mask[e]);
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const uint32_t n = scan_experts(total, start, a.experts, threadIdx.x);
-    if (threadIdx.x == 0) all = n;
-  }
-  __syncthreads();
+  const uint32_t all = scan_experts(total, start, a.experts);
   for (int e = threadIdx.x; e <= a.experts; e += kThreads) a.offsets[e] = (int32_t)(e < a.experts ? start[e] : all);
   place_tile(a, 0, mask, start, held);
   for (int i = (int)all + threadIdx.x; i < a.tokens * a.k; i += kThreads) a.rows[i] = -1;
@@ -277,55 +283,59 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const Route a) {
 __global__ void __launch_bounds__(kThreads) place_kernel(const Route a) {
   __shared__ uint32_t mask[kMaxExperts][kTile / 32];
   __shared__ uint32_t total[kMaxExperts], next[kMaxExperts], before[kMaxExperts];
-  __shared__ uint32_t all;
   __shared__ int16_t held[kTile * kMaxK];
   for (int e = threadIdx.x; e < a.experts; e += kThreads) total[e] = before[e] = 0;
+  clear(mask, a.experts);
   after_previous();
   let_next_begin();
+  // The choice of a tile, marked in its masks. The first one's is on its way beside the counts.
+  auto mark = [&](int first) {
+    const int pairs = (min(first + kTile, a.tokens) - first) * a.k;
+    for (int p = threadIdx.x; p < pairs; p += kThreads) {
+      const int id = a.ids[(int64_t)first * a.k + p], in = p / a.k;
+      held[p] = (int16_t)id;
+      if (id >= 0) atomicOr(&mask[id][in >> 5], 1u << (in & 31));
+    }
+  };
+  const int first0 = blockIdx.x * a.per * kTile;
   __syncthreads();
-  // a column of threads for each 32 experts' warp: warps take blocks in turn
+  // warps take columns of 32 experts, and where these are fewer than the warps share a column's blocks
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wide = (a.experts + 31) / 32;
-  for (int c = warp % wide; c < wide; c += kWarps) {
-    const int e = c * 32 + lane;
-    const int parts = wide < kWarps ? (kWarps - c + wide - 1) / wide : 1;  // warps that share column c
-    uint32_t n = 0, m = 0;
-    if (e < a.experts) {
+  const int c = warp % wide, e = c * 32 + lane, parts = (kWarps - c + wide - 1) / wide;  // wide is at most kWarps
+  uint32_t n = 0, m = 0;
+  if (e < a.experts) {
 #pragma unroll 16
-      for (int b = warp / wide; b < (int)gridDim.x; b += parts) {
-        const uint32_t v = a.counts[(int64_t)b * a.experts + e];
-        n += v;
-        if (b < (int)blockIdx.x) m += v;
-      }
-      atomicAdd(&total[e], n);
-      atomicAdd(&before[e], m);
+    for (int b = warp / wide; b < (int)gridDim.x; b += parts) {
+      const uint32_t v = a.counts[(int64_t)b * a.experts + e];
+      n += v;
+      if (b < (int)blockIdx.x) m += v;
     }
   }
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    const uint32_t n = scan_experts(total, next, a.experts, lane);
-    if (lane == 0) all = n;
+  mark(first0);
+  if (e < a.experts) {
+    atomicAdd(&total[e], n);
+    atomicAdd(&before[e], m);
   }
   __syncthreads();
+  const uint32_t all = scan_experts(total, next, a.experts);
   if (blockIdx.x == 0)
-    for (int e = threadIdx.x; e <= a.experts; e += kThreads) a.offsets[e] = (int32_t)(e < a.experts ? next[e] : all);
+    for (int i = threadIdx.x; i <= a.experts; i += kThreads) a.offsets[i] = (int32_t)(i < a.experts ? next[i] : all);
   __syncthreads();
-  for (int e = threadIdx.x; e < a.experts; e += kThreads) next[e] += before[e];
+  for (int i = threadIdx.x; i < a.experts; i += kThreads) next[i] += before[i];
+  __syncthreads();
   for (int i = 0; i < a.per; ++i) {
-    const int first = (blockIdx.x * a.per + i) * kTile;
+    const int first = first0 + i * kTile;
     if (first >= a.tokens) break;
-    clear(mask, a.experts);
-    const int pairs = (min(first + kTile, a.tokens) - first) * a.k;
-    for (int p = threadIdx.x; p < pairs; p += kThreads) held[p] = (int16_t)a.ids[(int64_t)first * a.k + p];
-    __syncthreads();
-    for (int p = threadIdx.x; p < pairs; p += kThreads) {
-      const int in = p / a.k;
-      if (held[p] >= 0) atomicOr(&mask[held[p]][in >> 5], 1u << (in & 31));
+    if (i > 0) {
+      clear(mask, a.experts);
+      __syncthreads();
+      mark(first);
+      __syncthreads();
     }
-    __syncthreads();
     place_tile(a, first, mask, next, held);
     __syncthreads();
-    for (int e = threadIdx.x; e < a.experts; e += kThreads) next[e] += count_of(mask[e]);
+    for (int x = threadIdx.x; x < a.experts; x += kThreads) next[x] += count_of(mask[x]);
     __syncthreads();
   }
   const int64_t pairs = (int64_t)a.tokens * a.k;
