@@ -6,13 +6,16 @@
 // tcgen05.mma of its own into tensor memory (four steps of 32 k, f32), and the epilogue warps add it, times its two scales,
 // to f32 sums in registers while the next blocks are multiplied.
 //
-// Two forms, by which operand takes the MMA's rows:
+// Two kinds, by which operand takes the MMA's rows:
 //  * Narrow, for few tokens: 128 weight rows, up to 32 tokens as columns. Bound by HBM: every weight once. Columns are dealt in steps of 16,
 //    so a group of one token costs little, and four blocks share an accumulator slot, so that handing it to the epilogue costs once
 //    for all four. A thread of the epilogue has one weight row; the tokens' scales come to it through shared memory.
-//  * Wide: 128 tokens as rows (256 of two CTAs, tcgen05's cta_group::2), 256 weight rows as columns. A thread of the epilogue has one
+//  * Wide: 128 tokens as rows (256 of two CTAs, tcgen05's cta_group::2), 256 or 128 weight rows as columns. A thread of the epilogue has one
 //    token, so a block's scales are one factor for all of its columns. (With tokens as columns every thread needs every token's
-//    factor: at 128 bytes a cycle shared memory gives those of 128 x 128 values in 512 cycles, in which the MMA takes 256.)
+//    factor: at 128 bytes a cycle shared memory gives those of 128 x 128 values in 512 cycles, in which the MMA takes 256.) Bound by
+//    the two accumulators' round: an MMA of 512 cycles, its commit, the epilogue's loads and 128 sums a thread, the arrival that frees it.
+// Measured (a B200, inputs larger than L2 where they can be): 1 row by 8192 x 8192 weights 19.9 us (3.4 TB/s of weights), by 28672 x 8192 43.5
+// (5.4 TB/s); 8192 rows by 8192 x 8192 538 us (2.04 PFLOP/s); 16384 rows of 8 experts by 4096 x 2048 163 us (1.68 PFLOP/s).
 #include "common.cuh"
 #include "divide.cuh"
 #include "launch.cuh"
@@ -23,6 +26,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cmath>
 #include <mutex>
 
 namespace up {
@@ -35,29 +39,30 @@ constexpr int kMaxExperts = 1024;
 constexpr int kRuns = 4;                  // runs of blocks that the roles may be apart
 constexpr int kMaxCtas = (UP_F8_COUNTER_BYTES - 64) / 4;  // a counter each
 
-template <int TOKENS>
 struct Narrow {
   static constexpr bool kWide = false;
-  static constexpr int kCtas = 1, kTokens = TOKENS, kStep = 16, kWeights = 128;  // of a tile; tokens go in steps
+  static constexpr int kCtas = 1, kTokens = 32, kStep = 16, kWeights = 128;  // of a tile; tokens go in steps
   static constexpr int kGroup = 4;                                  // blocks of an accumulator slot
-  static constexpr int kDBlock = TOKENS;                            // columns of tensor memory a block
-  static constexpr int kBBytes = TOKENS * kBlock, kStages = TOKENS == 64 ? 8 : 10;
-  static constexpr int kRunsWarp = 4, kEpi0 = 5;                    // the warp that deals the runs, the first of the epilogue's
-  static constexpr int kEpiWarps = TOKENS == 32 ? 4 : 8, kSums = TOKENS * 4 / kEpiWarps;  // sums a thread
-  static constexpr int kMinBlocks = 8;                              // of an owner: fewer do not pay for joining the parts
-  static constexpr int kScRing = 4, kScSlot = kGroup * TOKENS;  // tokens' scales in shared memory, a group a slot
+  static constexpr int kDBlock = 32;                                // columns of tensor memory a block
+  static constexpr int kBBytes = 32 * kBlock, kStages = 10;
+  static constexpr int kXWarp = 4, kEpi0 = 5;                       // the warp that loads the tokens, the first of the epilogue's
+  static constexpr int kEpiWarps = 4, kSums = 32;                   // sums a thread
+  static constexpr int kMinBlocks = 8, kJoinBlocks = 12;            // of an owner's share of a tile, at least; blocks that joining parts takes
+  static constexpr int kFactors = 32;                               // of a block, through shared memory: the tokens'
 };
-template <int CTAS>
+template <int CTAS, int WEIGHTS>
 struct Wide {
   static constexpr bool kWide = true;
-  static constexpr int kCtas = CTAS, kTokens = 128 * CTAS, kStep = kTokens, kWeights = 256;
+  static constexpr int kCtas = CTAS, kTokens = 128 * CTAS, kStep = kTokens, kWeights = WEIGHTS;
   static constexpr int kGroup = 1;
-  static constexpr int kDBlock = 256;
-  static constexpr int kBBytes = 256 / CTAS * kBlock, kStages = CTAS == 2 ? 6 : 4;
-  static constexpr int kRunsWarp = 2, kEpi0 = 4;
-  static constexpr int kEpiWarps = 8, kSums = 128;
-  static constexpr int kMinBlocks = 16;
-  static constexpr int kScRing = 0, kScSlot = 0;
+  static constexpr int kDBlock = WEIGHTS;
+  static constexpr int kBBytes = WEIGHTS / CTAS * kBlock, kStages = 204800 / (kTile + kBBytes) / 2 * 2;
+  static constexpr int kXWarp = 0, kEpi0 = 4;
+  static constexpr int kEpiWarps = 8, kSums = WEIGHTS / 2;
+  static constexpr int kMinBlocks = 16, kJoinBlocks = WEIGHTS == 256 ? 24 : 12;
+  // none through shared memory: a thread's row is one token, so it loads its own, some blocks ahead. Measured against a warp that hands them
+  // over as for the narrow forms: 8192 rows by 8192 x 8192 weights 543 against 580 us, 2048 by 4096 x 4096 (128 columns) 50 against 59
+  static constexpr int kFactors = 0;
 };
 // What follows from them.
 template <typename C>
@@ -65,12 +70,15 @@ struct Of {
   static constexpr int kStage = kTile + C::kBBytes;
   static constexpr int kDSlot = C::kDBlock * C::kGroup, kDRing = 512 / kDSlot;  // accumulators in tensor memory
   static constexpr int kEpiThreads = 32 * C::kEpiWarps, kThreads = 32 * C::kEpi0 + kEpiThreads;
+  static constexpr int kScRing = C::kFactors > 0 ? 4 : 0, kScSlot = 4 * C::kFactors;  // factors in shared memory, four blocks a slot
+  static constexpr int kStaged = C::kWide ? 32 * 17 : 0;             // values a warp, for rows of `out` that do not begin on 32 bytes
   static constexpr size_t kPart = (size_t)C::kSums * kEpiThreads;  // values of a CTA's part of a tile
   // One thread issues the MMAs and commits of a block in some 450 cycles, so two take the blocks in turn; the ring's even
   // depth then gives each stage to one of them, which sees all of its phases.
   static constexpr int kIssuers = 2;
-  static constexpr int kBars = 2 * C::kStages + 2 * kDRing + 2 * C::kScRing + 3 * kRuns + 3;
-  static constexpr int kSmem = 1024 + C::kStages * kStage + C::kScRing * C::kScSlot * 4 + kRuns * 48 + kBars * 8 + 16 + (kMaxExperts + 1) * 2 * 4;
+  static constexpr int kBars = 2 * C::kStages + 2 * kDRing + 2 * kScRing + 3 * kRuns + 3;
+  static constexpr int kSmem = 1024 + C::kStages * kStage + kScRing * kScSlot * 4 + kRuns * 48 + kBars * 8 + 16 + (kMaxExperts + 1) * 2 * 4 +
+                               C::kEpiWarps * kStaged * 4;
   static_assert(C::kStages % 2 == 0 && (C::kGroup > 1 || kDRing % 2 == 0) && kSmem <= 232448, "rings, shared memory");
 };
 
@@ -98,23 +106,12 @@ struct Args {
 
 // Waits for the barrier's phase, at most a.wait_ns; false when that ran out or another role gave up. The clock is read only after
 // many attempts.
-__device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(tc::smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, const Args& a, volatile int* abort) {
   for (int it = 0; it < 64; ++it)
-    if (try_wait(bar, parity)) return true;
+    if (tc::mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   for (uint32_t it = 1;; ++it) {
-    if (try_wait(bar, parity)) return true;
+    if (tc::mbar_try_wait(bar, parity)) return true;
     if ((it & 255u) == 0) {
       if (abort && *abort) return false;
       if (globaltimer_ns() - t0 > a.wait_ns) return false;
@@ -161,8 +158,10 @@ struct Walk {
     const int tiles = start[a.experts];
     const int rounds = (int)a.by_owners(tiles);
     int rest = tiles - rounds * owners;
-    if (10 * rest > 9 * owners) rest = 0;  // a last round that is nearly full: parts would cost more than they save
-    const int units = rest * groups, most = units * C::kGroup / C::kMinBlocks, sharers = most < 1 ? 1 : most < owners ? most : owners;
+    // shared only where that saves an owner more blocks than the joining of parts takes: else whole as well
+    const int most = min(owners, rest * groups * C::kGroup / C::kMinBlocks);
+    if (groups * C::kGroup * (most - rest) <= C::kJoinBlocks * most) rest = 0;
+    const int units = rest * groups, sharers = rest > 0 ? most : 1;
     base = sharers == owners ? (int)a.by_owners(units) : units / sharers, more = units - base * sharers;
     r.e = 0, r.t = 0, r.g0 = 0;
     if (owner < sharers) {
@@ -312,14 +311,8 @@ __device__ __forceinline__ constexpr uint32_t idesc_f8(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
-// 16 or 32 consecutive columns of this thread's lane of tensor memory. The registers hold them after wait_loads; what uses them is
+// 32 consecutive columns of this thread's lane of tensor memory. The registers hold them after wait_loads; what uses them is
 // volatile too, so nothing moves it before the wait.
-__device__ __forceinline__ void load16(uint32_t from, uint32_t (&v)[16]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-               : "r"(from)
-               : "memory");
-}
 __device__ __forceinline__ void load32(uint32_t from, uint32_t (&v)[32]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
@@ -388,11 +381,11 @@ template <typename C>
 __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMap& xmap, const CUtensorMap& xmap_full, const Args& a) {
   using O = Of<C>;
   constexpr bool PAIR = C::kCtas == 2;
-  constexpr int kGroup = C::kGroup, kStages = C::kStages, kDRing = O::kDRing, kScRing = C::kScRing, kSums = C::kSums;
+  constexpr int kGroup = C::kGroup, kStages = C::kStages, kDRing = O::kDRing, kScRing = O::kScRing, kSums = C::kSums;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* sc = reinterpret_cast<float*>(stages + kStages * O::kStage);  // [kScRing][4 blocks][32]
-  uint64_t* full = reinterpret_cast<uint64_t*>(sc + kScRing * C::kScSlot);
+  float* sc = reinterpret_cast<float*>(stages + kStages * O::kStage);  // [kScRing][4 blocks][kFactors]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sc + kScRing * O::kScSlot);
   uint64_t* empty = full + kStages;
   uint64_t* d_full = empty + kStages;
   uint64_t* d_empty = d_full + kDRing;
@@ -404,13 +397,14 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
   uint64_t* run_full = drain + 1;
   uint64_t* run_empty = run_full + kRuns;
   uint64_t* run_owners = run_empty + kRuns;
-  static_assert((kStages * O::kStage + kScRing * C::kScSlot * 4 + O::kBars * 8) % 8 == 0, "alignment");
+  static_assert((kStages * O::kStage + kScRing * O::kScSlot * 4 + O::kBars * 8) % 8 == 0, "alignment");
   Run* runs = reinterpret_cast<Run*>(run_owners + kRuns);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(runs + kRuns);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile uint32_t* verdict = tmem_slot + 2;
   int* start = reinterpret_cast<int*>(tmem_slot + 4);
   int* begin = start + kMaxExperts + 1;
+  float* staged = reinterpret_cast<float*>(begin + kMaxExperts + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cta_rank() : 0;
@@ -419,9 +413,10 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
       for (int s = 0; s < kStages; ++s) tc::mbar_init(&full[s], 1), tc::mbar_init(&empty[s], 1);
       for (int d = 0; d < kDRing; ++d) tc::mbar_init(&d_full[d], kGroup > 1 ? O::kIssuers : 1), tc::mbar_init(&d_empty[d], C::kEpiWarps * C::kCtas);
       for (int q = 0; q < kScRing; ++q) tc::mbar_init(&sc_full[q], 1), tc::mbar_init(&sc_empty[q], C::kEpiWarps);
-      // readers of the runs: the loads, the issuers (a pair's are the first CTA's), the scales, the epilogue's warps
+      // readers of the runs: the factors, the issuers (a pair's are the first CTA's), the tokens' loads, the epilogue's warps
       for (int i = 0; i < kRuns; ++i)
-        tc::mbar_init(&run_full[i], 1), tc::mbar_init(&run_owners[i], 1), tc::mbar_init(&run_empty[i], 1 + (rank == 0 ? O::kIssuers : 0) + (C::kWide ? 0 : 1) + C::kEpiWarps);
+        tc::mbar_init(&run_full[i], 1), tc::mbar_init(&run_owners[i], 1),
+            tc::mbar_init(&run_empty[i], (C::kFactors > 0 ? 1 : 0) + (rank == 0 ? O::kIssuers : 0) + (C::kWide ? 0 : 1) + C::kEpiWarps);
       tc::mbar_init(seg_in, C::kEpiWarps), tc::mbar_init(seg_out, 1), tc::mbar_init(drain, O::kIssuers);
       *abort_flag = 0;
       tc::mbar_fence_init();
@@ -452,48 +447,77 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
   };
 
   if (warp < C::kEpi0) {
-    if (C::kWide) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (C::kSums > 64) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");  // 56 x 128 + 224 x 256 threads: what 168 each are
     if (warp == 0) {
-      // ---------------- loads ----------------
+      // ---------------- runs, and the loads of weights (Wide: of tokens too) ----------------
       if (lane == 0) {
+        Walk<C> walk(a, start, begin, blockIdx.x / C::kCtas, gridDim.x / C::kCtas);
         int64_t issued = 0;
         int s = 0;
         uint32_t ph = 1;
         const uint32_t full0 = PAIR ? in_leader(full) : tc::smem_u32(full);  // a pair's loads all count on the leader's barriers
         bool good = true;
-        for (Runs at; take(at, good); at.next()) {
-          const Run w = runs[at.at];
-          tc::mbar_arrive(&run_empty[at.at]);
+        Runs at;
+        for (bool more = true; more && good; at.next()) {
+          more = walk.next();  // the run without groups is handed over too
+          good = wait(&run_empty[at.at], at.phase ^ 1u, a, abort_flag);
+          if (!good) break;
+          const Run w = walk.r;
+          runs[at.at] = w;
+          tc::mbar_arrive(&run_full[at.at]);
+          walk.passed();
           const int boxes = (w.n + kBox - 1) / kBox;
           const uint32_t bytes = C::kWide ? C::kCtas * O::kStage : kTile + boxes * (kBox * kBlock);
-          const int row = w.tb * C::kWeights + (int)rank * kBlock, m0 = w.m0 + (int)rank * 128;
+          const int row = w.tb * C::kWeights + (int)rank * (C::kWeights / C::kCtas);
           for (int kb = w.g0 * kGroup, end = min(a.kb, w.g1 * kGroup); kb < end; ++kb) {
             good = wait(&empty[s], ph, a, abort_flag);
             if (!good) break;
-            uint8_t* to = stages + (size_t)s * O::kStage;
+            uint8_t* to = stages + (size_t)s * O::kStage + (C::kWide ? kTile : 0);
             const uint32_t bar = full0 + 8 * s;
-            const int k = kb * kBlock;
             if (rank == 0) tc::mbar_arrive_expect_tx(&full[s], bytes);
-            if (C::kWide) {
-              load_w<PAIR>(to + kTile, &wmap, bar, k, row, w.e);
-              if (!PAIR) load_w<PAIR>(to + 2 * kTile, &wmap, bar, k, row + kBlock, w.e);
-              load_x<PAIR>(to, &xmap_full, bar, k, m0);
-            } else {
-              load_w<PAIR>(to, &wmap, bar, k, row, w.e);
-              if (boxes * kBox == C::kTokens)
-                load_x<PAIR>(to + kTile, &xmap_full, bar, k, m0);
-              else
-                for (int b = 0; b < boxes; ++b) load_x<PAIR>(to + kTile + b * (kBox * kBlock), &xmap, bar, k, m0 + b * kBox);
-            }
+            load_w<PAIR>(to, &wmap, bar, kb * kBlock, row, w.e);
+            if (C::kWeights / C::kCtas > 128) load_w<PAIR>(to + kTile, &wmap, bar, kb * kBlock, row + 128, w.e);
+            if (C::kWide) load_x<PAIR>(to - kTile, &xmap_full, bar, kb * kBlock, w.m0 + (int)rank * 128);
             ++issued;
             if (++s == kStages) s = 0, ph ^= 1u;
           }
+          // who shares the tile is needed last
+          if (w.g0 > 0 || w.g1 < a.groups) {
+            runs[at.at].c0 = walk.owner_of(w.t * a.groups);
+            runs[at.at].c1 = walk.owner_of(w.t * a.groups + a.groups - 1);
+          }
+          tc::mbar_arrive(&run_owners[at.at]);
         }
         if (!good) give_up();
         // every load lands before shared memory is released
         if (rank == 0)
           for (int64_t j = issued > kStages ? issued - kStages : 0; j < issued; ++j)
             wait(&full[j % kStages], (uint32_t)((j / kStages) & 1), a, nullptr);
+      }
+    } else if (!C::kWide && warp == C::kXWarp) {
+      // ---------------- the loads of tokens: on the same barriers, which the weights' loads give the bytes of both ----------------
+      if (lane == 0) {
+        int s = 0;
+        uint32_t ph = 1;
+        const uint32_t full0 = tc::smem_u32(full);
+        bool good = true;
+        for (Runs at; take(at, good); at.next()) {
+          const Run w = runs[at.at];
+          tc::mbar_arrive(&run_empty[at.at]);
+          const int boxes = (w.n + kBox - 1) / kBox;
+          for (int kb = w.g0 * kGroup, end = min(a.kb, w.g1 * kGroup); kb < end; ++kb) {
+            good = wait(&empty[s], ph, a, abort_flag);
+            if (!good) break;
+            uint8_t* to = stages + (size_t)s * O::kStage + kTile;
+            const uint32_t bar = full0 + 8 * s;
+            if (boxes * kBox == C::kTokens)
+              load_x<PAIR>(to, &xmap_full, bar, kb * kBlock, w.m0);
+            else
+              for (int b = 0; b < boxes; ++b) load_x<PAIR>(to + b * (kBox * kBlock), &xmap, bar, kb * kBlock, w.m0 + b * kBox);
+            if (++s == kStages) s = 0, ph ^= 1u;
+          }
+        }
+        if (!good) give_up();
       }
     } else if (warp == 1 || warp == 3) {
       // ---------------- MMA: the issuers take the blocks in turn; a group's accumulators are done when both have committed ----------------
@@ -505,22 +529,25 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
         for (Runs at; take(at, good); at.next()) {
           const Run w = runs[at.at];
           tc::mbar_arrive(&run_empty[at.at]);
-          const uint32_t id = C::kWide ? idesc_f8(128 * C::kCtas, 256) : idesc_f8(128, (w.n + 15) / 16 * 16);
+          const uint32_t id = C::kWide ? idesc_f8(128 * C::kCtas, C::kWeights) : idesc_f8(128, (w.n + 15) / 16 * 16);
           const int end = min(a.kb, w.g1 * kGroup);
           for (int kb = w.g0 * kGroup; kb < end && good; kb += kGroup) {
-            if (kGroup > 1 || mine) good = wait(&d_empty[d], dph, a, abort_flag);
+            if (kGroup > 1) good = wait(&d_empty[d], dph, a, abort_flag);
 #pragma unroll 1
             for (int j = 0; j < kGroup && kb + j < end && good; ++j, mine = !mine) {
               if (mine) {
+                // the operands first: they are there before the slot is free, which the next block's time hangs on
                 good = wait(&full[s], ph, a, abort_flag);
                 if (!good) break;
-                tc::fence_after_sync();
                 const uint32_t stage = tc::smem_u32(stages) + s * O::kStage;
                 const uint64_t ad = tc::sdesc_kmajor_sw128(stage), bd = tc::sdesc_kmajor_sw128(stage + kTile);
+                if (kGroup == 1) good = wait(&d_empty[d], dph, a, abort_flag);
+                if (!good) break;
+                tc::fence_after_sync();
 #pragma unroll
                 for (int i = 0; i < kBlock / 32; ++i) mma_f8<PAIR>(tmem + d * O::kDSlot + j * C::kDBlock, ad + 2 * i, bd + 2 * i, id, i > 0);
-                commit<PAIR>(&empty[s]);
                 if (kGroup == 1) commit<PAIR>(&d_full[d]);
+                commit<PAIR>(&empty[s]);
               }
               if (++s == kStages) s = 0, ph ^= 1u;
             }
@@ -532,95 +559,74 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
         commit<PAIR>(drain);
         wait(drain, 0, a, nullptr);
       }
-    } else if (warp == 2 && !C::kWide) {
-      // ---------------- scales: x's times the weight's, four blocks of a run at a time, the next four's loads on their way ----------------
-      constexpr int kEach = C::kTokens / 32;
-      float xs[2][4][kEach], ws[2];
-      int cnt[2], n[2], kb = 0, end = 0;
-      Run w;
-      Runs at;
-      bool good = true, more = true;
-      auto load = [&](int h) {
-        cnt[h] = 0;
-        if (kb >= end && more) {
-          more = __all_sync(0xffffffffu, take(at, good));
-          if (more) {
-            w = runs[at.at];
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&run_empty[at.at]);
-            at.next();
-            kb = w.g0 * kGroup, end = min(a.kb, w.g1 * kGroup);
-          }
-        }
-        if (more) {
-          cnt[h] = min(4, end - kb), n[h] = w.n;
-          ws[h] = lane < cnt[h] ? a.ws[((int64_t)w.e * a.nb + w.tb) * a.kb + kb + lane] : 0.f;
-          const float* from = a.xs + (w.m0 + lane) * a.xs_m + kb * a.xs_b;
-#pragma unroll
-          for (int c = 0; c < kEach; ++c)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) xs[h][j][c] = c * 32 + lane < w.n && j < cnt[h] ? from[c * 32 * a.xs_m + j * a.xs_b] : 0.f;
-          kb += 4;
-        }
-      };
-      int q = 0;
-      uint32_t ph = 1;
-      auto store = [&](int h) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j >= cnt[h]) break;
-          if (j % kGroup == 0) good = __all_sync(0xffffffffu, wait(&sc_empty[q], ph, a, abort_flag));
-          if (!good) break;
-          const float f = __shfl_sync(0xffffffffu, ws[h], j);
-#pragma unroll
-          for (int c = 0; c < kEach; ++c)
-            if (c * 32 < n[h]) sc[q * C::kScSlot + j % kGroup * C::kTokens + c * 32 + lane] = xs[h][j][c] * f;
-          if (j % kGroup == kGroup - 1 || j + 1 == cnt[h]) {
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&sc_full[q]);
-            if (++q == kScRing) q = 0, ph ^= 1u;
-          }
-        }
-      };
-      load(0);
-      while (cnt[0] > 0 && good) {
-        load(1);
-        store(0);
-        if (cnt[1] == 0 || !good) break;
-        load(0);
-        store(1);
-      }
-      if (!good) give_up();
-    } else if (warp == C::kRunsWarp) {
-      // ---------------- runs ----------------
-      if (lane == 0) {
-        Walk<C> w(a, start, begin, blockIdx.x / C::kCtas, gridDim.x / C::kCtas);
+    } else if (warp == 2) {
+      if constexpr (C::kFactors > 0) {
+        // ---------------- factors: x's scales times the weights', four blocks of a run at a time, the next four's loads on their way ----------------
+        constexpr int kEach = C::kFactors / 32;
+        float xs[2][4][kEach], ws[2];
+        int cnt[2], n[2], kb = 0, end = 0;
+        Run w;
         Runs at;
-        bool good = true;
-        for (bool more = true; more; at.next()) {
-          more = w.next();  // the run without groups is handed over too
-          good = wait(&run_empty[at.at], at.phase ^ 1u, a, abort_flag);
-          if (!good) break;
-          runs[at.at] = w.r;
-          tc::mbar_arrive(&run_full[at.at]);
-          if (w.r.g0 > 0 || w.r.g1 < a.groups) {  // who shares the tile is needed last
-            runs[at.at].c0 = w.owner_of(w.r.t * a.groups);
-            runs[at.at].c1 = w.owner_of(w.r.t * a.groups + a.groups - 1);
+        bool good = true, more = true;
+        auto load = [&](int h) {
+          cnt[h] = 0;
+          if (kb >= end && more) {
+            more = __all_sync(0xffffffffu, take(at, good));
+            if (more) {
+              w = runs[at.at];
+              __syncwarp();
+              if (lane == 0) tc::mbar_arrive(&run_empty[at.at]);
+              at.next();
+              kb = w.g0 * kGroup, end = min(a.kb, w.g1 * kGroup);
+            }
           }
-          tc::mbar_arrive(&run_owners[at.at]);
-          w.passed();
+          if (more) {
+            cnt[h] = min(4, end - kb), n[h] = w.n;
+            ws[h] = lane < cnt[h] ? a.ws[((int64_t)w.e * a.nb + w.tb) * a.kb + kb + lane] : 0.f;
+            const float* from = a.xs + (w.m0 + lane) * a.xs_m + kb * a.xs_b;
+  #pragma unroll
+            for (int c = 0; c < kEach; ++c)
+  #pragma unroll
+              for (int j = 0; j < 4; ++j) xs[h][j][c] = c * 32 + lane < w.n && j < cnt[h] ? from[c * 32 * a.xs_m + j * a.xs_b] : 0.f;
+            kb += 4;
+          }
+        };
+        int q = 0;
+        uint32_t ph = 1;
+        auto store = [&](int h) {
+          good = __all_sync(0xffffffffu, wait(&sc_empty[q], ph, a, abort_flag));
+          if (!good) return;
+  #pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float f = __shfl_sync(0xffffffffu, ws[h], j);
+            float* to = sc + q * O::kScSlot + j * C::kFactors + lane;
+  #pragma unroll
+            for (int c = 0; c < kEach; ++c)
+              if (c * 32 < n[h]) to[c * 32] = xs[h][j][c] * f;
+          }
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&sc_full[q]);
+          if (++q == kScRing) q = 0, ph ^= 1u;
+        };
+        load(0);
+        while (cnt[0] > 0 && good) {
+          load(1);
+          store(0);
+          if (cnt[1] == 0 || !good) break;
+          load(0);
+          store(1);
         }
         if (!good) give_up();
       }
     }
   } else {
     // ---------------- sums: lanes 32 (warp % 4) .. of tensor memory ----------------
-    if (C::kWide) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (C::kSums > 64) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int quarter = warp & 3, part = (warp - C::kEpi0) >> 2, thread = threadIdx.x - 32 * C::kEpi0, row = quarter * 32 + lane;
     const uint32_t d_empty0 = PAIR ? in_leader(d_empty) : 0;
     const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + kSums * part;
     float sum[kSums];
-    uint32_t v[2][C::kWide ? 16 : 32];
+    uint32_t v[2][32];
     int d = 0, q = 0;
     uint32_t dph = 0, qph = 0, joined = 0;
     bool good = true;
@@ -645,51 +651,49 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
       const volatile Run& w = runs[at.at];  // kept until the tile is written: read where it is needed, not held in registers
       const int first = w.g0 * kGroup, end = min(a.kb, w.g1 * kGroup);
       if constexpr (C::kWide) {
-        // The thread's row is a token, its columns 128 weight rows with one scale. A token behind the group's last one goes by the last one's
-        // scale, a block of weights behind the last by the last's; neither is written.
-        const int nb = min(w.tb * 2 + part, a.nb - 1), m = w.m0 + min((int)rank * 128 + row, w.n - 1);
+        // The thread's row is a token, its columns weight rows with one scale, so a block has one factor for it. A token behind the group's last one
+        // goes by the last one's scale, a block of weights behind the last by the last's; neither is written.
+        const int nb = min(w.tb * (C::kWeights / kBlock) + part * kSums / kBlock, a.nb - 1), m = w.m0 + min((int)rank * 128 + row, w.n - 1);
         const float* xs = a.xs + m * a.xs_m + first * a.xs_b;
         const float* ws = a.ws + ((int64_t)w.e * a.nb + nb) * a.kb + first;
-        constexpr int kAhead = 4;  // blocks whose scales are on their way
-        float xs_next[kAhead], ws_next[kAhead];
+        float xs_next[2], ws_next[2];  // two blocks' scales on their way
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
+        for (int j = 0; j < 2; ++j) {
           xs_next[j] = first + j < end ? xs[j * a.xs_b] : 0.f;
           ws_next[j] = first + j < end ? ws[j] : 0.f;
         }
         accumulators();
         if (!good) break;
-        // Two sets of 16 columns at a time; the next ones' loads run beside the sums, the next block's too. (Sets of 32 left too few
-        // registers for the 128 sums: 574 against 562 us for 8192 rows by 8192 x 8192 weights; packed fma.rn.f32x2 needs its operands moved: 565.)
-        load16(from + d * O::kDSlot, v[0]);
-        load16(from + d * O::kDSlot + 16, v[1]);
+        // Two sets of 32 columns at a time, whose successors' loads run beside the sums. A slot is free as soon as its last loads are
+        // done: a later block's MMA waits for that.
+        load32(from + d * O::kDSlot, v[0]);
+        load32(from + d * O::kDSlot + 32, v[1]);
         for (int kb = first; kb < end; ++kb) {
           const float f = xs_next[0] * ws_next[0];
-#pragma unroll
-          for (int j = 0; j + 1 < kAhead; ++j) xs_next[j] = xs_next[j + 1], ws_next[j] = ws_next[j + 1];
-          if (kb + kAhead < end) xs_next[kAhead - 1] = xs[kAhead * a.xs_b], ws_next[kAhead - 1] = ws[kAhead];
+          xs_next[0] = xs_next[1], ws_next[0] = ws_next[1];
+          if (kb + 2 < end) xs_next[1] = xs[2 * a.xs_b], ws_next[1] = ws[2];
           xs += a.xs_b, ++ws;
           const uint32_t in = from + d * O::kDSlot;
 #pragma unroll
-          for (int c = 0; c < kSums; c += 32) {
-            const bool last = c + 32 == kSums;
+          for (int c = 0; c < kSums; c += 64) {
+            const bool last = c + 64 == kSums;
             wait_loads();
             if (last) free_accumulators();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) fma_after(sum[c + j], v[0][j], f);
+            for (int j = 0; j < 32; ++j) fma_after(sum[c + j], v[0][j], f);
             if (!last) {
-              load16(in + c + 32, v[0]);
+              load32(in + c + 64, v[0]);
             } else if (kb + 1 < end) {
               accumulators();
               if (!good) break;
-              load16(from + d * O::kDSlot, v[0]);
+              load32(from + d * O::kDSlot, v[0]);
             }
 #pragma unroll
-            for (int j = 0; j < 16; ++j) fma_after(sum[c + 16 + j], v[1][j], f);
+            for (int j = 0; j < 32; ++j) fma_after(sum[c + 32 + j], v[1][j], f);
             if (!last)
-              load16(in + c + 48, v[1]);
+              load32(in + c + 96, v[1]);
             else if (kb + 1 < end)
-              load16(from + d * O::kDSlot + 16, v[1]);
+              load32(from + d * O::kDSlot + 32, v[1]);
           }
           if (!good) break;
         }
@@ -700,32 +704,24 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
           if (!good) break;
           good = __all_sync(0xffffffffu, wait(&sc_full[q], qph, a, abort_flag));
           if (!good) break;
-          const uint32_t f = tc::smem_u32(sc + q * C::kScSlot + kSums * part);
-          auto add = [&](int j, int c, const uint32_t(&x)[32]) {  // block j's columns c to c + 31
+          const uint32_t f = tc::smem_u32(sc + q * O::kScSlot + kSums * part);
+          auto add = [&](int j, const uint32_t(&x)[32]) {  // block j's
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              const float4 f4 = shared4(f + (j * C::kTokens + c + i) * 4);
-              fma_after(sum[c + i], x[i], f4.x), fma_after(sum[c + i + 1], x[i + 1], f4.y);
-              fma_after(sum[c + i + 2], x[i + 2], f4.z), fma_after(sum[c + i + 3], x[i + 3], f4.w);
+              const float4 f4 = shared4(f + (j * C::kFactors + i) * 4);
+              fma_after(sum[i], x[i], f4.x), fma_after(sum[i + 1], x[i + 1], f4.y);
+              fma_after(sum[i + 2], x[i + 2], f4.z), fma_after(sum[i + 3], x[i + 3], f4.w);
             }
           };
           const uint32_t in = from + d * O::kDSlot;
 #pragma unroll
-          for (int j = 0; j < kGroup; j += kSums > 32 ? 1 : 2) {
+          for (int j = 0; j < kGroup; j += 2) {
             if (kb + j >= end) break;
-            if constexpr (kSums > 32) {
-              load32(in + j * C::kDBlock, v[0]);
-              load32(in + j * C::kDBlock + 32, v[1]);
-              wait_loads();
-              add(j, 0, v[0]);
-              add(j, 32, v[1]);
-            } else {
-              load32(in + j * C::kDBlock, v[0]);
-              if (kb + j + 1 < end) load32(in + (j + 1) * C::kDBlock, v[1]);
-              wait_loads();
-              add(j, 0, v[0]);
-              if (kb + j + 1 < end) add(j + 1, 0, v[1]);
-            }
+            load32(in + j * C::kDBlock, v[0]);
+            if (kb + j + 1 < end) load32(in + (j + 1) * C::kDBlock, v[1]);
+            wait_loads();
+            add(j, v[0]);
+            if (kb + j + 1 < end) add(j + 1, v[1]);
           }
           free_accumulators();
           if (lane == 0) tc::mbar_arrive(&sc_empty[q]);  // free_accumulators synchronised the warp
@@ -736,7 +732,8 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
 
       bool write = true;
       if (w.g0 > 0 || w.g1 < a.groups) {
-        // A part of a tile: published, and whichever owner comes last adds the parts in the order of the owners.
+        // A part of a tile: published, and whichever owner comes last adds the parts in the order of the owners, its own among them, so that
+        // the sums do not depend on who that is.
         good = __all_sync(0xffffffffu, wait(&run_owners[at.at], at.phase, a, abort_flag));
         if (!good) break;
         const int c0 = w.c0, c1 = w.c1, owner = blockIdx.x / C::kCtas;
@@ -775,10 +772,9 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
 #pragma unroll
           for (int j = 0; j < kSums; j += kAt) {
             float x[kAt];
-            fetch(c0, j, x);
 #pragma unroll
-            for (int i = 0; i < kAt; ++i) sum[j + i] = x[i];
-            for (int p = c0 + 1; p <= c1; ++p) {
+            for (int i = 0; i < kAt; ++i) sum[j + i] = 0.f;
+            for (int p = c0; p <= c1; ++p) {
               fetch(p, j, x);
 #pragma unroll
               for (int i = 0; i < kAt; ++i) sum[j + i] += x[i];
@@ -790,22 +786,40 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
       if (!write) {
       } else if constexpr (C::kWide) {
         const int token = (int)rank * 128 + row, col0 = w.tb * C::kWeights + kSums * part;
-        if (token < w.n) {
+        if (!a.wide_out || col0 + kSums > a.n) {
+          // Stores of single values would each touch 32 rows, so 16 columns at a time go through shared memory and a store is 16
+          // neighbours of each of two rows.
+          float* own = staged + (warp - C::kEpi0) * O::kStaged;
+          const int n = w.n - (token - lane) < 32 ? w.n - (token - lane) : 32;  // the warp's rows
+          const int64_t at = (int64_t)(w.m0 + token - lane) * a.out_stride;
+#pragma unroll
+          for (int c = 0; c < kSums; c += 16) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) own[lane * 17 + i] = sum[c + i];
+            __syncwarp();
+            const int col = col0 + c + (lane & 15);
+#pragma unroll 4
+            for (int r = lane >> 4; r < n; r += 2) {
+              if (col >= a.n) break;
+              const float v = own[r * 17 + (lane & 15)];
+              const int64_t to = at + r * a.out_stride + col;
+              if (a.out_dtype == UP_EK_F32)
+                static_cast<float*>(a.out)[to] = v;
+              else
+                static_cast<uint16_t*>(a.out)[to] = (uint16_t)half_pair(v, 0.f, bf16);
+            }
+          }
+        } else if (token < w.n) {
           const int64_t at = (int64_t)(w.m0 + token) * a.out_stride + col0;
           if (a.out_dtype == UP_EK_F32) {
             float* to = static_cast<float*>(a.out) + at;
 #pragma unroll
             for (int j = 0; j < kSums; j += 8) {
-              if (a.wide_out && col0 + j + 8 <= a.n) {
-                uint32_t r[8];
+              uint32_t r[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(sum[j + i]);
-                store32(to + j, r);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  if (col0 + j + i < a.n) to[j + i] = sum[j + i];
-              }
+              for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(sum[j + i]);
+              store32(to + j, r);
             }
           } else {
             uint16_t* to = static_cast<uint16_t*>(a.out) + at;
@@ -814,13 +828,7 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
               uint32_t r[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) r[i] = half_pair(sum[j + 2 * i], sum[j + 2 * i + 1], bf16);
-              if (a.wide_out && col0 + j + 16 <= a.n) {
-                store32(to + j, r);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  if (col0 + j + i < a.n) to[j + i] = (uint16_t)(r[i >> 1] >> (16 * (i & 1)));
-              }
+              store32(to + j, r);
             }
           }
         }
@@ -860,37 +868,50 @@ __global__ void __launch_bounds__(Of<C>::kThreads, 1)
                   const __grid_constant__ CUtensorMap xmap_full, const __grid_constant__ Args a) {
   matmul<C>(wmap, xmap, xmap_full, a);
 }
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Of<Wide<2>>::kThreads, 1)
+template <typename C>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Of<C>::kThreads, 1)
     matmul_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                        const __grid_constant__ CUtensorMap xmap_full, const __grid_constant__ Args a) {
-  matmul<Wide<2>>(wmap, xmap, xmap_full, a);
+  matmul<C>(wmap, xmap, xmap_full, a);
 }
 
 // ---- host side ----
 // One CTA an SM.
 static int cta_count() { return sm_count() < kMaxCtas ? sm_count() : kMaxCtas; }
 
-enum Form { kNarrow32, kNarrow64, kWide, kPair };
+enum Form { kNarrow, kWide256, kPair256, kWide128 };
 
-// The form that takes the least time by a model of what was measured: a fixed part (launch, first loads, joining of parts) and so many
-// microseconds a block of an owner's tile, fitted to calls of 1 to 2048 rows by 1024 x 8192 to 28672 x 8192 weights. Measured, us,
-// Narrow<32>, Narrow<64>, Wide<1>, Wide<2>: by 8192 x 8192 weights 1 row 21, 23, 28, 37; 64 rows 27, 24, 29, 37; 128 rows 40, 31, 29, 37; 256
-// rows 72, 47, 40, 39; 2048 rows 501, 281, 151, 143. 128 experts of 4096 x 2048: 512 rows 162, 181, 171, 266; 8192 rows 439, 316, 213, 333;
-// 65536 rows 2327, 1685, 749, 784.
+// The form that takes the least time by a model: a fixed part (launch, first loads, output), then so many microseconds for each block of k of
+// the tiles of one owner, which Walk deals out. Fitted to 78 calls of 1 to 65536 rows, dense and by expert, by 512 x 1024 to 28672 x 8192
+// weights; the choice takes 0.6 % longer than the fastest form in the mean. Without one of the forms calls take 2 % longer in the mean, up to 30 %
+// where that one is the fastest. (A form of 64 tokens as columns was the fastest by 4 to 12 % for some calls of 64 to 256 rows, by
+// 0.2 % in the mean.) Measured, us, in the order of the table:
+//   rows by 2048 x 1024 weights:   1: 6.7, 8.4, 9.1, 6.4;     512: 9.2, 10.6, 11.2, 7.7;    8192: 68, 32, 31, 31
+//   rows by 8192 x 8192 weights:   1: 19.9, 26.9, 36.1, 30.1; 128: 34.4, 28.9, 35.1, 24.3;  512: 103, 40.8, 40.1, 50.8;  8192: 1561, 569, 538, 872
+//   128 experts' 4096 x 2048:      512: 149, 168, 244, 180;   8192: 303, 202, 302, 266;     65536: 1749, 714, 739, 872
 static Form form_of(int64_t m, int64_t experts, int64_t n, int64_t kb) {
   struct Cost {
-    int tokens, weights, ctas;  // of a tile
+    int tokens, weights, ctas, least, join;  // of a tile; Walk's
     double fixed, block;
   };
-  static const Cost cost[4] = {{32, 128, 1, 10.5, 0.275}, {64, 128, 1, 13, 0.30}, {128, 256, 1, 20, 0.59}, {256, 256, 2, 20, 0.56}};
+  static const Cost cost[4] = {{Narrow::kTokens, Narrow::kWeights, 1, Narrow::kMinBlocks, Narrow::kJoinBlocks, 1.7, 0.269},
+                               {128, 256, 1, Wide<1, 256>::kMinBlocks, Wide<1, 256>::kJoinBlocks, 3.1, 0.648},
+                               {256, 256, 2, Wide<2, 256>::kMinBlocks, Wide<2, 256>::kJoinBlocks, 4.6, 0.603},
+                               {128, 128, 1, Wide<1, 128>::kMinBlocks, Wide<1, 128>::kJoinBlocks, 1.7, 0.457}};
   const double used = (double)(m < experts ? m : experts), per = m / used;  // experts that have rows, at most; rows of each
   int best = 0;
   double least = 0;
   for (int i = 0; i < 4; ++i) {
     const Cost& c = cost[i];
+    const int owners = cta_count() / c.ctas;
     // a ragged group's last tile is half full in the mean
-    const double tiles = experts == 1 ? (double)((m + c.tokens - 1) / c.tokens) : per / c.tokens + 0.5 > 1 ? per / c.tokens + 0.5 : 1;
-    const double us = c.fixed + c.block * tiles * used * (double)((n + c.weights - 1) / c.weights) * (double)kb * c.ctas / cta_count();
+    const double wide = experts == 1 ? (double)((m + c.tokens - 1) / c.tokens) : per / c.tokens + 0.5 > 1 ? per / c.tokens + 0.5 : 1;
+    const double tiles = wide * used * (double)((n + c.weights - 1) / c.weights), rounds = floor(tiles / owners), rest = tiles - rounds * owners;
+    const double shares = rest * kb / c.least < owners ? rest * kb / c.least : owners;
+    const double blocks = rest == 0                                ? 0
+                          : kb * (shares - rest) <= c.join * shares ? (double)kb
+                                                                    : kb * rest / shares + c.join;
+    const double us = c.fixed + c.block * (rounds * kb + blocks);
     if (i == 0 || us < least) best = i, least = us;
   }
   return (Form)best;
@@ -931,7 +952,7 @@ static int launch(K kernel, unsigned grid, Args& a, const Operands& o, cudaStrea
   a.by_groups = Divide32(a.groups), a.by_owners = Divide32(grid / C::kCtas);
   a.tb = (a.nb + C::kWeights / kBlock - 1) / (C::kWeights / kBlock);
   CUtensorMap wmap, xmap, xmap_full;
-  if (!encode(&wmap, o.w, 3, o.k, o.n, o.experts, o.k, kBlock) || !encode(&xmap, o.x, 2, o.k, o.m, 1, o.x_stride, kBox) ||
+  if (!encode(&wmap, o.w, 3, o.k, o.n, o.experts, o.k, 128) || !encode(&xmap, o.x, 2, o.k, o.m, 1, o.x_stride, kBox) ||
       !encode(&xmap_full, o.x, 2, o.k, o.m, 1, o.x_stride, C::kTokens / C::kCtas))
     return fail_with(UP_ERR_CUDA, "cuTensorMapEncodeTiled refused an operand's tensor map");
   const cudaError_t e = ensure_smem_attr((const void*)kernel, Of<C>::kSmem);
@@ -950,7 +971,7 @@ using namespace up::f8;
 
 extern "C" size_t up_sm100_f8_matmul_workspace_bytes(int64_t m, int64_t experts, int64_t n, int64_t k) {
   if (m <= 0 || experts <= 0 || n <= 0 || k <= 0) return UP_F8_COUNTER_BYTES;
-  return UP_F8_COUNTER_BYTES + (size_t)cta_count() * 2 * Of<Wide<1>>::kPart * sizeof(float);
+  return UP_F8_COUNTER_BYTES + (size_t)cta_count() * 2 * Of<Wide<1, 256>>::kPart * sizeof(float);
 }
 
 extern "C" int up_sm100_f8_matmul(const uint8_t* x, int64_t m, int64_t x_stride, const float* x_scale, int64_t xs_stride_m,
@@ -976,23 +997,24 @@ extern "C" int up_sm100_f8_matmul(const uint8_t* x, int64_t m, int64_t x_stride,
   Args a{};
   a.xs = x_scale, a.ws = w_scale, a.xs_m = xs_stride_m, a.xs_b = xs_stride_b, a.m = m, a.experts = (int)experts, a.n = (int)n;
   a.kb = (int)kb, a.nb = (int)nb, a.offsets = offsets, a.out = out, a.out_stride = out_stride;
-  a.out_dtype = out_dtype, a.wide_out = out_stride % (out_dtype == UP_EK_F32 ? 8 : 16) == 0 && aligned(out, 32), a.header = static_cast<Header*>(workspace);
+  a.out_dtype = out_dtype, a.wide_out = out_stride % (out_dtype == UP_EK_F32 ? 8 : 16) == 0 && aligned(out, 32);
+  a.header = static_cast<Header*>(workspace);
   a.counters = reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + sizeof(Header));
   a.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + UP_F8_COUNTER_BYTES);
   a.wait_ns = wait_limit_ns();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (form_of(m, experts, n, kb)) {
-    case kPair: return launch<Wide<2>>(matmul_pair_kernel, (unsigned)(cta_count() & ~1), a, o, s);
-    case kWide: return launch<Wide<1>>(matmul_kernel<Wide<1>>, (unsigned)cta_count(), a, o, s);
-    case kNarrow64: return launch<Narrow<64>>(matmul_kernel<Narrow<64>>, (unsigned)cta_count(), a, o, s);
-    default: return launch<Narrow<32>>(matmul_kernel<Narrow<32>>, (unsigned)cta_count(), a, o, s);
+    case kWide256: return launch<Wide<1, 256>>(matmul_kernel<Wide<1, 256>>, (unsigned)cta_count(), a, o, s);
+    case kPair256: return launch<Wide<2, 256>>(matmul_pair_kernel<Wide<2, 256>>, (unsigned)(cta_count() & ~1), a, o, s);
+    case kWide128: return launch<Wide<1, 128>>(matmul_kernel<Wide<1, 128>>, (unsigned)cta_count(), a, o, s);
+    default: return launch<Narrow>(matmul_kernel<Narrow>, (unsigned)cta_count(), a, o, s);
   }
 }
 
 namespace up {
 size_t f8_matmul_smem_bytes() {  // for the kernel interface: the largest form's
   size_t most = 0;
-  for (const size_t n : {(size_t)Of<Narrow<32>>::kSmem, (size_t)Of<Narrow<64>>::kSmem, (size_t)Of<Wide<1>>::kSmem, (size_t)Of<Wide<2>>::kSmem})
+  for (const size_t n : {(size_t)Of<Narrow>::kSmem, (size_t)Of<Wide<1, 256>>::kSmem, (size_t)Of<Wide<2, 256>>::kSmem, (size_t)Of<Wide<1, 128>>::kSmem})
     most = n > most ? n : most;
   return most;
 }
