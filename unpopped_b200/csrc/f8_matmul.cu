@@ -334,12 +334,16 @@ __device__ __forceinline__ float4 shared4(uint32_t at) {
 template <typename C>
 __device__ __forceinline__ void schedule(const Args& a, int* start, int* begin, int lane) {
   constexpr int kTokens = C::kTokens;
+  if (a.offsets == nullptr) {  // one matrix and all rows
+    if (lane == 0) start[0] = begin[0] = 0, start[1] = (int)((a.m + kTokens - 1) / kTokens) * a.tb, begin[1] = (int)a.m;
+    return;
+  }
   int run_tiles = 0, run_row = 0;
   for (int e0 = 0; e0 <= a.experts; e0 += 32) {
     const int e = e0 + lane;
     int row = 0;
     if (e <= a.experts) {
-      const int64_t o = a.offsets ? (int64_t)a.offsets[e] : (e == 0 ? 0 : a.m);
+      const int64_t o = a.offsets[e];
       row = (int)(o < 0 ? 0 : o > a.m ? a.m : o);
     }
 #pragma unroll
@@ -425,16 +429,19 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
   } else if (warp == 1) {
     tmem_alloc<PAIR>(tmem_slot);
   } else if (warp == 2) {
-    after_previous();
+    if (a.offsets) after_previous();
     schedule<C>(a, start, begin, lane);
   }
-  after_previous();
+  // Nothing of the launch before is read until here without offsets, and then the first runs are dealt out beside its end too. No wait with a
+  // limit begins before that.
+  if (a.offsets) after_previous();
   let_next_begin();
   tc::fence_before_sync();
   __syncthreads();
   if (PAIR) cluster_sync();
   tc::fence_after_sync();
   const uint32_t tmem = *tmem_slot;
+  if (a.offsets == nullptr && warp > 0) after_previous();
 
   auto give_up = [&]() {
     *abort_flag = 1;
@@ -466,6 +473,7 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
           runs[at.at] = w;
           tc::mbar_arrive(&run_full[at.at]);
           walk.passed();
+          if (issued == 0 && a.offsets == nullptr) after_previous();
           const int boxes = (w.n + kBox - 1) / kBox;
           const uint32_t bytes = C::kWide ? C::kCtas * O::kStage : kTile + boxes * (kBox * kBlock);
           const int row = w.tb * C::kWeights + (int)rank * (C::kWeights / C::kCtas);
@@ -740,7 +748,10 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
         float* parts = a.partials + thread;
         float* to = parts + ((size_t)blockIdx.x * 2 + (c0 == owner ? 1 : 0)) * O::kPart;
 #pragma unroll
-        for (int j = 0; j < kSums; ++j) __stcg(to + j * O::kEpiThreads, sum[j]);
+        for (int j = 0; j < kSums; ++j) {
+          if (!C::kWide && j % C::kStep == 0 && j >= w.n) break;  // columns of no token
+          __stcg(to + j * O::kEpiThreads, sum[j]);
+        }
         __syncwarp();
         const uint32_t jp = joined & 1u;
         ++joined;
@@ -762,7 +773,7 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
         if (!good) break;
         write = *verdict != 0u;
         if (write) {
-          constexpr int kAt = kSums < 64 ? kSums : 64;  // values in flight
+          constexpr int kAt = C::kWide ? 64 : C::kStep;  // values of a part in flight
           const float* in = parts + (size_t)rank * 2 * O::kPart;
           auto fetch = [&](int p, int j, float(&x)[kAt]) {
             const float* of = in + ((size_t)p * C::kCtas * 2 + (p == c0 ? 1 : 0)) * O::kPart + j * O::kEpiThreads;
@@ -771,13 +782,28 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
           };
 #pragma unroll
           for (int j = 0; j < kSums; j += kAt) {
-            float x[kAt];
 #pragma unroll
             for (int i = 0; i < kAt; ++i) sum[j + i] = 0.f;
-            for (int p = c0; p <= c1; ++p) {
-              fetch(p, j, x);
+            if constexpr (C::kWide) {
+              for (int p = c0; p <= c1; ++p) {
+                float x[kAt];
+                fetch(p, j, x);
 #pragma unroll
-              for (int i = 0; i < kAt; ++i) sum[j + i] += x[i];
+                for (int i = 0; i < kAt; ++i) sum[j + i] += x[i];
+              }
+            } else {
+              if (j >= w.n) break;
+              float x[2][kAt];  // the next part's are on their way beside a part's sums
+              fetch(c0, j, x[0]);
+              for (int p = c0; p <= c1; p += 2) {
+                if (p + 1 <= c1) fetch(p + 1, j, x[1]);
+#pragma unroll
+                for (int i = 0; i < kAt; ++i) sum[j + i] += x[0][i];
+                if (p + 1 > c1) break;
+                if (p + 2 <= c1) fetch(p + 2, j, x[0]);
+#pragma unroll
+                for (int i = 0; i < kAt; ++i) sum[j + i] += x[1][i];
+              }
             }
           }
         }
@@ -839,13 +865,17 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
           if (a.out_dtype == UP_EK_F32) {
             float* to = static_cast<float*>(a.out) + at;
 #pragma unroll
-            for (int j = 0; j < kSums; ++j, to += a.out_stride)
-              if (j < n) *to = sum[j];
+            for (int j = 0; j < kSums; ++j, to += a.out_stride) {
+              if (j >= n) break;
+              *to = sum[j];
+            }
           } else {
             uint16_t* to = static_cast<uint16_t*>(a.out) + at;
 #pragma unroll
-            for (int j = 0; j < kSums; ++j, to += a.out_stride)
-              if (j < n) *to = half_bits(sum[j], bf16);
+            for (int j = 0; j < kSums; ++j, to += a.out_stride) {
+              if (j >= n) break;
+              *to = half_bits(sum[j], bf16);
+            }
           }
         }
       }
