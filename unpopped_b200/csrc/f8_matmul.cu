@@ -329,42 +329,37 @@ __device__ __forceinline__ float4 shared4(uint32_t at) {
   return f;
 }
 
-// The schedule: begin[e] (rows) and start[e] (tiles) of every expert, from the offsets on the device; each entry is held to
-// [0, m] and to its predecessors. One warp.
+// The schedule: begin[e] (rows) and start[e] (tiles) of every expert, from the offsets on the device, which all threads have put into
+// `begin` held to [0, m]; each entry is held to its predecessors. One warp, a lane with some experts that follow one another: one scan
+// of the lanes for the rows and one for the tiles.
 template <typename C>
 __device__ __forceinline__ void schedule(const Args& a, int* start, int* begin, int lane) {
   constexpr int kTokens = C::kTokens;
-  if (a.offsets == nullptr) {  // one matrix and all rows
-    if (lane == 0) start[0] = begin[0] = 0, start[1] = (int)((a.m + kTokens - 1) / kTokens) * a.tb, begin[1] = (int)a.m;
-    return;
-  }
-  int run_tiles = 0, run_row = 0;
-  for (int e0 = 0; e0 <= a.experts; e0 += 32) {
-    const int e = e0 + lane;
-    int row = 0;
-    if (e <= a.experts) {
-      const int64_t o = a.offsets[e];
-      row = (int)(o < 0 ? 0 : o > a.m ? a.m : o);
-    }
+  const int each = (a.experts + 32) / 32, e0 = min(lane * each, a.experts + 1), e1 = min(e0 + each, a.experts + 1);
+  int most = 0;
+  for (int e = e0; e < e1; ++e) most = max(most, begin[e]);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, row, o);
-      if (lane >= o) row = max(row, v);
-    }
-    row = max(row, run_row);
-    int before = __shfl_up_sync(0xffffffffu, row, 1);  // begin[e - 1]
-    if (lane == 0) before = run_row;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, most, o);
+    if (lane >= o) most = max(most, v);
+  }
+  int row = __shfl_up_sync(0xffffffffu, most, 1);  // where the expert before this lane's first entry begins
+  if (lane == 0) row = 0;
+  int tiles = 0;
+  for (int e = e0; e < e1; ++e) {
+    const int before = row;
+    row = max(row, begin[e]);
     // tiles of expert e - 1, which ends where e begins
-    int tiles = e >= 1 && e <= a.experts ? (row - before + kTokens - 1) / kTokens * a.tb : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, tiles, o);
-      if (lane >= o) tiles += v;
-    }
-    if (e <= a.experts) begin[e] = row, start[e] = run_tiles + tiles;
-    run_row = __shfl_sync(0xffffffffu, row, 31);
-    run_tiles += __shfl_sync(0xffffffffu, tiles, 31);
+    if (e > 0) tiles += (row - before + kTokens - 1) / kTokens * a.tb;
+    begin[e] = row, start[e] = tiles;
   }
+  int all = tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, all, o);
+    if (lane >= o) all += v;
+  }
+  for (int e = e0; e < e1; ++e) start[e] += all - tiles;
 }
 
 __device__ __forceinline__ uint16_t half_bits(float v, bool bf16) {
@@ -428,13 +423,17 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
     }
   } else if (warp == 1) {
     tmem_alloc<PAIR>(tmem_slot);
-  } else if (warp == 2) {
-    if (a.offsets) after_previous();
-    schedule<C>(a, start, begin, lane);
   }
-  // Nothing of the launch before is read until here without offsets, and then the first runs are dealt out beside its end too. No wait with a
-  // limit begins before that.
-  if (a.offsets) after_previous();
+  // Without offsets nothing of the launch before is read until after the first runs are dealt out. No wait with a limit begins before its end.
+  if (a.offsets) {
+    after_previous();
+    for (int e = threadIdx.x; e <= a.experts; e += O::kThreads) begin[e] = (int)min((int64_t)max(a.offsets[e], 0), a.m);
+    __syncthreads();
+    if (warp == 2) schedule<C>(a, start, begin, lane);
+  } else if (threadIdx.x == 64) {  // one matrix and all rows
+    start[0] = begin[0] = 0, begin[1] = (int)a.m;
+    start[1] = (int)((a.m + C::kTokens - 1) / C::kTokens) * a.tb;
+  }
   let_next_begin();
   tc::fence_before_sync();
   __syncthreads();
