@@ -157,6 +157,30 @@ def test_combine_of_views_in_place_and_of_rows_that_are_left_out():
             ops.expert_combine(**a)
 
 
+def test_offsets_that_pass_32_bits():
+    """Logits and rows of more than 2^31 values."""
+    tokens, experts, k = 4300000, 512, 2
+    logits = torch.zeros(tokens, experts, device=DEV, dtype=torch.float16)
+    logits[:, 7] = -1
+    logits[-1, 500], logits[-2, 7] = 2, 3
+    ids, weights, rows, slots, offsets = ops.expert_route(logits, k)
+    del logits
+    assert bool((ids[:-2] == torch.tensor([0, 1], device=DEV)).all()) and ids[-2:].tolist() == [[7, 0], [500, 0]]
+    assert offsets[[0, 1, 2, 7, 8, 500, 501, 512]].tolist() == [0, tokens, 2 * tokens - 2, 2 * tokens - 2, 2 * tokens - 1, 2 * tokens - 1,
+                                                                2 * tokens, 2 * tokens]
+    assert slots[-2:].tolist() == [[2 * tokens - 2, tokens - 2], [2 * tokens - 1, tokens - 1]]
+    assert torch.equal(rows[:tokens], torch.arange(tokens, device=DEV, dtype=torch.int32)) and rows[-2:].tolist() == [tokens - 2, tokens - 1]
+    assert torch.equal(rows[slots.long()], torch.arange(tokens, device=DEV, dtype=torch.int32)[:, None].expand(tokens, k))
+    del ids, weights, rows, slots
+    g = gen(17)
+    y = torch.zeros(300000, 8192, device=DEV, dtype=torch.bfloat16)
+    y[-40:] = torch.randn(40, 8192, generator=g, device=DEV).bfloat16()
+    slots = torch.randint(299960, 300000, (9, 3), generator=g, device=DEV, dtype=torch.int32)
+    w = torch.rand(9, 3, generator=g, device=DEV)
+    got = ops.expert_combine(y, slots, w)
+    assert torch.equal(got, check_combine(y[-40:].clone(), slots - 299960, w))
+
+
 # ---- a layer ----
 def layer(x, router, up, up_s, down, down_s, k, add=None):
     ids, weights, rows, slots, offsets = ops.expert_route(torch.matmul(x.float(), router.t()), k)
