@@ -101,6 +101,28 @@ def test_quantise_with_a_gate(dtype, tokens, k):
     assert bool((off <= (v.abs() * 2.0 ** -4).clamp(min=2.0 ** -10) + v.abs() * 2.0 ** -18).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantise_with_a_gate_far_from_0(dtype):
+    """x down to -126, where exp(-x) leaves f32 or its reciprocal does, times u up to 1e37: silu(x) u is a plain number. The argument |x| / 2
+    of exp, times log2(e), is below 128: its rounding is 2^-18 at most and its factor's as much, e^ of them 2^-17 of exp, which counts twice."""
+    g = gen(41)
+    x = torch.empty(64, 256, device=DEV)
+    x[:, :128] = -126 * torch.rand(64, 1, generator=g, device=DEV) - torch.rand(64, 128, generator=g, device=DEV)
+    x[:32, :128] = torch.linspace(-100, -80, 128, device=DEV)
+    x[:, 128:] = torch.randn(64, 128, generator=g, device=DEV).sign() * (1 + torch.rand(64, 128, generator=g, device=DEV)) * 5e36
+    x = x.to(dtype)
+    q, s = ops.f8_quantise(x, gate=True)
+    d = x.double()
+    y = d[:, :128] * torch.sigmoid(d[:, :128]) * d[:, 128:]
+    want = y.abs().amax(1, keepdim=True) / 448
+    there = want >= 2.0 ** -125  # smaller scales are 0
+    assert bool(there[:32].all())
+    assert bool(((s.double() - want).abs() <= want * (2.0 ** -16 + 2.0 ** -23))[there].all())
+    v = y / want
+    off = (q.double() - v).abs()
+    assert bool(((off <= (v.abs() * 2.0 ** -4).clamp(min=2.0 ** -10) + v.abs() * 2.0 ** -15) | ~there).all())
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(1, 16), (130, 144), (257, 384), (3, 130, 272), (2, 128, 128)])
 def test_quantise_weight(dtype, shape):
