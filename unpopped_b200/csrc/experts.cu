@@ -2,10 +2,12 @@
 //
 // Routing: a warp holds a token's logits as order-preserving 32-bit keys. The k-th largest of the lanes' own maxima is a bound that at
 // least k keys reach, and few more; those that do are collected in the experts' order, and each counts how many come before it, which is its
-// rank. (k rounds of a maximum over all keys took some 650 instructions a token of 256 experts, this takes about 250.) Then the pairs
+// rank. (k rounds of a maximum over lanes that held their keys sorted took 29 us for 16384 tokens of 256 experts, where this took 25.) Then the pairs
 // are counted and placed by expert. A pair's place is the number of pairs of lower experts plus that of the same
 // expert's earlier tokens, so it does not depend on the order in which anything runs: within 128 tokens the earlier
 // ones are the lower bits of a mask that each expert has (set by atomicOr, which commutes), before them the counts of earlier blocks.
+// Bound by instructions, not by the 19 MB: 520 a token in the choice, 215 in the placing. Measured: 1 token of 128 experts 3.3 us, 128 of 256
+// 12.2 (one block: up to there its time is less than a second launch's), 16384 of 256 22.5.
 #include "common.cuh"
 #include "divide.cuh"
 #include "launch.cuh"
@@ -444,7 +446,7 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 Vec<__nv_bfloat16, 1>::narrow(const float (&f)[1]) { return __float2bfloat16_rn(f[0]); }
 
 // A thread sums U pieces of V values (16 bytes each) over their token's slots. Bound by HBM: every chosen row once. With U pieces of up to
-// kAtOnce slots about 8 loads are on their way a thread.
+// kAtOnce slots about 8 loads are on their way a thread. Measured: 8192 tokens' 8 rows of 4096 bf16 values 104 us (5.8 TB/s).
 template <typename T, int V, int U, typename Div>
 __global__ void __launch_bounds__(kSumThreads)
     combine_kernel(const T* __restrict__ y, int64_t rows, int64_t ys, const int32_t* __restrict__ slots,

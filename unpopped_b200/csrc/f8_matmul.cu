@@ -14,8 +14,9 @@
 //    token, so a block's scales are one factor for all of its columns. (With tokens as columns every thread needs every token's
 //    factor: at 128 bytes a cycle shared memory gives those of 128 x 128 values in 512 cycles, in which the MMA takes 256.) Bound by
 //    the two accumulators' round: an MMA of 512 cycles, its commit, the epilogue's loads and 128 sums a thread, the arrival that frees it.
-// Measured (a B200, inputs larger than L2 where they can be): 1 row by 8192 x 8192 weights 19.9 us (3.4 TB/s of weights), by 28672 x 8192 43.5
-// (5.4 TB/s); 8192 rows by 8192 x 8192 538 us (2.04 PFLOP/s); 16384 rows of 8 experts by 4096 x 2048 163 us (1.68 PFLOP/s).
+// Measured: 1 row by 8192 x 8192 weights 18 us (3.7 TB/s of weights), by 28672 x 8192 42 (5.6 TB/s); 512 rows of 128 experts by 4096 x 2048
+// 149 (958 MB of weights: 6.4 TB/s); 8192 rows by 8192 x 8192 532 us (2.07 PFLOP/s; 617 where calls follow one another for seconds and
+// the clock falls to the power limit); 65536 rows of 128 experts by 4096 x 2048 710 (1.55 PFLOP/s).
 #include "common.cuh"
 #include "divide.cuh"
 #include "launch.cuh"
@@ -158,7 +159,8 @@ struct Walk {
     const int tiles = start[a.experts];
     const int rounds = (int)a.by_owners(tiles);
     int rest = tiles - rounds * owners;
-    // shared only where that saves an owner more blocks than the joining of parts takes: else whole as well
+    // Shared only where that saves an owner more blocks than the joining of parts takes: else whole as well. With 256 columns a part is 128 KB
+    // a CTA, written and read again by all at one time: 512 rows by 8192 x 8192 weights 53 us shared, 41 whole; 8 blocks: 53, 12 to 32: 41.
     const int most = min(owners, rest * groups * C::kGroup / C::kMinBlocks);
     if (groups * C::kGroup * (most - rest) <= C::kJoinBlocks * most) rest = 0;
     const int units = rest * groups, sharers = rest > 0 ? most : 1;
@@ -911,22 +913,22 @@ static int cta_count() { return sm_count() < kMaxCtas ? sm_count() : kMaxCtas; }
 enum Form { kNarrow, kWide256, kPair256, kWide128 };
 
 // The form that takes the least time by a model: a fixed part (launch, first loads, output), then so many microseconds for each block of k of
-// the tiles of one owner, which Walk deals out. Fitted to 78 calls of 1 to 65536 rows, dense and by expert, by 512 x 1024 to 28672 x 8192
-// weights; the choice takes 0.6 % longer than the fastest form in the mean. Without one of the forms calls take 2 % longer in the mean, up to 30 %
-// where that one is the fastest. (A form of 64 tokens as columns was the fastest by 4 to 12 % for some calls of 64 to 256 rows, by
-// 0.2 % in the mean.) Measured, us, in the order of the table:
-//   rows by 2048 x 1024 weights:   1: 6.7, 8.4, 9.1, 6.4;     512: 9.2, 10.6, 11.2, 7.7;    8192: 68, 32, 31, 31
-//   rows by 8192 x 8192 weights:   1: 19.9, 26.9, 36.1, 30.1; 128: 34.4, 28.9, 35.1, 24.3;  512: 103, 40.8, 40.1, 50.8;  8192: 1561, 569, 538, 872
-//   128 experts' 4096 x 2048:      512: 149, 168, 244, 180;   8192: 303, 202, 302, 266;     65536: 1749, 714, 739, 872
+// the tiles of one owner, which Walk deals out. Fitted to which form was the fastest in 86 calls of 1 to 65536 rows, dense and by expert, by
+// 512 x 1024 to 28672 x 8192 weights; the choice takes 0.3 % longer than the fastest in the mean, 10 % at most. Without one of the forms calls take
+// 1.7 to 6.9 % longer in the mean, 18 to 59 % at most. (A form of 64 tokens as columns was the fastest by 4 to 12 % for some calls
+// of 64 to 256 rows, by 0.2 % in the mean; one of 256 tokens by 128 weights never was.) Measured, us, in the order of the table:
+//   rows by 2048 x 1024 weights:   1: 6.0, 7.1, 7.7, 5.7;     512: 8.6, 9.1, 9.6, 6.5;      8192: 68, 30, 31, 32
+//   rows by 8192 x 8192 weights:   1: 17.8, 26.3, 34.6, 28.3; 128: 33.9, 28.7, 34.1, 23.7;  512: 100, 39.6, 38.4, 50.8;  8192: 1528, 575, 544, 839
+//   128 experts' 4096 x 2048:      512: 149, 168, 250, 188;   8192: 312, 207, 326, 277;     65536: 1795, 731, 758, 883
 static Form form_of(int64_t m, int64_t experts, int64_t n, int64_t kb) {
   struct Cost {
     int tokens, weights, ctas, least, join;  // of a tile; Walk's
     double fixed, block;
   };
-  static const Cost cost[4] = {{Narrow::kTokens, Narrow::kWeights, 1, Narrow::kMinBlocks, Narrow::kJoinBlocks, 1.7, 0.269},
-                               {128, 256, 1, Wide<1, 256>::kMinBlocks, Wide<1, 256>::kJoinBlocks, 3.1, 0.648},
-                               {256, 256, 2, Wide<2, 256>::kMinBlocks, Wide<2, 256>::kJoinBlocks, 4.6, 0.603},
-                               {128, 128, 1, Wide<1, 128>::kMinBlocks, Wide<1, 128>::kJoinBlocks, 1.7, 0.457}};
+  static const Cost cost[4] = {{Narrow::kTokens, Narrow::kWeights, 1, Narrow::kMinBlocks, Narrow::kJoinBlocks, 3.8, 0.214},
+                               {128, 256, 1, Wide<1, 256>::kMinBlocks, Wide<1, 256>::kJoinBlocks, 3.4, 0.653},
+                               {256, 256, 2, Wide<2, 256>::kMinBlocks, Wide<2, 256>::kJoinBlocks, 4.2, 0.600},
+                               {128, 128, 1, Wide<1, 128>::kMinBlocks, Wide<1, 128>::kJoinBlocks, 3.5, 0.415}};
   const double used = (double)(m < experts ? m : experts), per = m / used;  // experts that have rows, at most; rows of each
   int best = 0;
   double least = 0;

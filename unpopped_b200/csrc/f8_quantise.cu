@@ -5,7 +5,9 @@
 // with a gate, y itself goes by ex2.approx and rcp.approx (2^-19 of it for x within 16 of 0, 2^-16 within 128: the rounding of exp's
 // argument; e4m3's half step is 2^-4).
 //
-// Bound by HBM: 2 (4, 8) bytes read and 1.03 written a value.
+// Bound by HBM: 2 (4, 8) bytes read and 1.03 written a value. Measured: 32768 x 2048 gated bf16 values 59 us (5.6 TB/s), gated f32 86
+// (7.0), plain bf16 40 (5.1); 64 x 4096 x 2048 bf16 weights 5.3 TB/s. Neither a third fewer instructions nor blocks that walk over
+// the pieces with the next one's loads on their way (61 to 120 us gated) made it faster.
 #include "common.cuh"
 #include "divide.cuh"
 #include "launch.cuh"
