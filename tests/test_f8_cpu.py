@@ -183,6 +183,20 @@ def test_every_unit_has_one_owner(owners):
                 assert owner_of(bounds[o]) == o and owner_of(bounds[o + 1] - 1) == o
 
 
+@pytest.mark.parametrize("wide", [2, 3, 7, 32, 129])
+def test_panels_hold_every_tile_once(wide):
+    """Tiles of many rows: 16 tiles' weights at a time, token by token, the last panel with fewer."""
+    for across in (1, 2, 15, 16, 17, 33, 70):
+        seen = set()
+        for at in range(wide * across):
+            panel = at // (16 * wide)
+            left, n = at - panel * 16 * wide, min(16, across - panel * 16)
+            place, tile = left // n, panel * 16 + left % n
+            assert place < wide and tile < across
+            seen.add((tile, place))
+        assert len(seen) == wide * across
+
+
 @pytest.mark.parametrize("tokens,step", [(32, 16), (128, 128), (256, 256)])
 def test_a_groups_tiles_hold_its_rows(tokens, step):
     for rows in range(1, 3000):

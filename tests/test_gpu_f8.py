@@ -167,6 +167,13 @@ def test_matmul_of_few_tiles_that_many_share(m, n, k):
     assert torch.equal(ops.f8_matmul(x, xs, w, ws, dtype=torch.float32), got)
 
 
+@pytest.mark.parametrize("m,n,k", [(2100, 2049, 24576), (9000, 4500, 5136)])
+def test_matmul_of_more_rows_than_l2_holds(m, n, k):
+    """The tiles go by panels; every eighth row and all columns are looked at."""
+    x, xs, w, ws = problem(m + n, m, n, k)
+    check(ops.f8_matmul(x, xs, w, ws)[::8], x[::8], xs[::8], w, ws)
+
+
 def test_matmul_of_views():
     """Rows of a wider x and out, scales by rows and broadcast, a column slice of a projection's output."""
     m, n, k = 37, 200, 272

@@ -37,6 +37,11 @@ constexpr int kBlock = 128;               // k a scale, and weight rows a scale
 constexpr int kTile = 128 * kBlock;       // bytes of 128 rows of a block
 constexpr int kBox = 16;                  // tokens of a small TMA box
 constexpr int kMaxExperts = 1024;
+// The tiles of an expert with more rows than some 42 MB hold (a third of L2) go by panels of 16 tiles' weights, token by token; else those of one
+// tile's weights follow one another and the rows stay in L2. 8192 rows by 8192 x 8192 weights 544 us without panels, 502 with; 16384 rows
+// 1177, 991; but 4096 rows 247, 255. Panels of 8 tiles 510 and 1011, of 32 524 and 1044.
+constexpr int kPanel = 16;
+constexpr int64_t kPanelBytes = 42 << 20;
 constexpr int kRuns = 4;                  // runs of blocks that the roles may be apart
 constexpr int kMaxCtas = (UP_F8_COUNTER_BYTES - 64) / 4;  // a counter each
 
@@ -94,6 +99,7 @@ struct Args {
   int64_t xs_m, xs_b;
   int64_t m;
   int experts, n, kb, nb, tb, groups;     // kb: blocks of k, in `groups` groups; nb: of weight rows, in tb tiles
+  int panel_rows;                         // of an expert: more go by panels
   Divide32 by_owners = Divide32(1), by_groups = Divide32(1);
   const int32_t* offsets;
   void* out;
@@ -129,7 +135,7 @@ struct Runs {
   }
 };
 
-// A unit is one group of k of one tile; tiles are numbered by expert, then weight rows, then tokens, so the tiles that
+// A unit is one group of k of one tile; tiles are numbered by expert, then weight rows, then tokens (or by panels), so the tiles that
 // share weights are neighbours. An owner is a CTA, or a pair. Of the tiles, as many as fill whole rounds of the owners are dealt out one
 // by one; the units of the `rest` others, the first ones, are shared evenly, so that all owners end together. An owner's units are
 // runs of groups of a tile, one after the other: first its share of the rest, whose parts are then joined while others still
@@ -144,7 +150,7 @@ static_assert(sizeof(Run) == 48, "Run");
 template <typename C>
 struct Walk {
   const int *start, *begin;               // first tile, first row of each expert
-  int groups;                             // a tile's
+  int groups, tb, panel_rows;             // a tile's; tiles over the weight rows; Args'
   int base, more;                         // shares of the rest: base + 1 units for the first `more` owners, base for the others
   int left;                               // units of this owner's share, from r.g0 of tile r.t on
   int whole_t, whole_left, owners;        // the next of the tiles dealt out, and how many are left
@@ -155,7 +161,7 @@ struct Walk {
     return unit < more * (base + 1) ? unit / (base + 1) : more + (unit - more * (base + 1)) / base;
   }
   __device__ __forceinline__ Walk(const Args& a, const int* start_, const int* begin_, int owner, int owners_)
-      : start(start_), begin(begin_), groups(a.groups), left(0), owners(owners_) {
+      : start(start_), begin(begin_), groups(a.groups), tb(a.tb), panel_rows(a.panel_rows), left(0), owners(owners_) {
     const int tiles = start[a.experts];
     const int rounds = (int)a.by_owners(tiles);
     int rest = tiles - rounds * owners;
@@ -199,8 +205,16 @@ struct Walk {
     r.tb = at, r.m0 = begin[r.e], r.n = rows;
     if (wide > 1) {
       // the group's tokens in tiles of equal width; the last may have fewer, and has some: (wide - 1) * kTokens < rows
-      r.tb = at / wide;
-      const int each = ((rows + wide - 1) / wide + C::kStep - 1) / C::kStep * C::kStep, first = (at - r.tb * wide) * each;
+      int place;
+      if (C::kWide && rows > panel_rows) {
+        const int panel = at / (kPanel * wide), in = at - panel * (kPanel * wide), across = min(kPanel, tb - panel * kPanel);
+        place = in / across;
+        r.tb = panel * kPanel + in - place * across;
+      } else {
+        r.tb = at / wide;
+        place = at - r.tb * wide;
+      }
+      const int each = ((rows + wide - 1) / wide + C::kStep - 1) / C::kStep * C::kStep, first = place * each;
       r.m0 += first;
       r.n = min(each, rows - first);
     }
@@ -1027,6 +1041,7 @@ extern "C" int up_sm100_f8_matmul(const uint8_t* x, int64_t m, int64_t x_stride,
   const Operands o{x, w, m, x_stride, experts, n, k};
   Args a{};
   a.xs = x_scale, a.ws = w_scale, a.xs_m = xs_stride_m, a.xs_b = xs_stride_b, a.m = m, a.experts = (int)experts, a.n = (int)n;
+  a.panel_rows = (int)(kPanelBytes / (kb * kBlock));
   a.kb = (int)kb, a.nb = (int)nb, a.offsets = offsets, a.out = out, a.out_stride = out_stride;
   a.out_dtype = out_dtype, a.wide_out = out_stride % (out_dtype == UP_EK_F32 ? 8 : 16) == 0 && aligned(out, 32);
   a.header = static_cast<Header*>(workspace);
