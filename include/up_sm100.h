@@ -578,7 +578,7 @@ UP_API size_t up_sm100_expert_route_workspace_bytes(int64_t tokens, int64_t expe
 
 /* out[t] = add[t] + sum over j in order: weights[t][j] * y[slots[t][j]], in f32, rounded once; a slot outside [0, rows) adds
  * nothing, add NULL is zeros. y [rows, n], add and out [tokens, n] have one type (F32, F16 or BF16) and contiguous rows,
- * strides in elements; slots and weights [tokens, k] are dense. out may be add. */
+ * strides in elements; slots and weights [tokens, k] are dense. out may be add; else it overlaps nothing that is read. */
 UP_API int up_sm100_expert_combine(const void* y, int dtype, int64_t rows, int64_t y_stride, int64_t n,
                                    const int32_t* slots, const float* weights, int64_t tokens, int64_t k,
                                    const void* add, int64_t add_stride, void* out, int64_t out_stride, void* stream);

@@ -85,6 +85,25 @@ def test_route_of_many_tokens():
     assert torch.equal(offsets[1:].long(), torch.bincount(order.flatten(), minlength=16).cumsum(0))
 
 
+@pytest.mark.parametrize("tokens", [63, 64, 65, 96, 97, 1000, 4736, 4737, 9473, 14209, 18944, 18945, 32768, 32769])
+@pytest.mark.parametrize("experts,k", [(16, 2), (200, 8)])
+def test_route_where_the_blocks_tiles_change(tokens, experts, k):
+    """One launch or two, tiles of 32 to 128 tokens, blocks of one tile or more; every ninth token is padding."""
+    logits = torch.randn(tokens, experts, generator=gen(tokens), device=DEV)
+    logits[::9] = float("-inf")
+    ids, w, rows, slots, offsets = ops.expert_route(logits, k)
+    there = torch.ones(tokens, dtype=torch.bool, device=DEV)
+    there[::9] = False
+    top = torch.sort(logits, dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(ids[there].long(), top[there]) and bool((ids[~there] == -1).all()) and bool((slots[~there] == -1).all())
+    pairs = int(there.sum()) * k
+    flat = torch.where(there[:, None], top, experts).flatten()
+    by = torch.sort(flat, stable=True).indices[:pairs]
+    assert torch.equal(rows[:pairs].long(), by // k) and bool((rows[pairs:] == -1).all())
+    assert torch.equal(slots.flatten()[by].long(), torch.arange(pairs, device=DEV))
+    assert torch.equal(offsets[1:].long(), torch.bincount(flat, minlength=experts + 1)[:experts].cumsum(0)) and int(offsets[0]) == 0
+
+
 def test_route_of_views_and_no_tokens():
     wide = torch.randn(50, 3, 64, generator=gen(6), device=DEV)
     check_route(wide[:, 1], 4)
@@ -243,3 +262,37 @@ def test_route_where_more_experts_than_a_warp_has_lanes_reach_the_bound(experts,
     logits[7, 3::7] = -1e30
     check_route(logits, k, "sigmoid")
     check_route(logits[:5], k, "softmax", False)
+
+
+@pytest.mark.parametrize("tokens", [10, 200])
+def test_a_layer_of_a_padded_batch(tokens):
+    """Padded tokens have no experts: their rows are the residual, and the others are what they are alone."""
+    e, d, f, k = 8, 256, 128, 3
+    g = gen(tokens)
+    x = torch.randn(tokens, d, generator=g, device=DEV).bfloat16()
+    x[tokens // 2:] = float("nan")  # what lies in padded rows is not looked at
+    logits = torch.randn(tokens, e, generator=g, device=DEV)
+    logits[tokens // 2:] = float("-inf")
+    up, up_s = ops.f8_quantise_weight(torch.randn(e, 2 * f, d, generator=g, device=DEV).bfloat16())
+    down, down_s = ops.f8_quantise_weight(torch.randn(e, d, f, generator=g, device=DEV).bfloat16())
+
+    def run(x, logits, add):
+        ids, weights, rows, slots, offsets = ops.expert_route(logits, k)
+        h = ops.f8_expert_matmul(*ops.f8_quantise(x, rows), up, up_s, offsets)
+        y = ops.f8_expert_matmul(*ops.f8_quantise(h, gate=True), down, down_s, offsets)
+        return ops.expert_combine(y, slots, weights, add)
+
+    add = torch.randn(tokens, d, generator=g, device=DEV).bfloat16()
+    out, n = run(x, logits, add), tokens // 2
+    assert torch.equal(out[n:], add[n:]) and bool(out.isfinite().all())
+    want = run(x[:n], logits[:n], add[:n])
+    # With other counts of rows tiles may be split elsewhere and sums be added in another order: a code of h may then be its neighbour, 2^-3 of
+    # one of 128 terms of no common sign, 2^-3 / sqrt(128) = 2^-6.5 of a row's size
+    assert bool(((out[:n].double() - want.double()).abs() <= want.double().abs() * 2.0 ** -6 + 2.0 ** -6 * want.double().abs().max()).all())
+
+
+def test_combine_of_no_slots():
+    add = torch.randn(5, 24, generator=gen(1), device=DEV).bfloat16()
+    y = torch.randn(3, 24, generator=gen(2), device=DEV).bfloat16()
+    none, w = torch.empty(5, 0, dtype=torch.int32, device=DEV), torch.empty(5, 0, device=DEV)
+    assert torch.equal(ops.expert_combine(y, none, w, add), add) and not bool(ops.expert_combine(y, none, w).any())

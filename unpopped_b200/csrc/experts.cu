@@ -6,8 +6,8 @@
 // are counted and placed by expert. A pair's place is the number of pairs of lower experts plus that of the same
 // expert's earlier tokens, so it does not depend on the order in which anything runs: within 128 tokens the earlier
 // ones are the lower bits of a mask that each expert has (set by atomicOr, which commutes), before them the counts of earlier blocks.
-// Bound by instructions, not by the 19 MB: 520 a token in the choice, 215 in the placing. Measured: 1 token of 128 experts 3.3 us, 128 of 256
-// 12.2 (one block: up to there its time is less than a second launch's), 16384 of 256 22.5.
+// Bound by instructions, not by the 19 MB: 520 a token in the choice, 215 in the placing. Measured: 1 token of 128 experts 3.3 us, 64 of 256
+// 7.0, 2048 9.4, 16384 22.5.
 #include "common.cuh"
 #include "divide.cuh"
 #include "launch.cuh"
@@ -20,7 +20,8 @@ namespace experts {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxK = 32;
-constexpr int kTile = 128;            // tokens a tile: four words of mask an expert
+constexpr int kTile = 128;            // tokens a tile at most: four words of mask an expert
+constexpr int kOne = 64;              // tokens that one block takes in one launch: 7.0 us of 256 experts, where two launches take 7.6 (96: 8.0, 7.4)
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxBlocks = 256;       // each block of the placing kernel reads every block's counts
@@ -29,7 +30,7 @@ struct Route {
   const void* logits;
   int64_t stride;
   int tokens, experts, k, score, renormalise;
-  int per;                            // tiles a block
+  int span, per;                      // tokens a tile, tiles a block
   float gain;
   int32_t *ids, *rows, *slots, *offsets;
   float* weights;
@@ -147,7 +148,7 @@ __device__ __forceinline__ Choice choose(const uint32_t (&key)[PER], const Route
 template <int PER, typename T>
 __device__ __forceinline__ void choose_tile(const Route& a, int first, uint32_t (*mask)[kTile / 32], int16_t* held, Candidate* found) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int end = min(first + kTile, a.tokens);
+  const int end = min(first + a.span, a.tokens);
   constexpr int kEach = kTile / kWarps, kAtOnce = PER <= 4 ? kEach : PER <= 8 ? 2 : 1;
 #pragma unroll 1
   for (int t0 = first + warp; t0 < end; t0 += kAtOnce * kWarps) {
@@ -224,7 +225,7 @@ static_assert(kThreads == kMaxExperts && kWarps == 32, "a thread an expert, a la
 // Places the tile's pairs: next[e] is the place of expert e's first pair in it.
 __device__ __forceinline__ void place_tile(const Route& a, int first, const uint32_t (*mask)[kTile / 32], const uint32_t* next,
                                            const int16_t* held) {
-  const int pairs = (min(first + kTile, a.tokens) - first) * a.k;
+  const int pairs = (min(first + a.span, a.tokens) - first) * a.k;
   for (int p = threadIdx.x; p < pairs; p += kThreads) {
     const int in = p / a.k, id = held[p];
     int slot = -1;
@@ -238,7 +239,7 @@ __device__ __forceinline__ void place_tile(const Route& a, int first, const uint
   }
 }
 
-// All of it in one block, for at most kTile tokens.
+// All of it in one block, for at most kOne tokens.
 template <int PER, typename T>
 __global__ void __launch_bounds__(kThreads) route_one_kernel(const Route a) {
   __shared__ uint32_t mask[PER * 32][kTile / 32];
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) choose_kernel(const Route a) {
   after_previous();
   let_next_begin();
   for (int i = 0; i < a.per; ++i) {
-    const int first = (blockIdx.x * a.per + i) * kTile;
+    const int first = (blockIdx.x * a.per + i) * a.span;
     if (first >= a.tokens) break;
     clear(mask, a.experts);
     __syncthreads();
@@ -292,14 +293,14 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const Route a) {
   let_next_begin();
   // The choice of a tile, marked in its masks. The first one's is on its way beside the counts.
   auto mark = [&](int first) {
-    const int pairs = (min(first + kTile, a.tokens) - first) * a.k;
+    const int pairs = (min(first + a.span, a.tokens) - first) * a.k;
     for (int p = threadIdx.x; p < pairs; p += kThreads) {
       const int id = a.ids[(int64_t)first * a.k + p], in = p / a.k;
       held[p] = (int16_t)id;
       if (id >= 0) atomicOr(&mask[id][in >> 5], 1u << (in & 31));
     }
   };
-  const int first0 = blockIdx.x * a.per * kTile;
+  const int first0 = blockIdx.x * a.per * a.span;
   __syncthreads();
   // warps take columns of 32 experts, and where these are fewer than the warps share a column's blocks
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const Route a) {
   for (int i = threadIdx.x; i < a.experts; i += kThreads) next[i] += before[i];
   __syncthreads();
   for (int i = 0; i < a.per; ++i) {
-    const int first = first0 + i * kTile;
+    const int first = first0 + i * a.span;
     if (first >= a.tokens) break;
     if (i > 0) {
       clear(mask, a.experts);
@@ -345,22 +346,25 @@ __global__ void __launch_bounds__(kThreads) place_kernel(const Route a) {
     a.rows[i] = -1;
 }
 
-static int blocks_of(int64_t tokens, int* per) {
-  const int64_t tiles = (tokens + kTile - 1) / kTile;
+// Blocks of the two launches, their tiles and a tile's tokens: whole warps of them, as few as give every SM a block (2048 tokens of 256 experts:
+// 16.7 us in tiles of 128 on 16 SMs, 9.4 in tiles of 32 on 64).
+static int split(int64_t tokens, int* span, int* per) {
+  const int64_t each = ((tokens + sm_count() - 1) / sm_count() + kWarps - 1) / kWarps * kWarps;
+  *span = (int)(each < kTile ? each : kTile);
+  const int64_t tiles = (tokens + *span - 1) / *span;
   *per = (int)((tiles + kMaxBlocks - 1) / kMaxBlocks);
-  if (*per < 1) *per = 1;
   return (int)((tiles + *per - 1) / *per);
 }
 
 template <int PER, typename T>
 int route(Route& a, cudaStream_t s) {
-  if (a.tokens <= kTile) {
+  if (a.tokens <= kOne) {
     const cudaError_t e = launch_early(route_one_kernel<PER, T>, 1, kThreads, 0, s, a);
     if (e != cudaSuccess) return cuda_status(e);
     note_launch();
     return check_launch();
   }
-  const int blocks = blocks_of(a.tokens, &a.per);
+  const int blocks = split(a.tokens, &a.span, &a.per);
   cudaError_t e = launch_early(choose_kernel<PER, T>, blocks, kThreads, 0, s, a);
   if (e == cudaSuccess) e = launch_early(place_kernel, blocks, kThreads, 0, s, a);
   if (e != cudaSuccess) return cuda_status(e);
@@ -535,9 +539,9 @@ using namespace up;
 using namespace up::experts;
 
 extern "C" size_t up_sm100_expert_route_workspace_bytes(int64_t tokens, int64_t experts) {
-  if (tokens <= kTile || experts <= 0 || experts > kMaxExperts) return 256;
-  int per;
-  return (size_t)blocks_of(tokens, &per) * experts * sizeof(uint32_t);
+  if (tokens <= kOne || experts <= 0 || experts > kMaxExperts) return 256;
+  int span, per;
+  return (size_t)split(tokens, &span, &per) * experts * sizeof(uint32_t);
 }
 
 extern "C" int up_sm100_expert_route(const void* logits, int dtype, int64_t tokens, int64_t n_experts, int64_t stride,
@@ -555,7 +559,7 @@ extern "C" int up_sm100_expert_route(const void* logits, int dtype, int64_t toke
   Route a{};
   a.logits = logits, a.stride = stride, a.tokens = (int)tokens, a.experts = (int)n_experts, a.k = (int)k, a.score = score;
   a.renormalise = renormalise != 0, a.gain = gain, a.ids = ids, a.rows = rows, a.slots = slots, a.offsets = offsets;
-  a.weights = weights, a.counts = static_cast<uint32_t*>(workspace), a.per = 1;
+  a.weights = weights, a.counts = static_cast<uint32_t*>(workspace), a.span = kTile, a.per = 1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == UP_EK_F32) return route_sized<float>(a, s);
   if (dtype == UP_EK_F16) return route_sized<__half>(a, s);

@@ -109,7 +109,7 @@ static const char* interface_body(int id) {
     case UP_K_F8_MATMUL:
       return R"J({"entry_symbol":"up_sm100_f8_matmul","params":[{"name":"x","role":"read","elem":"FP8_E4M3FN","rank":2},{"name":"x_scale","role":"read","elem":"F32","rank":2},{"name":"w","role":"read","elem":"FP8_E4M3FN","rank":3},{"name":"w_scale","role":"read","elem":"F32","rank":3},{"name":"offsets","role":"read","elem":"I32","rank":1},{"name":"out","role":"write","elem":"F32|F16|BF16","rank":2}],"launch":{"block":[384,1,1],"grid":"persistent, one CTA per SM (blocks of 288 threads for few rows, of 384 and in pairs for many)","cluster":[2,1,1],"dynamic_shared_bytes":"up to %SMEM%"},"launch_bounds":{"max_threads":384,"min_blocks":1},"cooperative":false,"requires":["sm_100a","tcgen05","tensor_memory","tma","mbarrier","thread_block_clusters"],"fidelity_notes":["each block of 128 k summed in f32 by the tensor cores, the blocks times their scales in f32, one rounding to out","parts of split tiles are added in order: deterministic"],"workspace":"counters and parts of split tiles: up_sm100_f8_matmul_workspace_bytes, its first 8192 bytes zero-filled once"})J";
     case UP_K_EXPERT_ROUTE:
-      return R"J({"entry_symbol":"up_sm100_expert_route","params":[{"name":"logits","role":"read","elem":"F32|F16|BF16","rank":2},{"name":"ids","role":"write","elem":"I32","rank":2},{"name":"weights","role":"write","elem":"F32","rank":2},{"name":"rows","role":"write","elem":"I32","rank":1},{"name":"slots","role":"write","elem":"I32","rank":2},{"name":"offsets","role":"write","elem":"I32","rank":1},{"name":"k","role":"scalar","elem":"I64"},{"name":"score","role":"scalar","elem":"I32"},{"name":"renormalise","role":"scalar","elem":"I32"},{"name":"gain","role":"scalar","elem":"F32"}],"launch":{"block":[1024,1,1],"grid":"one CTA up to 128 tokens; else two launches of a CTA per 128 tokens, at most 256","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":1024,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["whole numbers are exact: largest logits, the lower expert of equal ones; weights in f32"],"workspace":"each CTA's counts: up_sm100_expert_route_workspace_bytes"})J";
+      return R"J({"entry_symbol":"up_sm100_expert_route","params":[{"name":"logits","role":"read","elem":"F32|F16|BF16","rank":2},{"name":"ids","role":"write","elem":"I32","rank":2},{"name":"weights","role":"write","elem":"F32","rank":2},{"name":"rows","role":"write","elem":"I32","rank":1},{"name":"slots","role":"write","elem":"I32","rank":2},{"name":"offsets","role":"write","elem":"I32","rank":1},{"name":"k","role":"scalar","elem":"I64"},{"name":"score","role":"scalar","elem":"I32"},{"name":"renormalise","role":"scalar","elem":"I32"},{"name":"gain","role":"scalar","elem":"F32"}],"launch":{"block":[1024,1,1],"grid":"one CTA up to 64 tokens; else two launches of a CTA per 32 to 128 tokens, at most 256","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":1024,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["whole numbers are exact: largest logits, the lower expert of equal ones; weights in f32"],"workspace":"each CTA's counts: up_sm100_expert_route_workspace_bytes"})J";
     case UP_K_EXPERT_COMBINE:
       return R"J({"entry_symbol":"up_sm100_expert_combine","params":[{"name":"y","role":"read","elem":"F32|F16|BF16","rank":2},{"name":"slots","role":"read","elem":"I32","rank":2},{"name":"weights","role":"read","elem":"F32","rank":2},{"name":"add","role":"read","elem":"F32|F16|BF16","rank":2},{"name":"out","role":"write","elem":"F32|F16|BF16","rank":2}],"launch":{"block":[256,1,1],"grid":"a thread per one to four 16-byte pieces of the output","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":256,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["fused multiply-adds in f32 in the slots' order, one rounding"],"workspace":null})J";
     default: return nullptr;
