@@ -159,7 +159,8 @@ def test_matmul_of_many_rows_whose_outputs_lie_oddly(m, n, k, dtype):
     check(ops.f8_matmul(x, xs, w, ws, dtype=dtype), x, xs, w, ws)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 130, 65552), (33, 300, 20496), (130, 130, 16400), (200, 300, 20480), (257, 513, 8208), (520, 300, 16384), (300, 4096, 8192)])
+@pytest.mark.parametrize("m,n,k", [(1, 130, 65552), (33, 300, 20496), (130, 130, 16400), (200, 300, 20480), (257, 513, 8208), (520, 300, 16384),
+                                   (300, 4096, 8192)])
 def test_matmul_of_few_tiles_that_many_share(m, n, k):
     x, xs, w, ws = problem(m + k, m, n, k)
     got = ops.f8_matmul(x, xs, w, ws, dtype=torch.float32)

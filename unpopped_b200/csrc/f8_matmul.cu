@@ -607,9 +607,9 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
             cnt[h] = min(4, end - kb), n[h] = w.n;
             ws[h] = lane < cnt[h] ? a.ws[((int64_t)w.e * a.nb + w.tb) * a.kb + kb + lane] : 0.f;
             const float* from = a.xs + (w.m0 + lane) * a.xs_m + kb * a.xs_b;
-  #pragma unroll
+#pragma unroll
             for (int c = 0; c < kEach; ++c)
-  #pragma unroll
+#pragma unroll
               for (int j = 0; j < 4; ++j) xs[h][j][c] = c * 32 + lane < w.n && j < cnt[h] ? from[c * 32 * a.xs_m + j * a.xs_b] : 0.f;
             kb += 4;
           }
@@ -619,11 +619,11 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
         auto store = [&](int h) {
           good = __all_sync(0xffffffffu, wait(&sc_empty[q], ph, a, abort_flag));
           if (!good) return;
-  #pragma unroll
+#pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float f = __shfl_sync(0xffffffffu, ws[h], j);
             float* to = sc + q * O::kScSlot + j * C::kFactors + lane;
-  #pragma unroll
+#pragma unroll
             for (int c = 0; c < kEach; ++c)
               if (c * 32 < n[h]) to[c * 32] = xs[h][j][c] * f;
           }
