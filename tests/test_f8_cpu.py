@@ -197,6 +197,14 @@ def test_panels_hold_every_tile_once(wide):
         assert len(seen) == wide * across
 
 
+def test_owners_a_tile_by_a_float_quotient():
+    """(most + 0.5) / rest, off by up to four steps of f32, has the whole part of most / rest: it is 0.5 / rest from a whole number at least."""
+    for rest in range(1, 2033):
+        for most in (0, 1, rest - 1, rest, rest + 1, 2 * rest - 1, 2 * rest, 5 * rest - 1, 5 * rest, 2032):
+            exact = (most + 0.5) / rest
+            assert int(exact * (1 - 2.0 ** -21)) == int(exact * (1 + 2.0 ** -21)) == most // rest
+
+
 @pytest.mark.parametrize("tokens,step", [(32, 16), (128, 128), (256, 256)])
 def test_a_groups_tiles_hold_its_rows(tokens, step):
     for rows in range(1, 3000):

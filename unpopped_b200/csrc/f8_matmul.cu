@@ -14,7 +14,7 @@
 //    token, so a block's scales are one factor for all of its columns. (With tokens as columns every thread needs every token's
 //    factor: at 128 bytes a cycle shared memory gives those of 128 x 128 values in 512 cycles, in which the MMA takes 256.) Bound by
 //    the two accumulators' round: an MMA of 512 cycles, its commit, the epilogue's loads and 128 sums a thread, the arrival that frees it.
-// Measured: 1 row by 8192 x 8192 weights 18 us (3.7 TB/s of weights), by 28672 x 8192 42 (5.6 TB/s); 512 rows of 128 experts by 4096 x 2048
+// Measured: 1 row by 8192 x 8192 weights 16.4 us (4.1 TB/s of weights), by 28672 x 8192 42 (5.6 TB/s); 512 rows of 128 experts by 4096 x 2048
 // 149 (958 MB of weights: 6.4 TB/s); 8192 rows by 8192 x 8192 496 us (2.22 PFLOP/s; 570 where calls follow one another for seconds and
 // the clock falls to the power limit); 65536 rows of 128 experts by 4096 x 2048 710 (1.55 PFLOP/s).
 #include "common.cuh"
@@ -167,8 +167,13 @@ struct Walk {
     int rest = tiles - rounds * owners;
     // Shared only where that saves an owner more blocks than the joining of parts takes: else whole as well. With 256 columns a part is 128 KB
     // a CTA, written and read again by all at one time: 512 rows by 8192 x 8192 weights 53 us shared, 41 whole; 8 blocks: 53, 12 to 32: 41.
-    const int most = min(owners, rest * groups * C::kGroup / C::kMinBlocks);
-    if (groups * C::kGroup * (most - rest) <= C::kJoinBlocks * most) rest = 0;
+    const int blocks = groups * C::kGroup;
+    int most = min(owners, rest * blocks / C::kMinBlocks);
+    // Equal numbers of owners a tile, where that leaves few of them idle and costs few blocks: fewer parts to join (1 row by 8192 x 8192 weights,
+    // 64 tiles: 18.1 us on 148 owners, 16.5 on 128; but 40 tiles of 5120 x 5120: 11.0 on 148, 11.6 on 120).
+    const int parts = (int)__fdividef(most + 0.5f, (float)max(rest, 1));  // most / rest: both are below 2^12
+    if (parts >= 2 && 6 * parts * rest >= 5 * most && blocks * (most - parts * rest) <= 8 * parts * most) most = parts * rest;
+    if (blocks * (most - rest) <= C::kJoinBlocks * most) rest = 0;
     const int units = rest * groups, sharers = rest > 0 ? most : 1;
     base = sharers == owners ? (int)a.by_owners(units) : units / sharers, more = units - base * sharers;
     r.e = 0, r.t = 0, r.g0 = 0;
@@ -932,7 +937,7 @@ enum Form { kNarrow, kWide256, kPair256, kWide128 };
 // 1.7 to 6.9 % longer in the mean, 18 to 59 % at most. (A form of 64 tokens as columns was the fastest by 4 to 12 % for some calls
 // of 64 to 256 rows, by 0.2 % in the mean; one of 256 tokens by 128 weights never was.) Measured, us, in the order of the table:
 //   rows by 2048 x 1024 weights:   1: 6.0, 7.1, 7.7, 5.7;     512: 8.6, 9.1, 9.6, 6.5;      8192: 68, 30, 31, 32
-//   rows by 8192 x 8192 weights:   1: 17.8, 26.3, 34.6, 28.3; 128: 33.9, 28.7, 34.1, 23.7;  512: 100, 39.6, 38.4, 50.8;  8192: 1528, 575, 544, 839 (496 by panels)
+//   rows by 8192 x 8192 weights:   1: 16.4, 26.3, 34.6, 28.3; 128: 33.9, 28.7, 34.1, 23.7;  512: 100, 39.6, 38.4, 50.8;  8192: 1528, 575, 544, 839 (496 by panels)
 //   128 experts' 4096 x 2048:      512: 149, 168, 250, 188;   8192: 312, 207, 326, 277;     65536: 1795, 731, 758, 883
 static Form form_of(int64_t m, int64_t experts, int64_t n, int64_t kb) {
   struct Cost {
