@@ -525,7 +525,7 @@ UP_API size_t up_sm100_kv4_attention_workspace_bytes(int64_t tokens, int64_t q_h
  * have one f32 scale for each 128 values of a row, weights one for each 128 x 128 block; a last block may be shorter. */
 
 /* Rows of x as 8-bit values. Row r of the result is y = x[rows[r]] (rows NULL: x[r], and n_rows = tokens), or with
- * `gate` != 0, where x holds 2k values a row, y[i] = x[i] / (1 + exp(-x[i])) * x[k + i]. For each 128 values of y, with a
+ * `gate` != 0, where x holds 2k values a row, y[i] = x[i] / (1 + exp(-x[i])) * x[k + i] in f32 (with no loss where exp(-x[i]) leaves f32). For each 128 values of y, with a
  * the largest magnitude of its finite ones: scale = a * f32(1/448), q = e4m3(y * (1/scale)), in f32. Where that scale is below 2^-126 it is
  * 0, and so is q. An infinity or a NaN gives the NaN code in its place. A row whose rows[r] is outside [0, tokens) gives
  * zeros, scales too. x [tokens, k] is F32, F16 or BF16, 16-byte aligned with rows of whole 16 bytes, k a multiple of 16

@@ -1,12 +1,12 @@
 // f8_quantise.cu — activations and weights as e4m3 values with an f32 scale for each block of 128.
 //
 // For a block with largest finite magnitude a: scale = a * f32(1/448), q = e4m3(y * (1/scale)). Every step is one IEEE
-// operation in f32 (1/scale is a correctly rounded division), so values and scales are the plain formula's bit for bit;
-// with a gate, y itself goes by ex2.approx and rcp.approx (2^-19 of it for x within 16 of 0, 2^-16 within 128: the rounding of exp's
-// argument; e4m3's half step is 2^-4).
+// operation in f32 (1/scale is a correctly rounded division), so values and scales are the plain formula's bit for bit, with a
+// gate too: y = x / (1 + exp(-x)) * u by f32's exponential and rounded quotient. (By ex2.approx and rcp.approx y was 2^-19 off, and a third more
+// codes than with these were on the other side of a border of e4m3's.)
 //
-// Bound by HBM: 2 (4, 8) bytes read and 1.03 written a value. Measured: 32768 x 2048 gated bf16 values 59 us (5.6 TB/s), gated f32 86
-// (7.0), plain bf16 40 (5.1); 64 x 4096 x 2048 bf16 weights 5.3 TB/s. Neither a third fewer instructions nor blocks that walk over
+// Bound by HBM: 2 (4, 8) bytes read and 1.03 written a value. Measured: 32768 x 2048 gated bf16 values 62.5 us (5.4 TB/s; 71 where
+// many of the gates are far from 0), gated f32 87 (7.0), plain bf16 40 (5.1); 64 x 4096 x 2048 bf16 weights 5.3 TB/s. Neither a third fewer instructions nor blocks that walk over
 // the pieces with the next one's loads on their way (61 to 120 us gated) made it faster.
 #include "common.cuh"
 #include "divide.cuh"
@@ -69,14 +69,23 @@ __device__ __forceinline__ void widen(const Raw<__nv_bfloat16>& r, float (&v)[16
   for (int i = 0; i < 8; ++i) v[2 * i] = __uint_as_float(r.w[i] << 16), v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
 }
 
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
 // Magnitudes compare as their bits do; those from kInfinity on are not finite.
 constexpr uint32_t kInfinity = 0x7f800000u;
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ float max_abs(float a, float b, float c) {  // a NaN if one of them is
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ uint32_t largest(const float (&v)[16]) {
-  uint32_t a = 0;
+  float a = v[0];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) a = max(a, magnitude(v[i]));
-  return a;
+  for (int i = 1; i < 15; i += 2) a = max_abs(a, v[i], v[i + 1]);
+  return magnitude(max_abs(a, v[15], 0.f));
 }
 __device__ __forceinline__ uint32_t largest_finite(const float (&v)[16]) {
   uint32_t a = 0;
@@ -122,33 +131,51 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
-__device__ __forceinline__ float exp2_approx(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 __device__ __forceinline__ float reciprocal_approx(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// x / (1 + exp(-x)) * g of two values. With h = exp(-|x| / 2) it is x * r * g for x >= 0 and h * x * r * g * h below, r = 1 / (1 + h^2): h is far from
-// the ends of f32's range wherever the result is not below it, so no factor is lost to underflow, and r is between a half and one.
+// x / (1 + exp(-x)) * g with f32's exponential and quotient. The quotient is x times an approximate reciprocal with one correction by its
+// remainder (Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990), of both by 1/4 so that the
+// reciprocal is a normal number: for each f32 x from -88.7 up, of 2^-100 at least, that is the rounded quotient (compared for all of them;
+// 63 us where the compiler's quotient takes 89). Below, where exp(-x) leaves f32, and for values that are not finite it gives a NaN.
 __device__ __forceinline__ void gated(float& x0, float& x1, float g0, float g1) {
-  constexpr float kRate = -0.72134752f;  // -log2(e) / 2
-  const float h0 = exp2_approx(fabsf(x0) * kRate), h1 = exp2_approx(fabsf(x1) * kRate);
-  const uint64_t h = pair_of(h0, h1), d = fma2(h, h, pair_of(1.f, 1.f));
-  const uint64_t r = pair_of(reciprocal_approx(__uint_as_float((uint32_t)d)), reciprocal_approx(__uint_as_float((uint32_t)(d >> 32))));
-  const uint64_t f = pair_of(x0 < 0.f ? h0 : 1.f, x1 < 0.f ? h1 : 1.f);
-  const uint64_t y = mul2(mul2(mul2(pair_of(x0, x1), f), mul2(r, pair_of(g0, g1))), f);
+  const float d0 = fmaf(expf(-x0), -0.25f, -0.25f), d1 = fmaf(expf(-x1), -0.25f, -0.25f);
+  const uint64_t d = pair_of(d0, d1), r = pair_of(reciprocal_approx(-d0), reciprocal_approx(-d1));
+  const uint64_t x = mul2(pair_of(x0, x1), pair_of(0.25f, 0.25f)), q = mul2(x, r);
+  const uint64_t y = mul2(fma2(fma2(d, q, x), r, q), pair_of(g0, g1));
   x0 = __uint_as_float((uint32_t)y), x1 = __uint_as_float((uint32_t)(y >> 32));
+}
+// The same for all values: with exp(-x) out of range 1 + exp(-x) is exp(-x) to the last bit, which goes by halves.
+__device__ __forceinline__ float gated_any(float x, float g) {
+  const float d = 1.f + expf(-x);
+  if (d < __uint_as_float(kInfinity)) return x / d * g;
+  const float h = expf(0.5f * x);
+  return x * h * g * h;
+}
+
+// Those of sixteen that are no finite numbers once more, from memory, so that the kernel need not hold its inputs for them.
+template <typename T>
+__device__ __forceinline__ void gate_again(const T* from, int k, float (&v)[16]) {
+  uint32_t bad = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) bad |= magnitude(v[i]) >= kInfinity ? 1u << i : 0u;
+#pragma unroll 1
+  for (; bad != 0; bad &= bad - 1) {
+    const int at = __ffs(bad) - 1;
+    const float y = gated_any(as_float(from[at]), as_float(from[k + at]));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = i == at ? y : v[i];
+  }
 }
 
 // A piece is 16 values; 8 pieces (a quarter of a warp) are a block. The last block of a row may have fewer. A thread has U pieces, whose loads
-// are all on their way before the first is looked at. (With 8 values a piece the blocks' own instructions, 150 a piece, were the bound:
+// are all on their way before the first is looked at. Gated 16-bit values are held to 40 registers a thread, six blocks an SM: 62.5 us where five
+// take 67. (With 8 values a piece the blocks' own instructions, 150 a piece, were the bound:
 // 8192 x 8192 bf16 values took 52 us.)
 template <typename T, bool GATE, int U, typename Div>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, GATE && sizeof(T) == 2 ? 6 : 0)
     quantise_kernel(const T* __restrict__ x, int64_t tokens, int64_t x_stride, const int32_t* __restrict__ rows,
                     typename Div::Int pieces, Div by_row, int k, bool wide, uint4* __restrict__ q, float* __restrict__ scale,
                     int64_t ss_r, int64_t ss_b) {
@@ -189,6 +216,10 @@ __global__ void __launch_bounds__(kThreads)
       for (int i = 0; i < 16; i += 2) gated(v[i], v[i + 1], g[i], g[i + 1]);
     }
     uint32_t a = largest(v);
+    if (GATE && a >= kInfinity) {
+      gate_again(x + (rows ? (int64_t)rows[row[u]] : (int64_t)row[u]) * x_stride + at[u], k, v);
+      a = largest(v);
+    }
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(mask, a, o));
     const bool fine = a < kInfinity;  // alike in the block's lanes

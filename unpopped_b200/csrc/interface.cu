@@ -105,7 +105,7 @@ static const char* interface_body(int id) {
     case UP_K_KV4_ATTENTION:
       return R"J({"entry_symbol":"up_sm100_kv4_attention","params":[{"name":"q","role":"read","elem":"F16|BF16","rank":3},{"name":"cache","role":"read","elem":"I4+F16","rank":4},{"name":"block_table","role":"read","elem":"I32","rank":2},{"name":"seq_lens","role":"read","elem":"I32","rank":1},{"name":"cu_q","role":"read","elem":"I32","rank":1},{"name":"out","role":"write","elem":"F16|BF16","rank":3},{"name":"lse","role":"write","elem":"F32","rank":2},{"name":"causal","role":"scalar","elem":"I32"},{"name":"window","role":"scalar","elem":"I64"},{"name":"scale","role":"scalar","elem":"F32"}],"launch":{"block":[128,1,1],"grid":"few query rows: two to four CTAs per SM over units of 128 cached tokens; prompts (block 576): a CTA per 256 query rows","cluster":null,"dynamic_shared_bytes":"up to 201728"},"launch_bounds":{"max_threads":576,"min_blocks":1},"cooperative":false,"requires":["sm_100a","cp.async","mma.sync","tcgen05","tensor_memory","mbarrier"],"fidelity_notes":["f32 sums, exact logits up to them; few query rows: p * v_scale rounded to f16; many: p, and with bf16 outputs nibble * v_scale","split tiles are added in order: deterministic"],"workspace":"counters and parts of split tiles: up_sm100_kv4_attention_workspace_bytes, zero-filled once"})J";
     case UP_K_F8_QUANTISE:
-      return R"J({"entry_symbol":"up_sm100_f8_quantise","params":[{"name":"x","role":"read","elem":"F32|F16|BF16","rank":2},{"name":"rows","role":"read","elem":"I32","rank":1},{"name":"q","role":"write","elem":"FP8_E4M3FN","rank":2},{"name":"scale","role":"write","elem":"F32","rank":2},{"name":"gate","role":"scalar","elem":"I32"}],"launch":{"block":[256,1,1],"grid":"a thread per one or two pieces of 16 values","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":256,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["values and scales are the stated f32 operations bit for bit; with a gate, exp and the quotient are approximate (2^-19 of a value for x within 16 of 0, 2^-16 within 128)"],"workspace":null})J";
+      return R"J({"entry_symbol":"up_sm100_f8_quantise","params":[{"name":"x","role":"read","elem":"F32|F16|BF16","rank":2},{"name":"rows","role":"read","elem":"I32","rank":1},{"name":"q","role":"write","elem":"FP8_E4M3FN","rank":2},{"name":"scale","role":"write","elem":"F32","rank":2},{"name":"gate","role":"scalar","elem":"I32"}],"launch":{"block":[256,1,1],"grid":"a thread per one or two pieces of 16 values","cluster":null,"dynamic_shared_bytes":0},"launch_bounds":{"max_threads":256,"min_blocks":0},"cooperative":false,"requires":["sm_100a"],"fidelity_notes":["values and scales are the stated f32 operations bit for bit, with a gate too where exp(-x) is a finite f32 number (below, x*h*g*h with h = exp(x/2))"],"workspace":null})J";
     case UP_K_F8_MATMUL:
       return R"J({"entry_symbol":"up_sm100_f8_matmul","params":[{"name":"x","role":"read","elem":"FP8_E4M3FN","rank":2},{"name":"x_scale","role":"read","elem":"F32","rank":2},{"name":"w","role":"read","elem":"FP8_E4M3FN","rank":3},{"name":"w_scale","role":"read","elem":"F32","rank":3},{"name":"offsets","role":"read","elem":"I32","rank":1},{"name":"out","role":"write","elem":"F32|F16|BF16","rank":2}],"launch":{"block":[384,1,1],"grid":"persistent, one CTA per SM (blocks of 288 threads for few rows, of 384 and in pairs for many)","cluster":[2,1,1],"dynamic_shared_bytes":"up to %SMEM%"},"launch_bounds":{"max_threads":384,"min_blocks":1},"cooperative":false,"requires":["sm_100a","tcgen05","tensor_memory","tma","mbarrier","thread_block_clusters"],"fidelity_notes":["each block of 128 k summed in f32 by the tensor cores, the blocks times their scales in f32, one rounding to out","parts of split tiles are added in order: deterministic"],"workspace":"counters and parts of split tiles: up_sm100_f8_matmul_workspace_bytes, its first 8192 bytes zero-filled once"})J";
     case UP_K_EXPERT_ROUTE:
