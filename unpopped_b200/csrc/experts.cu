@@ -453,9 +453,8 @@ __device__ __forceinline__ __nv_bfloat16 Vec<__nv_bfloat16, 1>::narrow(const flo
 // kAtOnce slots about 8 loads are on their way a thread. Measured: 8192 tokens' 8 rows of 4096 bf16 values 104 us (5.8 TB/s).
 template <typename T, int V, int U, typename Div>
 __global__ void __launch_bounds__(kSumThreads)
-    combine_kernel(const T* __restrict__ y, int64_t rows, int64_t ys, const int32_t* __restrict__ slots,
-                   const float* __restrict__ weights, int k, const T* add, int64_t as, T* out, int64_t os,
-                   typename Div::Int pieces, typename Div::Int row_pieces, Div by_row) {
+    combine_kernel(const T* y, int64_t rows, int64_t ys, const int32_t* slots, const float* weights, int k, const T* add, int64_t as,
+                   T* out, int64_t os, typename Div::Int pieces, typename Div::Int row_pieces, Div by_row) {
   using Int = typename Div::Int;
   using W = Vec<T, V>;
   constexpr int kAtOnce = 8 / U;

@@ -24,7 +24,7 @@ constexpr int kBlock = 128;           // values a scale
 constexpr float kMax = 448.f;         // e4m3's largest
 constexpr float kSmallest = 1.17549435e-38f;  // 2^-126: a smaller scale has no finite 1/scale to rely on
 
-// Sixteen values as they lie in memory (8 words of two, or 16), by loads of 32 bytes where they lie on such borders.
+// Sixteen values as they lie in memory (8 words of two, or 16), by loads of 32 bytes where they lie on such borders (ordinary ones: launch.cuh).
 template <typename T>
 struct Raw {
   uint32_t w[8];
@@ -35,12 +35,15 @@ struct Raw<float> {
 };
 __device__ __forceinline__ void load32(const void* p, uint32_t* w, bool wide) {
   if (wide) {
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
                  : "l"(p));
   } else {
-    const uint4 a = ld_nc_na_v4(p), b = ld_nc_na_v4(static_cast<const char*>(p) + 16);
-    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4)
+      asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                   : "l"(static_cast<const char*>(p) + 4 * i));
   }
 }
 template <typename T>
@@ -176,7 +179,7 @@ __device__ __forceinline__ void gate_again(const T* from, int k, float (&v)[16])
 // 8192 x 8192 bf16 values took 52 us.)
 template <typename T, bool GATE, int U, typename Div>
 __global__ void __launch_bounds__(kThreads, GATE && sizeof(T) == 2 ? 6 : 0)
-    quantise_kernel(const T* __restrict__ x, int64_t tokens, int64_t x_stride, const int32_t* __restrict__ rows,
+    quantise_kernel(const T* x, int64_t tokens, int64_t x_stride, const int32_t* rows,
                     typename Div::Int pieces, Div by_row, int k, bool wide, uint4* __restrict__ q, float* __restrict__ scale,
                     int64_t ss_r, int64_t ss_b) {
   using Int = typename Div::Int;
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, GATE && sizeof(T) == 2 ? 6 : 0)
 // One CTA a block of 128 x 128 weights: its values stay in registers between the maximum and the codes.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    weight_kernel(const T* __restrict__ w, int64_t n, int64_t k, int64_t stride_e, int64_t stride_n, uint32_t blocks_k,
+    weight_kernel(const T* w, int64_t n, int64_t k, int64_t stride_e, int64_t stride_n, uint32_t blocks_k,
                   uint32_t blocks_n, bool wide, uint4* __restrict__ q, float* __restrict__ scale) {
   const uint32_t rest = blockIdx.x / blocks_k, e = rest / blocks_n;
   const int64_t bk = blockIdx.x - rest * blocks_k, bn = rest - e * blocks_n;

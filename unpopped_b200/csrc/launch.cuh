@@ -6,7 +6,10 @@
 namespace up {
 
 // The kernel's CTAs may be placed as soon as every CTA of the kernel before has exited or called let_next_begin, so it calls
-// after_previous() in every thread that touches global memory, and before it does.
+// after_previous() in every thread that touches global memory, and before it does. Its lifetime then begins before the kernels ahead have
+// written: a CTA can be resident while the one before the one before still reads. So it reads what they may write by ordinary loads only. The
+// non-coherent path (ld.global.nc, __ldg, and what the compiler makes of const __restrict__ pointers) is for memory that does not
+// change in a kernel's lifetime; its loads may be served from lines that are already in L1 and be moved ahead of the wait.
 template <typename... P, typename... A>
 cudaError_t launch_early(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, A&&... args) {
   cudaLaunchAttribute attr;
