@@ -239,7 +239,9 @@ UP_API int up_sm100_launch(int kernel_id, const up_tensor* ins, int n_in, const 
                     void* stream);
 
 /* Waits for `stream`, then reads and clears the device error word of a workspace: UP_OK, or
- * UP_ERR_DEVICE_TIMEOUT when a bounded wait ran out during an earlier launch on it. */
+ * UP_ERR_DEVICE_TIMEOUT when a bounded wait ran out during an earlier launch on it. A launch that gave up may leave counters of
+ * unfinished tiles above zero, by which later launches would be wrong without a word: after UP_ERR_DEVICE_TIMEOUT zero-fill what was to be
+ * zero-filled before the first use again (a scan's workspace needs no more than this call). */
 UP_API int up_sm100_workspace_status(void* workspace, void* stream);
 
 /* ---- Typed entry points (what the generic launch dispatches to) ------------------------------------ */

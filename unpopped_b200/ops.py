@@ -64,11 +64,17 @@ def workspace(kind: str, nbytes: int, device: torch.device) -> torch.Tensor:
 
 
 def workspace_status(ws: torch.Tensor) -> int:
-    """Waits for the stream and returns UP_OK or UP_ERR_DEVICE_TIMEOUT (clearing the error word)."""
-    return _lib.load().up_sm100_workspace_status(ws.data_ptr(), _stream(ws))
+    """Waits for the stream and returns UP_OK or UP_ERR_DEVICE_TIMEOUT. After a wait that ran out the workspace is zero-filled, as before its
+    first use: a launch that gave up leaves counters of unfinished tiles behind, by which later launches would add parts that are not there."""
+    status = _lib.load().up_sm100_workspace_status(ws.data_ptr(), _stream(ws))
+    if status == _lib.UP_ERR_DEVICE_TIMEOUT:
+        ws.zero_()
+    return status
 
 
 def check_workspace(kind: str, device: torch.device):
+    """Raises UpError if a device wait of a call on the current stream ran out since the last check; the results of the calls between are not
+    to be used. The next call works again."""
     ws = _ws_cache.get(_ws_key(kind, device))
     if ws is not None:
         check(workspace_status(ws), f"{kind} device wait")
