@@ -566,7 +566,7 @@ typedef enum up_expert_score { UP_EXPERT_SOFTMAX = 0, UP_EXPERT_SIGMOID = 1 } up
 /* Routes tokens to experts and lays the pairs out by expert. Of each row of logits [tokens, experts] (F32, F16 or BF16) the
  * k largest are taken, largest first, the lower expert of equal ones, a NaN before all others; an expert whose logit is
  * -inf is never taken. ids[t][j] is the expert (-1 where none is left), weights[t][j] its score in f32 (0 there), divided by
- * the chosen ones' sum with `renormalise` != 0 (0 where that sum is 0), times gain. The pairs that were taken, in the order
+ * the chosen ones' sum with `renormalise` != 0 (0 where the largest is 0; shares of scores below 2^-126 are as precise as others), times gain. The pairs that were taken, in the order
  * of their expert and then of their token, have the places 0, 1, ...: slots[t][j] is a pair's place (-1 for none), rows[place] its
  * token (-1 behind the last), offsets[e] the first place of expert e and offsets[experts] the number of pairs. At most
  * 1024 experts, k at most 32 and at most experts, tokens * k below 2^31. `workspace` from

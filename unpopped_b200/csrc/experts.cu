@@ -135,8 +135,15 @@ __device__ __forceinline__ Choice choose(const uint32_t (&key)[PER], const Route
         if (key[i] > kMasked) total += expf(value_of(key[i]) - m);
       total = warp_sum(total);
     }
-  } else if (taken) {
-    w = 1.f / (1.f + expf(-l));
+  } else {
+    const float m = value_of(top);
+    // Shares of scores that are no normal numbers: exp(-m) times as large, which no quotient changes. None where the largest score is 0 in f32.
+    if (a.renormalise && m < 0.f && __any_sync(0xffffffffu, taken && l < -64.f)) {
+      if (taken && expf(m) > 0.f) w = expf(l - m) / (1.f + expf(l));
+    } else if (taken) {
+      const float d = 1.f + expf(-l);
+      w = d < __uint_as_float(0x7f800000u) ? 1.f / d : expf(l);  // below -88.7 they are one number
+    }
   }
   if (a.renormalise) total = warp_sum(w);
   c.weight = taken && !(total == 0.f) ? w / total * a.gain : 0.f;
