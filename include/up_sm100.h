@@ -542,7 +542,8 @@ UP_API int up_sm100_f8_quantise_weight(const void* w, int dtype, int64_t experts
                                        int64_t w_stride_e, int64_t w_stride_n, uint8_t* q, float* scale, void* stream);
 
 /* out[m][j] = sum over blocks b of 128: x_scale[m][b] * w_scale[e][j / 128][b] * (sum over k in b: x[m][k] w[e][j][k]),
- * each block's sum and the sum over blocks in f32 (tcgen05, block by block), rounded once to out_dtype (F32, F16 or BF16).
+ * each block's sum and the sum over blocks in f32 (tcgen05, block by block), rounded once to out_dtype (F32, F16 or BF16). Scales
+ * whose product leaves f32 are multiplied to a block's sum one after the other, so nothing that fits f32 is lost to it.
  * offsets NULL: one matrix (experts 1) for all rows. Otherwise (I32, experts + 1 entries, on the device) rows
  * [offsets[e], offsets[e + 1]) take matrix e; entries are held to [0, m] and to their predecessors, and rows that no
  * expert has are left as they were. x [m, k] e4m3, rows `x_stride` bytes apart; w [experts, n, k] e4m3, dense; both 16-byte

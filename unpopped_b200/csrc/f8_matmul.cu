@@ -29,6 +29,7 @@
 
 #include <cmath>
 #include <mutex>
+#include <type_traits>
 
 namespace up {
 namespace f8 {
@@ -76,7 +77,7 @@ struct Of {
   static constexpr int kStage = kTile + C::kBBytes;
   static constexpr int kDSlot = C::kDBlock * C::kGroup, kDRing = 512 / kDSlot;  // accumulators in tensor memory
   static constexpr int kEpiThreads = 32 * C::kEpiWarps, kThreads = 32 * C::kEpi0 + kEpiThreads;
-  static constexpr int kScRing = C::kFactors > 0 ? 4 : 0, kScSlot = 4 * C::kFactors;  // factors in shared memory, four blocks a slot
+  static constexpr int kScRing = C::kFactors > 0 ? 4 : 0, kScSlot = 8 * C::kFactors + 4;  // factors in shared memory, four blocks a slot, twice (Scales), and whether the second are there
   static constexpr int kStaged = C::kWide ? 32 * 17 : 0;             // values a warp, for rows of `out` that do not begin on 32 bytes
   static constexpr size_t kPart = (size_t)C::kSums * kEpiThreads;  // values of a CTA's part of a tile
   // One thread issues the MMAs and commits of a block in some 450 cycles, so two take the blocks in turn; the ring's even
@@ -343,6 +344,28 @@ __device__ __forceinline__ void load32(uint32_t from, uint32_t (&v)[32]) {
 __device__ __forceinline__ void wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fma_after(float& sum, uint32_t v, float f) {
   asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(sum) : "f"(__uint_as_float(v)), "f"(f));
+}
+__device__ __forceinline__ void mul_after(uint32_t& v, float f) {
+  float r;
+  asm volatile("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(v)), "f"(f));
+  v = __float_as_uint(r);
+}
+// Whether the product of two scales is no normal number (0 included). Then v * x * w goes by both, the larger first, as it may be an ordinary number
+// all the same: where x * w is too small, v * (the larger) is not too large, and where it is and x * w is as well, the result is.
+__device__ __forceinline__ bool out_of_range(float product) { return (__float_as_uint(product) << 1) - 0x01000000u >= 0xfe000000u; }
+struct Scales {
+  float first, then;
+  __device__ __forceinline__ Scales(float x, float w) : first(1.f), then(x * w) {
+    if (out_of_range(then) && x != 0.f && w != 0.f) {
+      const bool larger = fabsf(x) > fabsf(w);
+      first = larger ? x : w, then = larger ? w : x;
+    }
+  }
+};
+__device__ __forceinline__ float shared1(uint32_t at) {
+  float f;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(at));
+  return f;
 }
 __device__ __forceinline__ float4 shared4(uint32_t at) {
   float4 f;
@@ -624,14 +647,32 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
         auto store = [&](int h) {
           good = __all_sync(0xffffffffu, wait(&sc_empty[q], ph, a, abort_flag));
           if (!good) return;
+          float* slot = sc + q * O::kScSlot + lane;
+          bool odd = false;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float f = __shfl_sync(0xffffffffu, ws[h], j);
-            float* to = sc + q * O::kScSlot + j * C::kFactors + lane;
 #pragma unroll
             for (int c = 0; c < kEach; ++c)
-              if (c * 32 < n[h]) to[c * 32] = xs[h][j][c] * f;
+              if (c * 32 < n[h]) {
+                const float by = xs[h][j][c] * f;
+                slot[j * C::kFactors + c * 32] = by;
+                odd = odd || (out_of_range(by) && xs[h][j][c] != 0.f);
+              }
           }
+          odd = __any_sync(0xffffffffu, odd);
+          if (odd) {
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+              const float f = __shfl_sync(0xffffffffu, ws[h], j);
+#pragma unroll
+              for (int c = 0; c < kEach; ++c) {
+                const Scales two(j == 0 ? xs[h][0][c] : j == 1 ? xs[h][1][c] : j == 2 ? xs[h][2][c] : xs[h][3][c], f);
+                slot[j * C::kFactors + c * 32] = two.then, slot[(4 + j) * C::kFactors + c * 32] = two.first;
+              }
+            }
+          }
+          if (lane == 0) slot[8 * C::kFactors] = odd ? 1.f : 0.f;
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(&sc_full[q]);
           if (++q == kScRing) q = 0, ph ^= 1u;
@@ -693,27 +734,27 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
         accumulators();
         if (!good) break;
         // Two sets of 32 columns at a time, whose successors' loads run beside the sums. A slot is free as soon as its last loads are
-        // done: a later block's MMA waits for that.
+        // done: a later block's MMA waits for that. `odd`: the accumulators times g first (Scales).
         load32(from + d * O::kDSlot, v[0]);
         load32(from + d * O::kDSlot + 32, v[1]);
-        for (int kb = first; kb < end; ++kb) {
-          const float f = xs_next[0] * ws_next[0];
-          xs_next[0] = xs_next[1], ws_next[0] = ws_next[1];
-          if (kb + 2 < end) xs_next[1] = xs[2 * a.xs_b], ws_next[1] = ws[2];
-          xs += a.xs_b, ++ws;
+        auto block = [&](int kb, auto odd, float f, float g) {
           const uint32_t in = from + d * O::kDSlot;
 #pragma unroll
           for (int c = 0; c < kSums; c += 64) {
             const bool last = c + 64 == kSums;
             wait_loads();
             if (last) free_accumulators();
+            if constexpr (odd.value) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) mul_after(v[0][j], g), mul_after(v[1][j], g);
+            }
 #pragma unroll
             for (int j = 0; j < 32; ++j) fma_after(sum[c + j], v[0][j], f);
             if (!last) {
               load32(in + c + 64, v[0]);
             } else if (kb + 1 < end) {
               accumulators();
-              if (!good) break;
+              if (!good) return;
               load32(from + d * O::kDSlot, v[0]);
             }
 #pragma unroll
@@ -723,8 +764,38 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
             else if (kb + 1 < end)
               load32(from + d * O::kDSlot + 32, v[1]);
           }
+        };
+        float x_new, w_new;
+        auto fetch = [&](int kb) {
+          x_new = 0.f, w_new = 0.f;
+          if (kb + 2 < end) x_new = xs[2 * a.xs_b], w_new = ws[2];
+          xs += a.xs_b, ++ws;
+        };
+        auto move_up = [&]() { xs_next[0] = xs_next[1], ws_next[0] = ws_next[1], xs_next[1] = x_new, ws_next[1] = w_new; };
+        auto any_odd = [&](int j, float f) { return __any_sync(0xffffffffu, out_of_range(f) && xs_next[j] != 0.f && ws_next[j] != 0.f) != 0; };
+        // From the first block on where a row's scales leave f32's range, the run goes on in a loop of its own. The vote is on the block after, beside
+        // the wait for tensor memory: 8192 rows by 8192 x 8192 weights 503 us without any, 511 so, 514 to 542 with the vote or a branch in
+        // each block's own way.
+        int kb = first;
+        float f = xs_next[0] * ws_next[0];
+        for (bool odd = any_odd(0, f); kb < end && !odd; ++kb) {
+          fetch(kb);
+          const float f_next = xs_next[1] * ws_next[1];
+          odd = any_odd(1, f_next);
+          block(kb, std::false_type(), f, 1.f);
           if (!good) break;
+          move_up();
+          f = f_next;
         }
+        if (good)
+#pragma unroll 1
+          for (; kb < end; ++kb) {
+            const Scales two(xs_next[0], ws_next[0]);
+            fetch(kb);
+            block(kb, std::true_type(), two.then, two.first);
+            if (!good) break;
+            move_up();
+          }
       } else {
         // The thread's row is a weight row, its columns the tokens, each with a factor of its own.
         for (int kb = first; kb < end; kb += kGroup) {
@@ -733,24 +804,35 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
           good = __all_sync(0xffffffffu, wait(&sc_full[q], qph, a, abort_flag));
           if (!good) break;
           const uint32_t f = tc::smem_u32(sc + q * O::kScSlot + kSums * part);
-          auto add = [&](int j, const uint32_t(&x)[32]) {  // block j's
+          const float flag = shared1(f + 8 * C::kFactors * 4);
+          const uint32_t in = from + d * O::kDSlot;
+          auto blocks = [&](auto odd) {
+            auto add = [&](int j, uint32_t(&x)[32]) {  // block j's
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 f4 = shared4(f + (j * C::kFactors + i) * 4);
-              fma_after(sum[i], x[i], f4.x), fma_after(sum[i + 1], x[i + 1], f4.y);
-              fma_after(sum[i + 2], x[i + 2], f4.z), fma_after(sum[i + 3], x[i + 3], f4.w);
+              for (int i = 0; i < 32; i += 4) {
+                if constexpr (odd.value) {
+                  const float4 g4 = shared4(f + ((4 + j) * C::kFactors + i) * 4);
+                  mul_after(x[i], g4.x), mul_after(x[i + 1], g4.y), mul_after(x[i + 2], g4.z), mul_after(x[i + 3], g4.w);
+                }
+                const float4 f4 = shared4(f + (j * C::kFactors + i) * 4);
+                fma_after(sum[i], x[i], f4.x), fma_after(sum[i + 1], x[i + 1], f4.y);
+                fma_after(sum[i + 2], x[i + 2], f4.z), fma_after(sum[i + 3], x[i + 3], f4.w);
+              }
+            };
+#pragma unroll
+            for (int j = 0; j < kGroup; j += 2) {
+              if (kb + j >= end) break;
+              load32(in + j * C::kDBlock, v[0]);
+              if (kb + j + 1 < end) load32(in + (j + 1) * C::kDBlock, v[1]);
+              wait_loads();
+              add(j, v[0]);
+              if (kb + j + 1 < end) add(j + 1, v[1]);
             }
           };
-          const uint32_t in = from + d * O::kDSlot;
-#pragma unroll
-          for (int j = 0; j < kGroup; j += 2) {
-            if (kb + j >= end) break;
-            load32(in + j * C::kDBlock, v[0]);
-            if (kb + j + 1 < end) load32(in + (j + 1) * C::kDBlock, v[1]);
-            wait_loads();
-            add(j, v[0]);
-            if (kb + j + 1 < end) add(j + 1, v[1]);
-          }
+          if (__builtin_expect(flag != 0.f, 0))
+            blocks(std::true_type());
+          else
+            blocks(std::false_type());
           free_accumulators();
           if (lane == 0) tc::mbar_arrive(&sc_empty[q]);  // free_accumulators synchronised the warp
           if (++q == kScRing) q = 0, qph ^= 1u;
