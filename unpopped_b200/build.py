@@ -67,6 +67,9 @@ def revision_hash(path: str) -> int:
 # A serving operator's kernels are in more files than the one that its revision hash is of. That one holds a line with the
 # hash of the others, so the revision changes with any of them.
 OPERATOR_SOURCES = {
+    "experts.cu": ("divide.cuh", "launch.cuh"),
+    "f8_matmul.cu": ("divide.cuh", "launch.cuh"),
+    "f8_quantise.cu": ("divide.cuh", "launch.cuh"),
     "rope.cu": ("divide.cuh", "rope.cuh"),
     "kv4_append.cu": ("divide.cuh", "kv4.cuh", "rope.cuh"),
     "kv4_attention.cu": ("divide.cuh", "kv4.cuh", "kv4_attention.cuh", "kv4_prompt.cu", "kv4_split.cuh", "kv4_split_128.cu",
