@@ -9,7 +9,7 @@
 // Bound by instructions, not by the 19 MB: 520 a token in the choice, 215 in the placing. Measured: 1 token of 128 experts 3.3 us, 64 of 256
 // 7.0, 2048 9.4, 16384 22.5.
 // The operator's other sources, which its revision hash covers through this line (build.py --sources):
-// FNV-1a 64 of
+// FNV-1a 64 of divide.cuh, launch.cuh: 2e2d27af524d7113
 #include "common.cuh"
 #include "divide.cuh"
 #include "launch.cuh"

@@ -18,7 +18,7 @@
 // 149 (958 MB of weights: 6.4 TB/s); 8192 rows by 8192 x 8192 496 us (2.22 PFLOP/s; 570 where calls follow one another for seconds and
 // the clock falls to the power limit); 65536 rows of 128 experts by 4096 x 2048 710 (1.55 PFLOP/s).
 // The operator's other sources, which its revision hash covers through this line (build.py --sources):
-// FNV-1a 64 of
+// FNV-1a 64 of divide.cuh, launch.cuh: 2e2d27af524d7113
 #include "common.cuh"
 #include "divide.cuh"
 #include "launch.cuh"

@@ -9,7 +9,7 @@
 // many of the gates are far from 0), gated f32 87 (7.0), plain bf16 40 (5.1); 64 x 4096 x 2048 bf16 weights 5.3 TB/s. Neither a third fewer instructions nor blocks that walk over
 // the pieces with the next one's loads on their way (61 to 120 us gated) made it faster.
 // The operator's other sources, which its revision hash covers through this line (build.py --sources):
-// FNV-1a 64 of
+// FNV-1a 64 of divide.cuh, launch.cuh: 2e2d27af524d7113
 #include "common.cuh"
 #include "divide.cuh"
 #include "launch.cuh"
