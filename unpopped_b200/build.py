@@ -68,7 +68,7 @@ def revision_hash(path: str) -> int:
 # hash of the others, so the revision changes with any of them.
 OPERATOR_SOURCES = {
     "experts.cu": ("divide.cuh", "launch.cuh"),
-    "f8_matmul.cu": ("divide.cuh", "launch.cuh"),
+    "f8_matmul.cu": ("divide.cuh", "f8_walk.cuh", "launch.cuh"),
     "f8_quantise.cu": ("divide.cuh", "launch.cuh"),
     "rope.cu": ("divide.cuh", "rope.cuh"),
     "kv4_append.cu": ("divide.cuh", "kv4.cuh", "rope.cuh"),
