@@ -63,3 +63,43 @@ def test_a_sigmoid_of_logits_whose_scores_are_0(low):
     got = check(logits, 3, "sigmoid")
     assert not bool(got[1][3:].any()) and float(got[1][1, 0]) == 1 and bool((got[1][1:3, 1:] < 2.0 ** -140).all())  # exp(-101) is 10 times 2^-149
     check(logits, 3, "sigmoid", False, 2.0)
+
+
+@pytest.mark.parametrize("tokens", [70, 700])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalise", [True, False])
+def test_masked_experts(tokens, score, renormalise):
+    """Rows that have fewer experts than are asked for, or none."""
+    g = gen(tokens)
+    logits = 3 * torch.randn(tokens, 50, generator=g, device=DEV)
+    logits[torch.rand(tokens, 50, generator=g, device=DEV) < 0.9] = float("-inf")
+    logits[5] = float("-inf")
+    logits[-tokens // 4:] = float("-inf")
+    check(logits, 8, score, renormalise, 1.0 if renormalise else 2.5)
+
+
+@pytest.mark.parametrize("experts,k", [(40, 8), (64, 6), (256, 8), (256, 32), (1000, 32)])
+@pytest.mark.parametrize("score,renormalise", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+def test_equal_logits(experts, k, score, renormalise):
+    """More experts than a warp has lanes reach the k-th largest logit."""
+    logits = torch.randint(0, 3, (150, experts), generator=gen(experts), device=DEV).float()
+    logits[0] = 0.0
+    logits[1] = -0.0
+    logits[2, :k - 1] = 5.0
+    logits[3] = torch.arange(experts, device=DEV) % 32
+    logits[4] = torch.arange(experts, device=DEV) // 32
+    logits[7] = float("-inf")
+    logits[7, 3::7] = -20.0
+    check(logits, k, score, renormalise)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("value", [-3e38, -1e30, 1e30, 3e38])
+def test_logits_of_any_finite_size(score, value):
+    """A row of one huge value, beside ordinary rows whose bound does not know of it."""
+    logits = torch.randn(40, 30, generator=gen(7), device=DEV)
+    logits[7] = value
+    logits[9, 4] = value
+    got = check(logits, 5, score)
+    if score == "softmax" or value > 0:
+        assert bool(((got[1][7] - 0.2).abs() < 1e-6).all())
