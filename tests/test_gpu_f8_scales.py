@@ -3,12 +3,19 @@ import pytest
 import torch
 
 import f8_exact as ex
+import f8_walk
 from unpopped_b200 import ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 # few rows, rows of 128 x 128 tiles, of 128 x 256 ones and of pairs; tiles that are shared, and a last block of k that is short
-SHAPES = [(1, 200, 400), (21, 384, 4096), (40, 300, 272), (300, 1000, 528), (600, 4096, 1040), (300, 300, 8192), (1100, 4096, 528)]
+SHAPES = [(1, 200, 400), (21, 384, 4096), (40, 300, 272), (300, 1000, 528), (600, 4096, 1040), (300, 300, 8192), (1100, 4096, 528), (384, 4096, 4096), (513, 2051, 8192),
+          (1100, 4111, 8208), (2000, 2051, 8208)]
+
+
+def test_the_shapes_take_every_form():
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert {f8_walk.form(m, n, k, 1, sms) for m, n, k in SHAPES} == set(f8_walk.FORMS)
 
 
 def gen(seed):
