@@ -99,3 +99,9 @@ def test_the_choice_of_a_form_is_one_of_them_for_every_size():
         seen.add(f8_walk.form(log_int(rng, 1, 1 << 20), log_int(rng, 1, 30000), 16 * log_int(rng, 1, 2000), rng.choice([1, 1, 8, 128, 1024]),
                               rng.choice([1, 2, 132, 148])))
     assert seen == set(f8_walk.FORMS)
+
+
+def test_the_smoke_test_runs_every_form():
+    import __graft_entry__ as entry
+
+    assert [f8_walk.form(*shape) for shape in entry.F8_PRODUCTS] == ["narrow", "wide 128", "wide 256", "pair 256"]
