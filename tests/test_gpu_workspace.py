@@ -75,3 +75,21 @@ def test_kv4_attention():
     lens, cu = torch.tensor([1000], dtype=torch.int32, device=DEV), torch.tensor([0, 1], dtype=torch.int32, device=DEV)
     q = torch.randn(1, 4, 64, generator=g, device=DEV).bfloat16()
     recovers("kv4", 256, lambda: ops.kv4_attention(q, cache, table, lens, cu))
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 384, 8192), (384, 4096, 4096), (600, 4096, 8192), (5000, 512, 8192)])
+def test_f8_products_under_a_limit_that_no_wait_keeps(m, n, k):
+    """Whatever waits run out, the call ends, its status says so, and the next one is right."""
+    L = _lib.load()
+    p = f8_problem(m, n, k)
+    want = ops.f8_matmul(*p, dtype=torch.float32)
+    space = torch.zeros(L.up_sm100_f8_matmul_workspace_bytes(m, 1, n, k), dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    L.up_sm100_set_wait_limit_ns(1)
+    try:
+        got = ops.f8_matmul(*p, dtype=torch.float32, ws=space)
+        status = ops.workspace_status(space)
+    finally:
+        L.up_sm100_set_wait_limit_ns(1_000_000_000)
+    assert status == _lib.UP_ERR_DEVICE_TIMEOUT or (status == _lib.UP_OK and torch.equal(got, want))
+    assert torch.equal(ops.f8_matmul(*p, dtype=torch.float32, ws=space), want) and ops.workspace_status(space) == _lib.UP_OK

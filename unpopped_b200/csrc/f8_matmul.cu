@@ -38,6 +38,7 @@ namespace f8 {
 constexpr int kBox = 16;                  // tokens of a small TMA box
 constexpr int kMaxExperts = 1024;
 constexpr int kRuns = 4;                  // runs of blocks that the roles may be apart
+constexpr uint64_t kSettleNs = 10000000;  // loads land in some microseconds
 constexpr int kMaxCtas = (UP_F8_COUNTER_BYTES - 64) / 4;  // a counter each
 
 // What follows from a form (f8_walk.cuh).
@@ -413,11 +414,11 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
           }
           tc::mbar_arrive(&run_owners[at.at]);
         }
+        // every load lands before shared memory is released; where a role gave up, its loads' barriers may never complete (see the end)
+        if (rank == 0 && good)
+          for (int64_t j = issued > kStages ? issued - kStages : 0; j < issued && good; ++j)
+            good = wait(&full[j % kStages], (uint32_t)((j / kStages) & 1), a, abort_flag);
         if (!good) give_up();
-        // every load lands before shared memory is released
-        if (rank == 0)
-          for (int64_t j = issued > kStages ? issued - kStages : 0; j < issued; ++j)
-            wait(&full[j % kStages], (uint32_t)((j / kStages) & 1), a, nullptr);
       }
     } else if (!C::kWide && warp == C::kXWarp) {
       // ---------------- the loads of tokens: on the same barriers, which the weights' loads give the bytes of both ----------------
@@ -863,6 +864,12 @@ __device__ __forceinline__ void matmul(const CUtensorMap& wmap, const CUtensorMa
 
   tc::fence_before_sync();
   __syncthreads();
+  if (*abort_flag) {
+    // Some loads were issued whose others were not, so no barrier tells when they have landed: shared memory is kept for a time in which every
+    // load of this GPU's memory has.
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < kSettleNs) __nanosleep(1000);
+  }
   if (PAIR) cluster_sync();  // neither leaves while the other's MMAs or arrivals may still reach it
   tc::fence_after_sync();
   if (warp == 1) tmem_free<PAIR>(tmem);
