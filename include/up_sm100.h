@@ -527,11 +527,12 @@ UP_API size_t up_sm100_kv4_attention_workspace_bytes(int64_t tokens, int64_t q_h
  * have one f32 scale for each 128 values of a row, weights one for each 128 x 128 block; a last block may be shorter. */
 
 /* Rows of x as 8-bit values. Row r of the result is y = x[rows[r]] (rows NULL: x[r], and n_rows = tokens), or with
- * `gate` != 0, where x holds 2k values a row, y[i] = x[i] / (1 + exp(-x[i])) * x[k + i] in f32 (with no loss where exp(-x[i]) leaves f32). For each 128 values of y, with a
- * the largest magnitude of its finite ones: scale = a * f32(1/448), q = e4m3(y * (1/scale)), in f32. Where that scale is below 2^-126 it is
- * 0, and so is q. An infinity or a NaN gives the NaN code in its place. A row whose rows[r] is outside [0, tokens) gives
- * zeros, scales too. x [tokens, k] is F32, F16 or BF16, 16-byte aligned with rows of whole 16 bytes, k a multiple of 16
- * (UP_ERR_UNSUPPORTED else); q [n_rows, k] is dense and 16-byte aligned; scale [n_rows, ceil(k / 128)] has the strides given. */
+ * `gate` != 0, where x holds 2k values a row, y[i] = x[i] / (1 + exp(-x[i])) * x[k + i] in f32 (with no loss where exp(-x[i])
+ * leaves f32). For each 128 values of y, with a the largest magnitude of its finite ones: scale = a * f32(1/448),
+ * q = e4m3(y * (1/scale)), in f32. Where that scale is below 2^-126 it is 0, and so is q. An infinity or a NaN gives the NaN
+ * code in its place. A row whose rows[r] is outside [0, tokens) gives zeros, scales too. x [tokens, k] is F32, F16 or BF16,
+ * 16-byte aligned with rows of whole 16 bytes, k a multiple of 16 (UP_ERR_UNSUPPORTED else); q [n_rows, k] is dense and
+ * 16-byte aligned; scale [n_rows, ceil(k / 128)] has the strides given. */
 UP_API int up_sm100_f8_quantise(const void* x, int dtype, int64_t tokens, int64_t x_stride, const int32_t* rows,
                                 int64_t n_rows, int64_t k, int gate, uint8_t* q, float* scale, int64_t scale_stride_r,
                                 int64_t scale_stride_b, void* stream);
@@ -567,12 +568,12 @@ typedef enum up_expert_score { UP_EXPERT_SOFTMAX = 0, UP_EXPERT_SIGMOID = 1 } up
 /* Routes tokens to experts and lays the pairs out by expert. Of each row of logits [tokens, experts] (F32, F16 or BF16) the
  * k largest are taken, largest first, the lower expert of equal ones, a NaN before all others; an expert whose logit is
  * -inf is never taken. ids[t][j] is the expert (-1 where none is left), weights[t][j] its score in f32 (0 there), divided by
- * the chosen ones' sum with `renormalise` != 0 (0 where the largest is 0; shares of scores below 2^-126 are as precise as others), times gain. The pairs that were taken, in the order
- * of their expert and then of their token, have the places 0, 1, ...: slots[t][j] is a pair's place (-1 for none), rows[place] its
- * token (-1 behind the last), offsets[e] the first place of expert e and offsets[experts] the number of pairs. At most
- * 1024 experts, k at most 32 and at most experts, tokens * k below 2^31. `workspace` from
- * up_sm100_expert_route_workspace_bytes, 256-byte aligned; what it holds does not matter. Launches that overlap on the
- * GPU need separate workspaces. */
+ * the chosen ones' sum with `renormalise` != 0 (0 where the largest is 0; shares of scores below 2^-126 are as precise as
+ * others), times gain. The pairs that were taken, in the order of their expert and then of their token, have the places 0, 1,
+ * ...: slots[t][j] is a pair's place (-1 for none), rows[place] its token (-1 behind the last), offsets[e] the first place of
+ * expert e and offsets[experts] the number of pairs. At most 1024 experts, k at most 32 and at most experts, tokens * k below
+ * 2^31. `workspace` from up_sm100_expert_route_workspace_bytes, 256-byte aligned; what it holds does not matter. Launches that
+ * overlap on the GPU need separate workspaces. */
 UP_API int up_sm100_expert_route(const void* logits, int dtype, int64_t tokens, int64_t experts, int64_t stride, int64_t k,
                                  int score, int renormalise, float gain, int32_t* ids, float* weights, int32_t* rows,
                                  int32_t* slots, int32_t* offsets, void* workspace, size_t workspace_bytes,

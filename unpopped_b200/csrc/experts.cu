@@ -6,8 +6,8 @@
 // are counted and placed by expert. A pair's place is the number of pairs of lower experts plus that of the same
 // expert's earlier tokens, so it does not depend on the order in which anything runs: within 128 tokens the earlier
 // ones are the lower bits of a mask that each expert has (set by atomicOr, which commutes), before them the counts of earlier blocks.
-// Bound by instructions, not by the 19 MB: 520 a token in the choice, 215 in the placing. Measured: 1 token of 128 experts 3.3 us, 64 of 256
-// 7.0, 2048 9.4, 16384 22.5.
+// Bound by instructions, not by the 19 MB: 530 a token in the choice, 215 in the placing. Measured: 1 token of 128 experts 3.5 us, 64 of 256
+// 7.0, 2048 9.4, 16384 22.9. (With 513 to 1024 experts a lane holds 32 keys, and some 40 to 90 words of a thread's are kept in memory.)
 // The operator's other sources, which its revision hash covers through this line (build.py --sources):
 // FNV-1a 64 of divide.cuh, launch.cuh: 2e2d27af524d7113
 #include "common.cuh"

@@ -14,11 +14,11 @@
 //    token, so a block's scales are one factor for all of its columns. (With tokens as columns every thread needs every token's
 //    factor: at 128 bytes a cycle shared memory gives those of 128 x 128 values in 512 cycles, in which the MMA takes 256.) Bound by
 //    the two accumulators' round: an MMA of 512 cycles, its commit, the epilogue's loads and 128 sums a thread, the arrival that frees it.
-// Measured: 1 row by 8192 x 8192 weights 16.4 us (4.1 TB/s of weights), by 28672 x 8192 42 (5.6 TB/s); 512 rows of 128 experts by 4096 x 2048
-// 149 (958 MB of weights: 6.4 TB/s); 8192 rows by 8192 x 8192 496 us (2.22 PFLOP/s; 570 where calls follow one another for seconds and
-// the clock falls to the power limit); 65536 rows of 128 experts by 4096 x 2048 710 (1.55 PFLOP/s).
+// Measured: 1 row by 8192 x 8192 weights 16.3 us (4.1 TB/s of weights), by 28672 x 8192 42 (5.6 TB/s); 512 rows of 128 experts by 4096 x 2048
+// 150 (958 MB of weights: 6.4 TB/s). Where calls follow one another for seconds and the clock falls to the power limit, 8192 rows by
+// 8192 x 8192 take 583 us (1.89 PFLOP/s; 513 alone), 65536 rows of 128 experts by 4096 x 2048 853 (1.29 PFLOP/s; 729 alone).
 // The operator's other sources, which its revision hash covers through this line (build.py --sources):
-// FNV-1a 64 of divide.cuh, f8_walk.cuh, launch.cuh: dceec32fb00ae1e3
+// FNV-1a 64 of divide.cuh, f8_walk.cuh, launch.cuh: 45adde3f9cc64f52
 #include "common.cuh"
 #include "f8_walk.cuh"
 #include "launch.cuh"

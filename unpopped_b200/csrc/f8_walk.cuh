@@ -148,13 +148,15 @@ struct Walk {
 enum Form { kNarrow, kWide256, kPair256, kWide128 };
 
 // The form that takes the least time by a model: a fixed part (launch, first loads, output), then so many microseconds for each block of k of
-// the tiles of one owner, which Walk deals out. Fitted to which form was the fastest in 86 calls of 1 to 65536 rows, dense and by expert, by
-// 512 x 1024 to 28672 x 8192 weights; the choice takes 0.3 % longer than the fastest in the mean, 10 % at most. Without one of the forms calls take
-// 1.7 to 6.9 % longer in the mean, 18 to 59 % at most. (A form of 64 tokens as columns was the fastest by 4 to 12 % for some calls
-// of 64 to 256 rows, by 0.2 % in the mean; one of 256 tokens by 128 weights never was.) Measured, us, in the order of the table:
-//   rows by 2048 x 1024 weights:   1: 6.0, 7.1, 7.7, 5.7;     512: 8.6, 9.1, 9.6, 6.5;      8192: 68, 30, 31, 32
-//   rows by 8192 x 8192 weights:   1: 16.4, 26.3, 34.6, 28.3; 128: 33.9, 28.7, 34.1, 23.7;  512: 100, 39.6, 38.4, 50.8;  8192: 1528, 575, 544, 839 (496 by panels)
-//   128 experts' 4096 x 2048:      512: 149, 168, 250, 188;   8192: 312, 207, 326, 277;     65536: 1795, 731, 758, 883
+// the tiles of one owner. It was fitted before the tiles of many rows went by panels and those of few by equal numbers of owners, and knows of
+// neither: a tile's parts are counted here as if every owner had one share of them. Measured since, on 86 calls of 1 to 65536 rows, dense and by
+// expert, by 512 x 1024 to 28672 x 8192 weights, the choice takes 0.4 % longer than the fastest form in the mean, 9 % at most (2048 rows by
+// 1024 x 8192 weights: 32.4 us, where a pair takes 29.8). Without one of the forms the best of the others takes 1.0 to 5.4 % longer in the mean,
+// 12 to 47 % at most. (A form of 64 tokens as columns was the fastest by 4 to 12 % for some calls of 64 to 256 rows, by 0.2 % in the mean; one of
+// 256 tokens by 128 weights never was.) Measured, us, in the order of the table:
+//   rows by 2048 x 1024 weights:   512: 9.3, 9.4, 9.8, 6.6;     8192: 76, 30.5, 31.0, 31.6
+//   rows by 8192 x 8192 weights:   1: 16.5, 26.4, 30.2, 24.2;   128: 34.4, 28.6, 30.4, 24.3;  512: 102, 40.5, 39.3, 50.8;  8192: 1604, 539, 512, 853
+//   128 experts' 4096 x 2048:      512: 147, 165, 248, 188;     8192: 303, 210, 319, 269;     65536: 1732, 723, 758, 893
 inline Form form_of(int64_t m, int64_t experts, int64_t n, int64_t kb, int ctas) {
   struct Cost {
     int tokens, weights, ctas, least, join;  // of a tile; Walk's

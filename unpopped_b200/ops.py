@@ -501,7 +501,8 @@ def f8_quantise(x: torch.Tensor, rows: torch.Tensor | None = None, gate: bool = 
     float8_e4m3fn [n, k] with one f32 scale for each 128 values of a row, [n, ceil(k / 128)] (a block's scales lie beside one
     another in memory, as `f8_matmul` reads them fastest). rows (int32 [n]): row r is x[rows[r]], and zeros where that is no row of
     x (`expert_route`'s rows). gate: x holds 2k values a row, and y = silu(x[:, :k]) * x[:, k:] is quantised, in f32.
-    scale = max|y| / 448 over a block's finite values; an infinity or a NaN reads back as NaN. No part of autograd."""
+    scale = max|y| / 448 over a block's finite values; an infinity or a NaN reads back as NaN. q and scale are parts of one allocation (saving
+    one, or keeping it, saves or keeps both; clone it to part them). No part of autograd."""
     return _calls().f8_quantise(x, rows, gate)
 
 
@@ -516,7 +517,8 @@ def f8_matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     """[rows, n] = x [rows, k] times w [n, k], both float8_e4m3fn with their scales (`f8_quantise`, `f8_quantise_weight`):
     tcgen05 products of each block of 128, scaled and summed in f32, rounded once to `dtype` (bfloat16, float16 or float32;
     out's where it is given). Any number of rows and columns; k a multiple of 16. x's and out's rows may be views; out overlaps nothing
-    that is read.
+    that is read; w and w_scale are contiguous. Calls of one shape give the same bits each time. A row's last bits may differ between calls of other
+    numbers of rows, as sums are then taken in another order.
     ws: a workspace of the caller's, contiguous, its first 8192 bytes zero-filled once; without one the stream's is used, or
     a captured graph's own. Like `w4a16` it is no part of autograd."""
     return _calls().f8_matmul(x, x_scale, w, w_scale, None, dtype, out, ws)
@@ -541,7 +543,8 @@ def expert_route(logits: torch.Tensor, k: int, score: str = "softmax", renormali
     "softmax" over all experts or "sigmoid", divided by the chosen ones' sum (renormalise), times gain; 0 for -1. rows int32
     [tokens * k]: the token at each place, -1 behind the last (`f8_quantise` gathers by it). slots int32 [tokens, k]: each
     pair's place, or -1 (`expert_combine` reads it). offsets int32 [experts + 1]: where each expert's places begin
-    (`f8_expert_matmul` takes it). One launch up to 64 tokens, two above; nothing comes to the host."""
+    (`f8_expert_matmul` takes it). One launch up to 64 tokens, two above; nothing comes to the host. The five are parts of one allocation
+    (clone what is to be kept or saved alone). No part of autograd: the weights carry no gradient to the logits."""
     return _calls().expert_route(logits, k, score, renormalise, gain)
 
 
