@@ -47,7 +47,8 @@ struct Of {
   static constexpr int kStage = kTile + C::kBBytes;
   static constexpr int kDSlot = C::kDBlock * C::kGroup, kDRing = 512 / kDSlot;  // accumulators in tensor memory
   static constexpr int kEpiThreads = 32 * C::kEpiWarps, kThreads = 32 * C::kEpi0 + kEpiThreads;
-  static constexpr int kScRing = C::kFactors > 0 ? 4 : 0, kScSlot = 8 * C::kFactors + 4;  // factors in shared memory, four blocks a slot, twice (Scales), and whether the second are there
+  // factors in shared memory, four blocks a slot, twice (Scales), and whether the second are there
+  static constexpr int kScRing = C::kFactors > 0 ? 4 : 0, kScSlot = 8 * C::kFactors + 4;
   static constexpr int kStaged = C::kWide ? 32 * 17 : 0;             // values a warp, for rows of `out` that do not begin on 32 bytes
   static constexpr size_t kPart = (size_t)C::kSums * kEpiThreads;  // values of a CTA's part of a tile
   // One thread issues the MMAs and commits of a block in some 450 cycles, so two take the blocks in turn; the ring's even

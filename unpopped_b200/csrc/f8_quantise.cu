@@ -5,9 +5,10 @@
 // gate too: y = x / (1 + exp(-x)) * u by f32's exponential and rounded quotient. (By ex2.approx and rcp.approx y was 2^-19 off, and a third more
 // codes than with these were on the other side of a border of e4m3's.)
 //
-// Bound by HBM: 2 (4, 8) bytes read and 1.03 written a value. Measured: 32768 x 2048 gated bf16 values 62.5 us (5.4 TB/s; 71 where
-// many of the gates are far from 0), gated f32 87 (7.0), plain bf16 40 (5.1); 64 x 4096 x 2048 bf16 weights 5.3 TB/s. Neither a third fewer instructions nor blocks that walk over
-// the pieces with the next one's loads on their way (61 to 120 us gated) made it faster.
+// Bound by HBM: 2 (4, 8) bytes read and 1.03 written a value; gated 16-bit values by instructions as well (82 % of the issue slots). Measured:
+// 32768 x 2048 gated bf16 values 62.5 us (5.4 TB/s; 68 to 71 where many of the gates are far from 0), gated f32 87 (7.0), plain bf16 40
+// (5.1); 64 x 4096 x 2048 bf16 weights 5.3 TB/s. Blocks that walk over the pieces with the next one's loads on their way took 61 to 120
+// us where the same sums without took 59.
 // The operator's other sources, which its revision hash covers through this line (build.py --sources):
 // FNV-1a 64 of divide.cuh, launch.cuh: 2e2d27af524d7113
 #include "common.cuh"
